@@ -143,9 +143,9 @@ def _quantised(x, codes):
     if codes in ("bf16", "fp16"):
         return x.to(CODES[codes]), None
     a = x.abs().amax(-1)
-    inv = torch.where(a > 0, TOP[codes] / a, torch.zeros_like(a))
-    y = x * inv[..., None]
-    return (y.round() if codes == "int8" else y).to(CODES[codes]), a / TOP[codes]
+    top = torch.full_like(a, TOP[codes])  # a tensor: dividing by or into a number is a product with a reciprocal
+    y = x * torch.where(a > 0, top / a, 0.0)[..., None]
+    return (y.round() if codes == "int8" else y).to(CODES[codes]), a / top
 
 
 def _stored(heads, pages, page, dim, codes, g):
