@@ -518,6 +518,58 @@ int ng_batch_rows(const int* cells, const int* entries, ng_i64 n, ng_i64 capacit
 int ng_batch_rows_noalloc(const int* cells, const int* entries, ng_i64 n, ng_i64 capacity, int* out, ng_u64* total,
                           void* stream);
 
+/* ------------------------------------------------------------------------------------------------------------
+ * Model-side operators (no counterpart among the reference's kernels): hint rows embedded, a key/value cache held in 8
+ * bits, and attention for a tree of drafted tokens over it. Element types: 0 float32, 1 bfloat16, 2 float16.
+ * ------------------------------------------------------------------------------------------------------------ */
+
+/* Hint rows embedded (old_records/hint_runtime.py:381-418 is the contract): out [n, dim] (dtype, contiguous): out[i] =
+ * scale * the sum over position i's m entries with w != 0 and a cell of w * table[token]; table [V, dim] of row stride ld
+ * (elements); tokens [n, m] of tsize bytes (8 int64, 4 int32, 2 uint16); w float32 [n, m] or NULL (all 1); cell
+ * [n, m / entries] of csize bytes (8, 4, 2; signed) or NULL (every slot counts). A counted token outside [0, V) makes its
+ * row NaN. n * m < 2^31 - 64, V < 2^31.
+ * ng_embed_grad: grad [V, dim] (dtype, contiguous; every row written) = scale * the sum over the counted entries of each
+ * token of w * dout[position]; dout [n, dim] of row stride ld; work: ng_embed_grad_work(n * m, V, dim) bytes.
+ * ng_embed_weight_grad: dw float32 [n, m] = scale * <table[token], dout[position]> where the slot has a cell, else 0. */
+int ng_embed(const void* table, ng_i64 ld, ng_i64 V, int dim, int dtype, const void* tokens, int tsize, const float* w,
+             const void* cell, int csize, ng_i64 n, int m, int entries, float scale, void* out, void* stream);
+ng_i64 ng_embed_grad_work(ng_i64 entries, ng_i64 V, ng_i64 dim);
+int ng_embed_grad(const void* dout, ng_i64 ld, ng_i64 V, int dim, int dtype, const void* tokens, int tsize, const float* w,
+                  const void* cell, int csize, ng_i64 n, int m, int entries, float scale, void* grad, void* work,
+                  void* stream);
+int ng_embed_weight_grad(const void* table, ng_i64 ld, const void* dout, ng_i64 dld, ng_i64 V, int dim, int dtype,
+                         const void* tokens, int tsize, const void* cell, int csize, ng_i64 n, int m, int entries,
+                         float scale, float* dw, void* stream);
+
+/* A paged key/value cache. Codes [pages, heads, page, DP] (DP: dim to a multiple of 64), codes: 0 int8, 1 fp8 e4m3 (with
+ * float32 scales ks, vs [pages, heads, page]), 2 bfloat16, 3 float16 (no scales); page a power of two, 16 .. 4096; dim <=
+ * 256; codes and scales 16-byte aligned. slots int64 [n]: page * page size + row, not written / read as 0 where out of
+ * range.
+ * ng_kv_write: k, v [n, heads, dim] of dtype, strides of tokens and heads in elements. ng_kv_read: k, v [n, heads, dim] of
+ * dtype, contiguous. ng_kv_slots: out [B, count] = the slots of positions start[b] + i by the page tables [B, width] of row
+ * stride `stride`, -1 where there is none. */
+int ng_kv_write(const void* k, const void* v, ng_i64 k_tok, ng_i64 k_head, ng_i64 v_tok, ng_i64 v_head, int dtype,
+                const ng_i64* slots, ng_i64 n, void* kc, void* vc, float* ks, float* vs, ng_i64 pages, int page, int heads,
+                int dim, int codes, void* stream);
+int ng_kv_read(const void* kc, const void* vc, const float* ks, const float* vs, ng_i64 pages, int page, int heads,
+               int dim, int codes, const ng_i64* slots, ng_i64 n, void* k, void* v, int dtype, void* stream);
+int ng_kv_slots(const int* table, ng_i64 stride, int width, const int* start, int B, int count, ng_i64 pages, int page,
+                ng_i64* out, void* stream);
+
+/* Attention for trees of T <= 64 drafted tokens: q [B, T, H * G, dim] (strides qb, qt, qh in elements; qtype 1 or 2, a
+ * 16-bit cache's own) over the cache's H heads; sequence b's lengths[b] cached tokens, then its tree (token i at position
+ * lengths[b] + i); mask [B, T]: bit j of [b, i] lets token i see token j (NULL: 0 .. i); widths [B]: tree tokens in use
+ * (NULL: T). Table entries outside [0, pages) mask their keys; width * page <= 2^30. out [B, T, H * G, dim] contiguous of
+ * qtype; lse float32 [B, T, H * G] or NULL; work: ng_tree_attention_work(B, T, H, G, dim, codes, width * page) bytes (-1:
+ * out of range).
+ * ng_tree_mask: bits [B, T] of each token and its ancestors, from parents [B, T] (negative or not earlier: none). */
+ng_i64 ng_tree_attention_work(ng_i64 B, ng_i64 T, ng_i64 H, ng_i64 G, ng_i64 dim, ng_i64 codes, ng_i64 cap);
+int ng_tree_attention(const void* q, ng_i64 qb, ng_i64 qt, ng_i64 qh, int qtype, const void* k, const void* v,
+                      const float* ks, const float* vs, ng_i64 pages, int page, int codes, const int* table,
+                      ng_i64 table_stride, int width, const int* lengths, const int* widths, const ng_u64* mask, int B,
+                      int T, int H, int G, int dim, float scale, void* out, float* lse, void* work, void* stream);
+int ng_tree_mask(const int* parents, int B, int T, ng_u64* bits, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

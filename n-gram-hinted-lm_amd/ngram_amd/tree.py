@@ -1,0 +1,101 @@
+"""Attention for a tree of drafted tokens over a paged cache (kvcache.py): how a model verifies the continuations that this
+package's counts and matches draft. A sequence of lengths[b] cached tokens gets up to 64 drafted ones in a step, their keys
+and values written behind the cached ones (the token i of the tree at position lengths[b] + i); each sees the cached tokens
+and its own ancestors, so every path of the tree is scored as if it were the sequence's continuation. One token without a
+mask is ordinary decoding.
+
+  tree_attention(q, cache, table, lengths, mask=None, widths=None, scale=None, return_lse=False)
+  tree_mask(parents)    the ancestors' bits of trees given by their parents
+
+Everything runs on the current stream; lengths and widths are read on the device only. csrc/tree.hip has the kernels."""
+
+from __future__ import annotations
+
+import ctypes
+import functools
+import math
+
+import torch
+
+from .kvcache import KVCache, check_table
+from .lib import Lib, i32
+
+WIDEST = 64  # tokens of a tree: the bits of a mask
+DTYPES = {torch.bfloat16: 1, torch.float16: 2}
+
+
+@functools.lru_cache(maxsize=None)
+def _lib() -> Lib:
+    return Lib()
+
+
+@functools.lru_cache(maxsize=1024)
+def _work(B: int, T: int, H: int, G: int, dim: int, code: int, capacity: int) -> int:
+    n = _lib().size("ng_tree_attention_work", B, T, H, G, dim, code, capacity)
+    if n < 0:
+        raise ValueError(f"{B} sequences of {T} tokens, {H} heads x {G}, dim {dim}, tables of {capacity} tokens: out of "
+                         "range (tables hold at most 2^30 tokens)")
+    return n
+
+
+def tree_mask(parents: torch.Tensor) -> torch.Tensor:
+    """int64 [B, T]: bit j of [b, i] is set where token j is i or an ancestor of it. parents int32 [B, T], T <= 64: each
+    token's parent, an earlier token; negative (or not earlier): the last cached token."""
+    if parents.dtype != torch.int32 or parents.dim() != 2 or not 1 <= parents.shape[1] <= WIDEST or not parents.is_cuda:
+        raise ValueError(f"parents must be int32 [B, 1 to {WIDEST}] on the GPU: got {tuple(parents.shape)} "
+                         f"{parents.dtype} on {parents.device}")
+    out = torch.empty(parents.shape, dtype=torch.int64, device=parents.device)
+    with torch.cuda.device(parents.device):
+        _lib()("ng_tree_mask", parents.contiguous(), i32(parents.shape[0]), i32(parents.shape[1]), out)
+    return out
+
+
+def tree_attention(q: torch.Tensor, cache: KVCache, table: torch.Tensor, lengths: torch.Tensor,
+                   mask: torch.Tensor | None = None, widths: torch.Tensor | None = None, scale: float | None = None,
+                   return_lse: bool = False):
+    """Attention of q [B, T, heads * group, dim] (bfloat16 or float16, a 16-bit cache's own type; any strides over the
+    first three) over the cached tokens and the tree; query head h reads the cache's head h // group.
+
+    table    int32 [B, width]: the sequences' pages in order; keys whose entry is no page of the cache are masked
+    lengths  int32 [B]: the cached tokens before the tree (held to 0 .. what the table covers)
+    mask     int64 [B, T]: bit j of [b, i] lets tree token i see tree token j; None: a chain (i sees 0 .. i)
+    widths   int32 [B]: the tree tokens in use (None: all T); the rows past them are zeros, their keys masked
+    scale    the scores' factor, 1 / sqrt(dim) by default
+
+    Returns the output in q's shape and type, and with return_lse the float32 [B, T, heads * group] logarithms of the
+    softmax sums. A row that sees nothing is zeros, its logarithm -inf."""
+    if q.dim() != 4 or q.dtype not in DTYPES:
+        raise ValueError(f"q must be [B, T, heads, dim] in bfloat16 or float16: got {tuple(q.shape)} {q.dtype}")
+    B, T, heads, dim = q.shape
+    if dim != cache.dim or heads < 1 or heads % cache.heads or not 1 <= T <= WIDEST:
+        raise ValueError(f"q {tuple(q.shape)} does not go with {cache.heads} cached heads of {cache.dim}: a multiple of the "
+                         f"heads, 1 to {WIDEST} tokens")
+    if cache.code >= 2 and q.dtype != cache.k.dtype:
+        raise ValueError(f"a {cache.k.dtype} cache takes queries of its own type: got {q.dtype}")
+    device = cache.k.device
+    if q.device != device:
+        raise ValueError(f"q is on {q.device}, the cache on {device}")
+    check_table(cache, table)
+    for name, t, shape, dt in (("table", table, (B, table.shape[1]), torch.int32), ("lengths", lengths, (B,), torch.int32),
+                               ("mask", mask, (B, T), torch.int64), ("widths", widths, (B,), torch.int32)):
+        if t is not None and (t.shape != shape or t.dtype != dt or t.device != device):
+            raise ValueError(f"{name} must be {dt} {shape} on {device}: got {tuple(t.shape)} {t.dtype} on {t.device}")
+    scale = 1 / math.sqrt(dim) if scale is None else float(scale)
+    if not math.isfinite(scale):
+        raise ValueError(f"scale must be finite: {scale}")
+    if q.stride(3) != 1 and dim > 1:
+        q = q.contiguous()
+    lengths = lengths.contiguous()
+    mask = None if mask is None else mask.contiguous()
+    widths = None if widths is None else widths.contiguous()
+    group, width = heads // cache.heads, table.shape[1]
+    with torch.cuda.device(device):
+        out = torch.empty((B, T, heads, dim), dtype=q.dtype, device=device)
+        lse = torch.empty((B, T, heads), dtype=torch.float32, device=device) if return_lse else None
+        work = torch.empty(_work(B, T, cache.heads, group, dim, cache.code, width * cache.page), dtype=torch.uint8,
+                           device=device)
+        _lib()("ng_tree_attention", q, q.stride(0), q.stride(1), q.stride(2), i32(DTYPES[q.dtype]), cache.k, cache.v,
+               cache.k_scale, cache.v_scale, cache.pages, i32(cache.page), i32(cache.code), table, table.stride(0),
+               i32(width), lengths, widths, mask, i32(B), i32(T), i32(cache.heads), i32(group), i32(dim),
+               ctypes.c_float(scale), out, lse, work)
+    return (out, lse) if return_lse else out
