@@ -1,0 +1,726 @@
+// The tree attention kernel (tree.hip has the mathematics and the host's side; a file per cache type instantiates it).
+#pragma once
+#include "vals.h"
+
+typedef float f4 __attribute__((ext_vector_type(4)));
+typedef f16 h2 __attribute__((ext_vector_type(2)));
+typedef f16 h8 __attribute__((ext_vector_type(8)));
+typedef b16 b8 __attribute__((ext_vector_type(8)));
+
+#define TILE 128  // keys of a block's step: 32 a wave
+#define LOG2E 1.4426950408889634f
+#define LN2 0.6931471805599453f
+
+struct TreeArgs {
+    const void* q;
+    i64 qb, qt, qh;  // strides of q [B, T, H * G, dim] in elements
+    const void *k, *v;
+    const float *ks, *vs;
+    const int* table;
+    i64 table_stride;
+    const int *lengths, *widths;
+    const u64* mask;
+    void* out;   // [B, T, H * G, dim]
+    float* lse;  // [B, T, H * G] or NULL
+    float *po, *pm, *pl;  // partial sums [2 * blocks, rows a block, DP], maxima and sums [2 * blocks, rows a block]
+    i64 pages;
+    int B, T, H, G, dim, shift, width;  // width: the table's entries a sequence
+    int groups;  // row groups of a kv head
+    int qtype, vec;
+    float scale;
+};
+
+struct TreePlan {
+    int rpb, groups, dp;
+    int blocks;
+    bool join;
+    i64 po, pm, bytes;  // offsets in the workspace
+};
+
+// the launches for one cache type
+template <int CODES> int tree_codes(const TreeArgs& a, const TreePlan& p, hipStream_t st);
+
+struct Seq {
+    int len, w, n, tiles;
+};
+
+__device__ __forceinline__ Seq seq_of(const TreeArgs& a, int b) {
+    Seq s;
+    const i64 cap = (i64)a.width << a.shift;
+    const int l = a.lengths[b], w = a.widths ? a.widths[b] : a.T;
+    s.len = l < 0 ? 0 : (i64)l > cap ? (int)cap : l;
+    s.w = w < 0 ? 0 : w > a.T ? a.T : w;
+    const i64 n = (i64)s.len + s.w;
+    s.n = (int)(n < cap ? n : cap);
+    s.tiles = s.n > 0 ? (s.n + TILE - 1) / TILE : 1;
+    return s;
+}
+
+__device__ __forceinline__ int scan_wave(int x) {  // inclusive sum over the lanes
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+        const int up = __shfl_up(x, o, 64);
+        if (lane_id() >= o) x += up;
+    }
+    return x;
+}
+
+// The work laid end to end: sequence by sequence, in each its units (kv head, group of rows), in each its tiles. A share is
+// `per` tiles. Each wave finds its place by itself: one load and one scan for 64 sequences.
+struct Line {
+    Seq mine;  // of sequence lane_id()
+    int inc;   // tiles up to and with it
+    int total, per, shares;
+
+    __device__ __forceinline__ Line(const TreeArgs& a, int blocks) {
+        const int units = a.H * a.groups;
+        const int b = lane_id() < a.B ? lane_id() : a.B - 1;
+        mine = seq_of(a, b);
+        inc = scan_wave(lane_id() < a.B ? mine.tiles * units : 0);
+        total = __shfl(inc, 63, 64);
+        for (int b0 = 64; b0 < a.B; b0 += 64) {
+            int t = b0 + lane_id() < a.B ? seq_of(a, b0 + lane_id()).tiles * units : 0;
+            total += __shfl(scan_wave(t), 63, 64);
+        }
+        per = (total + blocks - 1) / blocks;
+        shares = (total + per - 1) / per;
+    }
+
+    // the sequence that holds tile x < total, and the tiles before it
+    __device__ __forceinline__ int at(const TreeArgs& a, int x, int& before, Seq& q) const {
+        const int units = a.H * a.groups;
+        u64 past = __ballot(inc > x);
+        if (past) {
+            const int l = __builtin_ctzll(past);
+            q.len = lane(mine.len, l), q.w = lane(mine.w, l), q.n = lane(mine.n, l), q.tiles = lane(mine.tiles, l);
+            before = lane(inc, l) - q.tiles * units;
+            return l;
+        }
+        int run = __shfl(inc, 63, 64);
+        for (int b0 = 64;; b0 += 64) {
+            Seq s;
+            s.len = s.w = s.n = s.tiles = 0;
+            if (b0 + lane_id() < a.B) s = seq_of(a, b0 + lane_id());
+            const int i = scan_wave(s.tiles * units);
+            past = __ballot(run + i > x);
+            if (past || b0 + 64 >= a.B) {
+                const int l = past ? __builtin_ctzll(past) : 63;
+                q.len = lane(s.len, l), q.w = lane(s.w, l), q.n = lane(s.n, l), q.tiles = lane(s.tiles, l);
+                before = run + lane(i, l) - q.tiles * units;
+                return b0 + l;
+            }
+            run += __shfl(i, 63, 64);
+        }
+    }
+
+    // the tiles before sequence b
+    __device__ __forceinline__ int before(const TreeArgs& a, int b, Seq& q) const {
+        const int units = a.H * a.groups;
+        int run = 0;
+        for (int b0 = 0;; b0 += 64) {
+            Seq s = mine;
+            int i = inc;
+            if (b0) {
+                s.len = s.w = s.n = s.tiles = 0;
+                if (b0 + lane_id() < a.B) s = seq_of(a, b0 + lane_id());
+                i = scan_wave(s.tiles * units);
+            }
+            if (b < b0 + 64) {
+                const int l = b - b0;
+                q.len = lane(s.len, l), q.w = lane(s.w, l), q.n = lane(s.n, l), q.tiles = lane(s.tiles, l);
+                return run + lane(i, l) - q.tiles * units;
+            }
+            run += __shfl(i, 63, 64);
+        }
+    }
+    static __device__ __forceinline__ int lane(int x, int l) { return __builtin_amdgcn_readlane(x, l); }
+};
+
+// ---------------------------------------------------------------------------------------------- codes to operands
+
+template <int CODES> struct op_t { typedef f16 type; };
+template <> struct op_t<KV_BF16> { typedef b16 type; };
+
+__device__ __forceinline__ f4 mma(h8 a, h8 b, f4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
+__device__ __forceinline__ f4 mma(b8 a, b8 b, f4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
+
+template <typename V8> union Words {
+    u32 u[4];
+    V8 v;
+};
+
+// Eight consecutive codes of a row (8 bits: two words; 16 bits: four) as an operand. int8 (its words' sign bits flipped
+// where they were loaded: c + 128): the bytes are taken for f16 as they stand, which are (c + 128) 2^-24 exactly (two
+// permutes a word and no conversion); the accumulators start at -128 2^-24 sum(q) (K_OFF) and the score's factor has 2^24.
+template <int CODES, typename V8> __device__ __forceinline__ V8 row_operand(const u32* w) {
+    Words<V8> x;
+    if constexpr (CODES == KV_INT8) {
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            x.u[2 * i] = __builtin_amdgcn_perm(0u, w[i], 0x0c010c00u);
+            x.u[2 * i + 1] = __builtin_amdgcn_perm(0u, w[i], 0x0c030c02u);
+        }
+    } else if constexpr (CODES == KV_FP8) {
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            x.u[2 * i] = __builtin_bit_cast(u32, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w[i], 1.f, false));
+            x.u[2 * i + 1] = __builtin_bit_cast(u32, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w[i], 1.f, true));
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) x.u[i] = w[i];
+    }
+    return x.v;
+}
+
+// Elements 2 p and 2 p + 1 of eight rows (v[row][words]) as two operands. int8: (c + 128) 2^-24 as above, then one
+// multiply-add to c 2^-9 (the outputs are multiplied by 2^9 at the end): a sum of c + 128 would lose what c's sum has.
+template <int CODES, typename V8, int VW>
+__device__ __forceinline__ void col_operands(const u32 (&v)[8][VW], int p, V8& lo, V8& hi) {
+    Words<V8> x, y;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        if constexpr (CODES == KV_INT8) {
+            const u32 a = v[2 * i][p >> 1], b = v[2 * i + 1][p >> 1], by = 2 * (p & 1);
+            const h2 k = {(f16)32768.f, (f16)32768.f}, o = {(f16)-0.25f, (f16)-0.25f};
+            const u32 s = 0x0c040c00u + by * 0x00010001u;
+            x.u[i] = __builtin_bit_cast(u32, __builtin_elementwise_fma(__builtin_bit_cast(h2, __builtin_amdgcn_perm(b, a, s)), k, o));
+            y.u[i] = __builtin_bit_cast(u32, __builtin_elementwise_fma(__builtin_bit_cast(h2, __builtin_amdgcn_perm(b, a, s + 0x00010001u)), k, o));
+        } else if constexpr (CODES == KV_FP8) {
+            const u32 by = 2 * (p & 1);
+            const u32 t = __builtin_amdgcn_perm(v[2 * i + 1][p >> 1], v[2 * i][p >> 1], 0x05010400u + by * 0x01010101u);
+            x.u[i] = __builtin_bit_cast(u32, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(t, 1.f, false));
+            y.u[i] = __builtin_bit_cast(u32, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(t, 1.f, true));
+        } else {
+            x.u[i] = __builtin_amdgcn_perm(v[2 * i + 1][p], v[2 * i][p], 0x05040100u);
+            y.u[i] = __builtin_amdgcn_perm(v[2 * i + 1][p], v[2 * i][p], 0x07060302u);
+        }
+    }
+    lo = x.v, hi = y.v;
+}
+
+// N words at p, which is aligned to a word at least (rows of 192 put a lane's values at multiples of 12 bytes)
+typedef u32 w4 __attribute__((ext_vector_type(4), aligned(4)));
+typedef u32 w2 __attribute__((ext_vector_type(2), aligned(4)));
+template <int N> __device__ __forceinline__ void load_words(const char* p, u32* w) {
+#pragma unroll
+    for (int i = 0; i + 4 <= N; i += 4) {
+        const w4 x = *(const w4*)(p + 4 * i);
+        w[i] = x[0], w[i + 1] = x[1], w[i + 2] = x[2], w[i + 3] = x[3];
+    }
+    if constexpr (N % 4 >= 2) {
+        const w2 x = *(const w2*)(p + 4 * (N / 4 * 4));
+        w[N / 4 * 4] = x[0], w[N / 4 * 4 + 1] = x[1];
+    }
+    if constexpr (N % 2 == 1) w[N - 1] = *(const u32*)(p + 4 * (N - 1));
+}
+
+__device__ __forceinline__ float max_quarters(float x) {  // over the lanes of one row: lane, lane ^ 16, lane ^ 32, ^ 48
+    x = fmaxf(x, __shfl_xor(x, 16, 64));
+    return fmaxf(x, __shfl_xor(x, 32, 64));
+}
+__device__ __forceinline__ float sum_quarters(float x) {
+    x += __shfl_xor(x, 16, 64);
+    return x + __shfl_xor(x, 32, 64);
+}
+
+// N outputs at element i of out, of which the first `have` exist
+template <int N> __device__ __forceinline__ void put(const TreeArgs& a, i64 i, int have, const float* x) {
+    u16 e[N];
+#pragma unroll
+    for (int j = 0; j < N; ++j)
+        e[j] = a.qtype == NG_BF16 ? __builtin_bit_cast(u16, (b16)x[j]) : __builtin_bit_cast(u16, (f16)x[j]);
+    u16* o = (u16*)a.out + i;
+#pragma unroll
+    for (int j = 0; j < N; j += 4) {
+        if (a.dim % 4 == 0) {
+            if (j < have) *(uint2*)(o + j) = make_uint2(e[j] | (u32)e[j + 1] << 16, e[j + 2] | (u32)e[j + 3] << 16);
+        } else
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+                if (j + k < have) o[j + k] = e[j + k];
+    }
+}
+
+// CODES: the cache's; DP: its padded row; R: rows a block / 16.
+template <int CODES, int DP, int R> struct Tree {
+    typedef typename op_t<CODES>::type T;
+    typedef T V8 __attribute__((ext_vector_type(8)));
+    static constexpr bool Q8 = CODES == KV_INT8 || CODES == KV_FP8;
+    static constexpr int ES = Q8 ? 1 : 2;       // bytes a code
+    static constexpr int KW = DP * ES / 16;     // words of a lane's quarter of a key row
+    static constexpr int VW = DP * ES / 64;     // words of a lane's sixteenth of a value row
+    static constexpr int KS = DP / 32;          // product steps over the dimension
+    static constexpr int NJ = DP / 16;          // 16-dimension tiles of the output
+    static constexpr float BIAS = Q8 ? 8.f : 0.f;   // P's exponent is raised by this: f16 holds 2^-32 of the largest
+    static constexpr float SLACK = 4.f;             // M follows the maximum only when that passes it by 2^SLACK
+    static constexpr float K_UP = CODES == KV_INT8 ? 16777216.f : 1.f, V_UP = CODES == KV_INT8 ? 512.f : 1.f;
+
+    struct Pages {
+        int k, v, s;  // of the keys this lane loads: key group c >> 2, value group g, scale group
+    };
+    struct Frag {
+        u32 k[2][KW], v[8][VW];
+        float s;   // lanes 0 .. 31: the key scale of key lane; 32 .. 63: the value scale of key lane - 32
+        bool ok;   // this lane's keys lie in a page of the cache
+        i64 row;   // its first value row
+    };
+
+    struct State {
+        V8 q[R][KS];
+        f4 o[R][NJ];
+        float m[R], l[R], off[R];
+        float c;  // scale * log2(e) / the queries' power of two
+    };
+
+    static constexpr int QLD = DP + 8;                    // a query row in LDS (16 rows' reads meet no bank twice)
+    static constexpr int NQ = (16 * R * DP / 8 + 255) / 256;  // groups of 8 query elements a thread brings
+
+    // The block's query rows, through LDS: each read once, for 8-bit caches scaled by the power of two that puts their
+    // largest element at 2^14 .. 2^15. top: 4 floats.
+    static __device__ __forceinline__ void load_q(const TreeArgs& a, int b, int head, int row0, T* lds, float* topl, State& s) {
+        const int c = lane_id() & 15, g = lane_id() >> 4, rows = a.T * a.G;
+        union Eight {
+            uint4 w;
+            u16 e[8];
+        } x[NQ];
+        float top = 0.f;
+#pragma unroll
+        for (int k = 0; k < NQ; ++k) {
+            const int i = threadIdx.x + 256 * k, row = row0 + i / (DP / 8), d0 = i % (DP / 8) * 8;
+            const int t = row / a.G, h = row - t * a.G;
+            const u16* p = (const u16*)a.q + b * a.qb + t * a.qt + (i64)(head * a.G + h) * a.qh + d0;
+            x[k].w = make_uint4(0, 0, 0, 0);
+            if (i < 16 * R * DP / 8 && row < rows) {
+                if (a.vec && d0 + 8 <= a.dim) x[k].w = *(const uint4*)p;
+                else
+                    for (int j = 0; j < 8; ++j)
+                        if (d0 + j < a.dim) x[k].e[j] = p[j];
+            }
+            if constexpr (Q8)
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    const float f = __builtin_fabsf(value(a, x[k].e[j]));
+                    top = finite_f(f) ? fmaxf(top, f) : top;
+                }
+        }
+        float up = 1.f;
+        s.c = a.scale * LOG2E;
+        if constexpr (Q8) {
+#pragma unroll
+            for (int o = 32; o; o >>= 1) top = fmaxf(top, __shfl_xor(top, o, 64));
+            if (lane_id() == 0) topl[threadIdx.x >> 6] = top;
+        }
+        __syncthreads();  // what LDS held before has been read, too
+        if constexpr (Q8) {
+            top = fmaxf(fmaxf(topl[0], topl[1]), fmaxf(topl[2], topl[3]));
+            if (top > 0.f) {
+                int e = 15 - __builtin_amdgcn_frexp_expf(top);
+                e = e > 100 ? 100 : e;
+                up = __builtin_amdgcn_ldexpf(1.f, e);
+                s.c *= __builtin_amdgcn_ldexpf(1.f, -e);
+            }
+            s.c *= K_UP;
+        }
+#pragma unroll
+        for (int k = 0; k < NQ; ++k) {
+            const int i = threadIdx.x + 256 * k;
+            if (i < 16 * R * DP / 8) {
+                Pack<T, 8> y;
+                if constexpr (Q8)
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) y.v[j] = (T)(value(a, x[k].e[j]) * up);
+                else y.r = x[k].w;
+                y.store(lds + i / (DP / 8) * QLD + i % (DP / 8) * 8);
+            }
+        }
+        __syncthreads();
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
+            float sum = 0.f;
+#pragma unroll
+            for (int st = 0; st < KS; ++st) {
+                s.q[r][st] = *(const V8*)(lds + (r * 16 + c) * QLD + g * (DP / 4) + st * 8);
+                if constexpr (CODES == KV_INT8)
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) sum += (float)s.q[r][st][j];
+            }
+            s.off[r] = CODES == KV_INT8 ? -128.f / K_UP * sum_quarters(sum) : 0.f;
+        }
+    }
+    static __device__ __forceinline__ float value(const TreeArgs& a, u16 e) {
+        return a.qtype == NG_BF16 ? __uint_as_float((u32)e << 16) : (float)__builtin_bit_cast(f16, e);
+    }
+
+    // the pages of this wave's 32 keys at `base` (any entry of the sequence where a key is past the table)
+    static __device__ __forceinline__ Pages pages_of(const TreeArgs& a, const int* tab, int base) {
+        const int c = lane_id() & 15, g = lane_id() >> 4, w = a.width - 1;
+        Pages p;
+        int e = (base + (c >> 2) * 8) >> a.shift;
+        p.k = tab[e < w ? e : w];
+        e = (base + g * 8) >> a.shift;
+        p.v = tab[e < w ? e : w];
+        e = (base + (lane_id() & 31)) >> a.shift;
+        p.s = Q8 ? tab[e < w ? e : w] : 0;
+        return p;
+    }
+
+    // a tile's keys and factors, and its values: each is loaded as soon as the one before it has left the registers, so that
+    // the next keys come while a tile's softmax and values are worked on, the next values while its scores are
+    static __device__ __forceinline__ void fetch_keys(const TreeArgs& a, int head, int base, const Pages& p, Frag& f) {
+        const int c = lane_id() & 15, g = lane_id() >> 4, in = (1 << a.shift) - 1;
+        const i64 pk = (u32)p.k < (u64)a.pages ? p.k : 0, ps = (u32)p.s < (u64)a.pages ? p.s : 0;
+        const i64 rk = ((pk * a.H + head) << a.shift) + ((base + (c >> 2) * 8) & in) + (c & 3);
+        const char* k = (const char*)a.k + rk * (DP * ES) + g * (DP * ES / 4);
+        load_words<KW>(k, f.k[0]);
+        load_words<KW>(k + 4 * DP * ES, f.k[1]);
+        if constexpr (Q8) {
+            const i64 rs = ((ps * a.H + head) << a.shift) + ((base + (lane_id() & 31)) & in);
+            f.s = (lane_id() < 32 ? a.ks : a.vs)[rs];
+        }
+    }
+    static __device__ __forceinline__ void fetch_values(const TreeArgs& a, int head, int base, const Pages& p, Frag& f) {
+        const int c = lane_id() & 15, g = lane_id() >> 4, in = (1 << a.shift) - 1;
+        f.ok = (u32)p.v < (u64)a.pages;
+        const i64 rv = ((((i64)(f.ok ? p.v : 0)) * a.H + head) << a.shift) + ((base + g * 8) & in);
+        if constexpr (!Q8) f.row = rv;
+        const char* v = (const char*)a.v + rv * (DP * ES) + c * (DP * ES / 16);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) load_words<VW>(v + i * DP * ES, f.v[i]);
+    }
+
+    // the tree tokens that a row sees
+    static __device__ __forceinline__ u64 bits_of(const TreeArgs& a, int b, const Seq& q, int row) {
+        const int t = row / a.G;
+        if (t >= q.w) return 0;
+        return a.mask ? a.mask[(i64)b * a.T + t] : (2ull << t) - 1;
+    }
+
+    // Values of a 16-bit cache that are not finite, in keys that only some rows see: they are 0 in the product (a masked
+    // key's P of 0 would make NaN of them) and are added here to the rows that do see them.
+    static __device__ __forceinline__ u32 take_out(Frag& f) {
+        constexpr u32 E = CODES == KV_BF16 ? 0x7F80u : 0x7C00u;
+        u32 bad = 0;
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+#pragma unroll
+            for (int w = 0; w < VW; ++w) {
+                const bool lo = (f.v[i][w] & E) == E, hi = (f.v[i][w] >> 16 & E) == E;
+                bad |= (lo || hi ? 1u : 0u) << i;
+                f.v[i][w] &= (lo ? 0u : 0xFFFFu) | (hi ? 0u : 0xFFFF0000u);
+            }
+        return bad;
+    }
+    static __device__ __forceinline__ void put_back(const TreeArgs& a, int b, const Seq& q, int base, int row0, const Frag& f,
+                                                    u32 bad, const V8 (&p)[R], State& s) {
+        const int c = lane_id() & 15, g = lane_id() >> 4;
+        for (int from = 0; from < 4; ++from) {
+            const i64 first = (i64)__shfl((long long)f.row, from * 16, 64);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                if (!__any(g == from && (bad >> i & 1))) continue;
+                const T* v = (const T*)a.v + (first + i) * DP;
+                const int j0 = base + from * 8 + i - q.len;
+#pragma unroll
+                for (int r = 0; r < R; ++r) {
+                    const float w = __shfl((float)p[r][i], from * 16 + c, 64);
+                    const bool sees = j0 < 0 || (bits_of(a, b, q, row0 + r * 16 + c) >> j0 & 1);
+#pragma unroll
+                    for (int j = 0; j < NJ; ++j)
+#pragma unroll
+                        for (int k = 0; k < 4; ++k) {
+                            const float x = (float)v[(4 * g + k) * NJ + j];
+                            if (sees && !finite_f(x)) s.o[r][j][k] += w * x;
+                        }
+                }
+            }
+        }
+    }
+
+    // This wave's keys from base up to stop, a tile of 32 in every TILE.
+    static __device__ __forceinline__ void keys(const TreeArgs& a, int b, int head, const Seq& q, int base, int stop, int row0,
+                                                State& s, float (*fac)[32]) {
+        if (base >= stop) return;
+        const int c = lane_id() & 15, g = lane_id() >> 4;
+        const int* tab = a.table + (i64)b * a.table_stride;
+        Frag f;
+        Pages next = pages_of(a, tab, base);
+        fetch_keys(a, head, base, next, f);
+        fetch_values(a, head, base, next, f);
+        next = pages_of(a, tab, base + TILE);
+        for (;;) {
+            const bool whole = base + 32 <= q.len && __all(f.ok);  // cached tokens in pages of the cache: all rows see them
+            const bool more = base + TILE < stop;
+            if constexpr (Q8) {  // the keys' factors, one lane each, handed to the lanes that hold their scores through LDS
+                const int key = lane_id() & 31;
+                if (lane_id() < 32) fac[0][key] = f.s * s.c;
+                else {
+                    // a row of zeros: any scale; the inverse of a subnormal one would overflow
+                    float x = f.s == 0.f ? 1.f : f.s < 0x1p-126f ? 0x1p-126f : f.s;
+                    x = base + key < q.n ? x : 1.f;
+                    fac[1][key] = __builtin_amdgcn_logf(x);
+                    fac[2][key] = __builtin_amdgcn_rcpf(x);
+                }
+                __builtin_amdgcn_wave_barrier();
+            }
+            f4 sc[R][2];
+#pragma unroll
+            for (int r = 0; r < R; ++r) sc[r][0] = sc[r][1] = f4{s.off[r], s.off[r], s.off[r], s.off[r]};
+#pragma unroll
+            for (int t = 0; t < 2; ++t)
+#pragma unroll
+                for (int st = 0; st < KS; ++st) {
+                    if constexpr (CODES == KV_INT8) f.k[t][2 * st] ^= 0x80808080u, f.k[t][2 * st + 1] ^= 0x80808080u;
+                    const V8 k = row_operand<CODES, V8>(f.k[t] + st * (Q8 ? 2 : 4));
+#pragma unroll
+                    for (int r = 0; r < R; ++r) sc[r][t] = mma(k, s.q[r][st], sc[r][t]);
+                }
+            if (more) fetch_keys(a, head, base + TILE, next, f);
+            float rv[8];
+            if constexpr (Q8)
+#pragma unroll
+                for (int i = 0; i < 8; ++i) rv[i] = fac[2][g * 8 + i];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const float kf = Q8 ? fac[0][g * 8 + i] : s.c, lv = Q8 ? fac[1][g * 8 + i] : 0.f;
+#pragma unroll
+                for (int r = 0; r < R; ++r) {
+                    const float x = sc[r][i >> 2][i & 3];
+                    sc[r][i >> 2][i & 3] = Q8 ? fmaf(x, kf, lv) : x * kf;
+                }
+            }
+            __builtin_amdgcn_wave_barrier();
+            u32 bad = 0;
+            if (!whole) {  // keys that a row does not see: nothing of those past the end or without a page enters a product
+                const int j0 = base + g * 8 - q.len;  // this lane's first key's place in the tree
+                const u32 in = !f.ok || q.n <= base + g * 8 ? 0u : q.n - base - g * 8 >= 8 ? 0xFFu : (1u << (q.n - base - g * 8)) - 1;
+                const u32 cached = j0 >= 0 ? 0u : j0 <= -8 ? 0xFFu : (1u << -j0) - 1;
+#pragma unroll
+                for (int i = 0; i < 8; ++i)
+#pragma unroll
+                    for (int w = 0; w < VW; ++w) f.v[i][w] = in >> i & 1 ? f.v[i][w] : 0u;
+                if constexpr (!Q8) bad = take_out(f);
+#pragma unroll
+                for (int r = 0; r < R; ++r) {
+                    const u64 bits = bits_of(a, b, q, row0 + r * 16 + c);
+                    const u32 tree = j0 >= 64 || j0 <= -8 ? 0u : j0 >= 0 ? (u32)(bits >> j0) : (u32)(bits << -j0);
+                    const u32 sees = in & (cached | tree);
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) {
+                        sc[r][i >> 2][i & 3] = sees >> i & 1 ? sc[r][i >> 2][i & 3] : -__builtin_inff();
+                        // a masked key's scale may be NaN: it does not enter the sum (a row that sees it has P of NaN)
+                        if constexpr (Q8) rv[i] = (sees >> i & 1) | finite_f(rv[i]) ? rv[i] : 1.f;
+                    }
+                }
+            }
+            bool grow = false;
+#pragma unroll
+            for (int r = 0; r < R; ++r) {
+                float top = sc[r][0][0];
+#pragma unroll
+                for (int i = 1; i < 8; ++i) top = fmaxf(top, sc[r][i >> 2][i & 3]);
+                grow |= top > s.m[r] + SLACK;
+            }
+            if (__any(grow)) {
+#pragma unroll
+                for (int r = 0; r < R; ++r) {
+                    float top = sc[r][0][0];
+#pragma unroll
+                    for (int i = 1; i < 8; ++i) top = fmaxf(top, sc[r][i >> 2][i & 3]);
+                    const float m = fmaxf(s.m[r], max_quarters(top));
+                    const float down = s.m[r] == -__builtin_inff() ? 0.f : __builtin_amdgcn_exp2f(s.m[r] - m);
+                    s.m[r] = m;
+                    s.l[r] *= down;
+#pragma unroll
+                    for (int j = 0; j < NJ; ++j) s.o[r][j] *= down;
+                }
+            }
+            V8 p[R];
+#pragma unroll
+            for (int r = 0; r < R; ++r) {
+                const float m0 = s.m[r] == -__builtin_inff() ? 0.f : s.m[r] - BIAS;
+                float add = 0.f;
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    const float e = __builtin_amdgcn_exp2f(sc[r][i >> 2][i & 3] - m0);
+                    if constexpr (Q8) add = fmaf(e, rv[i], add);
+                    else add += e;
+                    p[r][i] = (T)e;
+                }
+                s.l[r] += add;
+            }
+            if constexpr (CODES == KV_INT8)
+#pragma unroll
+                for (int i = 0; i < 8; ++i)
+#pragma unroll
+                    for (int w = 0; w < VW; ++w) f.v[i][w] ^= 0x80808080u;
+#pragma unroll
+            for (int j = 0; j < NJ; j += 2) {
+                V8 v0, v1;
+                col_operands<CODES, V8, VW>(f.v, j / 2, v0, v1);
+#pragma unroll
+                for (int r = 0; r < R; ++r) {
+                    s.o[r][j] = mma(v0, p[r], s.o[r][j]);
+                    s.o[r][j + 1] = mma(v1, p[r], s.o[r][j + 1]);
+                }
+            }
+            if constexpr (!Q8)
+                if (__any(bad != 0)) put_back(a, b, q, base, row0, f, bad, p, s);
+            base += TILE;
+            if (!more) break;
+            fetch_values(a, head, base, next, f);
+            next = pages_of(a, tab, base + TILE);
+        }
+    }
+};
+
+template <int CODES, int DP, int R> constexpr int tree_waves() { return R <= 2 && DP <= 128 ? 2 : 1; }
+
+template <int CODES, int DP, int R>
+__global__ __launch_bounds__(256, (tree_waves<CODES, DP, R>())) void tree_k(const TreeArgs a, int blocks) {
+    typedef Tree<CODES, DP, R> W;
+    constexpr int LD = DP + 4;
+    typedef float Lo[16][LD];
+    __shared__ __align__(16) char lds[sizeof(Lo) * 4 > 16 * R * W::QLD * 2 ? sizeof(Lo) * 4 : 16 * R * W::QLD * 2];
+    Lo* lo = (Lo*)lds;  // the waves' sums at a unit's end; at its beginning the queries
+    __shared__ float lm[4][16], ll[4][16], topl[4];
+    __shared__ __align__(16) float fac[4][3][32];
+    const Line line(a, blocks);
+    // neighbouring shares on one XCD (blocks go round the 8 XCDs): units that share keys meet in its L2
+    const int a8 = (line.shares + 7) / 8, me = (int)(blockIdx.x % 8) * a8 + (int)blockIdx.x / 8;
+    if ((int)blockIdx.x / 8 >= a8 || me >= line.shares) return;
+    const int wave = threadIdx.x >> 6, c = lane_id() & 15, g = lane_id() >> 4, units = a.H * a.groups;
+    int x = me * line.per;
+    const int end = line.total - x < line.per ? line.total : x + line.per;
+    int before;
+    Seq q;
+    int b = line.at(a, x, before, q);
+    while (x < end) {
+        while (x - before >= q.tiles * units) {
+            before += q.tiles * units;
+            q = seq_of(a, ++b);
+        }
+        const int unit = (x - before) / q.tiles, t0 = x - before - unit * q.tiles;
+        const int t1 = end - x < q.tiles - t0 ? t0 + (end - x) : q.tiles;
+        const int head = unit / a.groups, row0 = (unit - head * a.groups) * 16 * R;
+        typename W::State s;
+        W::load_q(a, b, head, row0, (typename W::T*)lds, topl, s);
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
+            s.m[r] = -__builtin_inff(), s.l[r] = 0.f;
+#pragma unroll
+            for (int j = 0; j < W::NJ; ++j) s.o[r][j] = f4{0.f, 0.f, 0.f, 0.f};
+        }
+        W::keys(a, b, head, q, t0 * TILE + wave * 32, t1 * TILE < q.n ? t1 * TILE : q.n, row0, s, fac[wave]);
+        const bool all = t0 == 0 && t1 == q.tiles;
+        const i64 slot = 2 * me + (t0 == 0 ? 1 : 0);
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
+            const float l = sum_quarters(s.l[r]);
+            __syncthreads();
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+#pragma unroll
+                for (int j = 0; j < W::NJ; ++j) lo[wave][c][(4 * g + i) * W::NJ + j] = s.o[r][j][i] * W::V_UP;
+            if (g == 0) lm[wave][c] = s.m[r], ll[wave][c] = l;
+            __syncthreads();
+            const int row = threadIdx.x >> 4, d0 = (threadIdx.x & 15) * W::NJ;
+            float m = lm[0][row];
+#pragma unroll
+            for (int w = 1; w < 4; ++w) m = fmaxf(m, lm[w][row]);
+            float sum = 0.f, o[W::NJ];
+#pragma unroll
+            for (int j = 0; j < W::NJ; ++j) o[j] = 0.f;
+#pragma unroll
+            for (int w = 0; w < 4; ++w) {
+                // a wave without a key that counts: sum and o are 0, or NaN where a NaN was seen
+                const float k = lm[w][row] == -__builtin_inff() ? 0.f : __builtin_amdgcn_exp2f(lm[w][row] - m);
+                sum = ll[w][row] == 0.f ? sum : fmaf(ll[w][row], k, sum);
+#pragma unroll
+                for (int j = 0; j < W::NJ; ++j) o[j] = fmaf(lo[w][row][d0 + j], k, o[j]);
+            }
+            const int at = row0 + r * 16 + row, t = at / a.G, h = at - t * a.G;
+            if (all) {
+                if (t < a.T) {
+                    const i64 i = ((i64)b * a.T + t) * a.H * a.G + head * a.G + h;
+                    const bool none = sum == 0.f || t >= q.w;
+                    const float inv = none ? 0.f : 1.f / sum;
+#pragma unroll
+                    for (int j = 0; j < W::NJ; ++j) o[j] = none ? 0.f : o[j] * inv;
+                    put<W::NJ>(a, i * a.dim + d0, a.dim - d0, o);
+                    if (a.lse && (threadIdx.x & 15) == 0)
+                        a.lse[i] = none ? -__builtin_inff() : LN2 * (m - W::BIAS + __builtin_amdgcn_logf(sum));
+                }
+            } else {
+                const i64 prow = slot * (16 * R) + r * 16 + row;
+#pragma unroll
+                for (int j = 0; j < W::NJ; ++j) a.po[prow * DP + d0 + j] = o[j];
+                if ((threadIdx.x & 15) == 0) a.pm[prow] = m, a.pl[prow] = sum;
+            }
+        }
+        x += t1 - t0;
+    }
+}
+
+// A block per (unit, 16 rows): the shares that hold part of the unit joined.
+template <int DP> __global__ __launch_bounds__(256) void tree_join_k(const TreeArgs a, int blocks, int rpb, float bias) {
+    constexpr int NJ = DP / 16;
+    const int sub = rpb / 16, u = blockIdx.x / sub, r16 = (int)(blockIdx.x - u * sub) * 16;
+    const int per = a.H * a.groups, b = u / per, unit = u - b * per;
+    const Line line(a, blocks);
+    Seq q;
+    const int x0 = line.before(a, b, q) + unit * q.tiles, x1 = x0 + q.tiles;
+    const int i0 = x0 / line.per, i1 = (x1 - 1) / line.per;
+    if (i0 == i1) return;
+    const int head = unit / a.groups, row0 = (unit - head * a.groups) * rpb;
+    const int row = threadIdx.x >> 4, d0 = (threadIdx.x & 15) * NJ;
+    const int at = row0 + r16 + row, t = at / a.G, h = at - t * a.G;
+    if (t >= a.T) return;
+    float m = -__builtin_inff(), sum = 0.f, o[NJ];
+#pragma unroll
+    for (int j = 0; j < NJ; ++j) o[j] = 0.f;
+    for (int i = i0; i <= i1; ++i) {
+        const i64 prow = (i64)(2 * i + (i == i0 ? 1 : 0)) * rpb + r16 + row;
+        const float pm = a.pm[prow], pl = a.pl[prow];
+        const float n = fmaxf(m, pm);
+        const float ko = m == -__builtin_inff() ? 0.f : __builtin_amdgcn_exp2f(m - n);
+        const float kp = pm == -__builtin_inff() ? 0.f : __builtin_amdgcn_exp2f(pm - n);
+        sum = (sum == 0.f ? 0.f : sum * ko) + (pl == 0.f ? 0.f : pl * kp);
+#pragma unroll
+        for (int j = 0; j < NJ; ++j) o[j] = o[j] * ko + a.po[prow * DP + d0 + j] * kp;
+        m = n;
+    }
+    const i64 i = ((i64)b * a.T + t) * a.H * a.G + head * a.G + h;
+    const bool none = sum == 0.f || t >= q.w;
+    const float inv = none ? 0.f : 1.f / sum;
+#pragma unroll
+    for (int j = 0; j < NJ; ++j) o[j] = none ? 0.f : o[j] * inv;
+    put<NJ>(a, i * a.dim + d0, a.dim - d0, o);
+    if (a.lse && (threadIdx.x & 15) == 0) a.lse[i] = none ? -__builtin_inff() : LN2 * (m - bias + __builtin_amdgcn_logf(sum));
+}
+
+// ------------------------------------------------------------------------------------------------------- the launches
+
+template <int CODES, int DP, int R> static int tree_run(const TreeArgs& a, const TreePlan& p, hipStream_t st) {
+    tree_k<CODES, DP, R><<<p.blocks, 256, 0, st>>>(a, p.blocks);
+    int rc = (int)hipGetLastError();
+    if (rc || !p.join) return rc;
+    tree_join_k<DP><<<a.B * a.H * a.groups * R, 256, 0, st>>>(a, p.blocks, 16 * R, Tree<CODES, DP, R>::BIAS);
+    return (int)hipGetLastError();
+}
+
+template <int CODES, int DP> static int tree_rows(const TreeArgs& a, const TreePlan& p, hipStream_t st) {
+    if (p.rpb == 16) return tree_run<CODES, DP, 1>(a, p, st);
+    if (p.rpb == 32) return tree_run<CODES, DP, 2>(a, p, st);
+    if constexpr (DP <= 128) return tree_run<CODES, DP, 4>(a, p, st);
+    return -1;
+}
+
+template <int CODES> int tree_codes(const TreeArgs& a, const TreePlan& p, hipStream_t st) {
+    switch (p.dp) {
+        case 64: return tree_rows<CODES, 64>(a, p, st);
+        case 128: return tree_rows<CODES, 128>(a, p, st);
+        case 192: return tree_rows<CODES, 192>(a, p, st);
+        default: return tree_rows<CODES, 256>(a, p, st);
+    }
+}

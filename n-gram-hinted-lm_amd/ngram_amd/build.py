@@ -35,7 +35,7 @@ LOCK_FILE = OUT_DIR / ".build.lock"
 LIBS = {
     LIB_NAME: ["prim.hip", "abi/owner.hip", "abi/gvs.hip", "gen.hip", "engine.hip", "part.hip", "table.hip",
                "online.hip", "online_counts.hip", "rows.hip", "hintrows.hip", "pairs32.hip", "embed.hip", "kvcache.hip",
-               "tree.hip"],
+               "tree.hip", "tree_int8.hip", "tree_fp8.hip", "tree_bf16.hip", "tree_f16.hip"],
     RECORD_LIB_NAME: ["prim.hip", "abi/owner.hip", "abi/record.hip"],
 }
 ARCH = os.environ.get("NGRAM_AMD_ARCH", "gfx950")
