@@ -56,6 +56,12 @@ __device__ __forceinline__ Seq seq_of(const TreeArgs& a, int b) {
     return s;
 }
 
+__device__ __forceinline__ Seq uniform(Seq s) {
+    s.len = __builtin_amdgcn_readfirstlane(s.len), s.w = __builtin_amdgcn_readfirstlane(s.w);
+    s.n = __builtin_amdgcn_readfirstlane(s.n), s.tiles = __builtin_amdgcn_readfirstlane(s.tiles);
+    return s;
+}
+
 __device__ __forceinline__ int scan_wave(int x) {  // inclusive sum over the lanes
 #pragma unroll
     for (int o = 1; o < 64; o <<= 1) {
@@ -77,10 +83,10 @@ struct Line {
         const int b = lane_id() < a.B ? lane_id() : a.B - 1;
         mine = seq_of(a, b);
         inc = scan_wave(lane_id() < a.B ? mine.tiles * units : 0);
-        total = __shfl(inc, 63, 64);
+        total = lane(inc, 63);
         for (int b0 = 64; b0 < a.B; b0 += 64) {
             int t = b0 + lane_id() < a.B ? seq_of(a, b0 + lane_id()).tiles * units : 0;
-            total += __shfl(scan_wave(t), 63, 64);
+            total += lane(scan_wave(t), 63);
         }
         per = (total + blocks - 1) / blocks;
         shares = (total + per - 1) / per;
@@ -96,7 +102,7 @@ struct Line {
             before = lane(inc, l) - q.tiles * units;
             return l;
         }
-        int run = __shfl(inc, 63, 64);
+        int run = lane(inc, 63);
         for (int b0 = 64;; b0 += 64) {
             Seq s;
             s.len = s.w = s.n = s.tiles = 0;
@@ -109,7 +115,7 @@ struct Line {
                 before = run + lane(i, l) - q.tiles * units;
                 return b0 + l;
             }
-            run += __shfl(i, 63, 64);
+            run += lane(i, 63);
         }
     }
 
@@ -130,7 +136,7 @@ struct Line {
                 q.len = lane(s.len, l), q.w = lane(s.w, l), q.n = lane(s.n, l), q.tiles = lane(s.tiles, l);
                 return run + lane(i, l) - q.tiles * units;
             }
-            run += __shfl(i, 63, 64);
+            run += lane(i, 63);
         }
     }
     static __device__ __forceinline__ int lane(int x, int l) { return __builtin_amdgcn_readlane(x, l); }
@@ -259,15 +265,20 @@ template <int CODES, int DP, int R> struct Tree {
     struct Pages {
         int k, v, s;  // of the keys this lane loads: key group c >> 2, value group g, scale group
     };
-    struct Frag {
-        u32 k[2][KW], v[8][VW];
+    struct Keys {
+        u32 k[2][KW];
         float s;   // lanes 0 .. 31: the key scale of key lane; 32 .. 63: the value scale of key lane - 32
+    };
+    struct Values {
+        u32 v[8][VW];
         bool ok;   // this lane's keys lie in a page of the cache
         i64 row;   // its first value row
     };
+    static constexpr bool QLDS = R >= 2;  // the queries are read from LDS for every tile: registers go to loads in flight
 
     struct State {
-        V8 q[R][KS];
+        V8 q[QLDS ? 1 : R][KS];
+        const T* ql;  // the queries in LDS, at this lane's row and quarter
         f4 o[R][NJ];
         float m[R], l[R], off[R];
         float c;  // scale * log2(e) / the queries' power of two
@@ -311,7 +322,7 @@ template <int CODES, int DP, int R> struct Tree {
             for (int o = 32; o; o >>= 1) top = fmaxf(top, __shfl_xor(top, o, 64));
             if (lane_id() == 0) topl[threadIdx.x >> 6] = top;
         }
-        __syncthreads();  // what LDS held before has been read, too
+        lds_barrier();  // what LDS held before has been read, too
         if constexpr (Q8) {
             top = fmaxf(fmaxf(topl[0], topl[1]), fmaxf(topl[2], topl[3]));
             if (top > 0.f) {
@@ -334,16 +345,18 @@ template <int CODES, int DP, int R> struct Tree {
                 y.store(lds + i / (DP / 8) * QLD + i % (DP / 8) * 8);
             }
         }
-        __syncthreads();
+        lds_barrier();
+        s.ql = lds + c * QLD + g * (DP / 4);
 #pragma unroll
         for (int r = 0; r < R; ++r) {
             float sum = 0.f;
 #pragma unroll
             for (int st = 0; st < KS; ++st) {
-                s.q[r][st] = *(const V8*)(lds + (r * 16 + c) * QLD + g * (DP / 4) + st * 8);
+                const V8 x = *(const V8*)(s.ql + r * 16 * QLD + st * 8);
+                if constexpr (!QLDS) s.q[r][st] = x;
                 if constexpr (CODES == KV_INT8)
 #pragma unroll
-                    for (int j = 0; j < 8; ++j) sum += (float)s.q[r][st][j];
+                    for (int j = 0; j < 8; ++j) sum += (float)x[j];
             }
             s.off[r] = CODES == KV_INT8 ? -128.f / K_UP * sum_quarters(sum) : 0.f;
         }
@@ -365,9 +378,9 @@ template <int CODES, int DP, int R> struct Tree {
         return p;
     }
 
-    // a tile's keys and factors, and its values: each is loaded as soon as the one before it has left the registers, so that
-    // the next keys come while a tile's softmax and values are worked on, the next values while its scores are
-    static __device__ __forceinline__ void fetch_keys(const TreeArgs& a, int head, int base, const Pages& p, Frag& f) {
+    // A tile's keys and factors, and its values. Both are asked for in the middle of the tile before: the keys into the
+    // registers that its keys have just left, the values into the other of two sets.
+    static __device__ __forceinline__ void fetch_keys(const TreeArgs& a, int head, int base, const Pages& p, Keys& f) {
         const int c = lane_id() & 15, g = lane_id() >> 4, in = (1 << a.shift) - 1;
         const i64 pk = (u32)p.k < (u64)a.pages ? p.k : 0, ps = (u32)p.s < (u64)a.pages ? p.s : 0;
         const i64 rk = ((pk * a.H + head) << a.shift) + ((base + (c >> 2) * 8) & in) + (c & 3);
@@ -379,7 +392,7 @@ template <int CODES, int DP, int R> struct Tree {
             f.s = (lane_id() < 32 ? a.ks : a.vs)[rs];
         }
     }
-    static __device__ __forceinline__ void fetch_values(const TreeArgs& a, int head, int base, const Pages& p, Frag& f) {
+    static __device__ __forceinline__ void fetch_values(const TreeArgs& a, int head, int base, const Pages& p, Values& f) {
         const int c = lane_id() & 15, g = lane_id() >> 4, in = (1 << a.shift) - 1;
         f.ok = (u32)p.v < (u64)a.pages;
         const i64 rv = ((((i64)(f.ok ? p.v : 0)) * a.H + head) << a.shift) + ((base + g * 8) & in);
@@ -398,7 +411,7 @@ template <int CODES, int DP, int R> struct Tree {
 
     // Values of a 16-bit cache that are not finite, in keys that only some rows see: they are 0 in the product (a masked
     // key's P of 0 would make NaN of them) and are added here to the rows that do see them.
-    static __device__ __forceinline__ u32 take_out(Frag& f) {
+    static __device__ __forceinline__ u32 take_out(Values& f) {
         constexpr u32 E = CODES == KV_BF16 ? 0x7F80u : 0x7C00u;
         u32 bad = 0;
 #pragma unroll
@@ -411,7 +424,7 @@ template <int CODES, int DP, int R> struct Tree {
             }
         return bad;
     }
-    static __device__ __forceinline__ void put_back(const TreeArgs& a, int b, const Seq& q, int base, int row0, const Frag& f,
+    static __device__ __forceinline__ void put_back(const TreeArgs& a, int b, const Seq& q, int base, int row0, const Values& f,
                                                     u32 bad, const V8 (&p)[R], State& s) {
         const int c = lane_id() & 15, g = lane_id() >> 4;
         for (int from = 0; from < 4; ++from) {
@@ -437,140 +450,199 @@ template <int CODES, int DP, int R> struct Tree {
         }
     }
 
-    // This wave's keys from base up to stop, a tile of 32 in every TILE.
-    static __device__ __forceinline__ void keys(const TreeArgs& a, int b, int head, const Seq& q, int base, int stop, int row0,
-                                                State& s, float (*fac)[32]) {
-        if (base >= stop) return;
-        const int c = lane_id() & 15, g = lane_id() >> 4;
-        const int* tab = a.table + (i64)b * a.table_stride;
-        Frag f;
-        Pages next = pages_of(a, tab, base);
-        fetch_keys(a, head, base, next, f);
-        fetch_values(a, head, base, next, f);
-        next = pages_of(a, tab, base + TILE);
-        for (;;) {
-            const bool whole = base + 32 <= q.len && __all(f.ok);  // cached tokens in pages of the cache: all rows see them
-            const bool more = base + TILE < stop;
-            if constexpr (Q8) {  // the keys' factors, one lane each, handed to the lanes that hold their scores through LDS
-                const int key = lane_id() & 31;
-                if (lane_id() < 32) fac[0][key] = f.s * s.c;
-                else {
-                    // a row of zeros: any scale; the inverse of a subnormal one would overflow
-                    float x = f.s == 0.f ? 1.f : f.s < 0x1p-126f ? 0x1p-126f : f.s;
-                    x = base + key < q.n ? x : 1.f;
-                    fac[1][key] = __builtin_amdgcn_logf(x);
-                    fac[2][key] = __builtin_amdgcn_rcpf(x);
-                }
-                __builtin_amdgcn_wave_barrier();
+    struct Run {
+        Keys k;
+        Values v;
+        Pages next;  // the pages of the tile whose loads come next
+    };
+
+    // The factors of a tile's keys, computed by one lane each and handed through LDS to the lanes that hold their scores:
+    // the score's factor, the logarithm and the inverse of the value scale.
+    static __device__ __forceinline__ void factors(float scale, bool in, const State& s, float (*fac)[32]) {
+        const int key = lane_id() & 31;
+        if (lane_id() < 32) fac[0][key] = scale * s.c;
+        else {
+            // a row of zeros: any scale; the inverse of a subnormal one would overflow
+            float x = scale == 0.f ? 1.f : scale < 0x1p-126f ? 0x1p-126f : scale;
+            x = in ? x : 1.f;
+            fac[1][key] = __builtin_amdgcn_logf(x);
+            fac[2][key] = __builtin_amdgcn_rcpf(x);
+        }
+        __builtin_amdgcn_wave_barrier();
+    }
+
+    static __device__ __forceinline__ void scores(Keys& k, const State& s, float (*fac)[32], f4 (&sc)[R][2]) {
+        const int g = lane_id() >> 4;
+#pragma unroll
+        for (int r = 0; r < R; ++r) sc[r][0] = sc[r][1] = f4{s.off[r], s.off[r], s.off[r], s.off[r]};
+#pragma unroll
+        for (int st = 0; st < KS; ++st) {
+            V8 x[R];
+#pragma unroll
+            for (int r = 0; r < R; ++r) x[r] = QLDS ? *(const V8*)(s.ql + r * 16 * QLD + st * 8) : s.q[QLDS ? 0 : r][st];
+#pragma unroll
+            for (int t = 0; t < 2; ++t) {
+                if constexpr (CODES == KV_INT8) k.k[t][2 * st] ^= 0x80808080u, k.k[t][2 * st + 1] ^= 0x80808080u;
+                const V8 e = row_operand<CODES, V8>(k.k[t] + st * (Q8 ? 2 : 4));
+#pragma unroll
+                for (int r = 0; r < R; ++r) sc[r][t] = mma(e, x[r], sc[r][t]);
             }
-            f4 sc[R][2];
+        }
 #pragma unroll
-            for (int r = 0; r < R; ++r) sc[r][0] = sc[r][1] = f4{s.off[r], s.off[r], s.off[r], s.off[r]};
+        for (int i = 0; i < 8; ++i) {
+            const float kf = Q8 ? fac[0][g * 8 + i] : s.c, lv = Q8 ? fac[1][g * 8 + i] : 0.f;
 #pragma unroll
-            for (int t = 0; t < 2; ++t)
-#pragma unroll
-                for (int st = 0; st < KS; ++st) {
-                    if constexpr (CODES == KV_INT8) f.k[t][2 * st] ^= 0x80808080u, f.k[t][2 * st + 1] ^= 0x80808080u;
-                    const V8 k = row_operand<CODES, V8>(f.k[t] + st * (Q8 ? 2 : 4));
-#pragma unroll
-                    for (int r = 0; r < R; ++r) sc[r][t] = mma(k, s.q[r][st], sc[r][t]);
-                }
-            if (more) fetch_keys(a, head, base + TILE, next, f);
-            float rv[8];
-            if constexpr (Q8)
-#pragma unroll
-                for (int i = 0; i < 8; ++i) rv[i] = fac[2][g * 8 + i];
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                const float kf = Q8 ? fac[0][g * 8 + i] : s.c, lv = Q8 ? fac[1][g * 8 + i] : 0.f;
-#pragma unroll
-                for (int r = 0; r < R; ++r) {
-                    const float x = sc[r][i >> 2][i & 3];
-                    sc[r][i >> 2][i & 3] = Q8 ? fmaf(x, kf, lv) : x * kf;
-                }
+            for (int r = 0; r < R; ++r) {
+                const float x = sc[r][i >> 2][i & 3];
+                sc[r][i >> 2][i & 3] = Q8 ? fmaf(x, kf, lv) : x * kf;
             }
-            __builtin_amdgcn_wave_barrier();
-            u32 bad = 0;
-            if (!whole) {  // keys that a row does not see: nothing of those past the end or without a page enters a product
-                const int j0 = base + g * 8 - q.len;  // this lane's first key's place in the tree
-                const u32 in = !f.ok || q.n <= base + g * 8 ? 0u : q.n - base - g * 8 >= 8 ? 0xFFu : (1u << (q.n - base - g * 8)) - 1;
-                const u32 cached = j0 >= 0 ? 0u : j0 <= -8 ? 0xFFu : (1u << -j0) - 1;
+        }
+    }
+
+    // The running maximum, and the scores as weights, their sum (rv: the inverses of the value scales).
+    static __device__ __forceinline__ void weights(f4 (&sc)[R][2], const float (&rv)[8], V8 (&p)[R], State& s) {
+        bool grow = false;
 #pragma unroll
-                for (int i = 0; i < 8; ++i)
+        for (int r = 0; r < R; ++r) {
+            float top = sc[r][0][0];
 #pragma unroll
-                    for (int w = 0; w < VW; ++w) f.v[i][w] = in >> i & 1 ? f.v[i][w] : 0u;
-                if constexpr (!Q8) bad = take_out(f);
-#pragma unroll
-                for (int r = 0; r < R; ++r) {
-                    const u64 bits = bits_of(a, b, q, row0 + r * 16 + c);
-                    const u32 tree = j0 >= 64 || j0 <= -8 ? 0u : j0 >= 0 ? (u32)(bits >> j0) : (u32)(bits << -j0);
-                    const u32 sees = in & (cached | tree);
-#pragma unroll
-                    for (int i = 0; i < 8; ++i) {
-                        sc[r][i >> 2][i & 3] = sees >> i & 1 ? sc[r][i >> 2][i & 3] : -__builtin_inff();
-                        // a masked key's scale may be NaN: it does not enter the sum (a row that sees it has P of NaN)
-                        if constexpr (Q8) rv[i] = (sees >> i & 1) | finite_f(rv[i]) ? rv[i] : 1.f;
-                    }
-                }
-            }
-            bool grow = false;
+            for (int i = 1; i < 8; ++i) top = fmaxf(top, sc[r][i >> 2][i & 3]);
+            grow |= top > s.m[r] + SLACK;
+        }
+        if (__any(grow)) {
 #pragma unroll
             for (int r = 0; r < R; ++r) {
                 float top = sc[r][0][0];
 #pragma unroll
                 for (int i = 1; i < 8; ++i) top = fmaxf(top, sc[r][i >> 2][i & 3]);
-                grow |= top > s.m[r] + SLACK;
+                const float m = fmaxf(s.m[r], max_quarters(top));
+                const float down = s.m[r] == -__builtin_inff() ? 0.f : __builtin_amdgcn_exp2f(s.m[r] - m);
+                s.m[r] = m;
+                s.l[r] *= down;
+#pragma unroll
+                for (int j = 0; j < NJ; ++j) s.o[r][j] *= down;
             }
-            if (__any(grow)) {
+        }
 #pragma unroll
-                for (int r = 0; r < R; ++r) {
-                    float top = sc[r][0][0];
+        for (int r = 0; r < R; ++r) {
+            const float m0 = s.m[r] == -__builtin_inff() ? 0.f : s.m[r] - BIAS;
+            float add = 0.f;
 #pragma unroll
-                    for (int i = 1; i < 8; ++i) top = fmaxf(top, sc[r][i >> 2][i & 3]);
-                    const float m = fmaxf(s.m[r], max_quarters(top));
-                    const float down = s.m[r] == -__builtin_inff() ? 0.f : __builtin_amdgcn_exp2f(s.m[r] - m);
-                    s.m[r] = m;
-                    s.l[r] *= down;
-#pragma unroll
-                    for (int j = 0; j < NJ; ++j) s.o[r][j] *= down;
-                }
+            for (int i = 0; i < 8; ++i) {
+                const float e = __builtin_amdgcn_exp2f(sc[r][i >> 2][i & 3] - m0);
+                if constexpr (Q8) add = fmaf(e, rv[i], add);
+                else add += e;
+                p[r][i] = (T)e;
             }
-            V8 p[R];
+            s.l[r] += add;
+        }
+    }
+
+    static __device__ __forceinline__ void values(Values& f, const V8 (&p)[R], State& s) {
+        if constexpr (CODES == KV_INT8)
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+#pragma unroll
+                for (int k = 0; k < VW; ++k) f.v[i][k] ^= 0x80808080u;
+#pragma unroll
+        for (int j = 0; j < NJ; j += 2) {
+            V8 v0, v1;
+            col_operands<CODES, V8, VW>(f.v, j / 2, v0, v1);
 #pragma unroll
             for (int r = 0; r < R; ++r) {
-                const float m0 = s.m[r] == -__builtin_inff() ? 0.f : s.m[r] - BIAS;
-                float add = 0.f;
+                s.o[r][j] = mma(v0, p[r], s.o[r][j]);
+                s.o[r][j + 1] = mma(v1, p[r], s.o[r][j + 1]);
+            }
+        }
+    }
+
+    // The first tile's loads.
+    static __device__ __forceinline__ void begin(const TreeArgs& a, int b, int head, int base, int stop, Run& w) {
+        if (base >= stop) return;
+        const int* tab = a.table + (i64)b * a.table_stride;
+        w.next = pages_of(a, tab, base);
+        fetch_keys(a, head, base, w.next, w.k);
+        fetch_values(a, head, base, w.next, w.v);
+        w.next = pages_of(a, tab, base + TILE);
+    }
+
+    // This wave's keys from base up to stop, a tile of 32 in every TILE; the first one's loads are under way. Only its last
+    // tile can hold keys past the cached tokens: the tree and the rest of a tile before it are at most 3 tiles in a row.
+    static __device__ __forceinline__ void keys(const TreeArgs& a, int b, int head, const Seq& q, int base, int stop, int row0,
+                                                Run& w, State& s, float (*fac)[32]) {
+        if (base >= stop) return;
+        const int g = lane_id() >> 4;
+        const int* tab = a.table + (i64)b * a.table_stride;
+        const int last = base + (stop - 1 - base) / TILE * TILE;
+        const int whole = stop < q.len - 31 ? stop : q.len - 31;
+        if (base < whole) do {
+            f4 sc[R][2];
+            V8 p[R];
+            float rv[8];
+            if constexpr (Q8) factors(w.k.s, true, s, fac);
+            scores(w.k, s, fac, sc);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) rv[i] = Q8 ? fac[2][g * 8 + i] : 1.f;
+            __builtin_amdgcn_wave_barrier();
+            const int nb = base + TILE < last ? base + TILE : last;  // past the last tile: that one again
+            const Pages pg = w.next;
+            fetch_keys(a, head, nb, pg, w.k);
+            w.next = pages_of(a, tab, nb + TILE < last ? nb + TILE : last);
+            if (!__all(w.v.ok)) {  // keys without a page: masked, nothing of them enters a product
 #pragma unroll
                 for (int i = 0; i < 8; ++i) {
-                    const float e = __builtin_amdgcn_exp2f(sc[r][i >> 2][i & 3] - m0);
-                    if constexpr (Q8) add = fmaf(e, rv[i], add);
-                    else add += e;
-                    p[r][i] = (T)e;
-                }
-                s.l[r] += add;
-            }
-            if constexpr (CODES == KV_INT8)
+                    rv[i] = w.v.ok ? rv[i] : 1.f;
 #pragma unroll
-                for (int i = 0; i < 8; ++i)
+                    for (int k = 0; k < VW; ++k) w.v.v[i][k] = w.v.ok ? w.v.v[i][k] : 0u;
 #pragma unroll
-                    for (int w = 0; w < VW; ++w) f.v[i][w] ^= 0x80808080u;
-#pragma unroll
-            for (int j = 0; j < NJ; j += 2) {
-                V8 v0, v1;
-                col_operands<CODES, V8, VW>(f.v, j / 2, v0, v1);
-#pragma unroll
-                for (int r = 0; r < R; ++r) {
-                    s.o[r][j] = mma(v0, p[r], s.o[r][j]);
-                    s.o[r][j + 1] = mma(v1, p[r], s.o[r][j + 1]);
+                    for (int r = 0; r < R; ++r) sc[r][i >> 2][i & 3] = w.v.ok ? sc[r][i >> 2][i & 3] : -__builtin_inff();
                 }
             }
-            if constexpr (!Q8)
-                if (__any(bad != 0)) put_back(a, b, q, base, row0, f, bad, p, s);
+            weights(sc, rv, p, s);
+            values(w.v, p, s);
+            fetch_values(a, head, nb, pg, w.v);
             base += TILE;
-            if (!more) break;
-            fetch_values(a, head, base, next, f);
-            next = pages_of(a, tab, base + TILE);
+        } while (base < whole);
+        if (base < stop) any_tile(a, b, head, q, base, row0, w, s, fac);
+    }
+
+    // A tile with keys that some row does not see.
+    static __device__ __forceinline__ void any_tile(const TreeArgs& a, int b, int head, const Seq& q, int base, int row0, Run& w,
+                                                    State& s, float (*fac)[32]) {
+        const int c = lane_id() & 15, g = lane_id() >> 4;
+        f4 sc[R][2];
+        V8 p[R];
+        float rv[8];
+        if constexpr (Q8) factors(w.k.s, base + (lane_id() & 31) < q.n, s, fac);
+        scores(w.k, s, fac, sc);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) rv[i] = Q8 ? fac[2][g * 8 + i] : 1.f;
+        __builtin_amdgcn_wave_barrier();
+        const int j0 = base + g * 8 - q.len, left = q.n - base - g * 8;  // this lane's first key's place in the tree
+        const u32 in = !w.v.ok || left <= 0 ? 0u : left >= 8 ? 0xFFu : (1u << left) - 1;
+        const u32 cached = j0 >= 0 ? 0u : j0 <= -8 ? 0xFFu : (1u << -j0) - 1;
+#pragma unroll
+        for (int i = 0; i < 8; ++i)  // nothing of a key past the end or without a page enters a product
+#pragma unroll
+            for (int k = 0; k < VW; ++k) w.v.v[i][k] = in >> i & 1 ? w.v.v[i][k] : 0u;
+        u32 bad = 0;
+        if constexpr (!Q8) bad = take_out(w.v);
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
+            const u64 bits = bits_of(a, b, q, row0 + r * 16 + c);
+            const u32 tree = j0 >= 64 || j0 <= -8 ? 0u : j0 >= 0 ? (u32)(bits >> j0) : (u32)(bits << -j0);
+            const u32 sees = in & (cached | tree);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                sc[r][i >> 2][i & 3] = sees >> i & 1 ? sc[r][i >> 2][i & 3] : -__builtin_inff();
+                // a masked key's scale may be NaN: it does not enter the sum (a row that sees it has P of NaN)
+                if constexpr (Q8) rv[i] = (sees >> i & 1) | finite_f(rv[i]) ? rv[i] : 1.f;
+            }
         }
+        weights(sc, rv, p, s);
+        values(w.v, p, s);
+        if constexpr (!Q8)
+            if (__any(bad != 0)) put_back(a, b, q, base, row0, w.v, bad, p, s);
     }
 };
 
@@ -582,14 +654,15 @@ __global__ __launch_bounds__(256, (tree_waves<CODES, DP, R>())) void tree_k(cons
     constexpr int LD = DP + 4;
     typedef float Lo[16][LD];
     __shared__ __align__(16) char lds[sizeof(Lo) * 4 > 16 * R * W::QLD * 2 ? sizeof(Lo) * 4 : 16 * R * W::QLD * 2];
-    Lo* lo = (Lo*)lds;  // the waves' sums at a unit's end; at its beginning the queries
+    Lo* lo = (Lo*)lds;  // the waves' sums at a unit's end; before that the queries
     __shared__ float lm[4][16], ll[4][16], topl[4];
     __shared__ __align__(16) float fac[4][3][32];
     const Line line(a, blocks);
     // neighbouring shares on one XCD (blocks go round the 8 XCDs): units that share keys meet in its L2
     const int a8 = (line.shares + 7) / 8, me = (int)(blockIdx.x % 8) * a8 + (int)blockIdx.x / 8;
     if ((int)blockIdx.x / 8 >= a8 || me >= line.shares) return;
-    const int wave = threadIdx.x >> 6, c = lane_id() & 15, g = lane_id() >> 4, units = a.H * a.groups;
+    // (uniform, and the compiler is to know it: a loop that lanes left one by one would keep two sets of sums)
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), c = lane_id() & 15, g = lane_id() >> 4, units = a.H * a.groups;
     int x = me * line.per;
     const int end = line.total - x < line.per ? line.total : x + line.per;
     int before;
@@ -598,12 +671,15 @@ __global__ __launch_bounds__(256, (tree_waves<CODES, DP, R>())) void tree_k(cons
     while (x < end) {
         while (x - before >= q.tiles * units) {
             before += q.tiles * units;
-            q = seq_of(a, ++b);
+            q = uniform(seq_of(a, ++b));
         }
         const int unit = (x - before) / q.tiles, t0 = x - before - unit * q.tiles;
         const int t1 = end - x < q.tiles - t0 ? t0 + (end - x) : q.tiles;
         const int head = unit / a.groups, row0 = (unit - head * a.groups) * 16 * R;
+        const int base = t0 * TILE + wave * 32, stop = t1 * TILE < q.n ? t1 * TILE : q.n;
         typename W::State s;
+        typename W::Run run;
+        W::begin(a, b, head, base, stop, run);
         W::load_q(a, b, head, row0, (typename W::T*)lds, topl, s);
 #pragma unroll
         for (int r = 0; r < R; ++r) {
@@ -611,7 +687,7 @@ __global__ __launch_bounds__(256, (tree_waves<CODES, DP, R>())) void tree_k(cons
 #pragma unroll
             for (int j = 0; j < W::NJ; ++j) s.o[r][j] = f4{0.f, 0.f, 0.f, 0.f};
         }
-        W::keys(a, b, head, q, t0 * TILE + wave * 32, t1 * TILE < q.n ? t1 * TILE : q.n, row0, s, fac[wave]);
+        W::keys(a, b, head, q, base, stop, row0, run, s, fac[wave]);
         const bool all = t0 == 0 && t1 == q.tiles;
         const i64 slot = 2 * me + (t0 == 0 ? 1 : 0);
 #pragma unroll

@@ -46,7 +46,7 @@ static bool tree_plan(int B, int T, int H, int G, int dim, int codes, i64 cap, T
         return false;
     p.dp = (dim + 63) / 64 * 64;
     const int rows = T * G;
-    p.rpb = rows <= 16 ? 16 : rows <= 32 || p.dp > 128 ? 32 : 64;
+    p.rpb = rows <= 16 ? 16 : 32;
     p.groups = (rows + p.rpb - 1) / p.rpb;
     const i64 units = (i64)B * H * p.groups, most = units * ((cap + TILE - 1) / TILE);
     if (units > 1 << 24 || most > (i64)1 << 30) return false;
