@@ -17,13 +17,12 @@ the current stream; csrc/embed.hip has the kernels."""
 
 from __future__ import annotations
 
-import ctypes
 import functools
 import math
 
 import torch
 
-from .lib import Lib, i32
+from .lib import Entry, Lib
 
 DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 _TOKENS = {torch.int64: 8, torch.int32: 4, torch.uint16: 2}
@@ -31,13 +30,14 @@ _CELLS = {torch.int64: 8, torch.int32: 4, torch.int16: 2}
 
 
 @functools.lru_cache(maxsize=None)
-def _lib() -> Lib:
-    return Lib()
+def _entries() -> tuple[Entry, Entry, Entry]:
+    return (Entry(name="ng_embed", types="pqqiipippiqiifp"), Entry(name="ng_embed_grad", types="pqqiipippiqiifpp"),
+            Entry(name="ng_embed_weight_grad", types="pqpqqiipipiqiifp"))
 
 
 @functools.lru_cache(maxsize=256)
 def _grad_work(entries: int, vocab: int, dim: int) -> int:
-    return _lib().size("ng_embed_grad_work", entries, vocab, dim)
+    return Lib().size("ng_embed_grad_work", entries, vocab, dim)
 
 
 def _rows(t: torch.Tensor) -> torch.Tensor:
@@ -45,87 +45,98 @@ def _rows(t: torch.Tensor) -> torch.Tensor:
     return t if t.stride(-1) == 1 or t.shape[-1] == 1 else t.contiguous()
 
 
-class _Plan:
-    """The checked arguments of one call: positions n, entries a position m, entries a slot, the leading shape."""
-
-    def __init__(self, weight, tokens, weights, cell, scale):
-        if weight.dim() != 2 or weight.dtype not in DTYPES:
-            raise ValueError(f"weight must be [vocab, dim] in float32, bfloat16 or float16: got {tuple(weight.shape)} "
-                             f"{weight.dtype}")
-        if weight.shape[0] < 1 or weight.shape[1] < 1 or (weight.stride(1) != 1 and weight.shape[1] > 1):
-            raise ValueError("weight's rows must be non-empty and contiguous")
-        if tokens.dtype not in _TOKENS:
-            raise ValueError(f"tokens must be int64, int32 or uint16: got {tokens.dtype}")
-        if not weight.is_cuda:
-            raise ValueError("embed runs on the GPU: weight is a CPU tensor")
-        for name, t in (("tokens", tokens), ("weights", weights), ("cell", cell)):
-            if t is not None and t.device != weight.device:
-                raise ValueError(f"{name} is on {t.device}, weight on {weight.device}")
-        if not math.isfinite(scale):
-            raise ValueError(f"scale must be finite: {scale}")
-        if weights is None:
-            if cell is not None:
-                raise ValueError("cell goes with weights")
-            self.lead, self.n, self.m, self.entries = tuple(tokens.shape), tokens.numel(), 1, 1
-        else:
-            if weights.shape != tokens.shape or tokens.dim() not in (2, 3) or weights.dtype != torch.float32:
-                raise ValueError(f"tokens and float32 weights must both be [n, entries] or [n, slots, entries]: got "
-                                 f"{tuple(tokens.shape)} and {tuple(weights.shape)} {weights.dtype}")
-            if tokens.shape[1:].numel() < 1:
-                raise ValueError("rows need at least one entry")
-            if cell is not None and (cell.shape != tokens.shape[:-1] or cell.dtype not in _CELLS):
-                raise ValueError(f"cell must be {tuple(tokens.shape[:-1])} in int64, int32 or int16: got "
-                                 f"{tuple(cell.shape)} {cell.dtype}")
-            self.lead, self.n = (tokens.shape[0],), tokens.shape[0]
-            self.m, self.entries = tokens.shape[1:].numel(), tokens.shape[-1]
-        self.vocab, self.dim = weight.shape
-        if self.n * self.m >= (1 << 31) - 64 or self.vocab >= 1 << 31:
-            raise ValueError(f"{self.n * self.m} entries over {self.vocab} rows: at most 2^31 - 64 and 2^31 - 1")
-        self.dtype, self.scale = i32(DTYPES[weight.dtype]), ctypes.c_float(scale)
-        self.tsize = i32(_TOKENS[tokens.dtype])
-        self.csize = i32(0 if cell is None else _CELLS[cell.dtype])
-        self.shape = i32(self.m), i32(self.entries)
-
-
 class _Embed(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, weight, tokens, weights, cell, plan):
-        out = torch.empty((*plan.lead, plan.dim), dtype=weight.dtype, device=weight.device)
-        with torch.cuda.device(weight.device):
-            _lib()("ng_embed", weight, weight.stride(0), plan.vocab, i32(plan.dim), plan.dtype, tokens, plan.tsize,
-                   weights, cell, plan.csize, plan.n, *plan.shape, plan.scale, out)
-        ctx.plan = plan
+    def forward(ctx, weight, tokens, weights, cell, shape, scale):
         ctx.save_for_backward(weight if ctx.needs_input_grad[2] else None, tokens, weights, cell)
-        ctx.like = weight.dtype, weight.device
-        return out
+        ctx.of = shape, scale, weight.shape, weight.dtype, weight.device
+        return _forward(weight, tokens, weights, cell, shape, scale)
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, up):
         weight, tokens, weights, cell = ctx.saved_tensors
-        plan, (dtype, device) = ctx.plan, ctx.like
-        up = _rows(up.reshape(plan.n, plan.dim))
+        (lead, n, m, entries), scale, (vocab, dim), dtype, device = ctx.of
+        up = _rows(up.reshape(n, dim))
+        dt, csize = DTYPES[dtype], 0 if cell is None else _CELLS[cell.dtype]
+        tsize, at = _TOKENS[tokens.dtype], _at(cell)
         dweight = dweights = None
-        with torch.cuda.device(device):
-            if ctx.needs_input_grad[0]:
-                dweight = torch.empty((plan.vocab, plan.dim), dtype=dtype, device=device)
-                work = torch.empty(_grad_work(plan.n * plan.m, plan.vocab, plan.dim), dtype=torch.uint8, device=device)
-                _lib()("ng_embed_grad", up, up.stride(0), plan.vocab, i32(plan.dim), plan.dtype, tokens, plan.tsize,
-                       weights, cell, plan.csize, plan.n, *plan.shape, plan.scale, dweight, work)
-            if ctx.needs_input_grad[2]:
-                dweights = torch.empty(weights.shape, dtype=torch.float32, device=device)
-                _lib()("ng_embed_weight_grad", weight, weight.stride(0), up, up.stride(0), plan.vocab, i32(plan.dim),
-                       plan.dtype, tokens, plan.tsize, cell, plan.csize, plan.n, *plan.shape, plan.scale, dweights)
-        return dweight, None, dweights, None, None
+        if ctx.needs_input_grad[0]:
+            dweight = torch.empty((vocab, dim), dtype=dtype, device=device)
+            work = torch.empty(_grad_work(n * m, vocab, dim), dtype=torch.uint8, device=device)
+            _entries()[1](device.index, up.data_ptr(), up.stride(0), vocab, dim, dt, tokens.data_ptr(), tsize, _at(weights),
+                          at, csize, n, m, entries, scale, dweight.data_ptr(), work.data_ptr())
+        if ctx.needs_input_grad[2]:
+            dweights = torch.empty(weights.shape, dtype=torch.float32, device=device)
+            _entries()[2](device.index, weight.data_ptr(), weight.stride(0), up.data_ptr(), up.stride(0), vocab, dim, dt,
+                          tokens.data_ptr(), tsize, at, csize, n, m, entries, scale, dweights.data_ptr())
+        return dweight, None, dweights, None, None, None
+
+
+def _at(t: torch.Tensor | None) -> int | None:
+    return None if t is None else t.data_ptr()
+
+
+def _forward(weight, tokens, weights, cell, shape, scale):
+    lead, n, m, entries = shape
+    vocab, dim = weight.shape
+    out = torch.empty((*lead, dim), dtype=weight.dtype, device=weight.device)
+    _entries()[0](weight.get_device(), weight.data_ptr(), weight.stride(0), vocab, dim, DTYPES[weight.dtype],
+                  tokens.data_ptr(), _TOKENS[tokens.dtype], _at(weights), _at(cell),
+                  0 if cell is None else _CELLS[cell.dtype], n, m, entries, scale, out.data_ptr())
+    return out
+
+
+def _check(weight, tokens, weights, cell, scale) -> tuple:
+    """The shape of the call: the output's leading shape, positions, entries a position and entries a slot."""
+    if weight.dim() != 2 or weight.dtype not in DTYPES:
+        raise ValueError(f"weight must be [vocab, dim] in float32, bfloat16 or float16: got {tuple(weight.shape)} "
+                         f"{weight.dtype}")
+    vocab, dim = weight.shape
+    if vocab < 1 or dim < 1 or (weight.stride(1) != 1 and dim > 1):
+        raise ValueError("weight's rows must be non-empty and contiguous")
+    if tokens.dtype not in _TOKENS:
+        raise ValueError(f"tokens must be int64, int32 or uint16: got {tokens.dtype}")
+    device = weight.get_device()
+    if device < 0:
+        raise ValueError("embed runs on the GPU: weight is a CPU tensor")
+    for name, t in (("tokens", tokens), ("weights", weights), ("cell", cell)):
+        if t is not None and t.get_device() != device:
+            raise ValueError(f"{name} is on {t.device}, weight on {weight.device}")
+    if not math.isfinite(scale):
+        raise ValueError(f"scale must be finite: {scale}")
+    size = tokens.shape
+    if weights is None:
+        if cell is not None:
+            raise ValueError("cell goes with weights")
+        shape = size, tokens.numel(), 1, 1
+    else:
+        if weights.shape != size or len(size) not in (2, 3) or weights.dtype != torch.float32:
+            raise ValueError(f"tokens and float32 weights must both be [n, entries] or [n, slots, entries]: got "
+                             f"{tuple(size)} and {tuple(weights.shape)} {weights.dtype}")
+        shape = size[:1], size[0], size[1:].numel(), size[-1]
+        if shape[2] < 1:
+            raise ValueError("rows need at least one entry")
+        if cell is not None and (cell.shape != size[:-1] or cell.dtype not in _CELLS):
+            raise ValueError(f"cell must be {tuple(size[:-1])} in int64, int32 or int16: got {tuple(cell.shape)} "
+                             f"{cell.dtype}")
+    if shape[1] * shape[2] >= (1 << 31) - 64 or vocab >= 1 << 31:
+        raise ValueError(f"{shape[1] * shape[2]} entries over {vocab} rows: at most 2^31 - 65 and 2^31 - 1")
+    return shape
 
 
 def embed(weight: torch.Tensor, tokens: torch.Tensor, weights: torch.Tensor | None = None,
           cell: torch.Tensor | None = None, scale: float = 1.0) -> torch.Tensor:
     """Embedded rows [n, dim] of tokens and float32 weights [n, entries] or [n, slots, entries], cell [n] or [n, slots]
     (None: every slot counts), or without weights the scaled lookup [*tokens.shape, dim]; in weight's type."""
-    plan = _Plan(weight, tokens, weights, cell, float(scale))
-    return _Embed.apply(weight, tokens.contiguous(), None if weights is None else weights.contiguous(),
-                        None if cell is None else cell.contiguous(), plan)
+    scale = float(scale)
+    shape = _check(weight, tokens, weights, cell, scale)
+    tokens = tokens.contiguous()
+    weights = None if weights is None else weights.contiguous()
+    cell = None if cell is None else cell.contiguous()
+    if torch.is_grad_enabled() and (weight.requires_grad or (weights is not None and weights.requires_grad)):
+        return _Embed.apply(weight, tokens, weights, cell, shape, scale)
+    return _forward(weight, tokens, weights, cell, shape, scale)
 
 
 class HintEmbedding(torch.nn.Module):

@@ -18,7 +18,7 @@ import functools
 
 import torch
 
-from .lib import Lib, i32
+from .lib import Entry
 
 CODES = {torch.int8: 0, torch.float8_e4m3fn: 1, torch.bfloat16: 2, torch.float16: 3}
 NAMES = {"int8": torch.int8, "fp8": torch.float8_e4m3fn, "bf16": torch.bfloat16, "fp16": torch.float16}
@@ -26,8 +26,9 @@ DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 
 
 @functools.lru_cache(maxsize=None)
-def _lib() -> Lib:
-    return Lib()
+def _entries() -> tuple[Entry, Entry, Entry]:
+    return (Entry(name="ng_kv_write", types="ppqqqqipqppppqiiii"), Entry(name="ng_kv_read", types="ppppqiiiipqppi"),
+            Entry(name="ng_kv_slots", types="pqipiiqip"))
 
 
 def padded(dim: int) -> int:
@@ -63,7 +64,8 @@ class KVCache:
             raise ValueError("a 16-bit cache has no scales")
         self.k, self.v, self.k_scale, self.v_scale = k, v, k_scale, v_scale
         self.pages, self.heads, self.page = pages, heads, page
-        self.code = CODES[k.dtype]
+        self.code, self.device = CODES[k.dtype], k.get_device()
+        self._at = (k.data_ptr(), v.data_ptr(), *((None, None) if k_scale is None else (k_scale.data_ptr(), v_scale.data_ptr())))
 
     @classmethod
     def empty(cls, pages: int, page: int, heads: int, dim: int, codes: str = "int8",
@@ -78,7 +80,7 @@ class KVCache:
         return cls(k.view(dt), v.view(dt), *scales, dim=dim)
 
     def _slots(self, slots: torch.Tensor, n: int) -> torch.Tensor:
-        if slots.dtype != torch.int64 or slots.shape != (n,) or slots.device != self.k.device:
+        if slots.dtype != torch.int64 or slots.shape != (n,) or slots.get_device() != self.device:
             raise ValueError(f"slots must be int64 [{n}] on {self.k.device}: got {tuple(slots.shape)} {slots.dtype} on "
                              f"{slots.device}")
         return slots.contiguous()
@@ -87,22 +89,22 @@ class KVCache:
         """The tokens' keys and values [n, heads, dim] (any strides over tokens and heads; float32, bfloat16 or float16,
         a 16-bit cache's own type) into their slots (int64 [n]); a token whose slot is negative or past the cache is not
         written. Slots given twice in one call leave either token."""
-        n = k.shape[0]
-        want = (n, self.heads, self.dim)
-        if k.shape != want or v.shape != want or k.dtype != v.dtype or k.dtype not in DTYPES:
+        size, dtype = k.shape, k.dtype
+        if (len(size) != 3 or size[1] != self.heads or size[2] != self.dim or v.shape != size or v.dtype != dtype
+                or dtype not in DTYPES):
             raise ValueError(f"k and v must both be [n, {self.heads}, {self.dim}] in float32, bfloat16 or float16: got "
-                             f"{tuple(k.shape)} {k.dtype} and {tuple(v.shape)} {v.dtype}")
-        if self.code >= 2 and k.dtype != self.k.dtype:
-            raise ValueError(f"a {self.k.dtype} cache takes its own type: got {k.dtype}")
-        if k.device != self.k.device or v.device != self.k.device:
+                             f"{tuple(size)} {dtype} and {tuple(v.shape)} {v.dtype}")
+        if self.code >= 2 and dtype != self.k.dtype:
+            raise ValueError(f"a {self.k.dtype} cache takes its own type: got {dtype}")
+        if k.get_device() != self.device or v.get_device() != self.device:
             raise ValueError(f"k and v must be on {self.k.device}")
-        if k.stride(2) != 1 or v.stride(2) != 1:
+        (kt, kh, kd), (vt, vh, vd) = k.stride(), v.stride()
+        if kd != 1 or vd != 1:
             k, v = k.contiguous(), v.contiguous()
-        slots = self._slots(slots, n)
-        with torch.cuda.device(self.k.device):
-            _lib()("ng_kv_write", k, v, k.stride(0), k.stride(1), v.stride(0), v.stride(1), i32(DTYPES[k.dtype]), slots,
-                   n, self.k, self.v, self.k_scale, self.v_scale, self.pages, i32(self.page), i32(self.heads),
-                   i32(self.dim), i32(self.code))
+            (kt, kh, _), (vt, vh, _) = k.stride(), v.stride()
+        slots = self._slots(slots, size[0])
+        _entries()[0](self.device, k.data_ptr(), v.data_ptr(), kt, kh, vt, vh, DTYPES[dtype], slots.data_ptr(), size[0],
+                      *self._at, self.pages, self.page, self.heads, self.dim, self.code)
 
     def read(self, slots: torch.Tensor, dtype: torch.dtype = torch.bfloat16) -> tuple[torch.Tensor, torch.Tensor]:
         """The keys and values held in slots (int64 [n]) as [n, heads, dim] of `dtype`: code * scale in 32 bits, rounded
@@ -111,30 +113,32 @@ class KVCache:
             raise ValueError(f"dtype must be float32, bfloat16 or float16: {dtype}")
         n = slots.shape[0] if slots.dim() else 0
         slots = self._slots(slots, n)
-        k, v = (torch.empty((n, self.heads, self.dim), dtype=dtype, device=self.k.device) for _ in range(2))
-        with torch.cuda.device(self.k.device):
-            _lib()("ng_kv_read", self.k, self.v, self.k_scale, self.v_scale, self.pages, i32(self.page),
-                   i32(self.heads), i32(self.dim), i32(self.code), slots, n, k, v, i32(DTYPES[dtype]))
+        k = torch.empty((n, self.heads, self.dim), dtype=dtype, device=self.k.device)
+        v = torch.empty_like(k)
+        _entries()[1](self.device, *self._at, self.pages, self.page, self.heads, self.dim, self.code, slots.data_ptr(), n,
+                      k.data_ptr(), v.data_ptr(), DTYPES[dtype])
         return k, v
 
     def slots(self, table: torch.Tensor, start: torch.Tensor, count: int) -> torch.Tensor:
         """int64 [B, count]: the slots of positions start[b], start[b] + 1, ... of sequences with page tables table
         (int32 [B, width]); -1 past a table or where its entry is no page of the cache. start int32 [B]."""
         check_table(self, table)
-        if start.dtype != torch.int32 or start.shape != table.shape[:1] or start.device != self.k.device:
-            raise ValueError(f"start must be int32 [{table.shape[0]}] on {self.k.device}")
+        B, width = table.shape
+        if start.dtype != torch.int32 or start.shape != (B,) or start.get_device() != self.device:
+            raise ValueError(f"start must be int32 [{B}] on {self.k.device}")
         if count < 0:
             raise ValueError(f"count must not be negative: {count}")
-        out = torch.empty((table.shape[0], count), dtype=torch.int64, device=self.k.device)
-        with torch.cuda.device(self.k.device):
-            _lib()("ng_kv_slots", table, table.stride(0), i32(table.shape[1]), start.contiguous(), i32(table.shape[0]),
-                   i32(count), self.pages, i32(self.page), out)
+        start = start.contiguous()
+        out = torch.empty((B, count), dtype=torch.int64, device=self.k.device)
+        _entries()[2](self.device, table.data_ptr(), table.stride(0), width, start.data_ptr(), B, count, self.pages,
+                      self.page, out.data_ptr())
         return out
 
 
 def check_table(cache: KVCache, table: torch.Tensor) -> None:
-    if table.dtype != torch.int32 or table.dim() != 2 or table.device != cache.k.device:
+    if table.dtype != torch.int32 or table.dim() != 2 or table.get_device() != cache.device:
         raise ValueError(f"the page table must be int32 [sequences, width] on {cache.k.device}: got "
                          f"{tuple(table.shape)} {table.dtype} on {table.device}")
-    if table.shape[1] < 1 or (table.shape[1] > 1 and table.stride(1) != 1):
+    width = table.shape[1]
+    if width < 1 or (width > 1 and table.stride(1) != 1):
         raise ValueError("the page table's rows must be non-empty and contiguous")

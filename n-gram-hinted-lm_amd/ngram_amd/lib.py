@@ -121,3 +121,27 @@ class Lib:
         fn = getattr(self.so, name)
         fn.restype = ctypes.c_int64
         return int(fn(*(ctypes.c_int64(a) for a in args)))
+
+
+_TYPES = {"p": _ptr, "q": _i64, "i": _i32, "f": ctypes.c_float}
+
+
+class Entry:
+    """One entry point with its argument types declared, for calls whose host time counts (ctypes then converts plain ints
+    and floats itself): `Entry(name="ng_x", types="ppqi")` has a letter an argument before the stream, p a pointer (an address or
+    None), q int64, i int, f float. Called with the device's index first; the stream is that device's current one."""
+
+    def __init__(self, name: str, types: str, path: str | Path | None = None):
+        self.name, self.types = name, types
+        self.fn = load(path)[name]
+        self.fn.restype = ctypes.c_int
+        self.fn.argtypes = [_TYPES[t] for t in types] + [_ptr]
+
+    def __call__(self, device: int, *args) -> None:
+        if _device() == device:
+            rc = self.fn(*args, _stream(device))
+        else:
+            with torch.cuda.device(device):
+                rc = self.fn(*args, _stream(device))
+        if rc:
+            raise RuntimeError(f"{self.name} returned {rc}")

@@ -11,27 +11,26 @@ Everything runs on the current stream; lengths and widths are read on the device
 
 from __future__ import annotations
 
-import ctypes
 import functools
 import math
 
 import torch
 
 from .kvcache import KVCache, check_table
-from .lib import Lib, i32
+from .lib import Entry, Lib
 
 WIDEST = 64  # tokens of a tree: the bits of a mask
 DTYPES = {torch.bfloat16: 1, torch.float16: 2}
 
 
 @functools.lru_cache(maxsize=None)
-def _lib() -> Lib:
-    return Lib()
+def _entries() -> tuple[Entry, Entry]:
+    return Entry(name="ng_tree_attention", types="pqqqippppqiipqipppiiiiifppp"), Entry(name="ng_tree_mask", types="piip")
 
 
 @functools.lru_cache(maxsize=1024)
 def _work(B: int, T: int, H: int, G: int, dim: int, code: int, capacity: int) -> int:
-    n = _lib().size("ng_tree_attention_work", B, T, H, G, dim, code, capacity)
+    n = Lib().size("ng_tree_attention_work", B, T, H, G, dim, code, capacity)
     if n < 0:
         raise ValueError(f"{B} sequences of {T} tokens, {H} heads x {G}, dim {dim}, tables of {capacity} tokens: out of "
                          "range (tables hold at most 2^30 tokens)")
@@ -44,10 +43,16 @@ def tree_mask(parents: torch.Tensor) -> torch.Tensor:
     if parents.dtype != torch.int32 or parents.dim() != 2 or not 1 <= parents.shape[1] <= WIDEST or not parents.is_cuda:
         raise ValueError(f"parents must be int32 [B, 1 to {WIDEST}] on the GPU: got {tuple(parents.shape)} "
                          f"{parents.dtype} on {parents.device}")
+    parents = parents.contiguous()
     out = torch.empty(parents.shape, dtype=torch.int64, device=parents.device)
-    with torch.cuda.device(parents.device):
-        _lib()("ng_tree_mask", parents.contiguous(), i32(parents.shape[0]), i32(parents.shape[1]), out)
+    _entries()[1](parents.get_device(), parents.data_ptr(), *parents.shape, out.data_ptr())
     return out
+
+
+def _check(name: str, t: torch.Tensor, shape: tuple, dtype: torch.dtype, cache: KVCache) -> torch.Tensor:
+    if t.dtype != dtype or t.shape != shape or t.get_device() != cache.device:
+        raise ValueError(f"{name} must be {dtype} {shape} on {cache.k.device}: got {tuple(t.shape)} {t.dtype} on {t.device}")
+    return t.contiguous()
 
 
 def tree_attention(q: torch.Tensor, cache: KVCache, table: torch.Tensor, lengths: torch.Tensor,
@@ -64,38 +69,40 @@ def tree_attention(q: torch.Tensor, cache: KVCache, table: torch.Tensor, lengths
 
     Returns the output in q's shape and type, and with return_lse the float32 [B, T, heads * group] logarithms of the
     softmax sums. A row that sees nothing is zeros, its logarithm -inf."""
-    if q.dim() != 4 or q.dtype not in DTYPES:
-        raise ValueError(f"q must be [B, T, heads, dim] in bfloat16 or float16: got {tuple(q.shape)} {q.dtype}")
-    B, T, heads, dim = q.shape
+    size, dtype = q.shape, q.dtype
+    if len(size) != 4 or dtype not in DTYPES:
+        raise ValueError(f"q must be [B, T, heads, dim] in bfloat16 or float16: got {tuple(size)} {dtype}")
+    B, T, heads, dim = size
     if dim != cache.dim or heads < 1 or heads % cache.heads or not 1 <= T <= WIDEST:
-        raise ValueError(f"q {tuple(q.shape)} does not go with {cache.heads} cached heads of {cache.dim}: a multiple of the "
+        raise ValueError(f"q {tuple(size)} does not go with {cache.heads} cached heads of {cache.dim}: a multiple of the "
                          f"heads, 1 to {WIDEST} tokens")
-    if cache.code >= 2 and q.dtype != cache.k.dtype:
-        raise ValueError(f"a {cache.k.dtype} cache takes queries of its own type: got {q.dtype}")
-    device = cache.k.device
-    if q.device != device:
-        raise ValueError(f"q is on {q.device}, the cache on {device}")
+    if cache.code >= 2 and dtype != cache.k.dtype:
+        raise ValueError(f"a {cache.k.dtype} cache takes queries of its own type: got {dtype}")
+    if q.get_device() != cache.device:
+        raise ValueError(f"q is on {q.device}, the cache on {cache.k.device}")
     check_table(cache, table)
-    for name, t, shape, dt in (("table", table, (B, table.shape[1]), torch.int32), ("lengths", lengths, (B,), torch.int32),
-                               ("mask", mask, (B, T), torch.int64), ("widths", widths, (B,), torch.int32)):
-        if t is not None and (t.shape != shape or t.dtype != dt or t.device != device):
-            raise ValueError(f"{name} must be {dt} {shape} on {device}: got {tuple(t.shape)} {t.dtype} on {t.device}")
+    tables, width = table.shape
+    if tables != B:
+        raise ValueError(f"{tables} page tables for {B} sequences")
+    lengths = _check("lengths", lengths, (B,), torch.int32, cache)
+    if mask is not None:
+        mask = _check("mask", mask, (B, T), torch.int64, cache)
+    if widths is not None:
+        widths = _check("widths", widths, (B,), torch.int32, cache)
     scale = 1 / math.sqrt(dim) if scale is None else float(scale)
     if not math.isfinite(scale):
         raise ValueError(f"scale must be finite: {scale}")
-    if q.stride(3) != 1 and dim > 1:
+    qb, qt, qh, qd = q.stride()
+    if qd != 1 and dim > 1:
         q = q.contiguous()
-    lengths = lengths.contiguous()
-    mask = None if mask is None else mask.contiguous()
-    widths = None if widths is None else widths.contiguous()
-    group, width = heads // cache.heads, table.shape[1]
-    with torch.cuda.device(device):
-        out = torch.empty((B, T, heads, dim), dtype=q.dtype, device=device)
-        lse = torch.empty((B, T, heads), dtype=torch.float32, device=device) if return_lse else None
-        work = torch.empty(_work(B, T, cache.heads, group, dim, cache.code, width * cache.page), dtype=torch.uint8,
-                           device=device)
-        _lib()("ng_tree_attention", q, q.stride(0), q.stride(1), q.stride(2), i32(DTYPES[q.dtype]), cache.k, cache.v,
-               cache.k_scale, cache.v_scale, cache.pages, i32(cache.page), i32(cache.code), table, table.stride(0),
-               i32(width), lengths, widths, mask, i32(B), i32(T), i32(cache.heads), i32(group), i32(dim),
-               ctypes.c_float(scale), out, lse, work)
+        qb, qt, qh, _ = q.stride()
+    device, group = cache.k.device, heads // cache.heads
+    out = torch.empty(size, dtype=dtype, device=device)
+    lse = torch.empty(size[:3], dtype=torch.float32, device=device) if return_lse else None
+    work = torch.empty(_work(B, T, cache.heads, group, dim, cache.code, width * cache.page), dtype=torch.uint8, device=device)
+    k, v, ks, vs = cache._at
+    _entries()[0](cache.device, q.data_ptr(), qb, qt, qh, DTYPES[dtype], k, v, ks, vs, cache.pages, cache.page, cache.code,
+                  table.data_ptr(), table.stride(0), width, lengths.data_ptr(),
+                  None if widths is None else widths.data_ptr(), None if mask is None else mask.data_ptr(), B, T,
+                  cache.heads, group, dim, scale, out.data_ptr(), None if lse is None else lse.data_ptr(), work.data_ptr())
     return (out, lse) if return_lse else out
