@@ -8,8 +8,8 @@
 // An entry that does not count is not read (its table row may hold anything). A counted token outside the table is never
 // read either: its position's output is NaN, its dw NaN, and it adds to no gradient. Sums are held in 32 bits, in a fixed
 // order, and rounded once.
-#include "prim.h"
 #include "vals.h"
+#include <type_traits>
 
 struct Rows {
     const void* tokens;  // int64, int32 or uint16 (tsize 8, 4, 2), [n, m]
@@ -47,50 +47,34 @@ template <typename T, int VEC> struct Acc {
 #pragma unroll
         for (int j = 0; j < VEC; ++j) v[j] = fmaf(w, (float)p.v[j], v[j]);
     }
-    __device__ __forceinline__ void store(T* o, float scale) const {
+    __device__ __forceinline__ void store(T* o, int have, float scale) const {
         Pack<T, VEC> p;
 #pragma unroll
         for (int j = 0; j < VEC; ++j) p.v[j] = (T)(v[j] * scale);
-        p.store(o);
+        p.store(o, have);
     }
 };
 
 __device__ __forceinline__ float lane_f(float x, int l) { return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(x), l)); }
 __device__ __forceinline__ int lane_i(int x, int l) { return __builtin_amdgcn_readlane(x, l); }
 
-// The rows that the lanes of `live` name (`row` of a lane, weighted `w`), added up at this lane's column: U rows' loads in
-// flight together.
+// The rows that the lanes of `live` name (`row` of a lane, weighted `w`), added up in order at this lane's column (of which
+// the row has `have` elements): U rows' loads in flight together.
 template <typename T, int VEC, int U>
-__device__ __forceinline__ void sum_rows(const T* __restrict__ base, i64 ld, int col, bool in, u64 live, int row, float w,
+__device__ __forceinline__ void sum_rows(const T* __restrict__ base, i64 ld, int col, int have, u64 live, int row, float w,
                                          Acc<T, VEC>& acc) {
     while (live) {
-        const int have = __popcll(live);
         int at[U];
-        u64 rest = live;
+        Pack<T, VEC> p[U];
 #pragma unroll
         for (int u = 0; u < U; ++u) {
-            at[u] = rest ? __builtin_ctzll(rest) : at[0];
-            rest &= rest - 1;
-        }
-        if (have >= U) {
-            Pack<T, VEC> p[U];
-            if (in)
-#pragma unroll
-                for (int u = 0; u < U; ++u) p[u].load(base + (i64)(u32)lane_i(row, at[u]) * ld + col);
-            if (in)
-#pragma unroll
-                for (int u = 0; u < U; ++u) acc.add(p[u], lane_f(w, at[u]));
-            live = rest;
-        } else {
-            const float x = lane_f(w, at[0]);
-            const i64 r = (u32)lane_i(row, at[0]);
-            if (in) {
-                Pack<T, VEC> p;
-                p.load(base + r * ld + col);
-                acc.add(p, x);
-            }
+            at[u] = live ? __builtin_ctzll(live) : -1;
             live &= live - 1;
+            if (at[u] >= 0 && have > 0) p[u].load(base + (i64)(u32)lane_i(row, at[u]) * ld + col, have);
         }
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+            if (at[u] >= 0 && have > 0) acc.add(p[u], lane_f(w, at[u]));
     }
 }
 
@@ -102,7 +86,7 @@ __global__ __launch_bounds__(256) void embed_rows_k(const Rows r, const T* __res
     for (i64 it = (i64)blockIdx.x * 4 + (threadIdx.x >> 6); it < items; it += step) {
         const i64 n = it / chunks;
         const int col = ((int)(it - n * chunks) * 64 + lane_id()) * VEC;
-        const bool in = col < dim;
+        const int have = dim - col;
         Acc<T, VEC> acc;
         acc.zero();
         bool bad = false;
@@ -116,12 +100,12 @@ __global__ __launch_bounds__(256) void embed_rows_k(const Rows r, const T* __res
             }
             const bool out_of = (u64)tok >= (u64)r.V;
             bad |= __ballot(out_of && w != 0.f) != 0;
-            sum_rows<T, VEC, 4>(table, ld, col, in, __ballot(w != 0.f && !out_of), (int)tok, w, acc);
+            sum_rows<T, VEC, 8>(table, ld, col, have, __ballot(w != 0.f && !out_of), (int)tok, w, acc);
         }
         if (bad)
 #pragma unroll
             for (int j = 0; j < VEC; ++j) acc.v[j] = __builtin_nanf("");
-        if (in) acc.store(out + n * dim + col, scale);
+        if (have > 0) acc.store(out + n * dim + col, have, scale);
     }
 }
 
@@ -141,7 +125,8 @@ __global__ __launch_bounds__(256) void embed_tokens_k(const Rows r, const T* __r
                 const i64 n = i / per;
                 const i64 tok = int_at(r.tokens, r.tsize, n);
                 ok[u] = (u64)tok < (u64)r.V;
-                if (ok[u]) p[u].load(table + tok * ld + (i - n * per) * VEC);
+                const int col = (int)(i - n * per) * VEC;
+                if (ok[u]) p[u].load(table + tok * ld + col, dim - col);
             }
         }
 #pragma unroll
@@ -155,35 +140,235 @@ __global__ __launch_bounds__(256) void embed_tokens_k(const Rows r, const T* __r
                 else
 #pragma unroll
                     for (int j = 0; j < VEC; ++j) acc.v[j] = __builtin_nanf("");
-                acc.store(out + n * dim + (i - n * per) * VEC, scale);
+                const int col = (int)(i - n * per) * VEC;
+                acc.store(out + n * dim + col, dim - col, scale);
             }
         }
     }
 }
 
 // ------------------------------------------------------------------------------------------------ the table's gradient
+//
+// The counted entries (about a quarter of a batch's) are sorted by token, stably, by digits of 8 bits, the first pass
+// leaving out the others: an entry is one 64-bit word, token << 32 | index. A pass is three launches over `tiles` spans of
+// the list: the spans' digit counts, their sums, and the words put in their places. A list of at most ONE entries is
+// sorted by one block in one launch.
 
-__global__ __launch_bounds__(256) void embed_emit_k(const Rows r, u64* __restrict__ keys, u32* __restrict__ vals) {
-    const i64 M = r.n * r.m;
-    for (i64 i = (i64)blockIdx.x * 256 + threadIdx.x; i < M; i += (i64)gridDim.x * 256) {
-        u64 k = (u64)r.V;
-        if (weight_of(r, i) != 0.f) {
-            const i64 t = int_at(r.tokens, r.tsize, i);
-            if ((u64)t < (u64)r.V) k = (u64)t;
+#define ONE 8192
+
+struct Source {  // what a pass reads: the entries themselves (list NULL), or the list of the pass before, count words long
+    Rows r;
+    const u64* list;
+    const u32* count;
+};
+
+template <bool FIRST> __device__ __forceinline__ u32 source_size(const Source& s) {
+    return FIRST ? (u32)(s.r.n * s.r.m) : *s.count;
+}
+
+template <bool FIRST> __device__ __forceinline__ bool word_at(const Source& s, u32 i, u64& w) {
+    if (!FIRST) {
+        w = s.list[i];
+        return true;
+    }
+    if (weight_of(s.r, i) == 0.f) return false;
+    const i64 t = int_at(s.r.tokens, s.r.tsize, i);
+    w = (u64)t << 32 | i;
+    return (u64)t < (u64)s.r.V;
+}
+
+// the wave's part of tile b: whole rounds of 64 words
+__device__ __forceinline__ void part_of(u32 n, u32 tile, int b, int waves, int wave, u32& lo, u32& hi) {
+    const u64 a = (u64)b * tile + (u64)(tile / waves) * wave, z = a + tile / waves;
+    lo = a < n ? (u32)a : n, hi = z < n ? (u32)z : n;
+}
+
+template <bool FIRST>
+__global__ __launch_bounds__(256) void embed_count_k(const Source s, u32 tile, int shift, int tiles, u32* __restrict__ hist) {
+    __shared__ u32 cnt[256];
+    cnt[threadIdx.x] = 0;
+    __syncthreads();
+    const u32 n = source_size<FIRST>(s);
+    const u64 a = (u64)blockIdx.x * tile, z = a + tile < n ? a + tile : n;
+    for (u64 i = a + threadIdx.x; i < z; i += 256) {
+        u64 w;
+        if (word_at<FIRST>(s, (u32)i, w)) atomicAdd(&cnt[(w >> 32 >> shift) & 255], 1u);
+    }
+    __syncthreads();
+    hist[(i64)threadIdx.x * tiles + blockIdx.x] = cnt[threadIdx.x];
+}
+
+// a block a digit: its counts become the sums before each tile, total[digit] their sum
+__global__ __launch_bounds__(256) void embed_sums_k(u32* __restrict__ hist, int tiles, u32* __restrict__ total) {
+    __shared__ u32 part[4];
+    u32* h = hist + (i64)blockIdx.x * tiles;
+    u32 run = 0;
+    for (int t0 = 0; t0 < tiles; t0 += 256) {
+        const int t = t0 + threadIdx.x;
+        const u32 x = t < tiles ? h[t] : 0;
+        u32 inc = x;
+#pragma unroll
+        for (int o = 1; o < 64; o <<= 1) {
+            const u32 up = (u32)__shfl_up((int)inc, o, 64);
+            if (lane_id() >= o) inc += up;
         }
-        keys[i] = k;
-        vals[i] = (u32)i;
+        __syncthreads();
+        if (lane_id() == 63) part[threadIdx.x >> 6] = inc;
+        __syncthreads();
+        u32 before = run;
+        for (int w = 0; w < (int)(threadIdx.x >> 6); ++w) before += part[w];
+        if (t < tiles) h[t] = before + inc - x;
+        run += part[0] + part[1] + part[2] + part[3];
+    }
+    if (threadIdx.x == 0) total[blockIdx.x] = run;
+}
+
+// the 256 digits' starts from their totals (every thread below 256 of the block: its digit's), and their sum
+__device__ __forceinline__ u32 digit_start(u32 mine, u32* lds, u32& sum) {
+    u32 inc = mine;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+        const u32 up = (u32)__shfl_up((int)inc, o, 64);
+        if (lane_id() >= o) inc += up;
+    }
+    if (threadIdx.x < 256 && lane_id() == 63) lds[threadIdx.x >> 6] = inc;
+    __syncthreads();
+    u32 before = 0;
+    for (int w = 0; w < 4; ++w) before += w < (int)(threadIdx.x >> 6) ? lds[w] : 0;
+    sum = lds[0] + lds[1] + lds[2] + lds[3];
+    return before + inc - mine;
+}
+
+// a wave's words [lo, hi) to their places: next[digit] the place of its next word of that digit
+template <bool FIRST>
+__device__ __forceinline__ void place_words(const Source& s, u32 lo, u32 hi, int shift, u32* next, u64* __restrict__ out) {
+    for (u32 i0 = lo; i0 < hi; i0 += 64) {
+        const u32 i = i0 + lane_id();
+        u64 w = 0;
+        const bool ok = i < hi && word_at<FIRST>(s, i, w);
+        const u32 d = (u32)(w >> 32 >> shift) & 255;
+        u64 same = __ballot(ok);
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+            const u64 one = __ballot(d >> k & 1);
+            same &= d >> k & 1 ? one : ~one;
+        }
+        const u32 at = ok ? next[d] : 0;
+        __builtin_amdgcn_wave_barrier();
+        if (ok && (same & lanemask_lt()) == 0) next[d] = at + (u32)__popcll(same);  // the first lane of each digit
+        __builtin_amdgcn_wave_barrier();
+        if (ok) out[at + (u32)__popcll(same & lanemask_lt())] = w;
     }
 }
 
-// start[v] = the first sorted entry whose token is >= v, v in [0, V]; a gap of many tokens is filled by the whole wave
-__global__ __launch_bounds__(256) void embed_starts_k(const u64* __restrict__ keys, i64 M, i64 V, u32* __restrict__ start) {
+template <bool FIRST>
+__device__ __forceinline__ void count_words(const Source& s, u32 lo, u32 hi, int shift, u32* cnt) {
+    for (u32 i = lo + lane_id(); i < hi; i += 64) {
+        u64 w;
+        if (word_at<FIRST>(s, i, w)) atomicAdd(&cnt[(w >> 32 >> shift) & 255], 1u);
+    }
+}
+
+template <bool FIRST>
+__global__ __launch_bounds__(256) void embed_place_k(const Source s, u32 tile, int shift, int tiles,
+                                                     const u32* __restrict__ hist, const u32* __restrict__ total,
+                                                     u64* __restrict__ out, u32* __restrict__ count) {
+    __shared__ u32 next[4][256];
+    __shared__ u32 part[4];
+    const int wave = threadIdx.x >> 6, d = threadIdx.x;
+#pragma unroll
+    for (int w = 0; w < 4; ++w) next[w][d] = 0;
+    u32 sum;
+    u32 at = digit_start(total[d], part, sum) + hist[(i64)d * tiles + blockIdx.x];
+    if (FIRST && blockIdx.x == 0 && d == 0) *count = sum;
+    __syncthreads();
+    u32 lo, hi;
+    part_of(source_size<FIRST>(s), tile, blockIdx.x, 4, wave, lo, hi);
+    count_words<FIRST>(s, lo, hi, shift, next[wave]);
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+        const u32 c = next[w][d];
+        next[w][d] = at;
+        at += c;
+    }
+    __syncthreads();
+    place_words<FIRST>(s, lo, hi, shift, next[wave], out);
+}
+
+// The whole sort of at most ONE entries by one block, the lists in LDS; the last pass writes out.
+__global__ __launch_bounds__(1024) void embed_sort_one_k(const Source src, int passes, u64* __restrict__ out,
+                                                         u32* __restrict__ count) {
+    __shared__ u64 list[ONE];
+    __shared__ u32 next[16][256];
+    __shared__ u32 part[4];
+    __shared__ u32 size;
+    const int wave = threadIdx.x >> 6, d = threadIdx.x & 255;
+    Source s = src;
+    for (int p = 0; p < passes; ++p) {
+        for (int i = threadIdx.x; i < 16 * 256; i += 1024) next[i >> 8][i & 255] = 0;
+        __syncthreads();
+        const u32 n = p ? size : (u32)(s.r.n * s.r.m);
+        const u32 tile = (n + 1023) / 1024 * 1024;
+        u32 lo, hi;
+        part_of(n, tile, 0, 16, wave, lo, hi);
+        u64 keep[ONE / 1024];  // the wave's words: they are written over the list they come from
+#pragma unroll
+        for (int k = 0; k < ONE / 1024; ++k) {
+            const u32 i = lo + k * 64 + lane_id();
+            keep[k] = ~0ull;
+            if (i < hi) {
+                if (p) keep[k] = list[i];
+                else if (u64 w; word_at<true>(s, i, w)) keep[k] = w;
+            }
+            if (keep[k] != ~0ull) atomicAdd(&next[wave][(keep[k] >> 32 >> (8 * p)) & 255], 1u);
+        }
+        __syncthreads();
+        u32 mine = 0;
+        if (threadIdx.x < 256)
+            for (int w = 0; w < 16; ++w) mine += next[w][d];
+        u32 sum, at = digit_start(mine, part, sum);
+        if (threadIdx.x < 256)
+            for (int w = 0; w < 16; ++w) {
+                const u32 c = next[w][d];
+                next[w][d] = at;
+                at += c;
+            }
+        if (p == 0 && threadIdx.x == 0) size = sum, *count = sum;
+        __syncthreads();
+        u64* to = p == passes - 1 ? out : list;
+#pragma unroll
+        for (int k = 0; k < ONE / 1024; ++k) {
+            const u64 w = keep[k];
+            const bool ok = w != ~0ull;
+            const u32 b = (u32)(w >> 32 >> (8 * p)) & 255;
+            u64 same = __ballot(ok);
+#pragma unroll
+            for (int q = 0; q < 8; ++q) {
+                const u64 one = __ballot(b >> q & 1);
+                same &= b >> q & 1 ? one : ~one;
+            }
+            const u32 to_at = ok ? next[wave][b] : 0;
+            __builtin_amdgcn_wave_barrier();
+            if (ok && (same & lanemask_lt()) == 0) next[wave][b] = to_at + (u32)__popcll(same);
+            __builtin_amdgcn_wave_barrier();
+            if (ok) to[to_at + (u32)__popcll(same & lanemask_lt())] = w;
+        }
+        __syncthreads();
+    }
+}
+
+// start[v] = the first sorted word whose token is >= v, v in [0, V]. Many words: each opens its token and the absent ones
+// before it (a gap of many tokens is filled by the whole wave).
+__global__ __launch_bounds__(256) void embed_starts_k(const u64* __restrict__ list, const u32* __restrict__ count, i64 V,
+                                                      u32* __restrict__ start) {
+    const i64 M = *count;
     for (i64 w0 = (i64)blockIdx.x * 256 + (threadIdx.x & ~63); w0 <= M; w0 += (i64)gridDim.x * 256) {
         const i64 i = w0 + lane_id();
-        i64 lo = 0, hi = 0;  // this entry opens the tokens [lo, hi)
+        i64 lo = 0, hi = 0;  // this word opens the tokens [lo, hi)
         if (i <= M) {
-            lo = i ? (i64)keys[i - 1] + 1 : 0;
-            hi = (i < M ? (i64)keys[i] : V) + 1;
+            lo = i ? (i64)(list[i - 1] >> 32) + 1 : 0;
+            hi = (i < M ? (i64)(list[i] >> 32) : V) + 1;
         }
         u64 wide = __ballot(hi - lo > 16);
         if (hi - lo <= 16)
@@ -197,82 +382,144 @@ __global__ __launch_bounds__(256) void embed_starts_k(const u64* __restrict__ ke
     }
 }
 
-#define PIECE 64  // a token with more entries than this is summed in pieces of the sorted list's chunks of this many
-
-// The sum over sorted entries [a, b) (at most 64) at this lane's column.
-template <typename T, int VEC>
-__device__ __forceinline__ void sum_entries(const u32* __restrict__ vals, u32 a, u32 b, const float* __restrict__ w, int m,
-                                            const T* __restrict__ dout, i64 ld, int col, bool in, Acc<T, VEC>& acc) {
-    const u32 i = a + lane_id();
-    int n = 0;
-    float x = 0.f;
-    if (i < b) {
-        const u32 e = vals[i];
-        x = w ? w[e] : 1.f;
-        n = (int)(e / (u32)m);
+// Few words (at most ONE): every token looks for its own, in LDS.
+__global__ __launch_bounds__(256) void embed_starts_one_k(const u64* __restrict__ list, const u32* __restrict__ count, i64 V,
+                                                          u32* __restrict__ start) {
+    __shared__ u32 tok[ONE];
+    const u32 M = *count;
+    for (u32 i = threadIdx.x; i < M; i += 256) tok[i] = (u32)(list[i] >> 32);
+    __syncthreads();
+    for (i64 v = (i64)blockIdx.x * 256 + threadIdx.x; v <= V; v += (i64)gridDim.x * 256) {
+        u32 lo = 0, hi = M;
+        while (lo < hi) {
+            const u32 mid = (lo + hi) / 2;
+            if ((i64)tok[mid] < v) lo = mid + 1;
+            else hi = mid;
+        }
+        start[v] = lo;
     }
-    sum_rows<T, VEC, 4>(dout, ld, col, in, __ballot(i < b), n, x, acc);
 }
 
-// A wave per (chunk of PIECE sorted entries, chunk of columns): the sums of a frequent token's part at the chunk's start
-// (slot 2 * chunk) and at its end (slot 2 * chunk + 1). A token with more than PIECE entries holds a chunk's first entry or
-// its last one wherever it touches it, so there are no others.
+// The sums. The sorted list is cut into chunks of 64 entries, a wave per chunk (and chunk of columns), whatever the tokens:
+// the work is even, and 8 rows' loads are in flight together whichever token they belong to. A token whose entries all lie
+// in one chunk has its gradient row stored there; one that crosses a chunk's end leaves a partial sum in each chunk that it
+// touches, slot 2 * chunk where it holds the chunk's first entry, else slot 2 * chunk + 1 (it then holds the last one), and
+// they are joined in order. Rows without entries are zeroed by a pass of their own.
+#define CHUNK 64
+
 template <typename T, int VEC>
-__global__ __launch_bounds__(256) void embed_pieces_k(const u64* __restrict__ keys, const u32* __restrict__ vals,
-                                                      const u32* __restrict__ start, i64 V, const float* __restrict__ w,
-                                                      int m, const T* __restrict__ dout, i64 ld, int dim, int chunks,
-                                                      i64 pieces, float* __restrict__ part) {
-    const u32 M = start[V];
-    const i64 items = pieces * chunks;
+__global__ __launch_bounds__(256) void embed_runs_k(const u64* __restrict__ list, const u32* __restrict__ count,
+                                                    const float* __restrict__ w, int m, const T* __restrict__ dout, i64 ld,
+                                                    int dim, int chunks, float scale, i64 spans, float* __restrict__ part,
+                                                    T* __restrict__ grad) {
+    constexpr int U = 8;
+    const u32 M = *count;
+    const i64 items = spans * chunks;
     for (i64 it = (i64)blockIdx.x * 4 + (threadIdx.x >> 6); it < items; it += (i64)gridDim.x * 4) {
         const i64 c = it / chunks;
-        const u32 c0 = (u32)(c * PIECE);
+        const u32 c0 = (u32)(c * CHUNK);
         if (c0 >= M) return;
-        const u32 c1 = M - c0 < PIECE ? M : c0 + PIECE;
-        const int col = ((int)(it - c * chunks) * 64 + lane_id()) * VEC;
-        const u32 t[2] = {(u32)keys[c0], (u32)keys[c1 - 1]};
+        const int last = M - c0 < CHUNK ? (int)(M - c0) - 1 : CHUNK - 1;
+        const int col = ((int)(it - c * chunks) * 64 + lane_id()) * VEC, have = dim - col;
+        const u32 i = c0 + (lane_id() < last ? lane_id() : last);
+        const u64 word = list[i];
+        const u32 tok = (u32)(word >> 32), before = i ? (u32)(list[i - 1] >> 32) : ~0u, after = i + 1 < M ? (u32)(list[i + 1] >> 32) : ~0u;
+        const int n = (int)((u32)word / (u32)m);
+        const float x = w ? w[(u32)word] : 1.f;
+        const u64 ends = __ballot(after != tok) | 1ull << last;
+        const bool from = lane_i((int)before, 0) == lane_i((int)tok, 0), on = lane_i((int)after, last) == lane_i((int)tok, last);
+        bool first = true;
+        Acc<T, VEC> acc;
+        acc.zero();
+        for (int l0 = 0; l0 <= last; l0 += U) {
+            Pack<T, VEC> r[U];
 #pragma unroll
-        for (int side = 0; side < 2; ++side) {
-            if (side && t[1] == t[0]) break;
-            const u32 s = start[t[side]], e = start[t[side] + 1];
-            if (e - s <= PIECE) continue;
-            Acc<T, VEC> acc;
-            acc.zero();
-            sum_entries<T, VEC>(vals, s > c0 ? s : c0, e < c1 ? e : c1, w, m, dout, ld, col, col < dim, acc);
-            if (col < dim) {
-                float* o = part + (2 * c + side) * dim + col;
+            for (int u = 0; u < U; ++u)
+                if (l0 + u <= last && have > 0) r[u].load(dout + (i64)(u32)lane_i(n, l0 + u) * ld + col, have);
 #pragma unroll
-                for (int j = 0; j < VEC; ++j) o[j] = acc.v[j];
+            for (int u = 0; u < U; ++u) {
+                const int l = l0 + u;
+                if (l > last) break;
+                if (have > 0) acc.add(r[u], lane_f(x, l));
+                if (ends >> l & 1) {
+                    if ((first && from) || (l == last && on)) {
+                        float* o = part + ((2 * c + (first ? 0 : 1)) * chunks * 64) * VEC + col;
+#pragma unroll
+                        for (int j = 0; j < VEC; ++j) o[j] = acc.v[j];
+                    } else if (have > 0) acc.store(grad + (i64)(u32)lane_i((int)tok, l) * dim + col, have, scale);
+                    acc.zero();
+                    first = false;
+                }
             }
         }
     }
 }
 
-// A wave per (token, chunk of columns): its gradient row, from its entries or from its pieces.
+// A block per (chunk, chunk of columns) in which a token begins that goes on in the next: its partial sums joined, each of
+// the eight waves in order, then the waves' sums.
 template <typename T, int VEC>
-__global__ __launch_bounds__(256) void embed_grad_k(const u32* __restrict__ vals, const u32* __restrict__ start, i64 V,
-                                                    const float* __restrict__ w, int m, const T* __restrict__ dout, i64 ld,
-                                                    int dim, int chunks, float scale, const float* __restrict__ part,
-                                                    T* __restrict__ grad) {
-    const i64 items = V * chunks;
-    for (i64 it = (i64)blockIdx.x * 4 + (threadIdx.x >> 6); it < items; it += (i64)gridDim.x * 4) {
-        const i64 v = it / chunks;
-        const int col = ((int)(it - v * chunks) * 64 + lane_id()) * VEC;
-        const bool in = col < dim;
-        const u32 s = start[v], e = start[v + 1];
-        Acc<T, VEC> acc;
-        acc.zero();
-        if (e - s <= PIECE) {
-            if (e > s) sum_entries<T, VEC>(vals, s, e, w, m, dout, ld, col, in, acc);
-        } else if (in) {
-            const i64 c0 = s / PIECE, c1 = (e - 1) / PIECE;
-            for (i64 c = c0; c <= c1; ++c) {
-                const float* p = part + (2 * c + (c == c0 && s % PIECE ? 1 : 0)) * dim + col;
+__global__ __launch_bounds__(512) void embed_join_k(const u64* __restrict__ list, const u32* __restrict__ count,
+                                                    const u32* __restrict__ start, int dim, int chunks, i64 spans, float scale,
+                                                    const float* __restrict__ part, T* __restrict__ grad) {
+    constexpr int U = 8;
+    __shared__ float sums[8][64 * VEC];
+    const u32 M = *count;
+    const i64 items = spans * chunks, row = (i64)chunks * 64 * VEC;
+    const int wave = threadIdx.x >> 6;
+    for (i64 it = blockIdx.x; it < items; it += gridDim.x) {
+        const i64 c = it / chunks;
+        const u32 c0 = (u32)(c * CHUNK);
+        if (c0 >= M) return;
+        const u32 c1 = M - c0 < CHUNK ? M : c0 + CHUNK;
+        const u32 t = (u32)(list[c1 - 1] >> 32), s = start[t], e = start[t + 1];
+        if (e <= c1 || s < c0) continue;
+        const int col = ((int)(it - c * chunks) * 64 + lane_id()) * VEC;
+        const i64 end = (e - 1) / CHUNK;
+        float acc[VEC];
 #pragma unroll
-                for (int j = 0; j < VEC; ++j) acc.v[j] += p[j];
+        for (int j = 0; j < VEC; ++j) acc[j] = 0.f;
+        for (i64 k = c + wave; k <= end; k += 8 * U) {
+            Pack<float, VEC> x[U];
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                const i64 q = k + 8 * u;
+                if (q <= end) x[u].load(part + (2 * q + (q == c && s != c0 ? 1 : 0)) * row + col);
             }
+#pragma unroll
+            for (int u = 0; u < U; ++u)
+                if (k + 8 * u <= end)
+#pragma unroll
+                    for (int j = 0; j < VEC; ++j) acc[j] += x[u].v[j];
         }
-        if (in) acc.store(grad + v * dim + col, scale);
+        __syncthreads();
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) sums[wave][j * 64 + lane_id()] = acc[j];
+        __syncthreads();
+        if (wave == 0 && col < dim) {
+            Acc<T, VEC> r;
+#pragma unroll
+            for (int j = 0; j < VEC; ++j) {
+                r.v[j] = sums[0][j * 64 + lane_id()];
+#pragma unroll
+                for (int k = 1; k < 8; ++k) r.v[j] += sums[k][j * 64 + lane_id()];
+            }
+            r.store(grad + t * (i64)dim + col, dim - col, scale);
+        }
+    }
+}
+
+// A thread per VEC columns of a row: rows without entries are zeros.
+template <typename T, int VEC>
+__global__ __launch_bounds__(256) void embed_zero_k(const u32* __restrict__ start, i64 V, int dim, int per, T* __restrict__ grad) {
+    const i64 items = V * per;
+    for (i64 i = (i64)blockIdx.x * 256 + threadIdx.x; i < items; i += (i64)gridDim.x * 256) {
+        const i64 v = i / per;
+        if (start[v] != start[v + 1]) continue;
+        const int col = (int)(i - v * per) * VEC;
+        Pack<T, VEC> z;
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) z.v[j] = (T)0.f;
+        z.store(grad + v * dim + col, dim - col);
     }
 }
 
@@ -303,10 +550,10 @@ __global__ __launch_bounds__(256) void embed_dw_k(const Rows r, const T* __restr
                 }
                 for (int col = lane_id() * VEC; col < dim; col += 64 * VEC) {
                     Pack<T, VEC> d, p[8];
-                    d.load(dout + n * dld + col);
+                    d.load(dout + n * dld + col, dim - col);
 #pragma unroll
                     for (int u = 0; u < 8; ++u)
-                        if (at[u] >= 0) p[u].load(table + (i64)(u32)lane_i((int)tok, at[u]) * ld + col);
+                        if (at[u] >= 0) p[u].load(table + (i64)(u32)lane_i((int)tok, at[u]) * ld + col, dim - col);
 #pragma unroll
                     for (int u = 0; u < 8; ++u)
                         if (at[u] >= 0)
@@ -339,11 +586,11 @@ static inline int wave_grid(i64 waves) {
     return (int)(g < 65536 ? (g > 0 ? g : 1) : 65536);
 }
 
-// The most elements of 16 bytes or fewer that a row's loads may take: every pointer and row stride a multiple of them, the
-// row a whole number of them, and (where a wave takes one row) more than `lanes` lanes with work.
-template <typename T> static int vec_of(u64 where, int dim, int lanes = 32) {
+// The elements a lane takes of a row: 16 bytes of them, or fewer where a short row would leave over half of a wave's lanes
+// without work.
+template <typename T> static int vec_of(int dim, int lanes = 32) {
     int v = 16 / (int)sizeof(T);
-    while (v > 1 && ((where & (v * sizeof(T) - 1)) || dim % v || dim / v <= lanes)) v >>= 1;
+    while (v > 1 && (dim + v - 1) / v <= lanes) v >>= 1;
     return v;
 }
 
@@ -358,12 +605,11 @@ template <typename T, typename F> static int with_vec(int v, F f) {
 
 template <typename T>
 static int embed_fwd(const Rows& r, const T* table, i64 ld, int dim, float scale, T* out, hipStream_t st) {
-    const u64 where = (u64)table | (u64)out | (u64)(ld * sizeof(T));
     const bool plain = !r.w && !r.cell && r.m == 1;
-    return with_vec<T>(vec_of<T>(where, dim, plain ? 0 : 32), [&](auto c) {
+    return with_vec<T>(vec_of<T>(dim, plain ? 0 : 32), [&](auto c) {
         constexpr int VEC = decltype(c)::value;
         if (plain) {
-            const int per = dim / VEC;
+            const int per = (dim + VEC - 1) / VEC;
             const i64 g = (r.n * per + 1023) / 1024;
             embed_tokens_k<T, VEC><<<(int)(g < 65536 ? g : 65536), 256, 0, st>>>(r, table, ld, dim, scale, out, per);
         } else {
@@ -375,11 +621,11 @@ static int embed_fwd(const Rows& r, const T* table, i64 ld, int dim, float scale
 }
 
 struct GradWork {
-    u64 *ka, *kb;
-    u32 *va, *vb, *start;
-    void* sort;
-    size_t sort_bytes;
+    u64 *la, *lb;
+    u32 *hist, *total, *count, *start;
     float* part;
+    u32 tile;   // entries of a span, a multiple of 256
+    int tiles;  // at most 2048 of them
     i64 bytes;
     GradWork(void* base, i64 M, i64 V, int dim) {
         char* p = (char*)base;
@@ -388,11 +634,14 @@ struct GradWork {
             p += (n + 255) / 256 * 256;
             return (void*)q;
         };
-        sort_bytes = prim::radix_sort_temp_bytes(M, true);
-        ka = (u64*)take(8 * M), kb = (u64*)take(8 * M), va = (u32*)take(4 * M), vb = (u32*)take(4 * M);
+        // spans of 1024 entries or more: 524288 entries fill the 256 compute units twice
+        const i64 t = (M + 2047) / 2048;
+        tile = (u32)((t < 1024 ? 1024 : t) + 255) / 256 * 256;
+        tiles = M > ONE ? (int)((M + tile - 1) / tile) : 0;
+        la = (u64*)take(8 * M), lb = (u64*)take(M > ONE ? 8 * M : 0);
+        hist = (u32*)take(1024ll * tiles), total = (u32*)take(1024), count = (u32*)take(4);
         start = (u32*)take(4 * (V + 1));
-        sort = take((i64)sort_bytes);
-        part = (float*)take((M + PIECE - 1) / PIECE * 2 * dim * 4);
+        part = (float*)take(M > CHUNK ? (M + CHUNK - 1) / CHUNK * 2 * ((dim + 511) / 512 * 512) * 4 : 0);  // 64 * VEC columns or more
         bytes = p - (char*)base;
     }
 };
@@ -401,23 +650,40 @@ template <typename T>
 static int embed_grad(const Rows& r, const T* dout, i64 ld, int dim, float scale, T* grad, void* work, hipStream_t st) {
     const i64 M = r.n * r.m;
     const GradWork g(work, M, r.V, dim);
-    int bits = 1;
-    while (bits < 32 && (r.V >> bits)) ++bits;
-    const int eg = grid_for(M, 256);
-    embed_emit_k<<<eg > 4096 ? 4096 : eg, 256, 0, st>>>(r, g.ka, g.va);
-    int rc = prim::radix_sort_pairs(g.ka, g.kb, g.va, g.vb, M, 0, bits, g.sort, g.sort_bytes, st);
-    if (rc) return rc;
-    const int sg = grid_for(M + 1, 256);
-    embed_starts_k<<<sg > 4096 ? 4096 : sg, 256, 0, st>>>(g.kb, M, r.V, g.start);
-    const u64 where = (u64)dout | (u64)grad | (u64)(ld * sizeof(T));
-    return with_vec<T>(vec_of<T>(where, dim), [&](auto c) {
+    int passes = 1;
+    while (passes < 4 && (r.V - 1) >> (8 * passes)) ++passes;
+    u64* list = g.la;
+    Source s;
+    s.r = r, s.list = nullptr, s.count = g.count;
+    if (M <= ONE) {
+        embed_sort_one_k<<<1, 1024, 0, st>>>(s, passes, list, g.count);
+        const int sg = grid_for(r.V + 1, 256);
+        embed_starts_one_k<<<sg > 1024 ? 1024 : sg, 256, 0, st>>>(list, g.count, r.V, g.start);
+    } else {
+        for (int p = 0; p < passes; ++p) {
+            u64* to = p & 1 ? g.lb : g.la;
+            if (p == 0) embed_count_k<true><<<g.tiles, 256, 0, st>>>(s, g.tile, 0, g.tiles, g.hist);
+            else embed_count_k<false><<<g.tiles, 256, 0, st>>>(s, g.tile, 8 * p, g.tiles, g.hist);
+            embed_sums_k<<<256, 256, 0, st>>>(g.hist, g.tiles, g.total);
+            if (p == 0) embed_place_k<true><<<g.tiles, 256, 0, st>>>(s, g.tile, 0, g.tiles, g.hist, g.total, to, g.count);
+            else embed_place_k<false><<<g.tiles, 256, 0, st>>>(s, g.tile, 8 * p, g.tiles, g.hist, g.total, to, g.count);
+            s.list = list = to;
+        }
+        const int sg = grid_for(M + 1, 256);
+        embed_starts_k<<<sg > 4096 ? 4096 : sg, 256, 0, st>>>(list, g.count, r.V, g.start);
+    }
+    return with_vec<T>(vec_of<T>(dim), [&](auto c) {
         constexpr int VEC = decltype(c)::value;
-        const int chunks = (dim + 64 * VEC - 1) / (64 * VEC);
-        const i64 pieces = (M + PIECE - 1) / PIECE;
-        embed_pieces_k<T, VEC><<<wave_grid(pieces * chunks), 256, 0, st>>>(g.kb, g.vb, g.start, r.V, r.w, r.m, dout, ld, dim,
-                                                                           chunks, pieces, g.part);
-        embed_grad_k<T, VEC><<<wave_grid(r.V * chunks), 256, 0, st>>>(g.vb, g.start, r.V, r.w, r.m, dout, ld, dim, chunks,
-                                                                      scale, g.part, grad);
+        const int chunks = (dim + 64 * VEC - 1) / (64 * VEC), per = (dim + VEC - 1) / VEC;
+        const i64 spans = (M + CHUNK - 1) / CHUNK, items = spans * chunks;
+        const int zg = grid_for(r.V * per, 256);
+        embed_zero_k<T, VEC><<<zg > 65536 ? 65536 : zg, 256, 0, st>>>(g.start, r.V, dim, per, grad);
+        if (M > 0)
+            embed_runs_k<T, VEC><<<wave_grid(items), 256, 0, st>>>(list, g.count, r.w, r.m, dout, ld, dim, chunks, scale, spans,
+                                                                   g.part, grad);
+        if (M > CHUNK)
+            embed_join_k<T, VEC><<<(int)(items < 65536 ? items : 65536), 512, 0, st>>>(list, g.count, g.start, dim, chunks, spans,
+                                                                                       scale, g.part, grad);
         return (int)hipGetLastError();
     });
 }
@@ -425,8 +691,7 @@ static int embed_grad(const Rows& r, const T* dout, i64 ld, int dim, float scale
 template <typename T>
 static int embed_dw(const Rows& r, const T* table, i64 ld, const T* dout, i64 dld, int dim, float scale, float* dw,
                     hipStream_t st) {
-    const u64 where = (u64)table | (u64)dout | (u64)((ld | dld) * sizeof(T));
-    return with_vec<T>(vec_of<T>(where, dim), [&](auto c) {
+    return with_vec<T>(vec_of<T>(dim), [&](auto c) {
         constexpr int VEC = decltype(c)::value;
         embed_dw_k<T, VEC><<<wave_grid(r.n), 256, 0, st>>>(r, table, ld, dout, dld, dim, scale, dw);
         return (int)hipGetLastError();

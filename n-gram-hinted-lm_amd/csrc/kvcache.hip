@@ -131,7 +131,8 @@ __global__ __launch_bounds__(256) void kv_read_k(const ReadArgs a) {
 #pragma unroll
                     for (int j = 0; j < 8; ++j) v[j] = (float)(signed char)k.v[j] * s;
                 } else {
-                    const u32 w[2] = {k.r.x, k.r.y};
+                    u32 w[2];
+                    __builtin_memcpy(w, k.v, 8);
 #pragma unroll
                     for (int h = 0; h < 2; ++h) {
                         const auto lo = __builtin_amdgcn_cvt_pk_f32_fp8((int)w[h], false);

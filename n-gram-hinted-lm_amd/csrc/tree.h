@@ -337,12 +337,15 @@ template <int CODES, int DP, int R> struct Tree {
         for (int k = 0; k < NQ; ++k) {
             const int i = threadIdx.x + 256 * k;
             if (i < 16 * R * DP / 8) {
-                Pack<T, 8> y;
+                union {
+                    T e[8];
+                    uint4 w;
+                } y;
                 if constexpr (Q8)
 #pragma unroll
-                    for (int j = 0; j < 8; ++j) y.v[j] = (T)(value(a, x[k].e[j]) * up);
-                else y.r = x[k].w;
-                y.store(lds + i / (DP / 8) * QLD + i % (DP / 8) * 8);
+                    for (int j = 0; j < 8; ++j) y.e[j] = (T)(value(a, x[k].e[j]) * up);
+                else y.w = x[k].w;
+                *(uint4*)(lds + i / (DP / 8) * QLD + i % (DP / 8) * 8) = y.w;
             }
         }
         lds_barrier();

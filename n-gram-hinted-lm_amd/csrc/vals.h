@@ -11,21 +11,38 @@ enum { NG_F32 = 0, NG_BF16 = 1, NG_F16 = 2 };
 // a cache's codes
 enum { KV_INT8 = 0, KV_FP8 = 1, KV_BF16 = 2, KV_F16 = 3 };
 
-template <int BYTES> struct raw_t;
+// N consecutive elements of T, moved as one load or store of N * sizeof(T) bytes, wherever p points (global memory takes
+// any alignment; rows whose length is odd run at the wide loads' rate but for the lines that two of them share)
+template <int BYTES> struct raw_t { typedef u32 type __attribute__((ext_vector_type(BYTES / 4), aligned(2))); };
 template <> struct raw_t<2> { typedef unsigned short type; };
-template <> struct raw_t<4> { typedef u32 type; };
-template <> struct raw_t<8> { typedef uint2 type; };
-template <> struct raw_t<16> { typedef uint4 type; };
+template <> struct raw_t<4> { typedef u32 type __attribute__((aligned(2))); };
 
-// N consecutive elements of T, moved as one load or store of N * sizeof(T) bytes (p aligned to that)
 template <typename T, int N> struct Pack {
+    T v[N];
     typedef typename raw_t<sizeof(T) * N>::type raw;
-    union {
+    __device__ __forceinline__ void load(const T* p) {
+        const raw r = *(const raw*)p;
+        __builtin_memcpy(v, &r, sizeof(raw));
+    }
+    __device__ __forceinline__ void store(T* p) const {
         raw r;
-        T v[N];
-    };
-    __device__ __forceinline__ void load(const T* p) { r = *(const raw*)p; }
-    __device__ __forceinline__ void store(T* p) const { *(raw*)p = r; }
+        __builtin_memcpy(&r, v, sizeof(raw));
+        *(raw*)p = r;
+    }
+    // of a row of `have` elements from p on
+    __device__ __forceinline__ void load(const T* p, int have) {
+        if (have >= N) load(p);
+        else
+#pragma unroll
+            for (int j = 0; j < N; ++j) v[j] = j < have ? p[j] : (T)0.f;
+    }
+    __device__ __forceinline__ void store(T* p, int have) const {
+        if (have >= N) store(p);
+        else
+#pragma unroll
+            for (int j = 0; j < N; ++j)
+                if (j < have) p[j] = v[j];
+    }
 };
 
 __device__ __forceinline__ bool finite_f(float x) { return __builtin_fabsf(x) < __builtin_inff(); }  // false for NaN
