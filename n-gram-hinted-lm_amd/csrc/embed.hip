@@ -47,21 +47,33 @@ template <typename T, int VEC> struct Acc {
 #pragma unroll
         for (int j = 0; j < VEC; ++j) v[j] = fmaf(w, (float)p.v[j], v[j]);
     }
-    __device__ __forceinline__ void store(T* o, int have, float scale) const {
+    __device__ __forceinline__ void store(T* o, float scale) const {
         Pack<T, VEC> p;
 #pragma unroll
         for (int j = 0; j < VEC; ++j) p.v[j] = (T)(v[j] * scale);
-        p.store(o, have);
+        p.store(o);
+    }
+};
+
+// The columns of a lane, [at, at + VEC) of the row: where the row ends inside them, or before, the row's last VEC columns
+// (dim >= VEC). So every load is a whole one: a row's last lane may compute columns of the lane before it once more, to the
+// same values, and a lane with nothing to do (in false) only stores nothing.
+template <int VEC> struct Cols {
+    int at, again;  // again: the first `again` of its columns are another lane's
+    bool in;
+    __device__ __forceinline__ Cols(int lane, int dim) {
+        const int col = lane * VEC;
+        in = col < dim, at = col < dim - VEC ? col : dim - VEC, again = in ? col - at : VEC;
     }
 };
 
 __device__ __forceinline__ float lane_f(float x, int l) { return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(x), l)); }
 __device__ __forceinline__ int lane_i(int x, int l) { return __builtin_amdgcn_readlane(x, l); }
 
-// The rows that the lanes of `live` name (`row` of a lane, weighted `w`), added up in order at this lane's column (of which
-// the row has `have` elements): U rows' loads in flight together.
+// The rows that the lanes of `live` name (`row` of a lane, weighted `w`), added up in order at this lane's column: U rows'
+// loads in flight together.
 template <typename T, int VEC, int U>
-__device__ __forceinline__ void sum_rows(const T* __restrict__ base, i64 ld, int col, int have, u64 live, int row, float w,
+__device__ __forceinline__ void sum_rows(const T* __restrict__ base, i64 ld, int col, u64 live, int row, float w,
                                          Acc<T, VEC>& acc) {
     while (live) {
         int at[U];
@@ -70,11 +82,11 @@ __device__ __forceinline__ void sum_rows(const T* __restrict__ base, i64 ld, int
         for (int u = 0; u < U; ++u) {
             at[u] = live ? __builtin_ctzll(live) : -1;
             live &= live - 1;
-            if (at[u] >= 0 && have > 0) p[u].load(base + (i64)(u32)lane_i(row, at[u]) * ld + col, have);
+            if (at[u] >= 0) p[u].load(base + (i64)(u32)lane_i(row, at[u]) * ld + col);
         }
 #pragma unroll
         for (int u = 0; u < U; ++u)
-            if (at[u] >= 0 && have > 0) acc.add(p[u], lane_f(w, at[u]));
+            if (at[u] >= 0) acc.add(p[u], lane_f(w, at[u]));
     }
 }
 
@@ -85,8 +97,7 @@ __global__ __launch_bounds__(256) void embed_rows_k(const Rows r, const T* __res
     const i64 items = r.n * chunks, step = (i64)gridDim.x * 4;
     for (i64 it = (i64)blockIdx.x * 4 + (threadIdx.x >> 6); it < items; it += step) {
         const i64 n = it / chunks;
-        const int col = ((int)(it - n * chunks) * 64 + lane_id()) * VEC;
-        const int have = dim - col;
+        const Cols<VEC> col((int)(it - n * chunks) * 64 + lane_id(), dim);
         Acc<T, VEC> acc;
         acc.zero();
         bool bad = false;
@@ -100,12 +111,12 @@ __global__ __launch_bounds__(256) void embed_rows_k(const Rows r, const T* __res
             }
             const bool out_of = (u64)tok >= (u64)r.V;
             bad |= __ballot(out_of && w != 0.f) != 0;
-            sum_rows<T, VEC, 8>(table, ld, col, have, __ballot(w != 0.f && !out_of), (int)tok, w, acc);
+            sum_rows<T, VEC, 4>(table, ld, col.at, __ballot(w != 0.f && !out_of), (int)tok, w, acc);
         }
         if (bad)
 #pragma unroll
             for (int j = 0; j < VEC; ++j) acc.v[j] = __builtin_nanf("");
-        if (have > 0) acc.store(out + n * dim + col, have, scale);
+        if (col.in) acc.store(out + n * dim + col.at, scale);
     }
 }
 
@@ -125,8 +136,7 @@ __global__ __launch_bounds__(256) void embed_tokens_k(const Rows r, const T* __r
                 const i64 n = i / per;
                 const i64 tok = int_at(r.tokens, r.tsize, n);
                 ok[u] = (u64)tok < (u64)r.V;
-                const int col = (int)(i - n * per) * VEC;
-                if (ok[u]) p[u].load(table + tok * ld + col, dim - col);
+                if (ok[u]) p[u].load(table + tok * ld + Cols<VEC>((int)(i - n * per), dim).at);
             }
         }
 #pragma unroll
@@ -140,8 +150,7 @@ __global__ __launch_bounds__(256) void embed_tokens_k(const Rows r, const T* __r
                 else
 #pragma unroll
                     for (int j = 0; j < VEC; ++j) acc.v[j] = __builtin_nanf("");
-                const int col = (int)(i - n * per) * VEC;
-                acc.store(out + n * dim + col, dim - col, scale);
+                acc.store(out + n * dim + Cols<VEC>((int)(i - n * per), dim).at, scale);
             }
         }
     }
@@ -420,7 +429,7 @@ __global__ __launch_bounds__(256) void embed_runs_k(const u64* __restrict__ list
         const u32 c0 = (u32)(c * CHUNK);
         if (c0 >= M) return;
         const int last = M - c0 < CHUNK ? (int)(M - c0) - 1 : CHUNK - 1;
-        const int col = ((int)(it - c * chunks) * 64 + lane_id()) * VEC, have = dim - col;
+        const Cols<VEC> col((int)(it - c * chunks) * 64 + lane_id(), dim);
         const u32 i = c0 + (lane_id() < last ? lane_id() : last);
         const u64 word = list[i];
         const u32 tok = (u32)(word >> 32), before = i ? (u32)(list[i - 1] >> 32) : ~0u, after = i + 1 < M ? (u32)(list[i + 1] >> 32) : ~0u;
@@ -435,18 +444,19 @@ __global__ __launch_bounds__(256) void embed_runs_k(const u64* __restrict__ list
             Pack<T, VEC> r[U];
 #pragma unroll
             for (int u = 0; u < U; ++u)
-                if (l0 + u <= last && have > 0) r[u].load(dout + (i64)(u32)lane_i(n, l0 + u) * ld + col, have);
+                if (l0 + u <= last) r[u].load(dout + (i64)(u32)lane_i(n, l0 + u) * ld + col.at);
 #pragma unroll
             for (int u = 0; u < U; ++u) {
                 const int l = l0 + u;
                 if (l > last) break;
-                if (have > 0) acc.add(r[u], lane_f(x, l));
+                acc.add(r[u], lane_f(x, l));
                 if (ends >> l & 1) {
                     if ((first && from) || (l == last && on)) {
-                        float* o = part + ((2 * c + (first ? 0 : 1)) * chunks * 64) * VEC + col;
+                        Pack<float, VEC> o;
 #pragma unroll
-                        for (int j = 0; j < VEC; ++j) o[j] = acc.v[j];
-                    } else if (have > 0) acc.store(grad + (i64)(u32)lane_i((int)tok, l) * dim + col, have, scale);
+                        for (int j = 0; j < VEC; ++j) o.v[j] = acc.v[j];
+                        if (col.in) o.store(part + (2 * c + (first ? 0 : 1)) * dim + col.at);
+                    } else if (col.in) acc.store(grad + (i64)(u32)lane_i((int)tok, l) * dim + col.at, scale);
                     acc.zero();
                     first = false;
                 }
@@ -464,7 +474,7 @@ __global__ __launch_bounds__(512) void embed_join_k(const u64* __restrict__ list
     constexpr int U = 8;
     __shared__ float sums[8][64 * VEC];
     const u32 M = *count;
-    const i64 items = spans * chunks, row = (i64)chunks * 64 * VEC;
+    const i64 items = spans * chunks;
     const int wave = threadIdx.x >> 6;
     for (i64 it = blockIdx.x; it < items; it += gridDim.x) {
         const i64 c = it / chunks;
@@ -473,7 +483,7 @@ __global__ __launch_bounds__(512) void embed_join_k(const u64* __restrict__ list
         const u32 c1 = M - c0 < CHUNK ? M : c0 + CHUNK;
         const u32 t = (u32)(list[c1 - 1] >> 32), s = start[t], e = start[t + 1];
         if (e <= c1 || s < c0) continue;
-        const int col = ((int)(it - c * chunks) * 64 + lane_id()) * VEC;
+        const Cols<VEC> col((int)(it - c * chunks) * 64 + lane_id(), dim);
         const i64 end = (e - 1) / CHUNK;
         float acc[VEC];
 #pragma unroll
@@ -483,7 +493,7 @@ __global__ __launch_bounds__(512) void embed_join_k(const u64* __restrict__ list
 #pragma unroll
             for (int u = 0; u < U; ++u) {
                 const i64 q = k + 8 * u;
-                if (q <= end) x[u].load(part + (2 * q + (q == c && s != c0 ? 1 : 0)) * row + col);
+                if (q <= end) x[u].load(part + (2 * q + (q == c && s != c0 ? 1 : 0)) * dim + col.at);
             }
 #pragma unroll
             for (int u = 0; u < U; ++u)
@@ -495,7 +505,7 @@ __global__ __launch_bounds__(512) void embed_join_k(const u64* __restrict__ list
 #pragma unroll
         for (int j = 0; j < VEC; ++j) sums[wave][j * 64 + lane_id()] = acc[j];
         __syncthreads();
-        if (wave == 0 && col < dim) {
+        if (wave == 0 && col.in) {
             Acc<T, VEC> r;
 #pragma unroll
             for (int j = 0; j < VEC; ++j) {
@@ -503,7 +513,7 @@ __global__ __launch_bounds__(512) void embed_join_k(const u64* __restrict__ list
 #pragma unroll
                 for (int k = 1; k < 8; ++k) r.v[j] += sums[k][j * 64 + lane_id()];
             }
-            r.store(grad + t * (i64)dim + col, dim - col, scale);
+            r.store(grad + t * (i64)dim + col.at, scale);
         }
     }
 }
@@ -515,11 +525,10 @@ __global__ __launch_bounds__(256) void embed_zero_k(const u32* __restrict__ star
     for (i64 i = (i64)blockIdx.x * 256 + threadIdx.x; i < items; i += (i64)gridDim.x * 256) {
         const i64 v = i / per;
         if (start[v] != start[v + 1]) continue;
-        const int col = (int)(i - v * per) * VEC;
         Pack<T, VEC> z;
 #pragma unroll
         for (int j = 0; j < VEC; ++j) z.v[j] = (T)0.f;
-        z.store(grad + v * dim + col, dim - col);
+        z.store(grad + v * dim + Cols<VEC>((int)(i - v * per), dim).at);
     }
 }
 
@@ -548,17 +557,21 @@ __global__ __launch_bounds__(256) void embed_dw_k(const Rows r, const T* __restr
                     live &= live - 1;
                     dot[u] = 0.f;
                 }
-                for (int col = lane_id() * VEC; col < dim; col += 64 * VEC) {
+                for (int k = 0; k * 64 * VEC < dim; ++k) {
+                    const Cols<VEC> col(k * 64 + lane_id(), dim);
                     Pack<T, VEC> d, p[8];
-                    d.load(dout + n * dld + col, dim - col);
+                    d.load(dout + n * dld + col.at);
 #pragma unroll
                     for (int u = 0; u < 8; ++u)
-                        if (at[u] >= 0) p[u].load(table + (i64)(u32)lane_i((int)tok, at[u]) * ld + col, dim - col);
+                        if (at[u] >= 0) p[u].load(table + (i64)(u32)lane_i((int)tok, at[u]) * ld + col.at);
+                    float f[VEC];
+#pragma unroll
+                    for (int j = 0; j < VEC; ++j) f[j] = j < col.again ? 0.f : (float)d.v[j];
 #pragma unroll
                     for (int u = 0; u < 8; ++u)
                         if (at[u] >= 0)
 #pragma unroll
-                            for (int k = 0; k < VEC; ++k) dot[u] = fmaf((float)d.v[k], (float)p[u].v[k], dot[u]);
+                            for (int j = 0; j < VEC; ++j) dot[u] = j < col.again ? dot[u] : fmaf(f[j], (float)p[u].v[j], dot[u]);
                 }
 #pragma unroll
                 for (int u = 0; u < 8; ++u) {
@@ -590,7 +603,7 @@ static inline int wave_grid(i64 waves) {
 // without work.
 template <typename T> static int vec_of(int dim, int lanes = 32) {
     int v = 16 / (int)sizeof(T);
-    while (v > 1 && (dim + v - 1) / v <= lanes) v >>= 1;
+    while (v > 1 && ((dim + v - 1) / v <= lanes || dim < v)) v >>= 1;
     return v;
 }
 
@@ -641,7 +654,7 @@ struct GradWork {
         la = (u64*)take(8 * M), lb = (u64*)take(M > ONE ? 8 * M : 0);
         hist = (u32*)take(1024ll * tiles), total = (u32*)take(1024), count = (u32*)take(4);
         start = (u32*)take(4 * (V + 1));
-        part = (float*)take(M > CHUNK ? (M + CHUNK - 1) / CHUNK * 2 * ((dim + 511) / 512 * 512) * 4 : 0);  // 64 * VEC columns or more
+        part = (float*)take(M > CHUNK ? (M + CHUNK - 1) / CHUNK * 2 * dim * 4 : 0);
         bytes = p - (char*)base;
     }
 };

@@ -29,20 +29,6 @@ template <typename T, int N> struct Pack {
         __builtin_memcpy(&r, v, sizeof(raw));
         *(raw*)p = r;
     }
-    // of a row of `have` elements from p on
-    __device__ __forceinline__ void load(const T* p, int have) {
-        if (have >= N) load(p);
-        else
-#pragma unroll
-            for (int j = 0; j < N; ++j) v[j] = j < have ? p[j] : (T)0.f;
-    }
-    __device__ __forceinline__ void store(T* p, int have) const {
-        if (have >= N) store(p);
-        else
-#pragma unroll
-            for (int j = 0; j < N; ++j)
-                if (j < have) p[j] = v[j];
-    }
 };
 
 __device__ __forceinline__ bool finite_f(float x) { return __builtin_fabsf(x) < __builtin_inff(); }  // false for NaN
