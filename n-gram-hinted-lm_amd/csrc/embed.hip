@@ -695,7 +695,7 @@ static int embed_grad(const Rows& r, const T* dout, i64 ld, int dim, float scale
             embed_runs_k<T, VEC><<<wave_grid(items), 256, 0, st>>>(list, g.count, r.w, r.m, dout, ld, dim, chunks, scale, spans,
                                                                    g.part, grad);
         if (M > CHUNK)
-            embed_join_k<T, VEC><<<(int)(items < 65536 ? items : 65536), 512, 0, st>>>(list, g.count, g.start, dim, chunks, spans,
+            embed_join_k<T, VEC><<<(int)(items < 2048 ? items : 2048), 512, 0, st>>>(list, g.count, g.start, dim, chunks, spans,
                                                                                        scale, g.part, grad);
         return (int)hipGetLastError();
     });

@@ -40,8 +40,12 @@ struct TreePlan {
 // the launches for one cache type
 template <int CODES> int tree_codes(const TreeArgs& a, const TreePlan& p, hipStream_t st);
 
+// A sequence's cached tokens, tree tokens, both, its tiles, and its units' span on the line: a unit costs its tiles and
+// START more, what its beginning and end take (queries, masks, the waves' joining) in tiles' time: a share of many short
+// units would else be a long one.
+#define START 3
 struct Seq {
-    int len, w, n, tiles;
+    int len, w, n, tiles, span;
 };
 
 __device__ __forceinline__ Seq seq_of(const TreeArgs& a, int b) {
@@ -53,12 +57,14 @@ __device__ __forceinline__ Seq seq_of(const TreeArgs& a, int b) {
     const i64 n = (i64)s.len + s.w;
     s.n = (int)(n < cap ? n : cap);
     s.tiles = s.n > 0 ? (s.n + TILE - 1) / TILE : 1;
+    s.span = s.tiles + START;
     return s;
 }
 
 __device__ __forceinline__ Seq uniform(Seq s) {
     s.len = __builtin_amdgcn_readfirstlane(s.len), s.w = __builtin_amdgcn_readfirstlane(s.w);
     s.n = __builtin_amdgcn_readfirstlane(s.n), s.tiles = __builtin_amdgcn_readfirstlane(s.tiles);
+    s.span = s.tiles + START;
     return s;
 }
 
@@ -71,55 +77,55 @@ __device__ __forceinline__ int scan_wave(int x) {  // inclusive sum over the lan
     return x;
 }
 
-// The work laid end to end: sequence by sequence, in each its units (kv head, group of rows), in each its tiles. A share is
-// `per` tiles. Each wave finds its place by itself: one load and one scan for 64 sequences.
+// The work laid end to end: sequence by sequence, in each its units (kv head, group of rows), in each its span. A share is
+// `per` places. Each wave finds its place by itself: one load and one scan for 64 sequences.
 struct Line {
     Seq mine;  // of sequence lane_id()
-    int inc;   // tiles up to and with it
+    int inc;   // places up to and with it
     int total, per, shares;
 
     __device__ __forceinline__ Line(const TreeArgs& a, int blocks) {
         const int units = a.H * a.groups;
         const int b = lane_id() < a.B ? lane_id() : a.B - 1;
         mine = seq_of(a, b);
-        inc = scan_wave(lane_id() < a.B ? mine.tiles * units : 0);
+        inc = scan_wave(lane_id() < a.B ? mine.span * units : 0);
         total = lane(inc, 63);
         for (int b0 = 64; b0 < a.B; b0 += 64) {
-            int t = b0 + lane_id() < a.B ? seq_of(a, b0 + lane_id()).tiles * units : 0;
+            int t = b0 + lane_id() < a.B ? seq_of(a, b0 + lane_id()).span * units : 0;
             total += lane(scan_wave(t), 63);
         }
         per = (total + blocks - 1) / blocks;
         shares = (total + per - 1) / per;
     }
 
-    // the sequence that holds tile x < total, and the tiles before it
+    // the sequence that holds place x < total, and the places before it
     __device__ __forceinline__ int at(const TreeArgs& a, int x, int& before, Seq& q) const {
         const int units = a.H * a.groups;
         u64 past = __ballot(inc > x);
         if (past) {
             const int l = __builtin_ctzll(past);
-            q.len = lane(mine.len, l), q.w = lane(mine.w, l), q.n = lane(mine.n, l), q.tiles = lane(mine.tiles, l);
-            before = lane(inc, l) - q.tiles * units;
+            q = pick(mine, l);
+            before = lane(inc, l) - q.span * units;
             return l;
         }
         int run = lane(inc, 63);
         for (int b0 = 64;; b0 += 64) {
             Seq s;
-            s.len = s.w = s.n = s.tiles = 0;
+            s.len = s.w = s.n = s.tiles = s.span = 0;
             if (b0 + lane_id() < a.B) s = seq_of(a, b0 + lane_id());
-            const int i = scan_wave(s.tiles * units);
+            const int i = scan_wave(s.span * units);
             past = __ballot(run + i > x);
             if (past || b0 + 64 >= a.B) {
                 const int l = past ? __builtin_ctzll(past) : 63;
-                q.len = lane(s.len, l), q.w = lane(s.w, l), q.n = lane(s.n, l), q.tiles = lane(s.tiles, l);
-                before = run + lane(i, l) - q.tiles * units;
+                q = pick(s, l);
+                before = run + lane(i, l) - q.span * units;
                 return b0 + l;
             }
             run += lane(i, 63);
         }
     }
 
-    // the tiles before sequence b
+    // the places before sequence b
     __device__ __forceinline__ int before(const TreeArgs& a, int b, Seq& q) const {
         const int units = a.H * a.groups;
         int run = 0;
@@ -127,17 +133,22 @@ struct Line {
             Seq s = mine;
             int i = inc;
             if (b0) {
-                s.len = s.w = s.n = s.tiles = 0;
+                s.len = s.w = s.n = s.tiles = s.span = 0;
                 if (b0 + lane_id() < a.B) s = seq_of(a, b0 + lane_id());
-                i = scan_wave(s.tiles * units);
+                i = scan_wave(s.span * units);
             }
             if (b < b0 + 64) {
                 const int l = b - b0;
-                q.len = lane(s.len, l), q.w = lane(s.w, l), q.n = lane(s.n, l), q.tiles = lane(s.tiles, l);
-                return run + lane(i, l) - q.tiles * units;
+                q = pick(s, l);
+                return run + lane(i, l) - q.span * units;
             }
             run += lane(i, 63);
         }
+    }
+    static __device__ __forceinline__ Seq pick(const Seq& s, int l) {
+        Seq q;
+        q.len = lane(s.len, l), q.w = lane(s.w, l), q.n = lane(s.n, l), q.tiles = lane(s.tiles, l), q.span = q.tiles + START;
+        return q;
     }
     static __device__ __forceinline__ int lane(int x, int l) { return __builtin_amdgcn_readlane(x, l); }
 };
@@ -289,8 +300,15 @@ template <int CODES, int DP, int R> struct Tree {
 
     // The block's query rows, through LDS: each read once, for 8-bit caches scaled by the power of two that puts their
     // largest element at 2^14 .. 2^15. top: 4 floats.
-    static __device__ __forceinline__ void load_q(const TreeArgs& a, int b, int head, int row0, T* lds, float* topl, State& s) {
+    // bits: the tree tokens that each row sees.
+    static __device__ __forceinline__ void load_q(const TreeArgs& a, int b, int head, const Seq& q, int row0, T* lds, float* topl,
+                                                  u64* bits, State& s) {
         const int c = lane_id() & 15, g = lane_id() >> 4, rows = a.T * a.G;
+        u64 seen = 0;
+        if (threadIdx.x < 16 * R) {
+            const int t = (row0 + threadIdx.x) / a.G;
+            if (t < q.w) seen = a.mask ? a.mask[(i64)b * a.T + t] : (2ull << t) - 1;
+        }
         union Eight {
             uint4 w;
             u16 e[8];
@@ -323,6 +341,7 @@ template <int CODES, int DP, int R> struct Tree {
             if (lane_id() == 0) topl[threadIdx.x >> 6] = top;
         }
         lds_barrier();  // what LDS held before has been read, too
+        if (threadIdx.x < 16 * R) bits[threadIdx.x] = seen;
         if constexpr (Q8) {
             top = fmaxf(fmaxf(topl[0], topl[1]), fmaxf(topl[2], topl[3]));
             if (top > 0.f) {
@@ -405,12 +424,6 @@ template <int CODES, int DP, int R> struct Tree {
         for (int i = 0; i < 8; ++i) load_words<VW>(v + i * DP * ES, f.v[i]);
     }
 
-    // the tree tokens that a row sees
-    static __device__ __forceinline__ u64 bits_of(const TreeArgs& a, int b, const Seq& q, int row) {
-        const int t = row / a.G;
-        if (t >= q.w) return 0;
-        return a.mask ? a.mask[(i64)b * a.T + t] : (2ull << t) - 1;
-    }
 
     // Values of a 16-bit cache that are not finite, in keys that only some rows see: they are 0 in the product (a masked
     // key's P of 0 would make NaN of them) and are added here to the rows that do see them.
@@ -427,7 +440,7 @@ template <int CODES, int DP, int R> struct Tree {
             }
         return bad;
     }
-    static __device__ __forceinline__ void put_back(const TreeArgs& a, int b, const Seq& q, int base, int row0, const Values& f,
+    static __device__ __forceinline__ void put_back(const TreeArgs& a, const Seq& q, int base, const u64* bits, const Values& f,
                                                     u32 bad, const V8 (&p)[R], State& s) {
         const int c = lane_id() & 15, g = lane_id() >> 4;
         for (int from = 0; from < 4; ++from) {
@@ -440,7 +453,7 @@ template <int CODES, int DP, int R> struct Tree {
 #pragma unroll
                 for (int r = 0; r < R; ++r) {
                     const float w = __shfl((float)p[r][i], from * 16 + c, 64);
-                    const bool sees = j0 < 0 || (bits_of(a, b, q, row0 + r * 16 + c) >> j0 & 1);
+                    const bool sees = j0 < 0 || (bits[r * 16 + c] >> j0 & 1);
 #pragma unroll
                     for (int j = 0; j < NJ; ++j)
 #pragma unroll
@@ -571,8 +584,8 @@ template <int CODES, int DP, int R> struct Tree {
 
     // This wave's keys from base up to stop, a tile of 32 in every TILE; the first one's loads are under way. Only its last
     // tile can hold keys past the cached tokens: the tree and the rest of a tile before it are at most 3 tiles in a row.
-    static __device__ __forceinline__ void keys(const TreeArgs& a, int b, int head, const Seq& q, int base, int stop, int row0,
-                                                Run& w, State& s, float (*fac)[32]) {
+    static __device__ __forceinline__ void keys(const TreeArgs& a, int b, int head, const Seq& q, int base, int stop,
+                                                const u64* bits, Run& w, State& s, float (*fac)[32]) {
         if (base >= stop) return;
         const int g = lane_id() >> 4;
         const int* tab = a.table + (i64)b * a.table_stride;
@@ -606,12 +619,12 @@ template <int CODES, int DP, int R> struct Tree {
             fetch_values(a, head, nb, pg, w.v);
             base += TILE;
         } while (base < whole);
-        if (base < stop) any_tile(a, b, head, q, base, row0, w, s, fac);
+        if (base < stop) any_tile(a, q, base, bits, w, s, fac);
     }
 
     // A tile with keys that some row does not see.
-    static __device__ __forceinline__ void any_tile(const TreeArgs& a, int b, int head, const Seq& q, int base, int row0, Run& w,
-                                                    State& s, float (*fac)[32]) {
+    static __device__ __forceinline__ void any_tile(const TreeArgs& a, const Seq& q, int base, const u64* bits, Run& w, State& s,
+                                                    float (*fac)[32]) {
         const int c = lane_id() & 15, g = lane_id() >> 4;
         f4 sc[R][2];
         V8 p[R];
@@ -632,8 +645,8 @@ template <int CODES, int DP, int R> struct Tree {
         if constexpr (!Q8) bad = take_out(w.v);
 #pragma unroll
         for (int r = 0; r < R; ++r) {
-            const u64 bits = bits_of(a, b, q, row0 + r * 16 + c);
-            const u32 tree = j0 >= 64 || j0 <= -8 ? 0u : j0 >= 0 ? (u32)(bits >> j0) : (u32)(bits << -j0);
+            const u64 see = bits[r * 16 + c];
+            const u32 tree = j0 >= 64 || j0 <= -8 ? 0u : j0 >= 0 ? (u32)(see >> j0) : (u32)(see << -j0);
             const u32 sees = in & (cached | tree);
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
@@ -645,7 +658,7 @@ template <int CODES, int DP, int R> struct Tree {
         weights(sc, rv, p, s);
         values(w.v, p, s);
         if constexpr (!Q8)
-            if (__any(bad != 0)) put_back(a, b, q, base, row0, w.v, bad, p, s);
+            if (__any(bad != 0)) put_back(a, q, base, bits, w.v, bad, p, s);
     }
 };
 
@@ -659,6 +672,7 @@ __global__ __launch_bounds__(256, (tree_waves<CODES, DP, R>())) void tree_k(cons
     __shared__ __align__(16) char lds[sizeof(Lo) * 4 > 16 * R * W::QLD * 2 ? sizeof(Lo) * 4 : 16 * R * W::QLD * 2];
     Lo* lo = (Lo*)lds;  // the waves' sums at a unit's end; before that the queries
     __shared__ float lm[4][16], ll[4][16], topl[4];
+    __shared__ u64 bits[16 * R];
     __shared__ __align__(16) float fac[4][3][32];
     const Line line(a, blocks);
     // neighbouring shares on one XCD (blocks go round the 8 XCDs): units that share keys meet in its L2
@@ -672,25 +686,28 @@ __global__ __launch_bounds__(256, (tree_waves<CODES, DP, R>())) void tree_k(cons
     Seq q;
     int b = line.at(a, x, before, q);
     while (x < end) {
-        while (x - before >= q.tiles * units) {
-            before += q.tiles * units;
+        while (x - before >= q.span * units) {
+            before += q.span * units;
             q = uniform(seq_of(a, ++b));
         }
-        const int unit = (x - before) / q.tiles, t0 = x - before - unit * q.tiles;
-        const int t1 = end - x < q.tiles - t0 ? t0 + (end - x) : q.tiles;
+        const int unit = (x - before) / q.span, from = x - before - unit * q.span;
+        const int to = end - x < q.span - from ? from + (end - x) : q.span;
+        const int t0 = from > START ? from - START : 0, t1 = to - START;
+        x += to - from;
+        if (t1 <= t0) continue;
         const int head = unit / a.groups, row0 = (unit - head * a.groups) * 16 * R;
         const int base = t0 * TILE + wave * 32, stop = t1 * TILE < q.n ? t1 * TILE : q.n;
         typename W::State s;
         typename W::Run run;
         W::begin(a, b, head, base, stop, run);
-        W::load_q(a, b, head, row0, (typename W::T*)lds, topl, s);
+        W::load_q(a, b, head, q, row0, (typename W::T*)lds, topl, bits, s);
 #pragma unroll
         for (int r = 0; r < R; ++r) {
             s.m[r] = -__builtin_inff(), s.l[r] = 0.f;
 #pragma unroll
             for (int j = 0; j < W::NJ; ++j) s.o[r][j] = f4{0.f, 0.f, 0.f, 0.f};
         }
-        W::keys(a, b, head, q, base, stop, row0, run, s, fac[wave]);
+        W::keys(a, b, head, q, base, stop, bits, run, s, fac[wave]);
         const bool all = t0 == 0 && t1 == q.tiles;
         const i64 slot = 2 * me + (t0 == 0 ? 1 : 0);
 #pragma unroll
@@ -737,7 +754,6 @@ __global__ __launch_bounds__(256, (tree_waves<CODES, DP, R>())) void tree_k(cons
                 if ((threadIdx.x & 15) == 0) a.pm[prow] = m, a.pl[prow] = sum;
             }
         }
-        x += t1 - t0;
     }
 }
 
@@ -748,8 +764,8 @@ template <int DP> __global__ __launch_bounds__(256) void tree_join_k(const TreeA
     const int per = a.H * a.groups, b = u / per, unit = u - b * per;
     const Line line(a, blocks);
     Seq q;
-    const int x0 = line.before(a, b, q) + unit * q.tiles, x1 = x0 + q.tiles;
-    const int i0 = x0 / line.per, i1 = (x1 - 1) / line.per;
+    const int x0 = line.before(a, b, q) + unit * q.span;
+    const int i0 = (x0 + START) / line.per, i1 = (x0 + q.span - 1) / line.per;  // the shares of its first and last tile
     if (i0 == i1) return;
     const int head = unit / a.groups, row0 = (unit - head * a.groups) * rpb;
     const int row = threadIdx.x >> 4, d0 = (threadIdx.x & 15) * NJ;

@@ -48,7 +48,7 @@ static bool tree_plan(int B, int T, int H, int G, int dim, int codes, i64 cap, T
     const int rows = T * G;
     p.rpb = rows <= 16 ? 16 : 32;
     p.groups = (rows + p.rpb - 1) / p.rpb;
-    const i64 units = (i64)B * H * p.groups, most = units * ((cap + TILE - 1) / TILE);
+    const i64 units = (i64)B * H * p.groups, most = units * ((cap + TILE - 1) / TILE + START);
     if (units > 1 << 24 || most > (i64)1 << 30) return false;
     p.blocks = most < MAX_BLOCKS ? (int)(most + 7) / 8 * 8 : MAX_BLOCKS;
     p.join = cap > TILE;
