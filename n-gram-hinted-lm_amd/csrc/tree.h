@@ -292,18 +292,29 @@ template <int CODES, int DP, int R> struct Tree {
         const T* ql;  // the queries in LDS, at this lane's row and quarter
         f4 o[R][NJ];
         float m[R], l[R], off[R];
-        float c;  // scale * log2(e) / the queries' power of two
+        float c;  // the scores' factor: scale * log2(e) / the queries' power of two (own: without powers of two)
     };
+
+    // A block's rows' largest elements (as bits: the largest of floats >= 0), zero between units, and their shifts.
+    struct Sizes {
+        u32 top[16 * R];
+        int shift[16 * R];
+    };
+    static constexpr int APART = 8;  // rows whose largest elements lie within 2^APART share one power of two
 
     static constexpr int QLD = DP + 8;                    // a query row in LDS (16 rows' reads meet no bank twice)
     static constexpr int NQ = (16 * R * DP / 8 + 255) / 256;  // groups of 8 query elements a thread brings
 
-    // The block's query rows, through LDS: each read once, for 8-bit caches scaled by the power of two that puts their
-    // largest element at 2^14 .. 2^15. top: 4 floats.
-    // bits: the tree tokens that each row sees.
-    static __device__ __forceinline__ void load_q(const TreeArgs& a, int b, int head, const Seq& q, int row0, T* lds, float* topl,
+    // The block's query rows in use, through LDS: each read once; a row past the tree's width is zeros, whatever it holds.
+    // For 8-bit caches the products run on f16: rows are scaled by the power of two that puts their largest finite element
+    // at 2^14 .. 2^15. Rows of about one size share it, the largest's (an element then keeps its bits down to 2^-22 of its
+    // own row's largest, and is off by 2^-31 of that below); where a row is over 2^APART smaller than another, or their size
+    // is far from 1 (its power of two times the scale or a key's scale could overflow), each has its own, and its scores
+    // take one more operation. bits: the tree tokens that each row sees.
+    // Returns whether each row has its own power of two (a score then takes 2^shift[row]).
+    static __device__ __forceinline__ bool load_q(const TreeArgs& a, int b, int head, const Seq& q, int row0, T* lds, Sizes& size,
                                                   u64* bits, State& s) {
-        const int c = lane_id() & 15, g = lane_id() >> 4, rows = a.T * a.G;
+        const int c = lane_id() & 15, g = lane_id() >> 4;
         u64 seen = 0;
         if (threadIdx.x < 16 * R) {
             const int t = (row0 + threadIdx.x) / a.G;
@@ -313,43 +324,54 @@ template <int CODES, int DP, int R> struct Tree {
             uint4 w;
             u16 e[8];
         } x[NQ];
-        float top = 0.f;
 #pragma unroll
         for (int k = 0; k < NQ; ++k) {
             const int i = threadIdx.x + 256 * k, row = row0 + i / (DP / 8), d0 = i % (DP / 8) * 8;
             const int t = row / a.G, h = row - t * a.G;
             const u16* p = (const u16*)a.q + b * a.qb + t * a.qt + (i64)(head * a.G + h) * a.qh + d0;
             x[k].w = make_uint4(0, 0, 0, 0);
-            if (i < 16 * R * DP / 8 && row < rows) {
+            if (i < 16 * R * DP / 8 && t < q.w) {
                 if (a.vec && d0 + 8 <= a.dim) x[k].w = *(const uint4*)p;
                 else
                     for (int j = 0; j < 8; ++j)
                         if (d0 + j < a.dim) x[k].e[j] = p[j];
             }
-            if constexpr (Q8)
+        }
+        if constexpr (Q8)
+#pragma unroll
+            for (int k = 0; k < NQ; ++k) {  // (apart from the loads, which are all asked for first)
+                const int i = threadIdx.x + 256 * k;
+                float top = 0.f;
 #pragma unroll
                 for (int j = 0; j < 8; ++j) {
                     const float f = __builtin_fabsf(value(a, x[k].e[j]));
                     top = finite_f(f) ? fmaxf(top, f) : top;
                 }
-        }
-        float up = 1.f;
-        s.c = a.scale * LOG2E;
-        if constexpr (Q8) {
-#pragma unroll
-            for (int o = 32; o; o >>= 1) top = fmaxf(top, __shfl_xor(top, o, 64));
-            if (lane_id() == 0) topl[threadIdx.x >> 6] = top;
-        }
+                if (i < 16 * R * DP / 8) atomicMax(&size.top[i / (DP / 8)], __float_as_uint(top));
+            }
         lds_barrier();  // what LDS held before has been read, too
         if (threadIdx.x < 16 * R) bits[threadIdx.x] = seen;
+        s.c = a.scale * LOG2E;
+        bool own = false;
+        int up = 0;  // the shared power of two
         if constexpr (Q8) {
-            top = fmaxf(fmaxf(topl[0], topl[1]), fmaxf(topl[2], topl[3]));
-            if (top > 0.f) {
-                int e = 15 - __builtin_amdgcn_frexp_expf(top);
-                e = e > 100 ? 100 : e;
-                up = __builtin_amdgcn_ldexpf(1.f, e);
-                s.c *= __builtin_amdgcn_ldexpf(1.f, -e);
+            u32 hi = size.top[lane_id() & (16 * R - 1)], lo = hi ? hi : ~0u;
+#pragma unroll
+            for (int o = 8 * R; o; o >>= 1) {
+                const u32 h = (u32)__shfl_xor((int)hi, o, 64), l = (u32)__shfl_xor((int)lo, o, 64);
+                hi = h > hi ? h : hi, lo = l < lo ? l : lo;
             }
+            hi = __builtin_amdgcn_readfirstlane(hi), lo = __builtin_amdgcn_readfirstlane(lo);
+            if (hi) {
+                const int eh = __builtin_amdgcn_frexp_expf(__uint_as_float(hi));
+                own = eh - __builtin_amdgcn_frexp_expf(__uint_as_float(lo)) > APART || eh > 40 || eh < -40;
+                up = 15 - eh;
+            }
+            if (own) {
+                if (threadIdx.x < 16 * R)
+                    size.shift[threadIdx.x] = __builtin_amdgcn_frexp_expf(s.c) - up_of(size.top[threadIdx.x]);
+                s.c = __builtin_amdgcn_frexp_mantf(s.c);
+            } else s.c = __builtin_amdgcn_ldexpf(s.c, -up);
             s.c *= K_UP;
         }
 #pragma unroll
@@ -360,14 +382,17 @@ template <int CODES, int DP, int R> struct Tree {
                     T e[8];
                     uint4 w;
                 } y;
-                if constexpr (Q8)
+                if constexpr (Q8) {
+                    if (own) up = up_of(size.top[i / (DP / 8)]);
 #pragma unroll
-                    for (int j = 0; j < 8; ++j) y.e[j] = (T)(value(a, x[k].e[j]) * up);
-                else y.w = x[k].w;
+                    for (int j = 0; j < 8; ++j) y.e[j] = (T)__builtin_amdgcn_ldexpf(value(a, x[k].e[j]), up);
+                } else y.w = x[k].w;
                 *(uint4*)(lds + i / (DP / 8) * QLD + i % (DP / 8) * 8) = y.w;
             }
         }
         lds_barrier();
+        if constexpr (Q8)
+            if (threadIdx.x < 16 * R) size.top[threadIdx.x] = 0;  // (the next unit's maxima come after the joining's barriers)
         s.ql = lds + c * QLD + g * (DP / 4);
 #pragma unroll
         for (int r = 0; r < R; ++r) {
@@ -382,6 +407,11 @@ template <int CODES, int DP, int R> struct Tree {
             }
             s.off[r] = CODES == KV_INT8 ? -128.f / K_UP * sum_quarters(sum) : 0.f;
         }
+        return own;
+    }
+    // the power of two that puts a row's largest element at 2^14 .. 2^15
+    static __device__ __forceinline__ int up_of(u32 top) {
+        return top ? 15 - __builtin_amdgcn_frexp_expf(__uint_as_float(top)) : 0;
     }
     static __device__ __forceinline__ float value(const TreeArgs& a, u16 e) {
         return a.qtype == NG_BF16 ? __uint_as_float((u32)e << 16) : (float)__builtin_bit_cast(f16, e);
@@ -487,8 +517,9 @@ template <int CODES, int DP, int R> struct Tree {
         __builtin_amdgcn_wave_barrier();
     }
 
-    static __device__ __forceinline__ void scores(Keys& k, const State& s, float (*fac)[32], f4 (&sc)[R][2]) {
-        const int g = lane_id() >> 4;
+    static __device__ __forceinline__ void scores(Keys& k, const State& s, const Sizes& size, bool own, float (*fac)[32],
+                                                  f4 (&sc)[R][2]) {
+        const int c = lane_id() & 15, g = lane_id() >> 4;
 #pragma unroll
         for (int r = 0; r < R; ++r) sc[r][0] = sc[r][1] = f4{s.off[r], s.off[r], s.off[r], s.off[r]};
 #pragma unroll
@@ -503,6 +534,15 @@ template <int CODES, int DP, int R> struct Tree {
 #pragma unroll
                 for (int r = 0; r < R; ++r) sc[r][t] = mma(e, x[r], sc[r][t]);
             }
+        }
+        if (Q8 && own) {  // (in this order nothing overflows that the score itself does not)
+#pragma unroll
+            for (int r = 0; r < R; ++r)
+#pragma unroll
+                for (int i = 0; i < 8; ++i)
+                    sc[r][i >> 2][i & 3] = __builtin_amdgcn_ldexpf(sc[r][i >> 2][i & 3] * fac[0][g * 8 + i], size.shift[r * 16 + c]) +
+                                           fac[1][g * 8 + i];
+            return;
         }
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
@@ -585,7 +625,8 @@ template <int CODES, int DP, int R> struct Tree {
     // This wave's keys from base up to stop, a tile of 32 in every TILE; the first one's loads are under way. Only its last
     // tile can hold keys past the cached tokens: the tree and the rest of a tile before it are at most 3 tiles in a row.
     static __device__ __forceinline__ void keys(const TreeArgs& a, int b, int head, const Seq& q, int base, int stop,
-                                                const u64* bits, Run& w, State& s, float (*fac)[32]) {
+                                                const u64* bits, const Sizes& size, bool own, Run& w, State& s,
+                                                float (*fac)[32]) {
         if (base >= stop) return;
         const int g = lane_id() >> 4;
         const int* tab = a.table + (i64)b * a.table_stride;
@@ -596,7 +637,7 @@ template <int CODES, int DP, int R> struct Tree {
             V8 p[R];
             float rv[8];
             if constexpr (Q8) factors(w.k.s, true, s, fac);
-            scores(w.k, s, fac, sc);
+            scores(w.k, s, size, own, fac, sc);
 #pragma unroll
             for (int i = 0; i < 8; ++i) rv[i] = Q8 ? fac[2][g * 8 + i] : 1.f;
             __builtin_amdgcn_wave_barrier();
@@ -619,18 +660,18 @@ template <int CODES, int DP, int R> struct Tree {
             fetch_values(a, head, nb, pg, w.v);
             base += TILE;
         } while (base < whole);
-        if (base < stop) any_tile(a, q, base, bits, w, s, fac);
+        if (base < stop) any_tile(a, q, base, bits, size, own, w, s, fac);
     }
 
     // A tile with keys that some row does not see.
-    static __device__ __forceinline__ void any_tile(const TreeArgs& a, const Seq& q, int base, const u64* bits, Run& w, State& s,
-                                                    float (*fac)[32]) {
+    static __device__ __forceinline__ void any_tile(const TreeArgs& a, const Seq& q, int base, const u64* bits, const Sizes& size,
+                                                    bool own, Run& w, State& s, float (*fac)[32]) {
         const int c = lane_id() & 15, g = lane_id() >> 4;
         f4 sc[R][2];
         V8 p[R];
         float rv[8];
         if constexpr (Q8) factors(w.k.s, base + (lane_id() & 31) < q.n, s, fac);
-        scores(w.k, s, fac, sc);
+        scores(w.k, s, size, own, fac, sc);
 #pragma unroll
         for (int i = 0; i < 8; ++i) rv[i] = Q8 ? fac[2][g * 8 + i] : 1.f;
         __builtin_amdgcn_wave_barrier();
@@ -671,7 +712,8 @@ __global__ __launch_bounds__(256, (tree_waves<CODES, DP, R>())) void tree_k(cons
     typedef float Lo[16][LD];
     __shared__ __align__(16) char lds[sizeof(Lo) * 4 > 16 * R * W::QLD * 2 ? sizeof(Lo) * 4 : 16 * R * W::QLD * 2];
     Lo* lo = (Lo*)lds;  // the waves' sums at a unit's end; before that the queries
-    __shared__ float lm[4][16], ll[4][16], topl[4];
+    __shared__ float lm[4][16], ll[4][16];
+    __shared__ typename W::Sizes size;
     __shared__ u64 bits[16 * R];
     __shared__ __align__(16) float fac[4][3][32];
     const Line line(a, blocks);
@@ -680,6 +722,10 @@ __global__ __launch_bounds__(256, (tree_waves<CODES, DP, R>())) void tree_k(cons
     if ((int)blockIdx.x / 8 >= a8 || me >= line.shares) return;
     // (uniform, and the compiler is to know it: a loop that lanes left one by one would keep two sets of sums)
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), c = lane_id() & 15, g = lane_id() >> 4, units = a.H * a.groups;
+    if constexpr (W::Q8) {
+        if (threadIdx.x < 16 * R) size.top[threadIdx.x] = 0;
+        lds_barrier();
+    }
     int x = me * line.per;
     const int end = line.total - x < line.per ? line.total : x + line.per;
     int before;
@@ -700,14 +746,14 @@ __global__ __launch_bounds__(256, (tree_waves<CODES, DP, R>())) void tree_k(cons
         typename W::State s;
         typename W::Run run;
         W::begin(a, b, head, base, stop, run);
-        W::load_q(a, b, head, q, row0, (typename W::T*)lds, topl, bits, s);
+        const bool own = W::load_q(a, b, head, q, row0, (typename W::T*)lds, size, bits, s);
 #pragma unroll
         for (int r = 0; r < R; ++r) {
             s.m[r] = -__builtin_inff(), s.l[r] = 0.f;
 #pragma unroll
             for (int j = 0; j < W::NJ; ++j) s.o[r][j] = f4{0.f, 0.f, 0.f, 0.f};
         }
-        W::keys(a, b, head, q, base, stop, bits, run, s, fac[wave]);
+        W::keys(a, b, head, q, base, stop, bits, size, own, run, s, fac[wave]);
         const bool all = t0 == 0 && t1 == q.tiles;
         const i64 slot = 2 * me + (t0 == 0 ? 1 : 0);
 #pragma unroll

@@ -337,3 +337,104 @@ def test_refusals(gpu):
               torch.zeros((2, 4), dtype=torch.int32)):
         with pytest.raises(ValueError):
             tree_mask(p)
+
+
+def _rows(got, q, cache, table, lengths, sees, scale=None, lse=None, skip=()):
+    """_check row by row (but those of skip, pairs of tree token and head), for rows whose sizes differ: every bound is the
+    row's own. The weights over 8-bit caches are resolved, a key, to 2^-33 of the largest weighted value (max of p times the
+    value row's largest element), or to 2^-97 times the largest code where a value row of scale below 2^-64 has the largest
+    weight. A row whose scores' error passes 1 has to be the value of its largest score, which then has to lead by more than
+    that error."""
+    B, T, heads, dim = q.shape
+    group = heads // cache.heads
+    scale = 1 / math.sqrt(dim) if scale is None else scale
+    for b in range(B):
+        n0 = int(lengths[b])
+        n = n0 + T
+        k, v, _ = _values(cache, table, b, n)
+        for t in range(T):
+            see = torch.ones(n, dtype=torch.bool)
+            see[n0:] = sees[b, t]
+            for h in range(heads):
+                if (t, h) in skip:
+                    continue
+                kh, vh = k[see, h // group], v[see, h // group]
+                x = q[b, t, h].double()
+                a = (kh @ x) * scale
+                d = (dim + 6) * 2.0**-24 * abs(scale) * float((kh.abs() @ x.abs()).max()) + 2.0**-22
+                z = torch.logsumexp(a, 0)
+                if d < 1:
+                    p = torch.exp(a - z)
+                    e = math.expm1(d)
+                else:
+                    top = a.topk(2).values
+                    assert top[0] - top[1] > 2 * d + 60, "the case: its row has no clear largest score"
+                    p, e = torch.nn.functional.one_hot(a.argmax(), len(a)).double(), 0.0
+                want, A = p @ vh, p @ vh.abs()
+                fine = (p * vh.abs().amax(1)).max() * n * 2.0**-33 + n * 2.0**-88
+                bound = U[q.dtype] * want.abs() + (UP[cache.k.dtype] + 2 * e + (n + 8) * 2.0**-24) * A + fine + (
+                    2.0**-25 if q.dtype == torch.float16 else 2.0**-134)
+                off = (got[b, t, h].double() - want).abs()
+                assert torch.isfinite(got[b, t, h]).all(), (b, t, h)
+                assert (off <= bound).all(), (b, t, h, float((off - bound).max()), float(off.max()), float(want.abs().max()))
+                if lse is not None:
+                    zb = d + (n + 8) * 2.0**-24 + 2.0**-22 * (abs(float(z)) + 16)
+                    assert abs(float(lse[b, t, h]) - float(z)) <= zb, (b, t, h, float(lse[b, t, h]), float(z), zb)
+
+
+def _chain(B, T):
+    return torch.tril(torch.ones(T, T, dtype=torch.bool)).expand(B, T, T)
+
+
+@pytest.mark.parametrize("codes,dtype", [("int8", torch.bfloat16), ("fp8", torch.bfloat16), ("int8", torch.float16),
+                                         ("fp16", torch.float16)])
+@pytest.mark.parametrize("T,group,dim", [(5, 3, 64), (20, 2, 128), (20, 4, 192)])
+def test_unused_rows_may_hold_anything(gpu, codes, dtype, T, group, dim):
+    """Rows at or past widths are never read: whatever they hold, the others' outputs are the same bit for bit."""
+    q, cache, table, ln, g = _make(31, 3, T, 2, group, dim, codes, dtype, [0, 200, 37])
+    widths = [T - 2, 3, T // 2]
+    wd = torch.tensor(widths, dtype=torch.int32).cuda()
+    want, wl = tree_attention(q, cache, table, ln, None, wd, return_lse=True)
+    _check(want, q, cache, table, ln, _chain(3, T), widths, lse=wl)
+    for x in (1e9, 3e38, float("inf"), float("nan")):
+        y = q.clone()
+        for b, w in enumerate(widths):
+            y[b, w:] = min(x, torch.finfo(dtype).max) if math.isfinite(x) else x
+        got, gl = tree_attention(y, cache, table, ln, None, wd, return_lse=True)
+        assert torch.equal(got, want) and torch.equal(gl, wl), x
+
+
+@pytest.mark.parametrize("codes", ["int8", "fp8"])
+@pytest.mark.parametrize("T,group,dim", [(5, 3, 64), (12, 4, 128), (9, 2, 192), (6, 1, 250)])
+def test_rows_of_different_sizes(gpu, codes, T, group, dim):
+    """Query rows 2^-60 to 2^100 of each other in one block of rows: each is as right as alone."""
+    q, cache, table, ln, g = _make(33, 2, T, 2, group, dim, codes, torch.bfloat16, [200, 33])
+    q[:, 1] *= 2.0**-60
+    q[:, 2] *= 2.0**40
+    q[:, 3, 0] *= 2.0**100
+    q[:, 3, -1] *= 2.0**20
+    q[:, 4, 1] = 0
+    out, lse = tree_attention(q, cache, table, ln, return_lse=True)
+    _rows(out, q, cache, table, ln, _chain(2, T), lse=lse)
+
+
+@pytest.mark.parametrize("size", [2.0**-126, 2.0**-100, 2.0**100, 2.0**120])
+def test_queries_of_extreme_sizes(gpu, size):
+    """Queries near the type's ends with a scale that makes ordinary scores of them."""
+    q, cache, table, ln, _ = _make(35, 2, 3, 1, 2, 64, "int8", torch.bfloat16, [300, 41])
+    q = (q.double() * size).bfloat16()
+    assert torch.isfinite(q).all()
+    scale = min(0.125 / size, 2.0**127)
+    out, lse = tree_attention(q, cache, table, ln, scale=scale, return_lse=True)
+    _rows(out, q, cache, table, ln, _chain(2, 3), scale=scale, lse=lse)
+
+
+def test_a_query_row_that_is_not_finite(gpu):
+    """An infinity or a NaN in a used row makes that row NaN and no other."""
+    q, cache, table, ln, _ = _make(37, 2, 5, 1, 2, 64, "int8", torch.bfloat16, [200, 33])
+    for x in (float("inf"), float("nan")):
+        y = q.clone()
+        y[:, 2, 1, 7] = x
+        got, lse = tree_attention(y, cache, table, ln, return_lse=True)
+        assert torch.isnan(got[:, 2, 1]).all()
+        _rows(got, y, cache, table, ln, _chain(2, 5), lse=lse, skip=[(2, 1)])
