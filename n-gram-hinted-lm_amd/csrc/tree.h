@@ -270,6 +270,7 @@ template <int CODES, int DP, int R> struct Tree {
     static constexpr int KS = DP / 32;          // product steps over the dimension
     static constexpr int NJ = DP / 16;          // 16-dimension tiles of the output
     static constexpr float BIAS = Q8 ? 8.f : 0.f;   // P's exponent is raised by this: f16 holds 2^-32 of the largest
+    static constexpr float NONE = 0x1p-64f;         // the scale taken for a value row of zeros
     static constexpr float SLACK = 4.f;             // M follows the maximum only when that passes it by 2^SLACK
     static constexpr float K_UP = CODES == KV_INT8 ? 16777216.f : 1.f, V_UP = CODES == KV_INT8 ? 512.f : 1.f;
 
@@ -508,8 +509,10 @@ template <int CODES, int DP, int R> struct Tree {
         const int key = lane_id() & 31;
         if (lane_id() < 32) fac[0][key] = scale * s.c;
         else {
-            // a row of zeros: any scale; the inverse of a subnormal one would overflow
-            float x = scale == 0.f ? 1.f : scale < 0x1p-126f ? 0x1p-126f : scale;
+            // A row of zeros: NONE, not 1. It counts in the sum (2^-64 * 2^64), and the maximum follows it only where its weight
+            // is 2^64 of the others' weighted values, which are then nothing: it takes none of their bits. (The inverse of a
+            // subnormal scale would overflow.)
+            float x = scale == 0.f ? NONE : scale < 0x1p-126f ? 0x1p-126f : scale;
             x = in ? x : 1.f;
             fac[1][key] = __builtin_amdgcn_logf(x);
             fac[2][key] = __builtin_amdgcn_rcpf(x);

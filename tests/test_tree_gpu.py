@@ -438,3 +438,34 @@ def test_a_query_row_that_is_not_finite(gpu):
         got, lse = tree_attention(y, cache, table, ln, return_lse=True)
         assert torch.isnan(got[:, 2, 1]).all()
         _rows(got, y, cache, table, ln, _chain(2, 5), lse=lse, skip=[(2, 1)])
+
+
+def _with_values(seed, codes, lengths, size, zeros, lead, T=2):
+    """A cache of values about `size`, zero rows at the positions `zeros` of every sequence, whose keys score `lead` more
+    than ordinary ones (every query is about one direction)."""
+    q, cache, table, ln, g = _make(seed, len(lengths), T, 1, 2, 64, codes, torch.bfloat16, lengths)
+    base = torch.randn(64, generator=g)
+    q = (base + 0.1 * torch.randn(q.shape, generator=g)).bfloat16().cuda()
+    n = cache.pages * cache.page
+    k = 0.3 * torch.randn((n, 1, 64), generator=g)
+    v = torch.randn((n, 1, 64), generator=g) * size
+    at = cache.slots(table, torch.zeros(len(lengths), dtype=torch.int32).cuda(), max(lengths) + T).cpu()
+    for b in range(len(lengths)):
+        for p in zeros:
+            if p < lengths[b] + T:
+                k[at[b, p]] = base * (lead * 8 / float(base @ base))  # scale 1/8: score `lead` with base
+                v[at[b, p]] = 0
+    cache.write(k.cuda(), v.cuda(), torch.arange(n).cuda())
+    return q, cache, table, ln
+
+
+@pytest.mark.parametrize("codes", ["int8", "fp8"])
+@pytest.mark.parametrize("size", [1.0, 1e-2, 1e-4, 1e-5, 2.0**-20, 2.0**-40])
+@pytest.mark.parametrize("lead", [0.0, 12.0, 40.0])
+def test_value_rows_of_zeros(gpu, codes, size, lead):
+    """Value rows of zeros take part in the softmax's sum and leave the others' weights their bits: at an ordinary score and
+    at one far above, first, in the middle, last, and in the tree."""
+    for zeros in ([0], [150], [5, 130, 201, 299], [300]):
+        q, cache, table, ln = _with_values(41, codes, [300, 1, 210], size, zeros, lead)
+        out, lse = tree_attention(q, cache, table, ln, return_lse=True)
+        _rows(out, q, cache, table, ln, _chain(3, 2), lse=lse)
