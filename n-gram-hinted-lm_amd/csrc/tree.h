@@ -270,7 +270,11 @@ template <int CODES, int DP, int R> struct Tree {
     static constexpr int KS = DP / 32;          // product steps over the dimension
     static constexpr int NJ = DP / 16;          // 16-dimension tiles of the output
     static constexpr float BIAS = Q8 ? 8.f : 0.f;   // P's exponent is raised by this: f16 holds 2^-32 of the largest
-    static constexpr float NONE = 0x1p-64f;         // the scale taken for a value row of zeros
+    // The scale taken for value rows of a smaller one, zeros among them; their weights in the product with the values then
+    // take the rest, scale / NONE. So such a row counts in the softmax's sum (2^-64 * 2^64: the inverse of a scale near the
+    // smallest float would overflow it), and the maximum follows it only where its weight is 2^64 of the others' weighted
+    // values, which are then nothing: it takes none of their bits, as a row of zeros with a scale of 1 would.
+    static constexpr float NONE = 0x1p-64f;
     static constexpr float SLACK = 4.f;             // M follows the maximum only when that passes it by 2^SLACK
     static constexpr float K_UP = CODES == KV_INT8 ? 16777216.f : 1.f, V_UP = CODES == KV_INT8 ? 512.f : 1.f;
 
@@ -505,19 +509,20 @@ template <int CODES, int DP, int R> struct Tree {
 
     // The factors of a tile's keys, computed by one lane each and handed through LDS to the lanes that hold their scores:
     // the score's factor, the logarithm and the inverse of the value scale.
-    static __device__ __forceinline__ void factors(float scale, bool in, const State& s, float (*fac)[32]) {
+    // True where a value scale is below NONE: the weights then take fac[3] more.
+    static __device__ __forceinline__ bool factors(float scale, bool in, const State& s, float (*fac)[32]) {
         const int key = lane_id() & 31;
+        const bool low = in && lane_id() >= 32 && scale < NONE;
         if (lane_id() < 32) fac[0][key] = scale * s.c;
         else {
-            // A row of zeros: NONE, not 1. It counts in the sum (2^-64 * 2^64), and the maximum follows it only where its weight
-            // is 2^64 of the others' weighted values, which are then nothing: it takes none of their bits. (The inverse of a
-            // subnormal scale would overflow.)
-            float x = scale == 0.f ? NONE : scale < 0x1p-126f ? 0x1p-126f : scale;
+            float x = low ? NONE : scale;
             x = in ? x : 1.f;
             fac[1][key] = __builtin_amdgcn_logf(x);
             fac[2][key] = __builtin_amdgcn_rcpf(x);
+            if (__any(low)) fac[3][key] = low ? scale * (1.f / NONE) : 1.f;
         }
         __builtin_amdgcn_wave_barrier();
+        return __any(low);
     }
 
     static __device__ __forceinline__ void scores(Keys& k, const State& s, const Sizes& size, bool own, float (*fac)[32],
@@ -597,6 +602,15 @@ template <int CODES, int DP, int R> struct Tree {
         }
     }
 
+    // The weights of value rows whose scale is below NONE.
+    static __device__ __forceinline__ void lower(const float (*fac)[32], V8 (&p)[R]) {
+        const int g = lane_id() >> 4;
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+#pragma unroll
+            for (int r = 0; r < R; ++r) p[r][i] = (T)((float)p[r][i] * fac[3][g * 8 + i]);
+    }
+
     static __device__ __forceinline__ void values(Values& f, const V8 (&p)[R], State& s) {
         if constexpr (CODES == KV_INT8)
 #pragma unroll
@@ -639,7 +653,8 @@ template <int CODES, int DP, int R> struct Tree {
             f4 sc[R][2];
             V8 p[R];
             float rv[8];
-            if constexpr (Q8) factors(w.k.s, true, s, fac);
+            bool low = false;
+            if constexpr (Q8) low = factors(w.k.s, true, s, fac);
             scores(w.k, s, size, own, fac, sc);
 #pragma unroll
             for (int i = 0; i < 8; ++i) rv[i] = Q8 ? fac[2][g * 8 + i] : 1.f;
@@ -659,6 +674,7 @@ template <int CODES, int DP, int R> struct Tree {
                 }
             }
             weights(sc, rv, p, s);
+            if (Q8 && low) lower(fac, p);
             values(w.v, p, s);
             fetch_values(a, head, nb, pg, w.v);
             base += TILE;
@@ -673,7 +689,8 @@ template <int CODES, int DP, int R> struct Tree {
         f4 sc[R][2];
         V8 p[R];
         float rv[8];
-        if constexpr (Q8) factors(w.k.s, base + (lane_id() & 31) < q.n, s, fac);
+        bool low = false;
+        if constexpr (Q8) low = factors(w.k.s, base + (lane_id() & 31) < q.n, s, fac);
         scores(w.k, s, size, own, fac, sc);
 #pragma unroll
         for (int i = 0; i < 8; ++i) rv[i] = Q8 ? fac[2][g * 8 + i] : 1.f;
@@ -700,6 +717,7 @@ template <int CODES, int DP, int R> struct Tree {
             }
         }
         weights(sc, rv, p, s);
+        if (Q8 && low) lower(fac, p);
         values(w.v, p, s);
         if constexpr (!Q8)
             if (__any(bad != 0)) put_back(a, q, base, bits, w.v, bad, p, s);
@@ -718,7 +736,7 @@ __global__ __launch_bounds__(256, (tree_waves<CODES, DP, R>())) void tree_k(cons
     __shared__ float lm[4][16], ll[4][16];
     __shared__ typename W::Sizes size;
     __shared__ u64 bits[16 * R];
-    __shared__ __align__(16) float fac[4][3][32];
+    __shared__ __align__(16) float fac[4][4][32];
     const Line line(a, blocks);
     // neighbouring shares on one XCD (blocks go round the 8 XCDs): units that share keys meet in its L2
     const int a8 = (line.shares + 7) / 8, me = (int)(blockIdx.x % 8) * a8 + (int)blockIdx.x / 8;

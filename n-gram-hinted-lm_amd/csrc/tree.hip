@@ -5,9 +5,17 @@
 //
 // Mathematics. One pass over the keys with a running maximum M and sum l per row, in base 2 and 32 bits. A cache held in
 // 8 bits is not dequantised: the key's scale multiplies the finished score, and the value's scale joins the exponent,
-// P = exp2(score + log2(vscale) - M), so that P stays in (0, 1] whatever the scales are and the product P V runs on the
-// codes; the sum of the softmax then takes P / vscale. Codes of 8 bits are exact in 16-bit floats. The 8-bit caches run
-// on f16 products (queries scaled by a power of two to f16's range), 16-bit caches on their own type.
+// P = exp2(score + log2(vscale) - M), so that P keeps its bits whatever the scales are to each other and the product P V
+// runs on the codes; the sum of the softmax takes P / vscale. (Value scales of 2^-64 to 2^40: a smaller one is split in
+// two factors, and beside a larger one weights below 2^-30 of the row's largest can be missing in the sum.) M follows the
+// maximum in steps of 2^4 at least, and over 8-bit caches P is raised by 2^8: it is at most 2^12. Codes of 8 bits are exact
+// in 16-bit floats. The 8-bit caches run on f16 products (queries scaled by a power of two to f16's range), 16-bit caches
+// on their own type.
+//
+// Rounding. Scores, M, l and the outputs' sums are held in 32 bits. P is rounded to 16 bits for its product with the
+// values (f16; bf16 over a bf16 cache), because the matrix instructions take no 32-bit operand at this rate: each key's
+// weight is off by up to 2^-11 (2^-8) of itself, against the 2^-9 to which bf16 outputs are rounded in any case, and over
+// 8-bit caches by up to 2^-33 of the largest weighted value. l sums P before that rounding.
 //
 // Layout. The scores are computed transposed (keys x rows), so that a lane holds 8 keys of one row: its maximum, sum and
 // rescaling are its own, and its P are the next product's operand as they stand, without a move between lanes. The output

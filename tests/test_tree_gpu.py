@@ -469,3 +469,47 @@ def test_value_rows_of_zeros(gpu, codes, size, lead):
         q, cache, table, ln = _with_values(41, codes, [300, 1, 210], size, zeros, lead)
         out, lse = tree_attention(q, cache, table, ln, return_lse=True)
         _rows(out, q, cache, table, ln, _chain(3, 2), lse=lse)
+
+
+@pytest.mark.parametrize("codes", ["int8", "fp8"])
+def test_scales_of_zero_stand_for_zeros(gpu, codes):
+    """A scale of 0 over codes that are not 0 (a cache from elsewhere): zeros, as read() has them."""
+    q, cache, table, ln = _with_values(43, codes, [300, 5], 1.0, [], 0.0)
+    cache.v_scale.view(-1)[::3] = 0
+    out, lse = tree_attention(q, cache, table, ln, return_lse=True)
+    _rows(out, q, cache, table, ln, _chain(2, 2), lse=lse)
+
+
+@pytest.mark.parametrize("codes", ["int8", "fp8"])
+@pytest.mark.parametrize("first", [1e-35, 1e-30, 1e-20, 1e-17])
+@pytest.mark.parametrize("rest", [1.0, 1e-4])
+def test_tiny_values_first(gpu, codes, first, rest):
+    """A first tile of values whose scales' inverses are near the largest float, then ordinary ones; and nothing else."""
+    q, cache, table, ln = _with_values(45, codes, [300, 100, 700], rest, [], 0.0)
+    n = cache.pages * cache.page
+    g = torch.Generator().manual_seed(5)
+    k, v = (torch.randn((n, 1, 64), generator=g) for _ in range(2))
+    v *= rest
+    at = cache.slots(table, torch.zeros(3, dtype=torch.int32).cuda(), 128).cpu()
+    for b in range(3):
+        for s in at[b]:
+            if s >= 0:
+                v[s] *= first / rest
+    cache.write(k.cuda(), v.cuda(), torch.arange(n).cuda())
+    out, lse = tree_attention(q, cache, table, ln, return_lse=True)
+    _rows(out, q, cache, table, ln, _chain(3, 2), lse=lse)
+
+
+@pytest.mark.parametrize("codes", ["int8", "fp8"])
+@pytest.mark.parametrize("zeros", [False, True])
+def test_value_sizes_far_apart(gpu, codes, zeros):
+    """Values 2^-40 to 2^40 of each other's, with and without rows of zeros."""
+    q, cache, table, ln, g = _make(47, 2, 3, 1, 2, 64, codes, torch.bfloat16, [300, 41])
+    n = cache.pages * cache.page
+    k = torch.randn((n, 1, 64), generator=g)
+    v = torch.randn((n, 1, 64), generator=g) * torch.exp2((torch.rand((n, 1, 1), generator=g) - 0.5) * 80)
+    if zeros:
+        v[::7] = 0
+    cache.write(k.cuda(), v.cuda(), torch.arange(n).cuda())
+    out, lse = tree_attention(q, cache, table, ln, return_lse=True)
+    _rows(out, q, cache, table, ln, _chain(2, 3), lse=lse)
