@@ -167,15 +167,16 @@ template <typename V8> union Words {
 };
 
 // Eight consecutive codes of a row (8 bits: two words; 16 bits: four) as an operand. int8 (its words' sign bits flipped
-// where they were loaded: c + 128): the bytes are taken for f16 as they stand, which are (c + 128) 2^-24 exactly (two
-// permutes a word and no conversion); the accumulators start at -128 2^-24 sum(q) (K_OFF) and the score's factor has 2^24.
+// where they were loaded: c + 128): the byte under 0x64 is the f16 1024 + (c + 128), exactly, and less 1152 it is c. (The
+// sum over c + 128, less 128 sum(q) at the end, saves that subtraction, but a key of small codes loses its sum in 128's.)
 template <int CODES, typename V8> __device__ __forceinline__ V8 row_operand(const u32* w) {
     Words<V8> x;
     if constexpr (CODES == KV_INT8) {
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
-            x.u[2 * i] = __builtin_amdgcn_perm(0u, w[i], 0x0c010c00u);
-            x.u[2 * i + 1] = __builtin_amdgcn_perm(0u, w[i], 0x0c030c02u);
+            const h2 o = {(f16)-1152.f, (f16)-1152.f};
+            x.u[2 * i] = __builtin_bit_cast(u32, __builtin_bit_cast(h2, __builtin_amdgcn_perm(0x64646464u, w[i], 0x04010400u)) + o);
+            x.u[2 * i + 1] = __builtin_bit_cast(u32, __builtin_bit_cast(h2, __builtin_amdgcn_perm(0x64646464u, w[i], 0x04030402u)) + o);
         }
     } else if constexpr (CODES == KV_FP8) {
 #pragma unroll
@@ -190,8 +191,8 @@ template <int CODES, typename V8> __device__ __forceinline__ V8 row_operand(cons
     return x.v;
 }
 
-// Elements 2 p and 2 p + 1 of eight rows (v[row][words]) as two operands. int8: (c + 128) 2^-24 as above, then one
-// multiply-add to c 2^-9 (the outputs are multiplied by 2^9 at the end): a sum of c + 128 would lose what c's sum has.
+// Elements 2 p and 2 p + 1 of eight rows (v[row][words]) as two operands. int8: the bytes are taken for f16 as they stand,
+// which are (c + 128) 2^-24 exactly, then one multiply-add to c 2^-9 (the outputs are multiplied by 2^9 at the end).
 template <int CODES, typename V8, int VW>
 __device__ __forceinline__ void col_operands(const u32 (&v)[8][VW], int p, V8& lo, V8& hi) {
     Words<V8> x, y;
@@ -276,7 +277,7 @@ template <int CODES, int DP, int R> struct Tree {
     // values, which are then nothing: it takes none of their bits, as a row of zeros with a scale of 1 would.
     static constexpr float NONE = 0x1p-64f;
     static constexpr float SLACK = 4.f;             // M follows the maximum only when that passes it by 2^SLACK
-    static constexpr float K_UP = CODES == KV_INT8 ? 16777216.f : 1.f, V_UP = CODES == KV_INT8 ? 512.f : 1.f;
+    static constexpr float V_UP = CODES == KV_INT8 ? 512.f : 1.f;
 
     struct Pages {
         int k, v, s;  // of the keys this lane loads: key group c >> 2, value group g, scale group
@@ -296,7 +297,7 @@ template <int CODES, int DP, int R> struct Tree {
         V8 q[QLDS ? 1 : R][KS];
         const T* ql;  // the queries in LDS, at this lane's row and quarter
         f4 o[R][NJ];
-        float m[R], l[R], off[R];
+        float m[R], l[R];
         float c;  // the scores' factor: scale * log2(e) / the queries' power of two (own: without powers of two)
     };
 
@@ -377,7 +378,6 @@ template <int CODES, int DP, int R> struct Tree {
                     size.shift[threadIdx.x] = __builtin_amdgcn_frexp_expf(s.c) - up_of(size.top[threadIdx.x]);
                 s.c = __builtin_amdgcn_frexp_mantf(s.c);
             } else s.c = __builtin_amdgcn_ldexpf(s.c, -up);
-            s.c *= K_UP;
         }
 #pragma unroll
         for (int k = 0; k < NQ; ++k) {
@@ -399,19 +399,11 @@ template <int CODES, int DP, int R> struct Tree {
         if constexpr (Q8)
             if (threadIdx.x < 16 * R) size.top[threadIdx.x] = 0;  // (the next unit's maxima come after the joining's barriers)
         s.ql = lds + c * QLD + g * (DP / 4);
+        if constexpr (!QLDS)
 #pragma unroll
-        for (int r = 0; r < R; ++r) {
-            float sum = 0.f;
+            for (int r = 0; r < R; ++r)
 #pragma unroll
-            for (int st = 0; st < KS; ++st) {
-                const V8 x = *(const V8*)(s.ql + r * 16 * QLD + st * 8);
-                if constexpr (!QLDS) s.q[r][st] = x;
-                if constexpr (CODES == KV_INT8)
-#pragma unroll
-                    for (int j = 0; j < 8; ++j) sum += (float)x[j];
-            }
-            s.off[r] = CODES == KV_INT8 ? -128.f / K_UP * sum_quarters(sum) : 0.f;
-        }
+                for (int st = 0; st < KS; ++st) s.q[r][st] = *(const V8*)(s.ql + r * 16 * QLD + st * 8);
         return own;
     }
     // the power of two that puts a row's largest element at 2^14 .. 2^15
@@ -529,7 +521,7 @@ template <int CODES, int DP, int R> struct Tree {
                                                   f4 (&sc)[R][2]) {
         const int c = lane_id() & 15, g = lane_id() >> 4;
 #pragma unroll
-        for (int r = 0; r < R; ++r) sc[r][0] = sc[r][1] = f4{s.off[r], s.off[r], s.off[r], s.off[r]};
+        for (int r = 0; r < R; ++r) sc[r][0] = sc[r][1] = f4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
         for (int st = 0; st < KS; ++st) {
             V8 x[R];

@@ -14,8 +14,8 @@
 //
 // Rounding. Scores, M, l and the outputs' sums are held in 32 bits. P is rounded to 16 bits for its product with the
 // values (f16; bf16 over a bf16 cache), because the matrix instructions take no 32-bit operand at this rate: each key's
-// weight is off by up to 2^-11 (2^-8) of itself, against the 2^-9 to which bf16 outputs are rounded in any case, and over
-// 8-bit caches by up to 2^-33 of the largest weighted value. l sums P before that rounding.
+// weight is off by up to 2^-11 (2^-8) of itself, as much as an output of that type is rounded in any case, and over 8-bit
+// caches by up to 2^-33 of the largest weighted value. l sums P before that rounding.
 //
 // Layout. The scores are computed transposed (keys x rows), so that a lane holds 8 keys of one row: its maximum, sum and
 // rescaling are its own, and its P are the next product's operand as they stand, without a move between lanes. The output

@@ -513,3 +513,25 @@ def test_value_sizes_far_apart(gpu, codes, zeros):
     cache.write(k.cuda(), v.cuda(), torch.arange(n).cuda())
     out, lse = tree_attention(q, cache, table, ln, return_lse=True)
     _rows(out, q, cache, table, ln, _chain(2, 3), lse=lse)
+
+
+@pytest.mark.parametrize("codes", ["int8", "fp8"])
+@pytest.mark.parametrize("dim", [64, 128, 256])
+def test_keys_with_one_large_channel(gpu, codes, dim):
+    """Keys whose codes are 0 but for a channel that the query has nothing in and another of the smallest code: a score is
+    one product, to the last bits of itself. One key a sequence, so its logarithm is the score."""
+    B = 40
+    g = torch.Generator().manual_seed(dim)
+    cache = KVCache.empty(B, 16, 1, dim, codes)
+    q = (torch.randn((B, 1, 1, dim), generator=g) * 1000).bfloat16()
+    k = torch.zeros((B, 1, dim))
+    for b in range(B):
+        top = 127.0 if codes == "int8" else 448.0
+        k[b, 0, b % dim], k[b, 0, (b + 5) % dim] = top, 1.0
+        q[b, 0, 0, b % dim] = 0
+    table = torch.arange(B, dtype=torch.int32).view(B, 1).cuda()
+    cache.write(k.cuda(), k.cuda(), torch.arange(B).cuda() * 16)
+    none = torch.zeros(B, dtype=torch.int32).cuda()
+    q = q.cuda()
+    out, lse = tree_attention(q, cache, table, none, scale=1.0, return_lse=True)
+    _rows(out, q, cache, table, none, _chain(B, 1), scale=1.0, lse=lse)
