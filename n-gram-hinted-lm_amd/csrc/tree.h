@@ -277,6 +277,7 @@ template <int CODES, int DP, int R> struct Tree {
     // values, which are then nothing: it takes none of their bits, as a row of zeros with a scale of 1 would.
     static constexpr float NONE = 0x1p-64f;
     static constexpr float SLACK = 4.f;             // M follows the maximum only when that passes it by 2^SLACK
+    static constexpr bool WILD = CODES != KV_INT8;  // codes can be NaN or infinite
     static constexpr float V_UP = CODES == KV_INT8 ? 512.f : 1.f;
 
     struct Pages {
@@ -445,14 +446,14 @@ template <int CODES, int DP, int R> struct Tree {
         const int c = lane_id() & 15, g = lane_id() >> 4, in = (1 << a.shift) - 1;
         f.ok = (u32)p.v < (u64)a.pages;
         const i64 rv = ((((i64)(f.ok ? p.v : 0)) * a.H + head) << a.shift) + ((base + g * 8) & in);
-        if constexpr (!Q8) f.row = rv;
+        if constexpr (WILD) f.row = rv;
         const char* v = (const char*)a.v + rv * (DP * ES) + c * (DP * ES / 16);
 #pragma unroll
         for (int i = 0; i < 8; ++i) load_words<VW>(v + i * DP * ES, f.v[i]);
     }
 
 
-    // Values of a 16-bit cache that are not finite, in keys that only some rows see: they are 0 in the product (a masked
+    // Values that are not finite (codes of NaN: fp8), in keys that only some rows see: they are 0 in the product (a masked
     // key's P of 0 would make NaN of them) and are added here to the rows that do see them.
     static __device__ __forceinline__ u32 take_out(Values& f) {
         constexpr u32 E = CODES == KV_BF16 ? 0x7F80u : 0x7C00u;
@@ -461,11 +462,22 @@ template <int CODES, int DP, int R> struct Tree {
         for (int i = 0; i < 8; ++i)
 #pragma unroll
             for (int w = 0; w < VW; ++w) {
-                const bool lo = (f.v[i][w] & E) == E, hi = (f.v[i][w] >> 16 & E) == E;
-                bad |= (lo || hi ? 1u : 0u) << i;
-                f.v[i][w] &= (lo ? 0u : 0xFFFFu) | (hi ? 0u : 0xFFFF0000u);
+                if constexpr (CODES == KV_FP8) {  // 0x7F and 0xFF
+                    const u32 nan = ((f.v[i][w] & 0x7F7F7F7Fu) + 0x01010101u) >> 7 & 0x01010101u;
+                    bad |= (nan ? 1u : 0u) << i;
+                    f.v[i][w] &= ~(nan * 0xFFu);
+                } else {
+                    const bool lo = (f.v[i][w] & E) == E, hi = (f.v[i][w] >> 16 & E) == E;
+                    bad |= (lo || hi ? 1u : 0u) << i;
+                    f.v[i][w] &= (lo ? 0u : 0xFFFFu) | (hi ? 0u : 0xFFFF0000u);
+                }
             }
         return bad;
+    }
+    // element `at` of the values held, where it is not finite (else anything finite)
+    static __device__ __forceinline__ float wild(const TreeArgs& a, i64 at) {
+        if constexpr (CODES == KV_FP8) return (((const unsigned char*)a.v)[at] & 0x7F) == 0x7F ? __builtin_nanf("") : 0.f;
+        else return (float)((const T*)a.v)[at];
     }
     static __device__ __forceinline__ void put_back(const TreeArgs& a, const Seq& q, int base, const u64* bits, const Values& f,
                                                     u32 bad, const V8 (&p)[R], State& s) {
@@ -475,7 +487,6 @@ template <int CODES, int DP, int R> struct Tree {
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
                 if (!__any(g == from && (bad >> i & 1))) continue;
-                const T* v = (const T*)a.v + (first + i) * DP;
                 const int j0 = base + from * 8 + i - q.len;
 #pragma unroll
                 for (int r = 0; r < R; ++r) {
@@ -485,7 +496,7 @@ template <int CODES, int DP, int R> struct Tree {
                     for (int j = 0; j < NJ; ++j)
 #pragma unroll
                         for (int k = 0; k < 4; ++k) {
-                            const float x = (float)v[(4 * g + k) * NJ + j];
+                            const float x = wild(a, (first + i) * DP + (4 * g + k) * NJ + j);
                             if (sees && !finite_f(x)) s.o[r][j][k] += w * x;
                         }
                 }
@@ -695,7 +706,7 @@ template <int CODES, int DP, int R> struct Tree {
 #pragma unroll
             for (int k = 0; k < VW; ++k) w.v.v[i][k] = in >> i & 1 ? w.v.v[i][k] : 0u;
         u32 bad = 0;
-        if constexpr (!Q8) bad = take_out(w.v);
+        if constexpr (WILD) bad = take_out(w.v);
 #pragma unroll
         for (int r = 0; r < R; ++r) {
             const u64 see = bits[r * 16 + c];
@@ -711,7 +722,7 @@ template <int CODES, int DP, int R> struct Tree {
         weights(sc, rv, p, s);
         if (Q8 && low) lower(fac, p);
         values(w.v, p, s);
-        if constexpr (!Q8)
+        if constexpr (WILD)
             if (__any(bad != 0)) put_back(a, q, base, bits, w.v, bad, p, s);
     }
 };

@@ -535,3 +535,26 @@ def test_keys_with_one_large_channel(gpu, codes, dim):
     q = q.cuda()
     out, lse = tree_attention(q, cache, table, none, scale=1.0, return_lse=True)
     _rows(out, q, cache, table, none, _chain(B, 1), scale=1.0, lse=lse)
+
+
+@pytest.mark.parametrize("side", [0, 1])
+def test_codes_of_nan_in_a_masked_token(gpu, side):
+    """An fp8 code that is itself NaN (a cache from elsewhere) in a tree token: only the rows that see it are NaN."""
+    T = 12
+    q, cache, table, ln, g = _make(49, 3, T, 2, 2, 64, "fp8", torch.bfloat16, [37, 128, 5])
+    m = _ancestors(_parents(3, T, g))
+    bits = _bits(m).cuda()
+    want, wl = tree_attention(q, cache, table, ln, bits, return_lse=True)
+    at = cache.slots(table, ln + 4, 1)[:, 0]
+    held = (cache.k, cache.v)[side].view(torch.uint8)
+    held[at // 16, :, at % 16, 9] = 0x7F
+    held[at // 16, :, at % 16, 33] = 0xFF
+    got, gl = tree_attention(q, cache, table, ln, bits, return_lse=True)
+    see = m[:, :, 4].cuda()
+    assert torch.equal(got[~see], want[~see]) and torch.equal(gl[~see], wl[~see])
+    if side == 0:
+        assert torch.isnan(got[see]).all()
+    else:
+        assert torch.isnan(got[see][..., [9, 33]]).all()
+        rest = [d for d in range(64) if d not in (9, 33)]
+        assert torch.equal(got[see][..., rest], want[see][..., rest]) and torch.equal(gl, wl)
