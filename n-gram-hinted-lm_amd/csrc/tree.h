@@ -260,7 +260,7 @@ template <int N> __device__ __forceinline__ void put(const TreeArgs& a, i64 i, i
     }
 }
 
-// CODES: the cache's; DP: its padded row; R: rows a block / 16.
+// CODES: the cache's; DP: its padded row; R: rows a block / 16, 1 or 2.
 template <int CODES, int DP, int R> struct Tree {
     typedef typename op_t<CODES>::type T;
     typedef T V8 __attribute__((ext_vector_type(8)));
@@ -292,7 +292,7 @@ template <int CODES, int DP, int R> struct Tree {
         bool ok;   // this lane's keys lie in a page of the cache
         i64 row;   // its first value row
     };
-    static constexpr bool QLDS = R >= 2;  // the queries are read from LDS for every tile: registers go to loads in flight
+    static constexpr bool QLDS = R == 2;  // the queries are read from LDS for every tile: registers go to loads in flight
 
     struct State {
         V8 q[QLDS ? 1 : R][KS];
@@ -727,10 +727,8 @@ template <int CODES, int DP, int R> struct Tree {
     }
 };
 
-template <int CODES, int DP, int R> constexpr int tree_waves() { return R <= 2 && DP <= 128 ? 2 : 1; }
-
 template <int CODES, int DP, int R>
-__global__ __launch_bounds__(256, (tree_waves<CODES, DP, R>())) void tree_k(const TreeArgs a, int blocks) {
+__global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void tree_k(const TreeArgs a, int blocks) {
     typedef Tree<CODES, DP, R> W;
     constexpr int LD = DP + 4;
     typedef float Lo[16][LD];
@@ -876,9 +874,7 @@ template <int CODES, int DP, int R> static int tree_run(const TreeArgs& a, const
 
 template <int CODES, int DP> static int tree_rows(const TreeArgs& a, const TreePlan& p, hipStream_t st) {
     if (p.rpb == 16) return tree_run<CODES, DP, 1>(a, p, st);
-    if (p.rpb == 32) return tree_run<CODES, DP, 2>(a, p, st);
-    if constexpr (DP <= 128) return tree_run<CODES, DP, 4>(a, p, st);
-    return -1;
+    return p.rpb == 32 ? tree_run<CODES, DP, 2>(a, p, st) : -1;
 }
 
 template <int CODES> int tree_codes(const TreeArgs& a, const TreePlan& p, hipStream_t st) {
