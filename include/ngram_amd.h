@@ -530,13 +530,18 @@ int ng_batch_rows_noalloc(const int* cells, const int* entries, ng_i64 n, ng_i64
  * row NaN. n * m < 2^31 - 64, V < 2^31.
  * ng_embed_grad: grad [V, dim] (dtype, contiguous; every row written) = scale * the sum over the counted entries of each
  * token of w * dout[position]; dout [n, dim] of row stride ld; work: ng_embed_grad_work(n * m, V, dim) bytes.
- * ng_embed_weight_grad: dw float32 [n, m] = scale * <table[token], dout[position]> where the slot has a cell, else 0. */
+ * ng_embed_slopes: dw float32 [n, m], the weights' gradient: scale * <table[token], dout[position]> where the slot has a
+ * cell, else 0. Where the token is outside the table: NaN, or 0 for a weight of 0 (padding). ng_embed_weight_grad: the same
+ * without weights (w NULL): every entry of a slot with a cell counts. */
 int ng_embed(const void* table, ng_i64 ld, ng_i64 V, int dim, int dtype, const void* tokens, int tsize, const float* w,
              const void* cell, int csize, ng_i64 n, int m, int entries, float scale, void* out, void* stream);
 ng_i64 ng_embed_grad_work(ng_i64 entries, ng_i64 V, ng_i64 dim);
 int ng_embed_grad(const void* dout, ng_i64 ld, ng_i64 V, int dim, int dtype, const void* tokens, int tsize, const float* w,
                   const void* cell, int csize, ng_i64 n, int m, int entries, float scale, void* grad, void* work,
                   void* stream);
+int ng_embed_slopes(const void* table, ng_i64 ld, const void* dout, ng_i64 dld, ng_i64 V, int dim, int dtype,
+                    const void* tokens, int tsize, const float* w, const void* cell, int csize, ng_i64 n, int m, int entries,
+                    float scale, float* dw, void* stream);
 int ng_embed_weight_grad(const void* table, ng_i64 ld, const void* dout, ng_i64 dld, ng_i64 V, int dim, int dtype,
                          const void* tokens, int tsize, const void* cell, int csize, ng_i64 n, int m, int entries,
                          float scale, float* dw, void* stream);

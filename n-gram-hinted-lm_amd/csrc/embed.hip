@@ -3,11 +3,12 @@
 //   out[n] = scale * sum_j w[n, j] * table[tok[n, j]]     over the entries j = (slot, candidate) of position n that count:
 //            w[n, j] != 0 and cell[n, slot] > 0; without weights one entry of weight 1
 //   grad[v] = scale * sum over the counted entries of token v of w[n, j] * dout[n]
-//   dw[n, j] = scale * <table[tok[n, j]], dout[n]> where the slot has a cell, else 0
+//   dw[n, j] = scale * <table[tok[n, j]], dout[n]> where the slot has a cell, else 0; also where w[n, j] = 0: the slope at 0
 //
-// An entry that does not count is not read (its table row may hold anything). A counted token outside the table is never
-// read either: its position's output is NaN, its dw NaN, and it adds to no gradient. Sums are held in 32 bits, in a fixed
-// order, and rounded once.
+// An entry that does not count is not read by the output and the table's gradient (its table row may hold anything); the
+// weights' gradient reads the row of an entry of weight 0 that has a cell, and is 0 where its token is outside the table. A
+// counted token outside the table is never read: its position's output is NaN, its dw NaN, and it adds to no gradient. Sums
+// are held in 32 bits, in a fixed order, and rounded once.
 #include "vals.h"
 #include <type_traits>
 
@@ -540,12 +541,12 @@ __global__ __launch_bounds__(256) void embed_dw_k(const Rows r, const T* __restr
         for (int base = 0; base < r.m; base += 64) {
             const int j = base + lane_id();
             i64 tok = -1;
-            bool counts = false;
+            bool has = false, counts = false;
             if (j < r.m) {
-                counts = has_cell(r, n * r.m + j);
-                if (counts) tok = int_at(r.tokens, r.tsize, n * r.m + j);
+                has = has_cell(r, n * r.m + j);
+                if (has) tok = int_at(r.tokens, r.tsize, n * r.m + j), counts = !r.w || r.w[n * r.m + j] != 0.f;
             }
-            const bool ok = counts && (u64)tok < (u64)r.V;
+            const bool ok = has && (u64)tok < (u64)r.V;
             float mine = counts && !ok ? __builtin_nanf("") : 0.f;
             u64 live = __ballot(ok);
             while (live) {
@@ -752,10 +753,10 @@ extern "C" int ng_embed_grad(const void* dout, i64 ld, i64 V, int dim, int dtype
     }
 }
 
-extern "C" int ng_embed_weight_grad(const void* table, i64 ld, const void* dout, i64 dld, i64 V, int dim, int dtype,
-                                    const void* tokens, int tsize, const void* cell, int csize, i64 n, int m, int entries,
-                                    float scale, float* dw, void* stream) {
-    const Rows r = rows_of(tokens, tsize, nullptr, cell, csize, n, m, entries, V);
+extern "C" int ng_embed_slopes(const void* table, i64 ld, const void* dout, i64 dld, i64 V, int dim, int dtype,
+                               const void* tokens, int tsize, const float* w, const void* cell, int csize, i64 n, int m,
+                               int entries, float scale, float* dw, void* stream) {
+    const Rows r = rows_of(tokens, tsize, w, cell, csize, n, m, entries, V);
     if (!rows_ok(r, dim)) return -1;
     if (n == 0) return 0;
     hipStream_t st = (hipStream_t)stream;
@@ -765,4 +766,11 @@ extern "C" int ng_embed_weight_grad(const void* table, i64 ld, const void* dout,
         case NG_F16: return embed_dw<f16>(r, (const f16*)table, ld, (const f16*)dout, dld, dim, scale, dw, st);
         default: return -1;
     }
+}
+
+extern "C" int ng_embed_weight_grad(const void* table, i64 ld, const void* dout, i64 dld, i64 V, int dim, int dtype,
+                                    const void* tokens, int tsize, const void* cell, int csize, i64 n, int m, int entries,
+                                    float scale, float* dw, void* stream) {
+    return ng_embed_slopes(table, ld, dout, dld, V, dim, dtype, tokens, tsize, nullptr, cell, csize, n, m, entries, scale, dw,
+                           stream);
 }

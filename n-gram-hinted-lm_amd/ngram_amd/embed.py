@@ -8,12 +8,14 @@ its row's weights, summed over its slots, zero where a slot has no cell).
       without weights a lookup: out = scale * weight[tokens]
   HintEmbedding(vocab, dim, ...)   a module that holds the table; forward takes HintRows
 
-Entries that do not count are not read. A counted token outside the table makes its position's output NaN (and adds to no
-gradient): an IndexError would cost a device synchronization a call.
+Entries that do not count are not read by the output and the table's gradient. A counted token outside the table makes its
+position's output NaN (and adds to no gradient): an IndexError would cost a device synchronization a call. The weights'
+gradient is the slope at 0 too: where a slot has a cell it reads the rows of weight 0, and is 0 for such an entry whose token
+is outside the table.
 
 Differentiable in weight and weights. The table's gradient is dense and the same on every run: entries are sorted by token
-(this library's stable radix sort) and each token's terms are added in order, in 32 bits, rounded once. Everything runs on
-the current stream; csrc/embed.hip has the kernels."""
+(stably, by radix) and each token's terms are added in a fixed order, in 32 bits, rounded once. Everything runs on the
+current stream; csrc/embed.hip has the kernels."""
 
 from __future__ import annotations
 
@@ -32,7 +34,7 @@ _CELLS = {torch.int64: 8, torch.int32: 4, torch.int16: 2}
 @functools.lru_cache(maxsize=None)
 def _entries() -> tuple[Entry, Entry, Entry]:
     return (Entry(name="ng_embed", types="pqqiipippiqiifp"), Entry(name="ng_embed_grad", types="pqqiipippiqiifpp"),
-            Entry(name="ng_embed_weight_grad", types="pqpqqiipipiqiifp"))
+            Entry(name="ng_embed_slopes", types="pqpqqiipippiqiifp"))
 
 
 @functools.lru_cache(maxsize=256)
@@ -69,7 +71,7 @@ class _Embed(torch.autograd.Function):
         if ctx.needs_input_grad[2]:
             dweights = torch.empty(weights.shape, dtype=torch.float32, device=device)
             _entries()[2](device.index, weight.data_ptr(), weight.stride(0), up.data_ptr(), up.stride(0), vocab, dim, dt,
-                          tokens.data_ptr(), tsize, at, csize, n, m, entries, scale, dweights.data_ptr())
+                          tokens.data_ptr(), tsize, _at(weights), at, csize, n, m, entries, scale, dweights.data_ptr())
         return dweight, None, dweights, None, None, None
 
 

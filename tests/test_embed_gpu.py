@@ -277,3 +277,22 @@ def test_refusals(gpu):
         embed(t, tok, w, c, float("nan"))
     with pytest.raises(ValueError):
         embed(t, tok[:1, :1].expand(1 << 20, 1 << 11), w[:1, :1].expand(1 << 20, 1 << 11))
+
+
+@pytest.mark.parametrize("dtype,dim", [(torch.float32, 72), (torch.bfloat16, 300)])
+def test_weights_gradient_of_entries_that_do_not_count(gpu, dtype, dim):
+    """Padding: a weight of 0, or a slot without a cell, before a token outside the table. Its slope is 0 as everything of
+    it; a weight of 0 before a token of the table has the slope that it would count with; without a cell, 0."""
+    table, tokens, weights, cell, up = _case(21, 50, 400, 2, 8, dim, dtype)
+    dead = (weights == 0) | (cell <= 0)[..., None]
+    outside = dead & (torch.rand(dead.shape, generator=torch.Generator().manual_seed(1)) < 0.5)
+    assert (outside & (weights == 0) & (cell > 0)[..., None]).any() and (dead & ~outside).any()
+    far = torch.tensor([-1, 50, 1 << 40])[torch.arange(outside.numel()).reshape(outside.shape) % 3]
+    out, grad, slopes = _run(table, torch.where(outside, far, tokens), weights, cell, up, 0.5)
+    o, g, (want, size, count) = _definition(table, tokens, weights, cell, up, 0.5)
+    _check(out, *o, dtype, "out")
+    _check(grad, *g, dtype, "grad")
+    off = outside.reshape(want.shape)
+    assert not slopes.cpu().reshape(want.shape)[off].any()  # 0, not NaN
+    _check(torch.where(off.cuda(), 0.0, slopes.reshape(want.shape)), torch.where(off, 0.0, want),
+           torch.where(off, 0.0, size), count, torch.float32, "slopes")
