@@ -13,9 +13,9 @@ position's output NaN (and adds to no gradient): an IndexError would cost a devi
 gradient is the slope at 0 too: where a slot has a cell it reads the rows of weight 0, and is 0 for such an entry whose token
 is outside the table.
 
-Differentiable in weight and weights. The table's gradient is dense and the same on every run: entries are sorted by token
-(stably, by radix) and each token's terms are added in a fixed order, in 32 bits, rounded once. Everything runs on the
-current stream; csrc/embed.hip has the kernels."""
+Differentiable in weight and weights, in reverse mode (a forward-mode tangent raises). The table's gradient is dense and the
+same on every run: entries are sorted by token (stably, by radix) and each token's terms are added in a fixed order, in 32
+bits, rounded once. Everything runs on the current stream; csrc/embed.hip has the kernels."""
 
 from __future__ import annotations
 
@@ -23,6 +23,7 @@ import functools
 import math
 
 import torch
+from torch.autograd import forward_ad
 
 from .lib import Entry, Lib
 
@@ -136,7 +137,8 @@ def embed(weight: torch.Tensor, tokens: torch.Tensor, weights: torch.Tensor | No
     tokens = tokens.contiguous()
     weights = None if weights is None else weights.contiguous()
     cell = None if cell is None else cell.contiguous()
-    if torch.is_grad_enabled() and (weight.requires_grad or (weights is not None and weights.requires_grad)):
+    if (torch.is_grad_enabled() and (weight.requires_grad or (weights is not None and weights.requires_grad))
+            or forward_ad._current_level >= 0):  # a level of forward mode is open: the function refuses tangents
         return _Embed.apply(weight, tokens, weights, cell, shape, scale)
     return _forward(weight, tokens, weights, cell, shape, scale)
 

@@ -296,3 +296,18 @@ def test_weights_gradient_of_entries_that_do_not_count(gpu, dtype, dim):
     assert not slopes.cpu().reshape(want.shape)[off].any()  # 0, not NaN
     _check(torch.where(off.cuda(), 0.0, slopes.reshape(want.shape)), torch.where(off, 0.0, want),
            torch.where(off, 0.0, size), count, torch.float32, "slopes")
+
+
+def test_forward_mode_is_refused(gpu):
+    """There is no forward-mode derivative: a tangent raises instead of being lost."""
+    import torch.autograd.forward_ad as fw
+
+    table, tokens, weights, cell, up = (x.cuda() for x in _case(23, 50, 40, 1, 8, 72, torch.float32))
+    want = embed(table, tokens, weights, cell)
+    with fw.dual_level():
+        for t, w in ((fw.make_dual(table, table), weights), (table, fw.make_dual(weights, weights))):
+            with pytest.raises(RuntimeError, match="jvp"):
+                embed(t, tokens, w, cell)
+        with pytest.raises(RuntimeError, match="jvp"):
+            embed(fw.make_dual(table, table), tokens)
+        assert torch.equal(embed(table, tokens, weights, cell), want)
