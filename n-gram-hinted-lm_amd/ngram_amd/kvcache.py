@@ -9,7 +9,8 @@ zero (or too small for its inverse) has scale 0; one that holds a NaN or an infi
 reads back as NaN and nothing of it enters where it is masked.
 
 A token's slot is page * page size + its row there; a sequence's page table lists its pages in order, and -1 stands for no
-slot. Which page belongs to whom is the caller's. Everything runs on the current stream, and nothing here synchronizes.
+slot. Which page belongs to whom is the caller's. Quantising has no backward pass: keys and values that require gradients
+(with gradients on) or carry tangents raise. Everything runs on the current stream, and nothing here synchronizes.
 csrc/kvcache.hip has the kernels."""
 
 from __future__ import annotations
@@ -17,6 +18,7 @@ from __future__ import annotations
 import functools
 
 import torch
+from torch.autograd import forward_ad
 
 from .lib import Entry
 
@@ -34,6 +36,14 @@ def _entries() -> tuple[Entry, Entry, Entry]:
 def padded(dim: int) -> int:
     """The length of a cached row of `dim` elements."""
     return (dim + 63) // 64 * 64
+
+
+def refuse_gradients(what: str, *tensors: torch.Tensor) -> None:
+    """Raises where gradients would be lost: a tensor that requires one while they are on, or has a forward-mode tangent."""
+    if torch.is_grad_enabled() and any(t.requires_grad for t in tensors) or (
+            forward_ad._current_level >= 0 and any(forward_ad.unpack_dual(t).tangent is not None for t in tensors)):
+        raise RuntimeError(f"{what} has no backward pass and its input requires a gradient: call it under torch.no_grad() or "
+                           "on detached tensors")
 
 
 class KVCache:
@@ -62,10 +72,23 @@ class KVCache:
                     raise ValueError(f"{name} must be contiguous float32 {(pages, heads, page)} beside 8-bit codes")
         elif k_scale is not None or v_scale is not None:
             raise ValueError("a 16-bit cache has no scales")
-        self.k, self.v, self.k_scale, self.v_scale = k, v, k_scale, v_scale
+        if any(t is not None and t.requires_grad for t in (k, v, k_scale, v_scale)):
+            raise ValueError("a cache's tensors take no gradients")
+        self._k, self._v, self._k_scale, self._v_scale = k, v, k_scale, v_scale
         self.pages, self.heads, self.page = pages, heads, page
         self.code, self.device = CODES[k.dtype], k.get_device()
-        self._at = (k.data_ptr(), v.data_ptr(), *((None, None) if k_scale is None else (k_scale.data_ptr(), v_scale.data_ptr())))
+
+    # The tensors are the cache's for good (its shape is theirs): a larger or moved cache is another KVCache.
+    k = property(lambda self: self._k, doc="the keys' codes [pages, heads, page size, row]")
+    v = property(lambda self: self._v, doc="the values' codes [pages, heads, page size, row]")
+    k_scale = property(lambda self: self._k_scale, doc="the keys' scales [pages, heads, page size], None in 16 bits")
+    v_scale = property(lambda self: self._v_scale, doc="the values' scales [pages, heads, page size], None in 16 bits")
+
+    def addresses(self) -> tuple:
+        """k, v, k_scale, v_scale as the kernels take them: where they lie now."""
+        if self._k_scale is None:
+            return self._k.data_ptr(), self._v.data_ptr(), None, None
+        return self._k.data_ptr(), self._v.data_ptr(), self._k_scale.data_ptr(), self._v_scale.data_ptr()
 
     @classmethod
     def empty(cls, pages: int, page: int, heads: int, dim: int, codes: str = "int8",
@@ -102,9 +125,10 @@ class KVCache:
         if kd != 1 or vd != 1:
             k, v = k.contiguous(), v.contiguous()
             (kt, kh, _), (vt, vh, _) = k.stride(), v.stride()
+        refuse_gradients("KVCache.write", k, v)
         slots = self._slots(slots, size[0])
         _entries()[0](self.device, k.data_ptr(), v.data_ptr(), kt, kh, vt, vh, DTYPES[dtype], slots.data_ptr(), size[0],
-                      *self._at, self.pages, self.page, self.heads, self.dim, self.code)
+                      *self.addresses(), self.pages, self.page, self.heads, self.dim, self.code)
 
     def read(self, slots: torch.Tensor, dtype: torch.dtype = torch.bfloat16) -> tuple[torch.Tensor, torch.Tensor]:
         """The keys and values held in slots (int64 [n]) as [n, heads, dim] of `dtype`: code * scale in 32 bits, rounded
@@ -115,8 +139,8 @@ class KVCache:
         slots = self._slots(slots, n)
         k = torch.empty((n, self.heads, self.dim), dtype=dtype, device=self.k.device)
         v = torch.empty_like(k)
-        _entries()[1](self.device, *self._at, self.pages, self.page, self.heads, self.dim, self.code, slots.data_ptr(), n,
-                      k.data_ptr(), v.data_ptr(), DTYPES[dtype])
+        _entries()[1](self.device, *self.addresses(), self.pages, self.page, self.heads, self.dim, self.code,
+                      slots.data_ptr(), n, k.data_ptr(), v.data_ptr(), DTYPES[dtype])
         return k, v
 
     def slots(self, table: torch.Tensor, start: torch.Tensor, count: int) -> torch.Tensor:

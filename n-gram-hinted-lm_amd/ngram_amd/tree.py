@@ -2,7 +2,7 @@
 package's counts and matches draft. A sequence of lengths[b] cached tokens gets up to 64 drafted ones in a step, their keys
 and values written behind the cached ones (the token i of the tree at position lengths[b] + i); each sees the cached tokens
 and its own ancestors, so every path of the tree is scored as if it were the sequence's continuation. One token without a
-mask is ordinary decoding.
+mask is ordinary decoding. There is no backward pass: queries that require gradients (with gradients on) raise.
 
   tree_attention(q, cache, table, lengths, mask=None, widths=None, scale=None, return_lse=False)
   tree_mask(parents)    the ancestors' bits of trees given by their parents
@@ -16,7 +16,7 @@ import math
 
 import torch
 
-from .kvcache import KVCache, check_table
+from .kvcache import KVCache, check_table, refuse_gradients
 from .lib import Entry, Lib
 
 WIDEST = 64  # tokens of a tree: the bits of a mask
@@ -80,6 +80,7 @@ def tree_attention(q: torch.Tensor, cache: KVCache, table: torch.Tensor, lengths
         raise ValueError(f"a {cache.k.dtype} cache takes queries of its own type: got {dtype}")
     if q.get_device() != cache.device:
         raise ValueError(f"q is on {q.device}, the cache on {cache.k.device}")
+    refuse_gradients("tree_attention", q)
     check_table(cache, table)
     tables, width = table.shape
     if tables != B:
@@ -100,7 +101,7 @@ def tree_attention(q: torch.Tensor, cache: KVCache, table: torch.Tensor, lengths
     out = torch.empty(size, dtype=dtype, device=device)
     lse = torch.empty(size[:3], dtype=torch.float32, device=device) if return_lse else None
     work = torch.empty(_work(B, T, cache.heads, group, dim, cache.code, width * cache.page), dtype=torch.uint8, device=device)
-    k, v, ks, vs = cache._at
+    k, v, ks, vs = cache.addresses()
     _entries()[0](cache.device, q.data_ptr(), qb, qt, qh, DTYPES[dtype], k, v, ks, vs, cache.pages, cache.page, cache.code,
                   table.data_ptr(), table.stride(0), width, lengths.data_ptr(),
                   None if widths is None else widths.data_ptr(), None if mask is None else mask.data_ptr(), B, T,

@@ -187,3 +187,41 @@ def test_refusals(gpu):
         c.slots(torch.zeros((1, 2)).cuda(), torch.zeros(1, dtype=torch.int32).cuda(), 1)
     with pytest.raises(ValueError):
         c.slots(torch.zeros((1, 2), dtype=torch.int32).cuda(), torch.zeros(2, dtype=torch.int32).cuda(), 1)
+
+
+def test_gradients_are_refused(gpu):
+    """Writing quantises and has no backward pass: keys or values that require gradients raise instead of losing them."""
+    import torch.autograd.forward_ad as fw
+
+    c = KVCache.empty(2, 16, 2, 64, "int8")
+    x, at = torch.randn(3, 2, 64).cuda(), torch.arange(3).cuda()
+    y = x.clone().requires_grad_(True)
+    for k, v in ((y, x), (x, y)):
+        with pytest.raises(RuntimeError, match="gradient"):
+            c.write(k, v, at)
+    with fw.dual_level(), pytest.raises(RuntimeError, match="gradient"):
+        c.write(fw.make_dual(x, x), x, at)
+    assert not c.k.any()
+    with torch.no_grad():
+        c.write(y, y, at)
+    assert c.k.any()
+    b = KVCache.empty(2, 16, 2, 64, "bf16")
+    with pytest.raises(ValueError):
+        KVCache(b.k.clone().requires_grad_(True), b.v)  # the cache is no leaf to train
+
+
+def test_the_tensors_are_not_replaced(gpu):
+    """The cache's tensors are its own for good: assigning others raises. One whose memory is exchanged in place is used
+    where it lies now."""
+    c = KVCache.empty(2, 16, 2, 64, "int8")
+    for name in ("k", "v", "k_scale", "v_scale"):
+        with pytest.raises(AttributeError):
+            setattr(c, name, getattr(c, name).clone())
+    x, at = torch.randn(3, 2, 64).cuda(), torch.arange(3).cuda()
+    before = [t.data for t in (c.k, c.v, c.k_scale, c.v_scale)]  # the old memory stays alive
+    for t in (c.k, c.v, c.k_scale, c.v_scale):
+        t.data = torch.zeros_like(t)
+    c.write(x, x, at)
+    assert not any(t.float().any() for t in before)
+    want, scale = _quantise(x, "int8")
+    assert torch.equal(c.read(at, torch.float32)[1], want * scale[..., None])

@@ -558,3 +558,22 @@ def test_codes_of_nan_in_a_masked_token(gpu, side):
         assert torch.isnan(got[see][..., [9, 33]]).all()
         rest = [d for d in range(64) if d not in (9, 33)]
         assert torch.equal(got[see][..., rest], want[see][..., rest]) and torch.equal(gl, wl)
+
+
+def test_gradients_are_refused(gpu):
+    """There is no backward pass: queries that require gradients raise instead of losing them."""
+    import torch.autograd.forward_ad as fw
+
+    q, cache, table, ln, _ = _make(51, 2, 2, 1, 1, 64, "int8", torch.bfloat16, [10, 20])
+    want = tree_attention(q, cache, table, ln)
+    x = q.clone().requires_grad_(True)
+    with pytest.raises(RuntimeError, match="gradient"):
+        tree_attention(x, cache, table, ln)
+    with torch.no_grad():
+        assert torch.equal(tree_attention(x, cache, table, ln), want)
+    with torch.inference_mode():
+        assert torch.equal(tree_attention(x, cache, table, ln), want)
+    with fw.dual_level():
+        with pytest.raises(RuntimeError, match="gradient"):
+            tree_attention(fw.make_dual(q, torch.ones_like(q)), cache, table, ln)
+        assert torch.equal(tree_attention(q, cache, table, ln), want)
