@@ -20,12 +20,11 @@ bits, rounded once. Everything runs on the current stream; csrc/embed.hip has th
 from __future__ import annotations
 
 import functools
-import math
 
 import torch
 from torch.autograd import forward_ad
 
-from .lib import Entry, Lib
+from .lib import Entry, Lib, float32
 
 DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 _TOKENS = {torch.int64: 8, torch.int32: 4, torch.uint16: 2}
@@ -90,7 +89,7 @@ def _forward(weight, tokens, weights, cell, shape, scale):
     return out
 
 
-def _check(weight, tokens, weights, cell, scale) -> tuple:
+def _check(weight, tokens, weights, cell) -> tuple:
     """The shape of the call: the output's leading shape, positions, entries a position and entries a slot."""
     if weight.dim() != 2 or weight.dtype not in DTYPES:
         raise ValueError(f"weight must be [vocab, dim] in float32, bfloat16 or float16: got {tuple(weight.shape)} "
@@ -106,8 +105,6 @@ def _check(weight, tokens, weights, cell, scale) -> tuple:
     for name, t in (("tokens", tokens), ("weights", weights), ("cell", cell)):
         if t is not None and t.get_device() != device:
             raise ValueError(f"{name} is on {t.device}, weight on {weight.device}")
-    if not math.isfinite(scale):
-        raise ValueError(f"scale must be finite: {scale}")
     size = tokens.shape
     if weights is None:
         if cell is not None:
@@ -132,8 +129,8 @@ def embed(weight: torch.Tensor, tokens: torch.Tensor, weights: torch.Tensor | No
           cell: torch.Tensor | None = None, scale: float = 1.0) -> torch.Tensor:
     """Embedded rows [n, dim] of tokens and float32 weights [n, entries] or [n, slots, entries], cell [n] or [n, slots]
     (None: every slot counts), or without weights the scaled lookup [*tokens.shape, dim]; in weight's type."""
-    scale = float(scale)
-    shape = _check(weight, tokens, weights, cell, scale)
+    scale = float32("scale", scale)
+    shape = _check(weight, tokens, weights, cell)
     tokens = tokens.contiguous()
     weights = None if weights is None else weights.contiguous()
     cell = None if cell is None else cell.contiguous()

@@ -123,6 +123,14 @@ class Lib:
         return int(fn(*(ctypes.c_int64(a) for a in args)))
 
 
+def float32(name: str, x: float) -> float:
+    """x as a float that a C float argument holds; ValueError where it would be infinite or NaN there."""
+    x = float(x)
+    if not abs(x) < 2.0**128 - 2.0**103:  # halfway from the largest float32 to 2^128
+        raise ValueError(f"{name} must be finite in float32: {x}")
+    return x
+
+
 _TYPES = {"p": _ptr, "q": _i64, "i": _i32, "f": ctypes.c_float}
 
 

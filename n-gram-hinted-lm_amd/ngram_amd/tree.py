@@ -17,7 +17,7 @@ import math
 import torch
 
 from .kvcache import KVCache, check_table, refuse_gradients
-from .lib import Entry, Lib
+from .lib import Entry, Lib, float32
 
 WIDEST = 64  # tokens of a tree: the bits of a mask
 DTYPES = {torch.bfloat16: 1, torch.float16: 2}
@@ -90,9 +90,7 @@ def tree_attention(q: torch.Tensor, cache: KVCache, table: torch.Tensor, lengths
         mask = _check("mask", mask, (B, T), torch.int64, cache)
     if widths is not None:
         widths = _check("widths", widths, (B,), torch.int32, cache)
-    scale = 1 / math.sqrt(dim) if scale is None else float(scale)
-    if not math.isfinite(scale):
-        raise ValueError(f"scale must be finite: {scale}")
+    scale = 1 / math.sqrt(dim) if scale is None else float32("scale", scale)
     qb, qt, qh, qd = q.stride()
     if qd != 1 and dim > 1:
         q = q.contiguous()

@@ -311,3 +311,10 @@ def test_forward_mode_is_refused(gpu):
         with pytest.raises(RuntimeError, match="jvp"):
             embed(fw.make_dual(table, table), tokens)
         assert torch.equal(embed(table, tokens, weights, cell), want)
+
+
+def test_scales_that_are_no_float32_are_refused(gpu):
+    t, tok = torch.randn(9, 16).cuda(), torch.zeros(5, dtype=torch.int64).cuda()
+    for scale in (1e39, -1e39, float("inf")):
+        with pytest.raises(ValueError, match="scale"):
+            embed(t, tok, scale=scale)

@@ -577,3 +577,10 @@ def test_gradients_are_refused(gpu):
         with pytest.raises(RuntimeError, match="gradient"):
             tree_attention(fw.make_dual(q, torch.ones_like(q)), cache, table, ln)
         assert torch.equal(tree_attention(q, cache, table, ln), want)
+
+
+def test_scales_that_are_no_float32_are_refused(gpu):
+    q, cache, table, ln, _ = _make(53, 2, 2, 1, 1, 64, "int8", torch.bfloat16, [10, 20])
+    for scale in (1e39, -1e39, float("nan")):
+        with pytest.raises(ValueError, match="scale"):
+            tree_attention(q, cache, table, ln, scale=scale)
