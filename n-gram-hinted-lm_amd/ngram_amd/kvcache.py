@@ -150,8 +150,8 @@ class KVCache:
         B, width = table.shape
         if start.dtype != torch.int32 or start.shape != (B,) or start.get_device() != self.device:
             raise ValueError(f"start must be int32 [{B}] on {self.k.device}")
-        if count < 0:
-            raise ValueError(f"count must not be negative: {count}")
+        if not 0 <= count < 1 << 31:
+            raise ValueError(f"count must be 0 to 2^31 - 1: {count}")
         start = start.contiguous()
         out = torch.empty((B, count), dtype=torch.int64, device=self.k.device)
         _entries()[2](self.device, table.data_ptr(), table.stride(0), width, start.data_ptr(), B, count, self.pages,

@@ -225,3 +225,11 @@ def test_the_tensors_are_not_replaced(gpu):
     assert not any(t.float().any() for t in before)
     want, scale = _quantise(x, "int8")
     assert torch.equal(c.read(at, torch.float32)[1], want * scale[..., None])
+
+
+def test_counts_past_32_bits_are_refused(gpu):
+    c = KVCache.empty(2, 16, 2, 64, "int8")
+    table, start = torch.zeros((1, 2), dtype=torch.int32).cuda(), torch.zeros(1, dtype=torch.int32).cuda()
+    for count in (1 << 31, (1 << 32) + 1):
+        with pytest.raises(ValueError):
+            c.slots(table, start, count)
