@@ -318,3 +318,42 @@ def test_scales_that_are_no_float32_are_refused(gpu):
     for scale in (1e39, -1e39, float("inf")):
         with pytest.raises(ValueError, match="scale"):
             embed(t, tok, scale=scale)
+
+
+def _sums(V, tok, up):
+    want = torch.zeros((V, up.shape[1]), device="cuda", dtype=torch.float64).index_add_(0, tok, up.double())
+    size = torch.zeros_like(want).index_add_(0, tok, up.double().abs())
+    return want, size, torch.zeros((V, 1), device="cuda", dtype=torch.float64).index_add_(
+        0, tok, torch.ones((len(tok), 1), device="cuda", dtype=torch.float64))
+
+
+def _check_sums(grad, tok, up):
+    want, size, many = _sums(grad.shape[0], tok, up)
+    bound = 2.0**-24 * want.abs() + (many + 4) * 2.0**-24 * size * (1 + 2.0**-24) + 2.0**-149
+    assert ((grad.double() - want).abs() <= bound).all()
+
+
+@pytest.mark.parametrize("n", [(1 << 21) + 1, 3000001])
+def test_gradient_of_many_entries(gpu, n):
+    """More than 2^21 entries: the sort's spans grow past their smallest."""
+    g = torch.Generator(device="cuda").manual_seed(n)
+    V = 70001
+    tok = (torch.rand(n, generator=g, device="cuda") ** 3 * V).long().clamp_(max=V - 1)
+    up = torch.randn((n, 4), generator=g, device="cuda")
+    t = torch.zeros((V, 4), device="cuda", requires_grad=True)
+    (grad,) = torch.autograd.grad(embed(t, tok), [t], up)
+    _check_sums(grad, tok, up)
+
+
+@pytest.mark.parametrize("n", [300, 50001])
+def test_gradient_of_a_table_past_24_bits(gpu, n):
+    """More than 2^24 rows: a fourth pass of digits, by one block and by many."""
+    g = torch.Generator(device="cuda").manual_seed(n)
+    V = (1 << 24) + 1001
+    tok = torch.randint(0, V, (n,), generator=g, device="cuda")
+    tok[:200] = V - 1 - tok[:200] % 7
+    tok[200:220] = tok[200:220] % 1000 + (1 << 24)
+    up = torch.randn((n, 2), generator=g, device="cuda")
+    t = torch.zeros((V, 2), device="cuda", requires_grad=True)
+    (grad,) = torch.autograd.grad(embed(t, tok), [t], up)
+    _check_sums(grad, tok, up)
