@@ -77,6 +77,7 @@ class KVCache:
         self._k, self._v, self._k_scale, self._v_scale = k, v, k_scale, v_scale
         self.pages, self.heads, self.page = pages, heads, page
         self.code, self.device = CODES[k.dtype], k.get_device()
+        self._ptr = tuple(None if t is None else t.data_ptr for t in (k, v, k_scale, v_scale))
 
     # The tensors are the cache's for good (its shape is theirs): a larger or moved cache is another KVCache.
     k = property(lambda self: self._k, doc="the keys' codes [pages, heads, page size, row]")
@@ -86,9 +87,8 @@ class KVCache:
 
     def addresses(self) -> tuple:
         """k, v, k_scale, v_scale as the kernels take them: where they lie now."""
-        if self._k_scale is None:
-            return self._k.data_ptr(), self._v.data_ptr(), None, None
-        return self._k.data_ptr(), self._v.data_ptr(), self._k_scale.data_ptr(), self._v_scale.data_ptr()
+        k, v, ks, vs = self._ptr
+        return k(), v(), ks and ks(), vs and vs()
 
     @classmethod
     def empty(cls, pages: int, page: int, heads: int, dim: int, codes: str = "int8",
@@ -125,7 +125,8 @@ class KVCache:
         if kd != 1 or vd != 1:
             k, v = k.contiguous(), v.contiguous()
             (kt, kh, _), (vt, vh, _) = k.stride(), v.stride()
-        refuse_gradients("KVCache.write", k, v)
+        if k.requires_grad or v.requires_grad or forward_ad._current_level >= 0:
+            refuse_gradients("KVCache.write", k, v)
         slots = self._slots(slots, size[0])
         _entries()[0](self.device, k.data_ptr(), v.data_ptr(), kt, kh, vt, vh, DTYPES[dtype], slots.data_ptr(), size[0],
                       *self.addresses(), self.pages, self.page, self.heads, self.dim, self.code)

@@ -15,6 +15,7 @@ import functools
 import math
 
 import torch
+from torch.autograd import forward_ad
 
 from .kvcache import KVCache, check_table, refuse_gradients
 from .lib import Entry, Lib, float32
@@ -80,7 +81,8 @@ def tree_attention(q: torch.Tensor, cache: KVCache, table: torch.Tensor, lengths
         raise ValueError(f"a {cache.k.dtype} cache takes queries of its own type: got {dtype}")
     if q.get_device() != cache.device:
         raise ValueError(f"q is on {q.device}, the cache on {cache.k.device}")
-    refuse_gradients("tree_attention", q)
+    if q.requires_grad or forward_ad._current_level >= 0:
+        refuse_gradients("tree_attention", q)
     check_table(cache, table)
     tables, width = table.shape
     if tables != B:
