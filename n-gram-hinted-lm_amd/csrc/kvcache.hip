@@ -8,7 +8,9 @@
 // and nothing of it reaches a row that masks it.
 //
 // Both directions move every byte once and compute little: memory bounds them. A row is 8 elements a lane (8, 16 or 32
-// lanes by DP), so that the 16-bit side moves 16 bytes a lane and a row's lanes cover whole 128-byte lines.
+// lanes by DP), so that the 16-bit side moves 16 bytes a lane and a row's lanes cover whole 128-byte lines. Measured, 8
+// heads of 128, bfloat16 to and from int8: 4096 tokens written 11.2 us (2.3 TB/s; one filling of the card, its start and
+// end count), 32768 read 45 us (4.5 TB/s); 8 tokens written 3.3 us, a launch.
 #include "vals.h"
 
 template <typename T> __device__ __forceinline__ void load8(const T* p, int d0, int dim, bool vec, float (&x)[8]) {

@@ -7,7 +7,9 @@ mask is ordinary decoding. There is no backward pass: queries that require gradi
   tree_attention(q, cache, table, lengths, mask=None, widths=None, scale=None, return_lse=False)
   tree_mask(parents)    the ancestors' bits of trees given by their parents
 
-Everything runs on the current stream; lengths and widths are read on the device only. csrc/tree.hip has the kernels."""
+Scores, the softmax's sums and the outputs' are held in 32 bits; a weight is rounded to 16 bits for its product with the
+values (float16, bfloat16 over a bfloat16 cache), as an output is. Everything runs on the current stream; lengths and widths
+are read on the device only. csrc/tree.hip has the kernels."""
 
 from __future__ import annotations
 
@@ -65,7 +67,8 @@ def tree_attention(q: torch.Tensor, cache: KVCache, table: torch.Tensor, lengths
     table    int32 [B, width]: the sequences' pages in order; keys whose entry is no page of the cache are masked
     lengths  int32 [B]: the cached tokens before the tree (held to 0 .. what the table covers)
     mask     int64 [B, T]: bit j of [b, i] lets tree token i see tree token j; None: a chain (i sees 0 .. i)
-    widths   int32 [B]: the tree tokens in use (None: all T); the rows past them are zeros, their keys masked
+    widths   int32 [B]: the tree tokens in use (None: all T); the rows past them are zeros, whatever q holds there, their
+             keys masked
     scale    the scores' factor, 1 / sqrt(dim) by default
 
     Returns the output in q's shape and type, and with return_lse the float32 [B, T, heads * group] logarithms of the
