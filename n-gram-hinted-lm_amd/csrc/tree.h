@@ -512,17 +512,17 @@ template <int CODES, int DP, int R> struct Tree {
 
     // The factors of a tile's keys, computed by one lane each and handed through LDS to the lanes that hold their scores:
     // the score's factor, the logarithm and the inverse of the value scale.
-    // True where a value scale is below NONE: the weights then take fac[3] more.
+    // True where a value scale is below NONE, or negative: the weights then take fac[3] more.
     static __device__ __forceinline__ bool factors(float scale, bool in, const State& s, float (*fac)[32]) {
         const int key = lane_id() & 31;
         const bool low = in && lane_id() >= 32 && scale < NONE;
         if (lane_id() < 32) fac[0][key] = scale * s.c;
         else {
-            float x = low ? NONE : scale;
+            float x = low ? fmaxf(__builtin_fabsf(scale), NONE) : scale;
             x = in ? x : 1.f;
             fac[1][key] = __builtin_amdgcn_logf(x);
             fac[2][key] = __builtin_amdgcn_rcpf(x);
-            if (__any(low)) fac[3][key] = low ? scale * (1.f / NONE) : 1.f;
+            if (__any(low)) fac[3][key] = low && finite_f(scale) ? scale * fac[2][key] : 1.f;  // (-inf: 0 times it is no 0)
         }
         __builtin_amdgcn_wave_barrier();
         return __any(low);
@@ -605,7 +605,7 @@ template <int CODES, int DP, int R> struct Tree {
         }
     }
 
-    // The weights of value rows whose scale is below NONE.
+    // The weights of value rows whose scale is below NONE, or negative.
     static __device__ __forceinline__ void lower(const float (*fac)[32], V8 (&p)[R]) {
         const int g = lane_id() >> 4;
 #pragma unroll

@@ -6,7 +6,7 @@ Codes lie in pages, [pages, heads, page size, dim padded with zeros to a multipl
   bf16, fp16   x itself
 and the 8-bit ones have a float32 scale a / 127 or a / 448 per token and head, [pages, heads, page size]. A row that is
 zero (or too small for its inverse) has scale 0; one that holds a NaN or an infinity has codes 0 and scale NaN, so that it
-reads back as NaN and nothing of it enters where it is masked. Scales are not negative; a scale of 0 stands for zeros.
+reads back as NaN and nothing of it enters where it is masked. A scale of 0 stands for zeros whatever the codes are.
 
 A token's slot is page * page size + its row there; a sequence's page table lists its pages in order, and -1 stands for no
 slot. Which page belongs to whom is the caller's. Quantising has no backward pass: keys and values that require gradients

@@ -584,3 +584,20 @@ def test_scales_that_are_no_float32_are_refused(gpu):
     for scale in (1e39, -1e39, float("nan")):
         with pytest.raises(ValueError, match="scale"):
             tree_attention(q, cache, table, ln, scale=scale)
+
+
+@pytest.mark.parametrize("codes", ["int8", "fp8"])
+def test_negative_scales(gpu, codes):
+    """Scales below 0 (a cache from elsewhere), of values and keys: code * scale, as read() has them; an infinite one in a
+    masked token shows nowhere else."""
+    q, cache, table, ln = _with_values(55, codes, [300, 5, 40], 1.0, [], 0.0)
+    cache.v_scale.view(-1)[::3] *= -1
+    cache.k_scale.view(-1)[1::5] *= -1
+    out, lse = tree_attention(q, cache, table, ln, return_lse=True)
+    _rows(out, q, cache, table, ln, _chain(3, 2), lse=lse)
+    at = cache.slots(table, ln + 1, 1)[:, 0]
+    for x in (-float("inf"), float("inf")):
+        cache.v_scale[at // 16, :, at % 16] = x  # the second token: the first does not see it
+        got, gl = tree_attention(q, cache, table, ln, return_lse=True)
+        assert torch.equal(got[:, 0], out[:, 0]) and torch.equal(gl[:, 0], lse[:, 0])
+        assert torch.isnan(got[:, 1]).any(-1).all()
