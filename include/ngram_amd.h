@@ -575,6 +575,63 @@ int ng_tree_attention(const void* q, ng_i64 qb, ng_i64 qt, ng_i64 qh, int qtype,
                       int T, int H, int G, int dim, float scale, void* out, float* lse, void* work, void* stream);
 int ng_tree_mask(const int* parents, int B, int T, ng_u64* bits, void* stream);
 
+/* A beam search's step: of the candidates of W beams (logits [B, W, V] of dtype, strides sb, sw in elements; scores float32
+ * [B, W]; lengths [B, W] of lsize bytes (4, 8) or NULL; finished bytes [B, W] or NULL) the K best, ranked by (score + logit - log sum exp) /
+ * max(length + 1, 1)^alpha; a finished beam has one, `pad` at its own score and length. out_scores, parents (b * W + w), tokens
+ * [B, K]; out_finished bytes [B, K] (token == end, or a finished parent) or NULL; out_lengths [B, K] or NULL; work:
+ * ng_beam_work(B, W, V, K) bytes (-1: out of range; W, K <= 128, V <= 2^25, K * V <= 2^27).
+ * ng_gather_rows: out row i = src row from[i], of `bytes` bytes at a multiple of `stride` bytes; zeros outside [0, rows). */
+ng_i64 ng_beam_work(ng_i64 B, ng_i64 W, ng_i64 V, ng_i64 K);
+int ng_beam_step(const void* logits, ng_i64 sb, ng_i64 sw, int dtype, const float* scores, const void* lengths,
+                 int lsize, const void* finished, int B, int W, int V, int K, int end, int pad, float alpha, float* out_scores,
+                 ng_i64* parents, ng_i64* tokens, void* out_finished, ng_i64* out_lengths, void* work, void* stream);
+int ng_gather_rows(const void* src, ng_i64 stride, ng_i64 rows, ng_i64 bytes, const ng_i64* from, ng_i64 n, void* out,
+                   void* stream);
+
+/* Who holds a cache's pages. state: ng_pool_state(pages) bytes, from ng_pool_clear on: int32 [pages] counts of the table
+ * entries that hold each page first, the int32 count of pages not to be had last. Tables int32 [S, width] of row stride
+ * `stride`, entries outside [0, pages) are no page.
+ * ng_pool_hold: a table's entries counted. ng_pool_fork: row s of table and lengths := row parents[s] (outside [0, S): empty);
+ * work: ng_pool_fork_work bytes. ng_pool_room: positions lengths[s] .. + count - 1 (counts[s] where counts is not NULL) get
+ * pages of the row's own, a shared page's first rows copied; slots [S, count], -1 where there is none; work:
+ * ng_pool_room_work(S, count, page) bytes. ng_pool_move: the pages in use, packed, to another pool's cache and state; out
+ * [S, width] the table there; bounds NULL or both. ng_copy_pages: page dst[i] := page src[i]. Caches as in ng_kv_write;
+ * bounds: bfloat16 [pages, heads, 2, DP]. */
+ng_i64 ng_pool_state(ng_i64 pages);
+int ng_pool_clear(void* state, ng_i64 pages, void* stream);
+int ng_pool_hold(void* state, ng_i64 pages, const int* table, ng_i64 stride, int S, int width, void* stream);
+ng_i64 ng_pool_fork_work(ng_i64 S, ng_i64 width);
+int ng_pool_fork(void* state, ng_i64 pages, int* table, ng_i64 stride, int S, int width, int* lengths, const ng_i64* parents,
+                 void* work, void* stream);
+ng_i64 ng_pool_room_work(ng_i64 S, ng_i64 count, ng_i64 page);
+int ng_pool_room(void* state, ng_i64 pages, int* table, ng_i64 stride, int S, int width, const int* lengths, const int* counts,
+                 int count, void* k, void* v, void* ks, void* vs, int page, int heads, int dim, int codes, ng_i64* slots,
+                 void* work, void* stream);
+ng_i64 ng_pool_move_work(ng_i64 pages, ng_i64 to_pages);
+int ng_pool_move(void* state, ng_i64 pages, const void* k, const void* v, const void* ks, const void* vs, const void* bounds,
+                 void* to_state, ng_i64 to_pages, void* to_k, void* to_v, void* to_ks, void* to_vs, void* to_bounds, int page,
+                 int heads, int dim, int codes, const int* table, ng_i64 stride, int S, int width, int* out, void* work,
+                 void* stream);
+int ng_copy_pages(const void* k, const void* v, const void* ks, const void* vs, const void* bounds, ng_i64 pages, void* to_k,
+                  void* to_v, void* to_ks, void* to_vs, void* to_bounds, ng_i64 to_pages, int page, int heads, int dim,
+                  int codes, const ng_i64* src, const ng_i64* dst, ng_i64 n, void* stream);
+
+/* Attention over the pages that a score keeps. bounds bfloat16 [pages, heads, 2, DP]: each page's smallest and largest key
+ * elements. ng_page_bounds: those of the pages that positions start[b] .. start[b] + count - 1 lie in and complete.
+ * ng_sparse_attention: q [B, T, H * G, dim] as in ng_tree_attention, token t of sequence b at position lengths[b] + t, widths
+ * [B] or NULL the tokens in use; of the pages up to its own each (token, cached head) keeps the `first` first, the `last` last
+ * and the best others, `keep` in all. out [B, T, H * G, dim]; lse [B, T, H * G] or NULL; chosen int32 [B, T, H, keep] or NULL;
+ * work: ng_sparse_work(B, T, H, G, dim, width, page, keep) bytes (-1: out of range; width <= 32768, width * page <= 2^30,
+ * keep <= 1024). */
+int ng_page_bounds(const void* k, const float* ks, ng_i64 pages, int page, int heads, int dim, int codes, const int* table,
+                   ng_i64 stride, int width, const int* start, int B, int count, void* bounds, void* stream);
+ng_i64 ng_sparse_work(ng_i64 B, ng_i64 T, ng_i64 H, ng_i64 G, ng_i64 dim, ng_i64 width, ng_i64 page, ng_i64 keep);
+int ng_sparse_attention(const void* q, ng_i64 qb, ng_i64 qt, ng_i64 qh, int qtype, const void* k, const void* v,
+                        const float* ks, const float* vs, const void* bounds, ng_i64 pages, int page, int codes,
+                        const int* table, ng_i64 table_stride, int width, const int* lengths, const int* widths, int B, int T,
+                        int H, int G, int dim, int keep, int first, int last, float scale, void* out, float* lse, int* chosen,
+                        void* work, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

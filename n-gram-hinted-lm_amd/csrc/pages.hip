@@ -1,0 +1,483 @@
+// The pages of a paged key/value cache: who holds them, room for more tokens, and copies of them.
+//
+// State: refs[p], the table entries that hold page p; free, a bit a page, set where refs is 0. asks and claim, 0 and INT_MAX
+// for each page between calls, are a reservation's own.
+//
+// Fork: row s of a table becomes what row parents[s] was. refs[p] += children(row) - 1 for each entry of each row, one atomic
+// an entry and none where a row has one child; every holder's change is -1 at least and refs counts them all, so a count
+// reaches 0 only by its last change, which sets the free bit. The entries go through a scratch table (rows read each
+// other), only the rows that move.
+//
+// Room: positions length .. length + count - 1 of each row, a request per page that holds any of them. A request is met by
+// the entry it finds where no other row holds that page, or where all that hold it request it here and this is the first of
+// them (atomic minimum and count: the order of atomics changes nothing); else by the lowest free pages in the order of rows.
+// One block does this, since each page given depends on all before it: the requests are scanned 1024 at a time and the free
+// bits 32768 pages at a time, up to the last one needed. The rows of a shared page that lie before the length are copied by
+// a second kernel, a block per row and head, which also writes the slots.
+//
+// Counts and pages are whole numbers and every choice is by order, so a call gives the same pages on every run.
+#include "vals.h"
+#include <climits>
+
+struct Pool {
+    int* refs;
+    u32* free;
+    int *asks, *claim;
+    int* missing;
+    i64 pages;
+};
+
+__device__ __forceinline__ int load_agent(const int* p) {  // past the L1: what atomics have made of it
+    return __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+
+__global__ __launch_bounds__(256) void pool_clear_k(const Pool p) {
+    const i64 words = (p.pages + 31) / 32, step = (i64)gridDim.x * 256;
+    for (i64 i = blockIdx.x * 256ll + threadIdx.x; i < p.pages; i += step) {
+        p.refs[i] = 0, p.asks[i] = 0, p.claim[i] = INT_MAX;
+        if (i < words) p.free[i] = i * 32 + 32 <= p.pages ? ~0u : (1u << (p.pages & 31)) - 1;
+        if (i == 0) *p.missing = 0;
+    }
+}
+
+__device__ __forceinline__ bool is_page(const Pool& p, int e) { return (u32)e < (u64)p.pages; }
+
+__global__ __launch_bounds__(256) void pool_hold_k(const Pool p, const int* __restrict__ table, i64 stride, int S, int width) {
+    const i64 n = (i64)S * width;
+    for (i64 i = blockIdx.x * 256ll + threadIdx.x; i < n; i += (i64)gridDim.x * 256) {
+        const i64 s = i / width;
+        const int e = table[s * stride + (i - s * width)];
+        if (is_page(p, e) && atomicAdd(&p.refs[e], 1) == 0) atomicAnd(&p.free[e >> 5], ~(1u << (e & 31)));
+    }
+}
+
+// ---------------------------------------------------------------------------------------------------------------- fork
+
+#define STRIP 2048  // a block's columns
+
+__global__ __launch_bounds__(256) void pool_fork_k(const Pool p, const int* __restrict__ table, i64 stride, int S, int width,
+                                                   const int* __restrict__ lengths, const i64* __restrict__ parents,
+                                                   int* __restrict__ moved, int* __restrict__ moved_len) {
+    __shared__ int children;
+    const int s = blockIdx.x, tid = threadIdx.x;
+    if (tid == 0) children = 0;
+    __syncthreads();
+    int n = 0;
+    for (int i = tid; i < S; i += 256) n += parents[i] == s;
+    if (n) atomicAdd(&children, n);
+    __syncthreads();
+    const int change = children - 1;
+    const i64 from = parents[s];
+    const bool is = (u64)from < (u64)S;
+    const int c1 = (blockIdx.y + 1) * STRIP < width ? (blockIdx.y + 1) * STRIP : width;
+    for (int c = blockIdx.y * STRIP + tid; c < c1; c += 256) {
+        if (change) {
+            const int e = table[s * stride + c];
+            if (is_page(p, e) && atomicAdd(&p.refs[e], change) + change == 0) atomicOr(&p.free[e >> 5], 1u << (e & 31));
+        }
+        if (from != s) moved[(i64)s * width + c] = is ? table[from * stride + c] : -1;
+    }
+    if (blockIdx.y == 0 && tid == 0) moved_len[s] = is ? lengths[from] : 0;
+}
+
+__global__ __launch_bounds__(256) void pool_moved_k(int* __restrict__ table, i64 stride, int width, int* __restrict__ lengths,
+                                                    const i64* __restrict__ parents, const int* __restrict__ moved,
+                                                    const int* __restrict__ moved_len) {
+    const int s = blockIdx.x;
+    if (parents[s] == s) return;
+    const int c1 = (blockIdx.y + 1) * STRIP < width ? (blockIdx.y + 1) * STRIP : width;
+    for (int c = blockIdx.y * STRIP + threadIdx.x; c < c1; c += 256) table[s * stride + c] = moved[(i64)s * width + c];
+    if (blockIdx.y == 0 && threadIdx.x == 0) lengths[s] = moved_len[s];
+}
+
+// ---------------------------------------------------------------------------------------------------------------- room
+
+struct Room {
+    int* table;
+    i64 stride;
+    const int *lengths, *counts;  // counts: NULL, or each row's own
+    int S, width, count, shift, per;  // per: requests a row
+    int* rank;    // [S * per]: a request's place among those for a free page; KEPT, NONE
+    int* page;    // [S * per]: the page a request found, then the one it has got; -1
+    int* given;   // [S * per]: the lowest free pages
+    int* source;  // [S]: the page whose first rows are copied to page[s * per], -1
+};
+enum { KEPT = -1, NONE = -2 };
+
+struct Ask {
+    int column, entry;
+    bool is, held;
+};
+
+__device__ __forceinline__ int row_count(const Room& r, int s) {
+    const int n = r.counts ? r.counts[s] : r.count;
+    return n < 0 ? 0 : n < r.count ? n : r.count;
+}
+
+__device__ __forceinline__ Ask ask_of(const Pool& p, const Room& r, int i) {
+    const int s = i / r.per, j = i - s * r.per, len = r.lengths[s] < 0 ? 0 : r.lengths[s];
+    Ask q;
+    q.column = (len >> r.shift) + j;
+    q.is = ((i64)q.column << r.shift) < (i64)len + row_count(r, s) && q.column < r.width && row_count(r, s) > 0;
+    q.entry = q.is ? r.table[s * r.stride + q.column] : -1;
+    q.held = q.is && is_page(p, q.entry) && p.refs[q.entry] > 0;  // (an entry that was never counted is none)
+    return q;
+}
+
+// The sum over a block of 1024 of the threads before this one, and the whole.
+__device__ __forceinline__ int scan_block(int x, int* lds, int& total) {
+    int inc = x;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+        const int up = __shfl_up(inc, o, 64);
+        if (lane_id() >= o) inc += up;
+    }
+    __syncthreads();  // (lds was read by the call before)
+    if (lane_id() == 63) lds[threadIdx.x >> 6] = inc;
+    __syncthreads();
+    int before = 0;
+    total = 0;
+#pragma unroll
+    for (int w = 0; w < 16; ++w) {
+        before += w < (int)(threadIdx.x >> 6) ? lds[w] : 0;
+        total += lds[w];
+    }
+    return before + inc - x;
+}
+
+__global__ __launch_bounds__(1024) void pool_room_k(const Pool p, const Room r) {
+    __shared__ int sums[16];
+    const int n = r.S * r.per, tid = threadIdx.x;
+    // who else asks for a shared page
+    for (int i = tid; i < n; i += 1024) {
+        const Ask q = ask_of(p, r, i);
+        if (q.held && p.refs[q.entry] != 1) {
+            atomicAdd(&p.asks[q.entry], 1);
+            atomicMin(&p.claim[q.entry], i);
+        }
+    }
+    __syncthreads();
+    int wanted = 0;
+    for (int i0 = 0; i0 < n; i0 += 1024) {
+        const int i = i0 + tid;
+        bool want = false, is = false;
+        int entry = -1;
+        if (i < n) {
+            const Ask q = ask_of(p, r, i);
+            is = q.is;
+            want = q.is;
+            if (q.held) {
+                entry = q.entry;
+                const int refs = p.refs[q.entry];
+                want = refs != 1 && !(refs == load_agent(&p.asks[q.entry]) && load_agent(&p.claim[q.entry]) == i);
+            }
+        }
+        int total;
+        const int at = scan_block(want, sums, total);
+        if (i < n) r.rank[i] = want ? wanted + at : is ? KEPT : NONE, r.page[i] = entry;
+        wanted += total;
+    }
+    // the lowest free pages
+    const i64 words = (p.pages + 31) / 32;
+    int found = 0;
+    for (i64 w0 = 0; w0 < words && found < wanted; w0 += 1024) {
+        u32 bits = w0 + tid < words ? p.free[w0 + tid] : 0u;
+        int total, at = found + scan_block(__popc(bits), sums, total);
+        for (; bits && at < wanted; ++at, bits &= bits - 1) r.given[at] = (int)((w0 + tid) * 32 + __builtin_ctz(bits));
+        found += total;
+    }
+    if (found > wanted) found = wanted;
+    if (tid == 0 && wanted > found) *p.missing += wanted - found;
+    __syncthreads();
+    for (int i = tid; i < n; i += 1024) {
+        const int k = r.rank[i], held = r.page[i], s = i / r.per, j = i - s * r.per;
+        int page = k == KEPT ? held : -1, source = -1;
+        if (k >= 0 && k < found) {
+            page = r.given[k];
+            r.table[s * r.stride + ((r.lengths[s] < 0 ? 0 : r.lengths[s]) >> r.shift) + j] = page;
+            p.refs[page] = 1;
+            atomicAnd(&p.free[page >> 5], ~(1u << (page & 31)));
+            if (held >= 0) {
+                atomicSub(&p.refs[held], 1);
+                source = held;
+            }
+        }
+        if (held >= 0) p.asks[held] = 0, p.claim[held] = INT_MAX;
+        r.page[i] = page;
+        if (j == 0) r.source[s] = source;
+    }
+}
+
+// ------------------------------------------------------------------------------------------------------------- copies
+
+// What a page is made of: parts of `bytes` a row and head. (The bounds have one row a page and head.)
+struct Part {
+    const char* src;
+    char* dst;
+    i64 bytes;  // a row
+};
+struct Parts {
+    Part part[5];
+    int n, H, shift;
+    i64 src_pages, dst_pages;
+};
+
+__device__ __forceinline__ void copy_bytes(const char* s, char* d, i64 bytes) {  // both at multiples of 16 bytes
+    const i64 n = bytes / 16;
+    i64 i = threadIdx.x;
+    for (; i + 768 < n; i += 1024) {
+        uint4 x[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) x[k] = ((const uint4*)s)[i + k * 256];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) ((uint4*)d)[i + k * 256] = x[k];
+    }
+    for (; i < n; i += 256) ((uint4*)d)[i] = ((const uint4*)s)[i];
+    for (i = n * 4 + threadIdx.x; i < bytes / 4; i += 256) ((u32*)d)[i] = ((const u32*)s)[i];
+}
+
+// A block per (row, head): the slots of the row's positions (head 0), and the rows of a copied page.
+__global__ __launch_bounds__(256) void pool_slots_k(const Pool p, const Room r, const Parts c, i64* __restrict__ slots) {
+    const int s = blockIdx.x / c.H, h = blockIdx.x - s * c.H;
+    const int len = r.lengths[s] < 0 ? 0 : r.lengths[s], in = (1 << r.shift) - 1;
+    if (h == 0) {
+        const int own = row_count(r, s);
+        for (int i = threadIdx.x; i < r.count; i += 256) {
+            const i64 pos = (i64)len + i;
+            const int page = i < own ? r.page[s * r.per + (int)((pos >> r.shift) - (len >> r.shift))] : -1;
+            slots[(i64)s * r.count + i] = page < 0 ? -1 : ((i64)page << r.shift) + (pos & in);
+        }
+    }
+    const int rows = len & in, from = r.source[s];
+    if (!rows || from < 0) return;
+    const int to = r.page[s * r.per];
+    for (int k = 0; k < c.n; ++k) {
+        const Part& t = c.part[k];
+        copy_bytes(t.src + (((i64)from * c.H + h) << c.shift) * t.bytes, t.dst + (((i64)to * c.H + h) << c.shift) * t.bytes,
+                   rows * t.bytes);
+    }
+}
+
+// Page dst[i] of one cache := page src[i] of another, in pieces of PIECE bytes; entries that are no pages are passed over.
+// (src NULL: the list of `from`'s live pages, packed.)
+#define PIECE 65536
+template <typename I>
+__global__ __launch_bounds__(256) void copy_pages_k(const Parts c, const I* __restrict__ src, const I* __restrict__ dst, i64 n,
+                                                    int pieces) {
+    const i64 i = blockIdx.x / pieces;
+    const int piece = (int)(blockIdx.x - i * pieces);
+    const i64 a = src[i], b = dst ? (i64)dst[i] : i;
+    if ((u64)a >= (u64)c.src_pages || (u64)b >= (u64)c.dst_pages) return;
+    i64 at = (i64)piece * PIECE, end = at + PIECE;
+    for (int k = 0; k < c.n; ++k) {  // the parts laid end to end
+        const Part& t = c.part[k];
+        const i64 size = t.bytes * c.H << (k < 4 ? c.shift : 0);
+        const i64 x = at < 0 ? 0 : at, y = end < size ? end : size;
+        if (x < y) copy_bytes(t.src + a * size + x, t.dst + b * size + x, y - x);
+        at -= size, end -= size;
+        if (end <= 0) break;
+    }
+}
+
+// The live pages in order: list[i] = the i-th, map[p] = its place (-1), and the other pool's state. A block per 1024 words of
+// free bits, which counts the words before its own by itself.
+__global__ __launch_bounds__(1024) void pool_pack_k(const Pool p, const Pool to, int* __restrict__ list, int* __restrict__ map) {
+    __shared__ int sums[16];
+    const i64 words = (p.pages + 31) / 32;
+    const int tid = threadIdx.x;
+    auto live = [&](i64 w) {
+        return w < words ? ~p.free[w] & (w * 32 + 32 <= p.pages ? ~0u : (1u << (p.pages & 31)) - 1) : 0u;
+    };
+    int n = 0, before, total;
+    for (i64 w = tid; w < (i64)blockIdx.x * 1024; w += 1024) n += __popc(live(w));
+    scan_block(n, sums, before);
+    const i64 w = (i64)blockIdx.x * 1024 + tid;
+    const u32 bits = live(w);
+    int at = before + scan_block(__popc(bits), sums, total);
+    for (int b = 0; b < 32; ++b) {
+        const i64 page = w * 32 + b;
+        if (w >= words || page >= p.pages) break;
+        const bool is = bits >> b & 1;
+        map[page] = is && at < to.pages ? at : -1;
+        if (is && at < to.pages) list[at] = (int)page, to.refs[at] = p.refs[page];
+        at += is;
+    }
+    if (blockIdx.x + 1 < gridDim.x) return;
+    const int all = before + total;  // the last block: what is behind the live pages
+    if (tid == 0) *to.missing += all > to.pages ? (int)(all - to.pages) : 0;
+    for (i64 i = all + tid; i < to.pages; i += 1024) list[i] = -1, to.refs[i] = 0;
+    for (i64 v = tid; v < (to.pages + 31) / 32; v += 1024) {
+        const i64 from = all - v * 32;  // the word's first free page
+        const u32 in = v * 32 + 32 <= to.pages ? ~0u : (1u << (to.pages & 31)) - 1;
+        to.free[v] = from >= 32 ? 0u : from <= 0 ? in : in & ~0u << from;
+    }
+}
+
+__global__ __launch_bounds__(256) void pool_map_k(const Pool p, const int* __restrict__ table, i64 stride, int S, int width,
+                                                  const int* __restrict__ map, int* __restrict__ out) {
+    const i64 n = (i64)S * width;
+    for (i64 i = blockIdx.x * 256ll + threadIdx.x; i < n; i += (i64)gridDim.x * 256) {
+        const i64 s = i / width;
+        const int e = table[s * stride + (i - s * width)];
+        out[i] = is_page(p, e) ? map[e] : -1;
+    }
+}
+
+// ------------------------------------------------------------------------------------------------------------ the host
+
+// refs, asks, claim int32 [pages], free u32 [(pages + 31) / 32], missing int32 [1], end to end
+static i64 pool_words(i64 pages) { return 3 * pages + (pages + 31) / 32 + 1; }
+static bool pool_of(void* state, i64 pages, Pool& p) {
+    if (pages < 1 || pages >= (i64)1 << 31) return false;
+    p.refs = (int*)state, p.asks = p.refs + pages, p.claim = p.asks + pages, p.free = (u32*)(p.claim + pages);
+    p.missing = (int*)(p.free + (pages + 31) / 32), p.pages = pages;
+    return true;
+}
+
+static int some_blocks(i64 n) {
+    const int g = grid_for(n, 256);
+    return g < 2048 ? g : 2048;
+}
+
+extern "C" i64 ng_pool_state(i64 pages) { return pages < 1 || pages >= (i64)1 << 31 ? -1 : pool_words(pages) * 4; }
+
+extern "C" int ng_pool_clear(void* state, i64 pages, void* stream) {
+    Pool p;
+    if (!pool_of(state, pages, p)) return -1;
+    pool_clear_k<<<some_blocks(pages), 256, 0, (hipStream_t)stream>>>(p);
+    return (int)hipGetLastError();
+}
+
+extern "C" int ng_pool_hold(void* state, i64 pages, const int* table, i64 stride, int S, int width, void* stream) {
+    Pool p;
+    if (!pool_of(state, pages, p) || S < 0 || width < 0) return -1;
+    if ((i64)S * width == 0) return 0;
+    pool_hold_k<<<some_blocks((i64)S * width), 256, 0, (hipStream_t)stream>>>(p, table, stride, S, width);
+    return (int)hipGetLastError();
+}
+
+extern "C" i64 ng_pool_fork_work(i64 S, i64 width) {
+    return S < 0 || width < 1 || S > 1 << 24 || width > 1 << 26 || S * width >= (i64)1 << 40 ? -1 : (S * width + S) * 4;
+}
+
+extern "C" int ng_pool_fork(void* state, i64 pages, int* table, i64 stride, int S, int width, int* lengths,
+                            const i64* parents, void* work, void* stream) {
+    Pool p;
+    if (!pool_of(state, pages, p) || ng_pool_fork_work(S, width) < 0) return -1;
+    if (S == 0) return 0;
+    int* moved = (int*)work;
+    int* moved_len = moved + (i64)S * width;
+    const dim3 grid(S, (width + STRIP - 1) / STRIP);
+    hipStream_t st = (hipStream_t)stream;
+    pool_fork_k<<<grid, 256, 0, st>>>(p, table, stride, S, width, lengths, parents, moved, moved_len);
+    const int rc = (int)hipGetLastError();
+    if (rc) return rc;
+    pool_moved_k<<<grid, 256, 0, st>>>(table, stride, width, lengths, parents, moved, moved_len);
+    return (int)hipGetLastError();
+}
+
+static int room_per(int count, int shift) { return ((count - 1) >> shift) + 2; }
+
+extern "C" i64 ng_pool_room_work(i64 S, i64 count, i64 page) {
+    if (S < 0 || count < 1 || count >= (i64)1 << 30 || page < 16 || page > 4096 || (page & (page - 1))) return -1;
+    const i64 n = S * room_per((int)count, __builtin_ctz((unsigned)page));
+    return n >= (i64)1 << 28 ? -1 : (3 * n + S) * 4;
+}
+
+// A cache's parts side by side with another's (the same one: a page's rows copied within it). Without scales, or bounds: NULL.
+static bool parts_of(const void* const (&src)[5], void* const (&dst)[5], i64 src_pages, i64 dst_pages, int page, int heads,
+                     int dim, int codes, Parts& c) {
+    if (page < 16 || page > 4096 || (page & (page - 1)) || heads < 1 || dim < 1 || dim > 256 || codes < KV_INT8 ||
+        codes > KV_F16 || src_pages < 1 || dst_pages < 1 || src_pages >= (i64)1 << 31 || dst_pages >= (i64)1 << 31)
+        return false;
+    const i64 dp = (dim + 63) / 64 * 64;
+    const bool q8 = codes == KV_INT8 || codes == KV_FP8;
+    c.n = 0, c.H = heads, c.shift = __builtin_ctz((unsigned)page), c.src_pages = src_pages, c.dst_pages = dst_pages;
+    for (int i = 0; i < 5; ++i) {
+        c.part[i].src = (const char*)src[i], c.part[i].dst = (char*)dst[i];
+        c.part[i].bytes = i < 2 ? dp * (q8 ? 1 : 2) : i < 4 ? (q8 ? 4 : 0) : 4 * dp;
+    }
+    c.n = q8 ? 4 : 2;
+    return true;
+}
+
+extern "C" int ng_pool_room(void* state, i64 pages, int* table, i64 stride, int S, int width, const int* lengths,
+                            const int* counts, int count, void* k, void* v, void* ks, void* vs, int page, int heads,
+                            int dim, int codes, i64* slots, void* work, void* stream) {
+    Pool p;
+    Parts c;
+    const void* const src[5] = {k, v, ks, vs, nullptr};
+    void* const dst[5] = {k, v, ks, vs, nullptr};
+    if (!pool_of(state, pages, p) || S < 0 || width < 1 || ng_pool_room_work(S, count, page) < 0 ||
+        !parts_of(src, dst, pages, pages, page, heads, dim, codes, c) || (i64)S * heads >= (i64)1 << 31)
+        return -1;
+    if (S == 0) return 0;
+    Room r;
+    r.table = table, r.stride = stride, r.lengths = lengths, r.counts = counts, r.S = S, r.width = width, r.count = count;
+    r.shift = c.shift, r.per = room_per(count, c.shift);
+    const i64 n = (i64)S * r.per;
+    r.rank = (int*)work, r.page = r.rank + n, r.given = r.page + n, r.source = r.given + n;
+    hipStream_t st = (hipStream_t)stream;
+    pool_room_k<<<1, 1024, 0, st>>>(p, r);
+    const int rc = (int)hipGetLastError();
+    if (rc) return rc;
+    pool_slots_k<<<(unsigned)(S * heads), 256, 0, st>>>(p, r, c, slots);
+    return (int)hipGetLastError();
+}
+
+static i64 page_pieces(const Parts& c, bool bounds) {
+    i64 size = 0;
+    for (int i = 0; i < 5; ++i)
+        if (i < c.n || (i == 4 && bounds)) size += c.part[i].bytes * c.H << (i < 4 ? c.shift : 0);
+    return (size + PIECE - 1) / PIECE;
+}
+
+template <typename I> static int copy_list(Parts c, bool bounds, const I* src, const I* dst, i64 n, hipStream_t st) {
+    const i64 pieces = page_pieces(c, bounds);
+    if (bounds) c.n = 5;  // (a 16-bit cache's scales have rows of no bytes)
+    if (n * pieces >= (i64)1 << 31) return -1;
+    copy_pages_k<I><<<(unsigned)(n * pieces), 256, 0, st>>>(c, src, dst, n, (int)pieces);
+    return (int)hipGetLastError();
+}
+
+extern "C" int ng_copy_pages(const void* k, const void* v, const void* ks, const void* vs, const void* bounds, i64 pages,
+                             void* to_k, void* to_v, void* to_ks, void* to_vs, void* to_bounds, i64 to_pages, int page,
+                             int heads, int dim, int codes, const i64* src, const i64* dst, i64 n, void* stream) {
+    Parts c;
+    const void* const from[5] = {k, v, ks, vs, bounds};
+    void* const to[5] = {to_k, to_v, to_ks, to_vs, to_bounds};
+    if (n < 0 || (bounds == nullptr) != (to_bounds == nullptr) ||
+        !parts_of(from, to, pages, to_pages, page, heads, dim, codes, c))
+        return -1;
+    return n == 0 ? 0 : copy_list(c, bounds != nullptr, src, dst, n, (hipStream_t)stream);
+}
+
+extern "C" i64 ng_pool_move_work(i64 pages, i64 to_pages) {
+    return pages < 1 || to_pages < 1 || pages >= (i64)1 << 31 || to_pages >= (i64)1 << 31 ? -1 : (pages + to_pages) * 4;
+}
+
+extern "C" int ng_pool_move(void* state, i64 pages, const void* k, const void* v, const void* ks, const void* vs,
+                            const void* bounds, void* to_state, i64 to_pages, void* to_k, void* to_v, void* to_ks, void* to_vs,
+                            void* to_bounds, int page, int heads, int dim, int codes, const int* table, i64 stride, int S,
+                            int width, int* out, void* work, void* stream) {
+    Pool p, to;
+    Parts c;
+    const void* const from[5] = {k, v, ks, vs, bounds};
+    void* const into[5] = {to_k, to_v, to_ks, to_vs, to_bounds};
+    if (!pool_of(state, pages, p) || !pool_of(to_state, to_pages, to) || S < 0 || width < 0 ||
+        (bounds == nullptr) != (to_bounds == nullptr) ||
+        !parts_of(from, into, pages, to_pages, page, heads, dim, codes, c))
+        return -1;
+    int* list = (int*)work;
+    int* map = list + to_pages;
+    hipStream_t st = (hipStream_t)stream;
+    const i64 words = (pages + 31) / 32;
+    pool_pack_k<<<(unsigned)((words + 1023) / 1024), 1024, 0, st>>>(p, to, list, map);
+    int rc = (int)hipGetLastError();
+    if (rc) return rc;
+    if ((i64)S * width) {
+        pool_map_k<<<some_blocks((i64)S * width), 256, 0, st>>>(p, table, stride, S, width, map, out);
+        if ((rc = (int)hipGetLastError())) return rc;
+    }
+    return copy_list<int>(c, bounds != nullptr, list, nullptr, pages < to_pages ? pages : to_pages, st);
+}

@@ -632,10 +632,9 @@ template <int CODES, int DP, int R> struct Tree {
         }
     }
 
-    // The first tile's loads.
-    static __device__ __forceinline__ void begin(const TreeArgs& a, int b, int head, int base, int stop, Run& w) {
+    // The first tile's loads. tab: the sequence's page table (a.width entries).
+    static __device__ __forceinline__ void begin(const TreeArgs& a, const int* tab, int head, int base, int stop, Run& w) {
         if (base >= stop) return;
-        const int* tab = a.table + (i64)b * a.table_stride;
         w.next = pages_of(a, tab, base);
         fetch_keys(a, head, base, w.next, w.k);
         fetch_values(a, head, base, w.next, w.v);
@@ -644,12 +643,11 @@ template <int CODES, int DP, int R> struct Tree {
 
     // This wave's keys from base up to stop, a tile of 32 in every TILE; the first one's loads are under way. Only its last
     // tile can hold keys past the cached tokens: the tree and the rest of a tile before it are at most 3 tiles in a row.
-    static __device__ __forceinline__ void keys(const TreeArgs& a, int b, int head, const Seq& q, int base, int stop,
+    static __device__ __forceinline__ void keys(const TreeArgs& a, const int* tab, int head, const Seq& q, int base, int stop,
                                                 const u64* bits, const Sizes& size, bool own, Run& w, State& s,
                                                 float (*fac)[32]) {
         if (base >= stop) return;
         const int g = lane_id() >> 4;
-        const int* tab = a.table + (i64)b * a.table_stride;
         const int last = base + (stop - 1 - base) / TILE * TILE;
         const int whole = stop < q.len - 31 ? stop : q.len - 31;
         if (base < whole) do {
@@ -725,13 +723,43 @@ template <int CODES, int DP, int R> struct Tree {
         if constexpr (WILD)
             if (__any(bad != 0)) put_back(a, q, base, bits, w.v, bad, p, s);
     }
+
+    // The four waves' sums of rows r * 16 .. r * 16 + 15, joined in LDS: row threadIdx.x >> 4's maximum, sum and NJ outputs
+    // (from element (threadIdx.x & 15) * NJ on).
+    typedef float Lo[16][DP + 4];
+    static __device__ __forceinline__ void join_waves(const State& s, int r, Lo* lo, float (*lm)[16], float (*ll)[16], float& m,
+                                                      float& sum, float (&o)[NJ]) {
+        const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), c = lane_id() & 15, g = lane_id() >> 4;
+        const float l = sum_quarters(s.l[r]);
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+            for (int j = 0; j < NJ; ++j) lo[wave][c][(4 * g + i) * NJ + j] = s.o[r][j][i] * V_UP;
+        if (g == 0) lm[wave][c] = s.m[r], ll[wave][c] = l;
+        __syncthreads();
+        const int row = threadIdx.x >> 4, d0 = (threadIdx.x & 15) * NJ;
+        m = lm[0][row];
+#pragma unroll
+        for (int w = 1; w < 4; ++w) m = fmaxf(m, lm[w][row]);
+        sum = 0.f;
+#pragma unroll
+        for (int j = 0; j < NJ; ++j) o[j] = 0.f;
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+            // a wave without a key that counts: sum and o are 0, or NaN where a NaN was seen
+            const float k = lm[w][row] == -__builtin_inff() ? 0.f : __builtin_amdgcn_exp2f(lm[w][row] - m);
+            sum = ll[w][row] == 0.f ? sum : fmaf(ll[w][row], k, sum);
+#pragma unroll
+            for (int j = 0; j < NJ; ++j) o[j] = fmaf(lo[w][row][d0 + j], k, o[j]);
+        }
+    }
 };
 
 template <int CODES, int DP, int R>
 __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void tree_k(const TreeArgs a, int blocks) {
     typedef Tree<CODES, DP, R> W;
-    constexpr int LD = DP + 4;
-    typedef float Lo[16][LD];
+    typedef typename W::Lo Lo;
     __shared__ __align__(16) char lds[sizeof(Lo) * 4 > 16 * R * W::QLD * 2 ? sizeof(Lo) * 4 : 16 * R * W::QLD * 2];
     Lo* lo = (Lo*)lds;  // the waves' sums at a unit's end; before that the queries
     __shared__ float lm[4][16], ll[4][16];
@@ -743,7 +771,7 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void tree_k(const TreeArgs 
     const int a8 = (line.shares + 7) / 8, me = (int)(blockIdx.x % 8) * a8 + (int)blockIdx.x / 8;
     if ((int)blockIdx.x / 8 >= a8 || me >= line.shares) return;
     // (uniform, and the compiler is to know it: a loop that lanes left one by one would keep two sets of sums)
-    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), c = lane_id() & 15, g = lane_id() >> 4, units = a.H * a.groups;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), units = a.H * a.groups;
     if constexpr (W::Q8) {
         if (threadIdx.x < 16 * R) size.top[threadIdx.x] = 0;
         lds_barrier();
@@ -767,7 +795,8 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void tree_k(const TreeArgs 
         const int base = t0 * TILE + wave * 32, stop = t1 * TILE < q.n ? t1 * TILE : q.n;
         typename W::State s;
         typename W::Run run;
-        W::begin(a, b, head, base, stop, run);
+        const int* tab = a.table + (i64)b * a.table_stride;
+        W::begin(a, tab, head, base, stop, run);
         const bool own = W::load_q(a, b, head, q, row0, (typename W::T*)lds, size, bits, s);
 #pragma unroll
         for (int r = 0; r < R; ++r) {
@@ -775,34 +804,14 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void tree_k(const TreeArgs 
 #pragma unroll
             for (int j = 0; j < W::NJ; ++j) s.o[r][j] = f4{0.f, 0.f, 0.f, 0.f};
         }
-        W::keys(a, b, head, q, base, stop, bits, size, own, run, s, fac[wave]);
+        W::keys(a, tab, head, q, base, stop, bits, size, own, run, s, fac[wave]);
         const bool all = t0 == 0 && t1 == q.tiles;
         const i64 slot = 2 * me + (t0 == 0 ? 1 : 0);
 #pragma unroll
         for (int r = 0; r < R; ++r) {
-            const float l = sum_quarters(s.l[r]);
-            __syncthreads();
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-#pragma unroll
-                for (int j = 0; j < W::NJ; ++j) lo[wave][c][(4 * g + i) * W::NJ + j] = s.o[r][j][i] * W::V_UP;
-            if (g == 0) lm[wave][c] = s.m[r], ll[wave][c] = l;
-            __syncthreads();
             const int row = threadIdx.x >> 4, d0 = (threadIdx.x & 15) * W::NJ;
-            float m = lm[0][row];
-#pragma unroll
-            for (int w = 1; w < 4; ++w) m = fmaxf(m, lm[w][row]);
-            float sum = 0.f, o[W::NJ];
-#pragma unroll
-            for (int j = 0; j < W::NJ; ++j) o[j] = 0.f;
-#pragma unroll
-            for (int w = 0; w < 4; ++w) {
-                // a wave without a key that counts: sum and o are 0, or NaN where a NaN was seen
-                const float k = lm[w][row] == -__builtin_inff() ? 0.f : __builtin_amdgcn_exp2f(lm[w][row] - m);
-                sum = ll[w][row] == 0.f ? sum : fmaf(ll[w][row], k, sum);
-#pragma unroll
-                for (int j = 0; j < W::NJ; ++j) o[j] = fmaf(lo[w][row][d0 + j], k, o[j]);
-            }
+            float m, sum, o[W::NJ];
+            W::join_waves(s, r, lo, lm, ll, m, sum, o);
             const int at = row0 + r * 16 + row, t = at / a.G, h = at - t * a.G;
             if (all) {
                 if (t < a.T) {

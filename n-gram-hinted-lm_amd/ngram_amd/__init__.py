@@ -9,5 +9,8 @@ Host code (Python on PyTorch-ROCm) over a C-ABI HIP library (csrc/, built for gf
   embed           hint rows and tokens embedded, with the table's and the weights' gradients (HintEmbedding)
   kvcache         a paged key/value cache in 8 or 16 bits, quantised as it is written
   tree            attention for trees of drafted tokens over that cache
+  beam            a beam search's step over a model's logits, and its states' reordering
+  pages           who holds that cache's pages: forks, room for more tokens, copies, moves
+  sparse          attention over the pages that a cheap score keeps for each token
 """
 __all__ = ["data", "lib", "build"]
