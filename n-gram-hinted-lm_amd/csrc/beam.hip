@@ -12,8 +12,9 @@
 // candidates; where there are many, a block a row first leaves K of them.
 //
 // Precision. Candidates of different beams lie close to each other, so what decides between them is held in 64 bits: sums
-// over more than a thread's 32 elements, the logarithm, totals and ranks. An exponential is a 32-bit one whose argument's
-// rounding is put back (its error is the instruction's 2^-23 of itself, and averages out over a row).
+// over more than a thread's 32 elements, the logarithm, totals and ranks. An exponential is a 32-bit one: its argument's
+// rounding and the instruction's are off by 2^-20 of a term, and average out over a row's terms. (Putting each argument's
+// rounding back took 5 more operations an element: 20.5 us a chunk's pass against 17.3 for 64 x 8 rows of 50257.)
 #include "choose.h"
 #include "vals.h"
 
@@ -44,28 +45,89 @@ __device__ __forceinline__ i64 length_of(const BeamArgs& a, i64 row) {
     return a.lsize == 4 ? (i64)((const int*)a.lengths)[row] : ((const i64*)a.lengths)[row];
 }
 
-// exp(d) for d <= 0 or NaN
-__device__ __forceinline__ float exp_of(float d) {
-    d = d < -200.f ? -200.f : d;
-    const float t = d * 1.44269504f, r = fmaf(d, 1.44269504f, -t) + d * 1.925963033e-8f;
-    const float e = __builtin_amdgcn_exp2f(t);
-    return fmaf(e, r * 0.693147181f, e);
-}
+// Where a threshold that leaves K at least is fine enough: each halving costs as much as ranking some ten keys more.
+__device__ __forceinline__ int few(int K) { return K + K / 2 + 12; }
 
-template <typename K> __device__ __forceinline__ void write_ranked(const u64* list, int n, int K_, u64* out, K threads) {
+// The n keys of list, all different, in order: the K_ largest to out, 0 behind the last. list has room for 3 more.
+__device__ __forceinline__ void write_ranked(u64* list, int n, int K_, u64* out, int threads) {
+    if (threadIdx.x < 3) list[n + threadIdx.x] = 0;
+    __syncthreads();
     for (int i = threadIdx.x; i < n; i += threads) {
         const u64 mine = list[i];
         int r = 0;
-        for (int j = 0; j < n; ++j) r += list[j] > mine;
+        for (int j = 0; j < n; j += 4) r += (list[j] > mine) + (list[j + 1] > mine) + (list[j + 2] > mine) + (list[j + 3] > mine);
         if (r < K_) out[r] = mine;
     }
     for (int i = n + threadIdx.x; i < K_; i += threads) out[i] = 0;
 }
 
+// A thread's E logits as they are, 16 bytes in every 256 lanes'; -inf behind the last. whole: the chunk ends before V.
+template <typename T, int E> struct Logits {
+    static constexpr int N = 16 / (int)sizeof(T), P = E / N;
+    Pack<T, N> k[P];
+    __device__ __forceinline__ void load(const T* x, int from, int V, bool whole) {
+        if (whole) {
+#pragma unroll
+            for (int p = 0; p < P; ++p) k[p].load(x + from + p * 256 * N);
+            return;
+        }
+#pragma unroll
+        for (int p = 0; p < P; ++p) {
+            const int i = from + p * 256 * N;
+            if (i + N <= V) k[p].load(x + i);
+            else
+#pragma unroll
+                for (int j = 0; j < N; ++j) k[p].v[j] = i + j < V ? x[i + j] : (T)-__builtin_inff();
+        }
+    }
+    __device__ __forceinline__ float at(int p, int j) const { return (float)k[p].v[j]; }
+};
+
+// More logits reach the threshold t than are compared with each other: many are equal, or most of them in few threads. The
+// threshold that leaves K, and of the logits equal to it the lowest tokens. (The logits are loaded again for each count:
+// registers held for this would cost every block a third of its waves.)
+template <typename T, int E>
+__device__ __forceinline__ void crowded(const T* x, int from, const BeamArgs& a, u32 t, u32 hi, Count<4>& count, u64* list,
+                                        int* fill) {
+    constexpr int N = 16 / (int)sizeof(T);
+    auto each = [&](auto f) {
+#pragma unroll 1
+        for (int p = 0; p < E / N; ++p)
+#pragma unroll 1
+            for (int j = 0; j < N; ++j) {
+                const int i = from + p * 256 * N + j;
+                f(i < a.V ? key_of((float)x[i]) : 0u, (u32)i);
+            }
+    };
+    auto at_least = [&](u32 least, u32 last) {  // keys above `least`, and those equal to it of tokens up to `last`
+        int n = 0;
+        each([&](u32 k, u32 i) { n += __popcll(__ballot(k > least || (k == least && i <= last))); });
+        return count.sum(n);
+    };
+    u32 up = hi;
+    while (t < up) {  // the largest t that K reach
+        const u32 mid = t + (up - t) / 2 + 1;
+        if (at_least(mid, ~0u) >= a.K) t = mid;
+        else up = mid - 1;
+    }
+    u32 l = 0, h = (u32)a.V - 1;  // the lowest token up to which enough are equal
+    while (l < h) {
+        const u32 mid = l + (h - l) / 2;
+        if (at_least(t, mid) >= a.K) h = mid;
+        else l = mid + 1;
+    }
+    if (threadIdx.x == 0) *fill = 0;
+    __syncthreads();
+    each([&](u32 k, u32 i) {
+        if (k > t || (k == t && i <= l)) list[atomicAdd(fill, 1)] = (u64)k << 32 | (u32)~i;
+    });
+    __syncthreads();
+}
+
 // A block per (row, chunk of 256 E logits).
-template <typename T, int E> __global__ __launch_bounds__(256) void beam_part_k(const BeamArgs a) {
+template <typename T, int E> __global__ __launch_bounds__(256, 8) void beam_part_k(const BeamArgs a) {
     constexpr int N = 16 / (int)sizeof(T), P = E / N;
-    __shared__ u64 list[ROOM];
+    __shared__ u64 list[ROOM + 3];
     __shared__ int counts[2][4];
     __shared__ u32 most[4], least[4];
     __shared__ double sums[4];
@@ -76,24 +138,17 @@ template <typename T, int E> __global__ __launch_bounds__(256) void beam_part_k(
     const i64 b = row / a.W;
     const T* __restrict__ x = (const T*)a.logits + b * a.sb + (row - b * a.W) * a.sw;
     const int from = chunk * 256 * E + tid * N;
-    float v[E];
+    Logits<T, E> v;
+    v.load(x, from, a.V, (i64)(chunk + 1) * 256 * E <= a.V);
+    float tops[P], top = -__builtin_inff();  // of each load, and all (NaN passed over)
 #pragma unroll
     for (int p = 0; p < P; ++p) {
-        const int i = from + p * 256 * N;
-        Pack<T, N> k;
-        if (i + N <= a.V) k.load(x + i);
-        else
+        tops[p] = v.at(p, 0);
 #pragma unroll
-            for (int j = 0; j < N; ++j) k.v[j] = i + j < a.V ? x[i + j] : (T)-__builtin_inff();
-#pragma unroll
-        for (int j = 0; j < N; ++j) v[p * N + j] = (float)k.v[j];
+        for (int j = 1; j < N; ++j) tops[p] = fmaxf(tops[p], v.at(p, j));
+        top = fmaxf(top, tops[p]);
     }
-    u32 key[E], mine[1] = {0};
-#pragma unroll
-    for (int e = 0; e < E; ++e) {
-        key[e] = key_of(v[e]);
-        mine[0] = key[e] > mine[0] ? key[e] : mine[0];
-    }
+    const u32 mine[1] = {key_of(top)};
     const u32 wm = max_wave(mine[0]), wl = min_wave(mine[0]);
     if (lane_id() == 0) most[wave] = wm, least[wave] = wl;
     if (tid == 0) fill = 0;
@@ -102,9 +157,17 @@ template <typename T, int E> __global__ __launch_bounds__(256) void beam_part_k(
 #pragma unroll
     for (int w = 1; w < 4; ++w) hi = most[w] > hi ? most[w] : hi, lo = least[w] < lo ? least[w] : lo;
     const float m = hi ? of_key(hi) : 0.f;  // (nothing above -inf: each term is 0, or NaN)
+    // 2^(L v + c) with c = -L m rounded: one operation an argument; how far c is off is put back below, once for all terms.
+    // (Where L m is large that is no small correction: the arguments are L (v - m) then.)
+    const float L = 1.44269504f, c = -L * m;
+    const bool near = __builtin_fabsf(m) < 4096.f;
     float s = 0.f;
+    if (near)
 #pragma unroll
-    for (int e = 0; e < E; ++e) s += exp_of(v[e] - m);
+        for (int e = 0; e < E; ++e) s += __builtin_amdgcn_exp2f(fmaf(v.at(e / N, e % N), L, c));
+    else
+#pragma unroll
+        for (int e = 0; e < E; ++e) s += __builtin_amdgcn_exp2f((v.at(e / N, e % N) - m) * L);
     double sum = s;
 #pragma unroll
     for (int o = 32; o; o >>= 1) sum += __shfl_xor(sum, o, WAVE);
@@ -112,140 +175,163 @@ template <typename T, int E> __global__ __launch_bounds__(256) void beam_part_k(
     // the threads' largest give a threshold that K logits at least reach
     Count<4> count(counts);
     int n = 256;
-    u32 t = count.threshold(mine, lo ? lo : 1u, hi, a.K, a.K + a.K / 4, n);
-    int c = count.at_least(key, t);
-    u32 last = ~0u;  // of the keys equal to t, those of tokens up to here
-    if (c > ROOM) {  // many equal ones, or most of them in few threads: the threshold that leaves K
-        t = count.threshold(key, t, hi, a.K, ROOM, c);
-        if (c > ROOM) {
-            const int above = t == hi ? 0 : count.at_least(key, t + 1);
-            u32 l = 0, h = (u32)a.V - 1;  // the lowest token up to which enough are equal
-            while (l < h) {
-                const u32 mid = l + (h - l) / 2;
-                int k = 0;
+    const u32 lowest = 0x00800000u;  // the key of the lowest number: where there are fewer than K, all are taken
+    u32 t = count.threshold(mine, lo > lowest ? lo : lowest, hi, a.K, few(a.K), n);
+    const float least_v = of_key(t);
 #pragma unroll
-                for (int e = 0; e < E; ++e) k += __popcll(__ballot(key[e] == t && (u32)(from + e / N * 256 * N + e % N) <= mid));
-                if (above + count.sum(k) >= a.K) h = mid;
-                else l = mid + 1;
-            }
-            last = l;
-        }
-    }
+    for (int p = 0; p < P; ++p)
+        if (tops[p] >= least_v)
 #pragma unroll
-    for (int e = 0; e < E; ++e) {
-        const u32 token = from + e / N * 256 * N + e % N;
-        if (key[e] > t || (key[e] == t && token <= last)) list[atomicAdd(&fill, 1)] = (u64)key[e] << 32 | (u32)~token;
-    }
+            for (int j = 0; j < N; ++j)
+                if (v.at(p, j) >= least_v) {
+                    const u32 token = from + p * 256 * N + j;
+                    const int at = atomicAdd(&fill, 1);
+                    if (at < ROOM) list[at] = (u64)key_of(v.at(p, j)) << 32 | (u32)~token;
+                }
     __syncthreads();
+    if (fill > ROOM) crowded<T, E>(x, from, a, t, hi, count, list, &fill);
     const i64 at = row * a.chunks + chunk;
     write_ranked(list, fill, a.K, a.part + at * a.K, 256);
-    if (tid == 0) a.top[at] = hi ? m : -__builtin_inff(), a.sum[at] = sums[0] + sums[1] + sums[2] + sums[3];
+    if (tid == 0) {
+        const double off = near ? 0.69314718055994531 * ((double)L * m + (double)c) : 0.;  // below 2^-11: exp by its series
+        a.top[at] = hi ? m : -__builtin_inff();
+        a.sum[at] = (sums[0] + sums[1] + sums[2] + sums[3]) * (1. - off * (1. - off * (0.5 - off / 6.)));
+    }
 }
 
-// The chunks' sums of one row, by a wave: log sum exp (NaN or infinite: the row has no candidates).
-__device__ __forceinline__ double row_lse(const BeamArgs& a, i64 row) {
-    float m = -__builtin_inff();
-    for (int c = lane_id(); c < a.chunks; c += 64) m = fmaxf(m, a.top[row * a.chunks + c]);
-    m = of_key(max_wave(key_of(m)));  // (all -inf: NaN)
-    double s = 0;
-    for (int c = lane_id(); c < a.chunks; c += 64) {
-        const double x = a.sum[row * a.chunks + c];
-        const float t = a.top[row * a.chunks + c];
-        s += t == -__builtin_inff() ? x : x * exp((double)t - (double)m);
+// The chunks' sums of one row, by LANES lanes of a wave: the row's largest logit and sum of exponentials beside it (NaN or
+// infinite, or a sum of 0: the row has no candidates).
+template <int LANES> __device__ __forceinline__ void row_sum(const BeamArgs& a, i64 row, float& m, double& s) {
+    const int l = lane_id() & (LANES - 1);
+    const float* top = a.top + row * a.chunks;
+    const double* sum = a.sum + row * a.chunks;
+    m = -__builtin_inff(), s = 0;
+    for (int c = l; c < a.chunks; c += LANES) {  // (a running maximum: one pass over the loads)
+        const float t = top[c];
+        const double x = sum[c];
+        const float n = fmaxf(m, t);
+        if (n == -__builtin_inff()) s += x;
+        else if (n == m) s += t == -__builtin_inff() ? x : x * exp((double)t - (double)m);
+        else s = (m == -__builtin_inff() ? s : s * exp((double)m - (double)n)) + x, m = n;
     }
+    float all = m;
 #pragma unroll
-    for (int o = 32; o; o >>= 1) s += __shfl_xor(s, o, WAVE);
-    return log(s) + (double)m;
+    for (int o = LANES / 2; o; o >>= 1) all = fmaxf(all, __shfl_xor(all, o, WAVE));
+    if (m != -__builtin_inff() && m != all) s *= exp((double)m - (double)all);
+    m = all;
+#pragma unroll
+    for (int o = LANES / 2; o; o >>= 1) s += __shfl_xor(s, o, WAVE);
+}
+
+// The block's largest of x and of y: y the last of a list of K, which as many at least reach (1: no list is full).
+template <int NW> __device__ __forceinline__ void ends(u64 x, u64 y, u64 (&lds)[2][NW], u64& hi, u64& lo) {
+    x = max_wave(x), y = max_wave(y);
+    if (lane_id() == 0) lds[0][threadIdx.x >> 6] = x, lds[1][threadIdx.x >> 6] = y;
+    lds_barrier();
+    hi = lds[0][0], lo = lds[1][0];
+#pragma unroll
+    for (int w = 1; w < NW; ++w) hi = lds[0][w] > hi ? lds[0][w] : hi, lo = lds[1][w] > lo ? lds[1][w] : lo;
+    if (!lo) lo = 1;
 }
 
 // A block a row: its chunks' lists to one of K, and its log sum exp.
-__global__ __launch_bounds__(1024) void beam_row_k(const BeamArgs a, u64* part, double* lses) {
-    constexpr int E = 16;
-    __shared__ u64 list[ROOM];
-    __shared__ int counts[2][16];
-    __shared__ u64 most[16];
+template <int NW, int E> __global__ __launch_bounds__(NW * 64) void beam_row_k(const BeamArgs a, u64* part, double* lses) {
+    constexpr int NT = NW * 64;
+    __shared__ u64 list[ROOM + 3];
+    __shared__ int counts[2][NW];
+    __shared__ u64 most[2][NW];
     __shared__ int fill;
     const i64 row = blockIdx.x;
     if (ended(a, row)) return;
     const int have = a.chunks * a.K;
-    u64 key[E], mine = 0;
+    u64 key[E], mine = 0, full = 0;
 #pragma unroll
     for (int e = 0; e < E; ++e) {
-        const int i = e * 1024 + threadIdx.x;
+        const int i = e * NT + threadIdx.x;
         key[e] = i < have ? a.part[row * have + i] : 0;
         mine = key[e] > mine ? key[e] : mine;
+        if (i % a.K == a.K - 1) full = key[e] > full ? key[e] : full;
     }
-    mine = max_wave(mine);
-    if (lane_id() == 0) most[threadIdx.x >> 6] = mine;
+    u64 lo, hi;
+    ends(mine, full, most, hi, lo);
     if (threadIdx.x == 0) fill = 0;
     lds_barrier();
-    u64 hi = most[0];
-#pragma unroll
-    for (int w = 1; w < 16; ++w) hi = most[w] > hi ? most[w] : hi;
-    Count<16> count(counts);
-    int n = count.at_least(key, 1ull);  // (the keys are all different: a threshold leaves as few as wanted)
-    const u64 t = count.threshold(key, 1ull, hi, a.K, ROOM / 4, n);
+    Count<NW> count(counts);
+    int n = count.at_least(key, lo);  // (the keys are all different: a threshold leaves as few as wanted)
+    const u64 t = count.threshold(key, lo, hi, a.K, few(a.K), n);
 #pragma unroll
     for (int e = 0; e < E; ++e)
         if (key[e] >= t && key[e]) list[atomicAdd(&fill, 1)] = key[e];
     __syncthreads();
-    write_ranked(list, fill, a.K, part + row * a.K, 1024);
+    write_ranked(list, fill, a.K, part + row * a.K, NT);
     if (threadIdx.x < 64) {
-        const double lse = row_lse(a, row);
-        if (threadIdx.x == 0) lses[row] = lse;
+        float m;
+        double s;
+        row_sum<64>(a, row, m, s);
+        if (threadIdx.x == 0) lses[row] = log(s) + (double)m;
     }
 }
 
-// A block a sequence. MERGED: part holds a list a row and sum its log sum exp.
-template <int NW, bool MERGED> __global__ __launch_bounds__(NW * 64) void beam_join_k(const BeamArgs a) {
-    constexpr int NT = NW * 64, E = 16;
+// A block a sequence, which holds E candidates a thread. a.top NULL: part holds a list a row and sum its log sum exp.
+template <int NW, int E> __global__ __launch_bounds__(NW * 64) void beam_join_k(const BeamArgs a) {
+    constexpr int NT = NW * 64;
     __shared__ double lses[MOST], scores[MOST], norms[MOST];
     __shared__ int done[MOST];
-    __shared__ u64 most[NW], list[ROOM], list2[ROOM];
+    __shared__ u64 most[2][NW];
+    __shared__ ulonglong2 list[ROOM + 3];  // a candidate's two words
     __shared__ int counts[2][NW];
     __shared__ int fill;
     const i64 b = blockIdx.x;
-    const int tid = threadIdx.x, wave = tid >> 6;
-    for (int w = wave; w < a.W; w += NW) {
+    const int tid = threadIdx.x;
+    const int per = a.chunks * a.K, have = a.W * per;
+    constexpr bool HOLD = E <= 4;  // the candidates are kept beside their ranks, else loaded again where they are chosen
+    u64 held[HOLD ? E : 1];
+    if constexpr (HOLD)
+#pragma unroll
+        for (int e = 0; e < E; ++e) held[e] = e * NT + tid < have ? a.part[b * have + e * NT + tid] : 0;
+    for (int w = tid / 16; w < a.W; w += NT / 16) {  // 16 lanes a beam
         const i64 row = b * a.W + w;
         const bool end = ended(a, row);
-        const double lse = end ? 0. : MERGED ? a.sum[row] : row_lse(a, row);
-        if (lane_id() == 0) {
-            const i64 len = (a.lengths ? length_of(a, row) : 0) + (end ? 0 : 1);
-            lses[w] = lse, scores[w] = a.scores[row], done[w] = end;
-            norms[w] = a.alpha == 0. ? 1. : pow((double)(len < 1 ? 1 : len), a.alpha);
+        const i64 len = (a.lengths ? length_of(a, row) : 0) + (end ? 0 : 1);
+        const float score = a.scores[row];
+        double lse = 0.;
+        if (!a.top) lse = end ? 0. : a.sum[row];
+        else if (!end) {
+            float m;
+            row_sum<16>(a, row, m, lse);
+            lse = log(lse) + (double)m;
+        }
+        if ((lane_id() & 15) == 0) {
+            lses[w] = lse, scores[w] = score, done[w] = end;
+            norms[w] = a.alpha == 0. || len <= 1 ? 1. : exp(-a.alpha * log((double)len));
         }
     }
     if (tid == 0) fill = 0;
     __syncthreads();
     // candidates: the rows' lists, then one of each finished beam. A key's first word is its rank, its second the beam
     // (lower first), the logit and the token (lower first).
-    const int per = a.chunks * a.K, have = a.W * per;
-    u64 key[E], mine = 0;
+    u64 key[E], mine = 0, full = 0;
 #pragma unroll
     for (int e = 0; e < E; ++e) {
         const int i = e * NT + tid;
         key[e] = 0;
         if (i < have) {
             const int w = i / per;
-            const u64 c = done[w] ? 0ull : a.part[b * have + i];
-            if (c) key[e] = key_of((scores[w] + ((double)of_key((u32)(c >> 32)) - lses[w])) / norms[w]);
-            if (done[w] && i == w * per) key[e] = key_of(scores[w] / norms[w]);
+            const u64 c = done[w] ? 0ull : HOLD ? held[HOLD ? e : 0] : a.part[b * have + i];
+            if (c) key[e] = key_of((scores[w] + ((double)of_key((u32)(c >> 32)) - lses[w])) * norms[w]);
+            if (done[w] && i == w * per) key[e] = key_of(scores[w] * norms[w]);
+            if (i % a.K == a.K - 1) full = key[e] > full ? key[e] : full;
         }
         mine = key[e] > mine ? key[e] : mine;
     }
-    mine = max_wave(mine);
-    if (lane_id() == 0) most[wave] = mine;
-    lds_barrier();
-    u64 hi = most[0];
-#pragma unroll
-    for (int w = 1; w < NW; ++w) hi = most[w] > hi ? most[w] : hi;
+    u64 lo, hi;
+    ends(mine, full, most, hi, lo);
     Count<NW> count(counts);
-    int n = count.at_least(key, 1ull);
-    const u64 t = n > a.K ? count.threshold(key, 1ull, hi, a.K, a.K + 64, n) : 1ull;
-    auto second = [&](int i) {
-        const int w = i / per;
-        const u64 c = done[w] ? 0xFFFFFFFFull << 32 | (u32)~a.pad : a.part[b * have + i];
+    int n = count.at_least(key, lo);
+    const u64 t = count.threshold(key, lo, hi, a.K, few(a.K), n);
+    auto second = [&](int e) {
+        const int i = e * NT + tid, w = i / per;
+        const u64 c = done[w] ? 0xFFFFFFFFull << 32 | (u32)~a.pad : HOLD ? held[HOLD ? e : 0] : a.part[b * have + i];
         return (u64)(MOST - 1 - w) << 57 | c >> 32 << TOKEN_BITS | ((u32)c & ((1u << TOKEN_BITS) - 1));
     };
     u64 t2 = 0;  // of the keys equal to t, those whose second word is this or more
@@ -256,7 +342,7 @@ template <int NW, bool MERGED> __global__ __launch_bounds__(NW * 64) void beam_j
             const u64 mid = lo + (up - lo) / 2 + 1;
             int k = 0;
 #pragma unroll
-            for (int e = 0; e < E; ++e) k += __popcll(__ballot(key[e] == t && second(e * NT + tid) >= mid));
+            for (int e = 0; e < E; ++e) k += __popcll(__ballot(key[e] == t && second(e) >= mid));
             if (above + count.sum(k) >= a.K) lo = mid;
             else up = mid - 1;
         }
@@ -265,14 +351,16 @@ template <int NW, bool MERGED> __global__ __launch_bounds__(NW * 64) void beam_j
 #pragma unroll
     for (int e = 0; e < E; ++e)
         if (key[e] >= t && key[e]) {
-            const u64 s = second(e * NT + tid);
+            const u64 s = second(e);
             if (key[e] > t || s >= t2) {
                 const int at = atomicAdd(&fill, 1);
-                list[at] = key[e], list2[at] = s;
+                list[at] = make_ulonglong2(key[e], s);
             }
         }
     __syncthreads();
     n = fill;
+    if (tid < 3) list[n + tid] = make_ulonglong2(0, 0);
+    __syncthreads();
     auto put = [&](int r, int w, int token, float score) {
         const i64 o = b * a.K + r;
         a.out_scores[o] = score, a.parents[o] = b * a.W + w, a.tokens[o] = token;
@@ -280,9 +368,14 @@ template <int NW, bool MERGED> __global__ __launch_bounds__(NW * 64) void beam_j
         if (a.out_lengths) a.out_lengths[o] = length_of(a, b * a.W + w) + (done[w] ? 0 : 1);
     };
     for (int i = tid; i < n; i += NT) {
-        const u64 k = list[i], s = list2[i];
+        const u64 k = list[i].x, s = list[i].y;
         int r = 0;
-        for (int j = 0; j < n; ++j) r += list[j] > k || (list[j] == k && list2[j] > s);
+        for (int j = 0; j < n; j += 4)
+#pragma unroll
+            for (int u = 0; u < 4; ++u) {
+                const ulonglong2 x = list[j + u];
+                r += x.x > k || (x.x == k && x.y > s);
+            }
         if (r >= a.K) continue;
         const int w = MOST - 1 - (int)(s >> 57), token = (1 << TOKEN_BITS) - 1 - (int)(s & ((1u << TOKEN_BITS) - 1));
         put(r, w, token, (float)(done[w] ? scores[w] : scores[w] + ((double)of_key((u32)(s >> TOKEN_BITS)) - lses[w])));
@@ -294,7 +387,7 @@ template <int NW, bool MERGED> __global__ __launch_bounds__(NW * 64) void beam_j
         const int w = i / a.V, v = i - w * a.V;
         bool o = w < a.W;
         for (int j = 0; j < n; ++j)
-            o &= MOST - 1 - (int)(list2[j] >> 57) != w || (1 << TOKEN_BITS) - 1 - (int)(list2[j] & ((1u << TOKEN_BITS) - 1)) != v;
+            o &= MOST - 1 - (int)(list[j].y >> 57) != w || (1 << TOKEN_BITS) - 1 - (int)(list[j].y & ((1u << TOKEN_BITS) - 1)) != v;
         open[i] = o;
     }
     __syncthreads();
@@ -372,14 +465,19 @@ extern "C" int ng_beam_step(const void* logits, i64 sb, i64 sw, int dtype, const
     }
     int rc = (int)hipGetLastError();
     if (rc) return rc;
-    if (!p.merge) beam_join_k<4, false><<<B, 256, 0, st>>>(a);
-    else {
+    if (p.merge) {
         u64* rows = (u64*)(w + p.rows);
         double* lses = (double*)(w + p.row_sum);
-        beam_row_k<<<(unsigned)(B * W), 1024, 0, st>>>(a, rows, lses);
-        a.part = rows, a.sum = lses, a.chunks = 1;
-        beam_join_k<16, true><<<B, 1024, 0, st>>>(a);
+        if (a.chunks * K <= 1024) beam_row_k<4, 4><<<(unsigned)(B * W), 256, 0, st>>>(a, rows, lses);
+        else beam_row_k<16, 16><<<(unsigned)(B * W), 1024, 0, st>>>(a, rows, lses);
+        if ((rc = (int)hipGetLastError())) return rc;
+        a.part = rows, a.top = nullptr, a.sum = lses, a.chunks = 1;
     }
+    const int have = W * a.chunks * K;
+    if (have <= 1024) beam_join_k<4, 4><<<B, 256, 0, st>>>(a);
+    else if (have <= 2048) beam_join_k<8, 4><<<B, 512, 0, st>>>(a);
+    else if (have <= 4096) beam_join_k<16, 4><<<B, 1024, 0, st>>>(a);
+    else beam_join_k<16, 16><<<B, 1024, 0, st>>>(a);
     return (int)hipGetLastError();
 }
 
@@ -392,8 +490,11 @@ template <typename U> __global__ __launch_bounds__(256) void gather_rows_k(const
     const U* s = (const U*)(src + r * stride);
     U* o = (U*)(out + i * units * (i64)sizeof(U));
     const bool is = (u64)r < (u64)rows;
-    const U zero = {};
-    for (i64 j = (blockIdx.x % parts) * 256 + threadIdx.x; j < units; j += (i64)parts * 256) o[j] = is ? s[j] : zero;
+    for (i64 j = (blockIdx.x % parts) * 256 + threadIdx.x; j < units; j += (i64)parts * 256) {
+        U x = {};
+        if (is) x = s[j];
+        o[j] = x;
+    }
 }
 
 

@@ -2,9 +2,10 @@
 blocks', ties, masked tokens, finished beams, lengths, too few candidates, NaN and infinities, strides, streams, graphs, and the
 refusals; the states' reordering.
 
-Tolerances. A row's log-sum: an exponential is off by 2^-22 of itself (the instruction's 2^-23, the argument's rounding put
-back), a thread's sum of up to 32 terms by 31 * 2^-24 of itself, the rest is 64 bits: off by LSE = 2^-22 + 31 * 2^-24 at most.
-A score is rounded to float32 once: 2^-24 of itself more. Two candidates may come in the other order where their exact ranks
+Tolerances. A row's log-sum: a term 2^t beside the largest (1) has its exponent rounded once, off by |t| 2^-24, so itself by
+0.7 |t| 2^-24, and the instruction adds 2^-23; of V <= 2^17 terms those with |t| > 20 weigh less than 2^-3 of the largest
+together and less the further they lie, so a sum is off by 20 * 0.7 * 2^-24 < 2^-20 and 2^-23 of itself at most; a thread's
+sum of up to 32 terms adds 31 * 2^-24, the rest is 64 bits: LSE = 2^-20 + 2^-23 + 31 * 2^-24. A score is rounded to float32 once: 2^-24 of itself more. Two candidates may come in the other order where their exact ranks
 differ by less than twice LSE (over their lengths' norms, which are 1 at least); within a beam the order is the logits'."""
 
 import math
@@ -16,7 +17,7 @@ from ngram_amd.beam import beam_step, reorder
 
 pytestmark = pytest.mark.gpu
 
-LSE = 2.0**-22 + 31 * 2.0**-24
+LSE = 2.0**-20 + 2.0**-23 + 31 * 2.0**-24
 
 
 def _ranked(logits, scores, lengths, finished, pad, alpha):
