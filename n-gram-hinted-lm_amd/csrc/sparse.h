@@ -6,13 +6,25 @@ struct SparseArgs {
     TreeArgs a;  // q, the cache, out, lse; a.table: the chosen pages [rows, keep], a.width: keep
     const int2* rows;  // [rows]: a row's keys over its chosen pages (0: none), and whether it is in use
     int T, splits;     // the tokens of a sequence; the blocks a unit
-    i64 first_row;     // the row (sequence, token, head) that row 0 of the workspace is
+    int b0, t0, nt;    // this pass: tokens t0 .. t0 + nt - 1 of sequences b0 on
     i64 units;         // rows x groups of 16 query heads
 };
 
 template <int CODES> int sparse_codes(const SparseArgs& s, int dp, hipStream_t st);
 template <int CODES> int bounds_codes(const void* k, const float* ks, i64 pages, int shift, int H, int dim, const int* table,
                                       i64 stride, int width, const int* start, int B, int count, b16* bounds, hipStream_t st);
+
+// A row's sequence, token and head.
+struct At {
+    i64 b;
+    int t, head;
+};
+__device__ __forceinline__ At at_of(const SparseArgs& s, i64 row) {
+    const i64 token = row / s.a.H, b = token / s.nt;
+    At p;
+    p.b = s.b0 + b, p.t = s.t0 + (int)(token - b * s.nt), p.head = (int)(row - token * s.a.H);
+    return p;
+}
 
 // The tiles of a unit that its block `split` takes: [t0, t1), and how many of its blocks have any.
 struct Share {
@@ -41,9 +53,10 @@ template <int CODES, int DP> __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1
     const i64 blocks = s.units * s.splits, a8 = (blocks + 7) / 8, me = (i64)(blockIdx.x % 8) * a8 + blockIdx.x / 8;
     if ((i64)blockIdx.x / 8 >= a8 || me >= blocks) return;
     const i64 unit = me / s.splits;
-    const int split = (int)(me - unit * s.splits), groups = s.a.groups, H = s.a.H, G = s.a.G;
-    const i64 row = unit / groups, token = (s.first_row + row) / H, b = token / s.T;
-    const int group = (int)(unit - row * groups), head = (int)(s.first_row + row - token * H), t = (int)(token - b * s.T);
+    const int split = (int)(me - unit * s.splits), groups = s.a.groups, G = s.a.G;
+    const i64 row = unit / groups;
+    const int group = (int)(unit - row * groups);
+    const At p = at_of(s, row);
     const int2 r = s.rows[row];
     const int n = __builtin_amdgcn_readfirstlane(r.x);
     const Share mine = share_of(n, s.splits, split);
@@ -54,25 +67,25 @@ template <int CODES, int DP> __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1
         lds_barrier();
     }
     TreeArgs a = s.a;
-    a.q = (const u16*)a.q + b * a.qb + t * a.qt, a.T = 1, a.mask = nullptr;
+    a.q = (const u16*)a.q + p.b * a.qb + p.t * a.qt, a.T = 1, a.mask = nullptr;
     Seq q;
     q.w = __builtin_amdgcn_readfirstlane(r.y), q.len = n > 0 ? n - 1 : 0, q.n = n, q.tiles = 0, q.span = 0;
     const int base = mine.t0 * TILE + wave * 32, stop = mine.t1 * TILE < n ? mine.t1 * TILE : n;
     typename W::State st;
     typename W::Run run;
     const int* tab = a.table + row * a.width;
-    W::begin(a, tab, head, base, stop, run);
-    const bool own = W::load_q(a, 0, head, q, group * 16, (typename W::T*)lds, size, bits, st);
+    W::begin(a, tab, p.head, base, stop, run);
+    const bool own = W::load_q(a, 0, p.head, q, group * 16, (typename W::T*)lds, size, bits, st);
     st.m[0] = -__builtin_inff(), st.l[0] = 0.f;
 #pragma unroll
     for (int j = 0; j < W::NJ; ++j) st.o[0][j] = f4{0.f, 0.f, 0.f, 0.f};
-    W::keys(a, tab, head, q, base, stop, bits, size, own, run, st, fac[wave]);
+    W::keys(a, tab, p.head, q, base, stop, bits, size, own, run, st, fac[wave]);
     float m, sum, o[W::NJ];
     W::join_waves(st, 0, lo, lm, ll, m, sum, o);
     const int at = threadIdx.x >> 4, d0 = (threadIdx.x & 15) * W::NJ, h = group * 16 + at;
     if (h >= G) return;
     if (mine.blocks <= 1) {
-        const i64 i = token * H * G + head * G + h;
+        const i64 i = (p.b * s.T + p.t) * a.H * G + p.head * G + h;
         const bool none = sum == 0.f;
         const float inv = none ? 0.f : 1.f / sum;
 #pragma unroll
@@ -92,8 +105,9 @@ template <int CODES, int DP> __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1
 template <int DP> __global__ __launch_bounds__(256) void sparse_join_k(const SparseArgs s, float bias) {
     constexpr int NJ = DP / 16;
     const TreeArgs& a = s.a;
-    const i64 unit = blockIdx.x, row = unit / a.groups, token = (s.first_row + row) / a.H;
-    const int head = (int)(s.first_row + row - token * a.H), h = (int)(unit - row * a.groups) * 16 + (threadIdx.x >> 4);
+    const i64 unit = blockIdx.x, row = unit / a.groups;
+    const int h = (int)(unit - row * a.groups) * 16 + (threadIdx.x >> 4);
+    const At p = at_of(s, row);
     const int parts = share_of(s.rows[row].x, s.splits, 0).blocks;
     if (parts <= 1 || h >= a.G) return;
     const int d0 = (threadIdx.x & 15) * NJ;
@@ -111,7 +125,7 @@ template <int DP> __global__ __launch_bounds__(256) void sparse_join_k(const Spa
         for (int j = 0; j < NJ; ++j) o[j] = o[j] * ko + a.po[prow * DP + d0 + j] * kp;
         m = n;
     }
-    const i64 i = token * a.H * a.G + head * a.G + h;
+    const i64 i = (p.b * s.T + p.t) * a.H * a.G + p.head * a.G + h;
     const bool none = sum == 0.f;
     const float inv = none ? 0.f : 1.f / sum;
 #pragma unroll

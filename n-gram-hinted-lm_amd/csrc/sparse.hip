@@ -21,107 +21,219 @@
 struct ScoreArgs {
     const void* q;
     i64 qb, qt, qh;
-    const b16* bounds;  // [pages, H, 2, DP]
+    const b16* bounds;  // [pages, H, 2, DP], zeros behind dim
     const int* table;
     i64 table_stride, pages;
     const int *lengths, *widths;
     int B, T, H, G, dim, shift, width, keep, first, last, qtype, vec;
-    i64 first_row, rows;  // those of this pass: (sequence, token, head)
+    int b0, t0, nt;       // this pass: tokens t0 .. t0 + nt - 1 of sequences b0 on
+    i64 rows;             // its rows: (sequence, token, head)
     u64* score;           // [rows, width]
     int* table_out;       // [rows, keep]: the kept pages of the cache
     int2* row_out;        // [rows]
     int* chosen;          // [B, T, H, keep] or NULL: the kept pages' places in the sequence, -1 behind them
-    int chunks;
+    int chunks, per;      // blocks a row, and the pages of each
 };
 
 // A row's token: whether it is in use, the pages it sees, and its keys' number over all of them.
 struct Place {
     bool is;
     int b, t, h, pages;
-    i64 keys;
+    i64 len, keys;  // the tokens before the sequence's first of the call, and those that it sees
 };
-__device__ __forceinline__ Place place_of(const ScoreArgs& a, i64 row) {
+__device__ __forceinline__ Place place_of(const ScoreArgs& a, u32 row) {  // (a pass has fewer than 2^31 rows)
     Place p;
-    const i64 at = a.first_row + row, token = at / a.H, cap = (i64)a.width << a.shift;
-    p.h = (int)(at - token * a.H), p.b = (int)(token / a.T), p.t = (int)(token - (i64)p.b * a.T);
+    const u32 token = row / (u32)a.H, b = token / (u32)a.nt;
+    const i64 cap = (i64)a.width << a.shift;
+    p.h = (int)(row - token * a.H), p.b = a.b0 + (int)b, p.t = a.t0 + (int)(token - b * a.nt);
     const int l = a.lengths[p.b], w = a.widths ? a.widths[p.b] : a.T;
-    const i64 len = l < 0 ? 0 : l > cap ? cap : l;
+    p.len = l < 0 ? 0 : l > cap ? cap : l;
     p.is = p.t < w;
-    p.keys = len + p.t + 1 < cap ? len + p.t + 1 : cap;
+    p.keys = p.len + p.t + 1 < cap ? p.len + p.t + 1 : cap;
     p.pages = (int)((p.keys + (1 << a.shift) - 1) >> a.shift);
     return p;
 }
 
-// A block per (row, 256 pages); GS lanes a page, each of 8 elements.
-template <int DP, int GS> __global__ __launch_bounds__(256) void score_k(const ScoreArgs a) {
-    constexpr int U = 4;
-    const i64 row = blockIdx.x / a.chunks;
+__device__ __forceinline__ float query_at(const ScoreArgs& a, u16 e) {
+    return a.qtype == NG_BF16 ? __uint_as_float((u32)e << 16) : (float)__builtin_bit_cast(f16, e);
+}
+
+// A score as a key: a page of none of the cache's ranks last, one whose score is NaN first.
+__device__ __forceinline__ u64 score_key(bool is, double x) {
+    const u64 u = (u64)__double_as_longlong(x + 0.);
+    return !is ? 1ull : x != x ? ~1ull : u >> 63 ? ~u : u | 1ull << 63;
+}
+
+// The pairs of elements of four words, 16 bits each, in 64 bits.
+__device__ __forceinline__ double low(u32 w) { return (double)__uint_as_float(w << 16); }
+__device__ __forceinline__ double high(u32 w) { return (double)__uint_as_float(w & 0xFFFF0000u); }
+
+// One token a sequence: a block per (row, a.per pages); GS lanes a page, each of 8 elements, 4 pages at a time.
+template <int DP, int GS> __global__ __launch_bounds__(256) void score_one_k(const ScoreArgs a) {
+    constexpr int U = 4, STEP = 256 / GS;
+    const i64 row = blockIdx.x / (u32)a.chunks;
     const int chunk = (int)(blockIdx.x - row * a.chunks);
-    const Place p = place_of(a, row);
-    const int end = p.pages - a.last, from = chunk * 256 > a.first ? chunk * 256 : a.first;
-    const int to = chunk * 256 + 256 < end ? chunk * 256 + 256 : end;
-    if (!p.is || p.pages <= a.keep || from >= to) return;
     const int sub = threadIdx.x % GS, group = threadIdx.x / GS, d0 = sub * 8;
+    const Place p = place_of(a, (u32)row);
+    const int from = chunk * a.per, stop = from + a.per < a.width ? from + a.per : a.width;
+    const int* tab = a.table + p.b * a.table_stride;
+    int e[U], next[U];  // (asked for before the sequence's length is known)
+#pragma unroll
+    for (int u = 0; u < U; ++u) e[u] = from + group + u * STEP < stop ? tab[from + group + u * STEP] : -1;
     double up[8], down[8];
 #pragma unroll
     for (int j = 0; j < 8; ++j) up[j] = down[j] = 0.;
     const u16* q = (const u16*)a.q + p.b * a.qb + p.t * a.qt + (i64)p.h * a.G * a.qh + d0;
-    for (int g = 0; g < a.G; ++g, q += a.qh) {
-        union {
-            uint4 w;
-            u16 e[8];
-        } x;
-        x.w = make_uint4(0, 0, 0, 0);
-        if (a.vec && d0 + 8 <= a.dim) x.w = *(const uint4*)q;
-        else
-            for (int j = 0; j < 8; ++j)
-                if (d0 + j < a.dim) x.e[j] = q[j];
+    if (p.is)
+        for (int g = 0; g < a.G; ++g, q += a.qh) {
+            union {
+                uint4 w;
+                u16 e[8];
+            } x;
+            x.w = make_uint4(0, 0, 0, 0);
+            if (a.vec && d0 + 8 <= a.dim) x.w = *(const uint4*)q;
+            else
+                for (int j = 0; j < 8; ++j)
+                    if (d0 + j < a.dim) x.e[j] = q[j];
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            const float f = a.qtype == NG_BF16 ? __uint_as_float((u32)x.e[j] << 16) : (float)__builtin_bit_cast(f16, x.e[j]);
-            up[j] += f > 0.f || f != f ? (double)f : 0.;
-            down[j] += f < 0.f ? (double)f : 0.;
+            for (int j = 0; j < 8; ++j) {
+                const float f = query_at(a, x.e[j]);
+                up[j] += f > 0.f || f != f ? (double)f : 0.;
+                down[j] += f < 0.f ? (double)f : 0.;
+            }
         }
-    }
-    const int* tab = a.table + p.b * a.table_stride;
-    for (int j0 = from + group; j0 < to; j0 += (256 / GS) * U) {
-        double acc[U];
+    const int end = p.pages - a.last < stop ? p.pages - a.last : stop;
+    if (!p.is || p.pages <= a.keep || from >= end) return;
+    for (int j0 = from + group; j0 < end; j0 += STEP * U) {
         uint4 lo[U], hi[U];
         bool is[U];
 #pragma unroll
         for (int u = 0; u < U; ++u) {
-            const int j = j0 + u * (256 / GS);
-            const int e = j < to ? tab[j] : -1;
-            is[u] = (u32)e < (u64)a.pages;
+            const int j = j0 + u * STEP;
+            is[u] = (u32)e[u] < (u64)a.pages;
             lo[u] = hi[u] = make_uint4(0, 0, 0, 0);
-            if (is[u] && d0 < DP) {
-                const b16* x = a.bounds + ((i64)e * a.H + p.h) * 2 * DP + d0;
+            if (is[u] && j < end && d0 < DP) {
+                const b16* x = a.bounds + ((i64)e[u] * a.H + p.h) * 2 * DP + d0;
                 lo[u] = *(const uint4*)x, hi[u] = *(const uint4*)(x + DP);
             }
+            next[u] = j + STEP * U < stop ? tab[j + STEP * U] : -1;
         }
+        double acc[U];
 #pragma unroll
         for (int u = 0; u < U; ++u) {
             acc[u] = 0.;
             const u32 l[4] = {lo[u].x, lo[u].y, lo[u].z, lo[u].w}, h[4] = {hi[u].x, hi[u].y, hi[u].z, hi[u].w};
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
-                if (d0 + j >= a.dim) continue;
-                const float x = __uint_as_float(j & 1 ? l[j / 2] & 0xFFFF0000u : l[j / 2] << 16);
-                const float y = __uint_as_float(j & 1 ? h[j / 2] & 0xFFFF0000u : h[j / 2] << 16);
-                acc[u] = fma(down[j], (double)x, fma(up[j], (double)y, acc[u]));
+                const double x = j & 1 ? high(l[j / 2]) : low(l[j / 2]), y = j & 1 ? high(h[j / 2]) : low(h[j / 2]);
+                acc[u] = fma(down[j], x, fma(up[j], y, acc[u]));
+            }
+        }
+        // the four pages' sums over the lanes, each step for half as many pages: a quarter of the lanes ends with each
+        const bool a1 = sub & (GS / 2), a2 = sub & (GS / 4);
+        double x = (a1 ? acc[2] : acc[0]) + __shfl_xor(a1 ? acc[0] : acc[2], GS / 2, GS);
+        double y = (a1 ? acc[3] : acc[1]) + __shfl_xor(a1 ? acc[1] : acc[3], GS / 2, GS);
+        x = (a2 ? y : x) + __shfl_xor(a2 ? x : y, GS / 4, GS);
+#pragma unroll
+        for (int o = GS / 8; o; o >>= 1) x += __shfl_xor(x, o, GS);
+        const int u = (a1 ? 2 : 0) + (a2 ? 1 : 0), j = j0 + u * STEP;
+        const bool mine = a1 ? (a2 ? is[3] : is[2]) : (a2 ? is[1] : is[0]);
+        if (j >= a.first && j < end && sub % (GS / 4) == 0) a.score[row * a.width + j] = score_key(mine, x);
+#pragma unroll
+        for (int u = 0; u < U; ++u) e[u] = next[u];
+    }
+}
+
+typedef double d4 __attribute__((ext_vector_type(4)));
+
+// Several tokens a sequence: a block per (16 tokens of a sequence and head, a.per pages), on the matrix units: tokens x pages,
+// 16 of each a wave at a time. A lane's operand is 8 in 32 elements of a page's bounds (of one page in 16) and the same ones
+// of a token's sums, which lie in LDS.
+template <int DP> __global__ __launch_bounds__(256, DP <= 128 ? 4 : 2) void score_k(const ScoreArgs a) {
+    constexpr int LD = 2 * DP + 2;  // (16 rows' reads of 16 bytes meet no bank twice)
+    __shared__ __align__(16) double sums[16 * LD];
+    const int c = lane_id() & 15, g = lane_id() >> 4, wave = threadIdx.x >> 6;
+    const u32 tiles = (a.nt + 15) / 16, unit = blockIdx.x / (u32)a.chunks, bh = unit / tiles;  // (sequence, head, 16 tokens)
+    const u32 at = bh / (u32)a.H;
+    const int chunk = (int)(blockIdx.x - unit * a.chunks), tile = (int)(unit - bh * tiles) * 16;
+    const int h = (int)(bh - at * a.H), b = a.b0 + (int)at, t0 = a.t0 + tile;
+    const int n = a.nt - tile < 16 ? a.nt - tile : 16;
+    const i64 row0 = ((i64)at * a.nt + tile) * a.H + h;
+    const Place whole = place_of(a, (u32)(row0 + (i64)(n - 1) * a.H));  // the last token sees the most pages
+    const int from = chunk * a.per;
+    const int stop = from + a.per < whole.pages - a.last ? from + a.per : whole.pages - a.last;
+    if (whole.pages <= a.keep || from >= stop) return;
+    const int w = a.widths ? a.widths[b] : a.T;
+    if (t0 >= w) return;
+    for (int i = threadIdx.x; i < 16 * DP / 8; i += 256) {
+        const int t = i / (DP / 8), d0 = i % (DP / 8) * 8;
+        double up[8], down[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) up[j] = down[j] = 0.;
+        if (t < n && t0 + t < w) {
+            const u16* q = (const u16*)a.q + b * a.qb + (t0 + t) * a.qt + (i64)h * a.G * a.qh + d0;
+            for (int k = 0; k < a.G; ++k, q += a.qh) {
+                union {
+                    uint4 w;
+                    u16 e[8];
+                } x;
+                x.w = make_uint4(0, 0, 0, 0);
+                if (a.vec && d0 + 8 <= a.dim) x.w = *(const uint4*)q;
+                else
+                    for (int j = 0; j < 8; ++j)
+                        if (d0 + j < a.dim) x.e[j] = q[j];
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    const float f = query_at(a, x.e[j]);
+                    up[j] += f > 0.f || f != f ? (double)f : 0.;
+                    down[j] += f < 0.f ? (double)f : 0.;
+                }
             }
         }
 #pragma unroll
-        for (int u = 0; u < U; ++u) {
+        for (int j = 0; j < 8; ++j) sums[t * LD + d0 + j] = up[j], sums[t * LD + DP + d0 + j] = down[j];
+    }
+    __syncthreads();
+    const int* tab = a.table + b * a.table_stride;
+    const double* mine = sums + c * LD + g * 8;
+    const int steps = (a.dim + 31) / 32;
+    u64* out = a.score + (row0 + (i64)g * a.H) * a.width;
+    int ends[4];  // behind the last page that a token's score is wanted of
 #pragma unroll
-            for (int o = GS / 2; o; o >>= 1) acc[u] += __shfl_xor(acc[u], o, GS);
-            const int j = j0 + u * (256 / GS);
-            if (j < to && sub == 0) {
-                // a page of none of the cache's ranks last, one whose score is NaN first
-                const u64 x = (u64)__double_as_longlong(acc[u] + 0.);
-                a.score[row * a.width + j] = !is[u] ? 1ull : acc[u] != acc[u] ? ~1ull : x >> 63 ? ~x : x | 1ull << 63;
+    for (int r = 0; r < 4; ++r) {
+        const int t = 4 * r + g;
+        const i64 keys = whole.len + t0 + t + 1, cap = (i64)a.width << a.shift;
+        const int pages = (int)(((keys < cap ? keys : cap) + (1 << a.shift) - 1) >> a.shift);
+        ends[r] = t < n && t0 + t < w ? (pages - a.last < stop ? pages - a.last : stop) : 0;
+    }
+    auto entry = [&](int j) { return j + c < stop ? tab[j + c] : -1; };
+    auto page = [&](int e) { return a.bounds + ((i64)((u32)e < (u64)a.pages ? e : 0) * a.H + h) * 2 * DP + g * 8; };
+    int e = entry(from + wave * 16), next = entry(from + wave * 16 + 64);
+    const b16* x = page(e);
+    uint4 lo = *(const uint4*)x, hi = *(const uint4*)(x + DP);
+    for (int j0 = from + wave * 16; j0 < stop; j0 += 64) {
+        const bool is = (u32)e < (u64)a.pages;
+        const b16* then = page(next);
+        e = next, next = entry(j0 + 128);
+        d4 acc = {0., 0., 0., 0.}, more = {0., 0., 0., 0.};
+#pragma unroll 1
+        for (int i = 0; i < steps; ++i) {  // (the next eight elements, or the next page's first, are under way)
+            const u32 l[4] = {lo.x, lo.y, lo.z, lo.w}, k[4] = {hi.x, hi.y, hi.z, hi.w};
+            x = i + 1 < steps ? x + 32 : then;
+            lo = *(const uint4*)x, hi = *(const uint4*)(x + DP);
+#pragma unroll
+            for (int j = 0; j < 8; j += 2) {
+                const double2 up = *(const double2*)(mine + i * 32 + j), down = *(const double2*)(mine + DP + i * 32 + j);
+                acc = __builtin_amdgcn_mfma_f64_16x16x4f64(up.x, low(k[j / 2]), acc, 0, 0, 0);
+                more = __builtin_amdgcn_mfma_f64_16x16x4f64(down.x, low(l[j / 2]), more, 0, 0, 0);
+                acc = __builtin_amdgcn_mfma_f64_16x16x4f64(up.y, high(k[j / 2]), acc, 0, 0, 0);
+                more = __builtin_amdgcn_mfma_f64_16x16x4f64(down.y, high(l[j / 2]), more, 0, 0, 0);
             }
         }
+        const int j = j0 + c;  // this lane's page; its tokens: 4 r + g
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+            if (j >= a.first && j < ends[r]) out[(i64)r * 4 * a.H * a.width + j] = score_key(is, acc[r] + more[r]);
     }
 }
 
@@ -129,14 +241,14 @@ template <int DP, int GS> __global__ __launch_bounds__(256) void score_k(const S
 template <int NW, int E> __global__ __launch_bounds__(NW == 1 ? 256 : NW * 64) void choose_k(const ScoreArgs a) {
     constexpr int NT = NW * 64;
     __shared__ int counts[2][NW], before[NW == 1 ? 1 : E * NW];
-    __shared__ u64 ends[2][NW];
+    __shared__ u32 ends[2][NW];
     const i64 row = NW == 1 ? (i64)blockIdx.x * 4 + (threadIdx.x >> 6) : (i64)blockIdx.x;
     if (row >= a.rows) return;
     const int tid = NW == 1 ? lane_id() : (int)threadIdx.x, wave = NW == 1 ? 0 : tid >> 6;
-    const Place p = place_of(a, row);
+    const Place p = place_of(a, (u32)row);
     const int* tab = a.table + p.b * a.table_stride;
     int* out = a.table_out + row * a.keep;
-    int* chosen = a.chosen ? a.chosen + (a.first_row + row) * a.keep : nullptr;
+    int* chosen = a.chosen ? a.chosen + (((i64)p.b * a.T + p.t) * a.H + p.h) * a.keep : nullptr;
     const int n = p.is ? p.pages : 0, kept = n < a.keep ? n : a.keep;
     if (tid == 0) {
         const int rest = n ? (int)(p.keys - ((i64)(n - 1) << a.shift)) : 0;
@@ -153,14 +265,16 @@ template <int NW, int E> __global__ __launch_bounds__(NW == 1 ? 256 : NW * 64) v
         }
         return;
     }
-    u64 key[E], lo = ~0ull, hi = 0;
+    // the upper words of the scores decide but where they are equal (a score's first 20 bits): then the lower ones
+    u32 key[E], rest[E], lo = ~0u, hi = 0;
 #pragma unroll
     for (int e = 0; e < E; ++e) {
         const int j = e * NT + tid;
-        key[e] = 0;
-        if (j < n) key[e] = j < a.first || j >= n - a.last ? ~0ull : a.score[row * a.width + j];
+        u64 k = 0;
+        if (j < n) k = j < a.first || j >= n - a.last ? ~0ull : a.score[row * a.width + j];
+        key[e] = (u32)(k >> 32), rest[e] = (u32)k;
         if (j < n) lo = key[e] < lo ? key[e] : lo;
-        if (key[e] != ~0ull) hi = key[e] > hi ? key[e] : hi;
+        if (key[e] != ~0u) hi = key[e] > hi ? key[e] : hi;
     }
     lo = min_wave(lo), hi = max_wave(hi);
     if constexpr (NW > 1) {
@@ -170,11 +284,23 @@ template <int NW, int E> __global__ __launch_bounds__(NW == 1 ? 256 : NW * 64) v
         for (int w = 0; w < NW; ++w) lo = ends[0][w] < lo ? ends[0][w] : lo, hi = ends[1][w] > hi ? ends[1][w] : hi;
     }
     Count<NW> count(counts);
-    int c = n;
-    const int forced = a.first + a.last;
-    const u64 t = forced == a.keep ? ~0ull : count.threshold(key, lo, hi, a.keep, a.keep, c);
-    int equal = E * NT;  // of the scores equal to t, the first so many
-    if (forced < a.keep && c > a.keep) equal = a.keep - count.at_least(key, t + 1);
+    int c;
+    // (an upper word of ones: a page always kept, or a NaN, whose lower word is one less; hi is below both)
+    u32 t = ~0u, t2 = 0;
+    int equal = E * NT;  // of the scores equal to t and t2, the first so many
+    c = count.at_least(key, t);
+    if (c < a.keep) {
+        c = n;
+        t = count.threshold(key, lo, hi, a.keep, a.keep, c);
+    }
+    if (c > a.keep) {
+        const int above = t == ~0u ? 0 : count.at_least(key, t + 1);
+#pragma unroll
+        for (int e = 0; e < E; ++e) rest[e] = key[e] == t ? rest[e] : 0u;
+        c -= above;
+        t2 = count.threshold(rest, 0u, ~0u, a.keep - above, a.keep - above, c);
+        if (c > a.keep - above) equal = a.keep - above - (t2 == ~0u ? 0 : count.at_least(rest, t2 + 1));
+    }
     // in order of the pages: first how many of each wave's 64 come before
     auto place = [&](auto is, auto got) {
         int run = 0;
@@ -207,8 +333,12 @@ template <int NW, int E> __global__ __launch_bounds__(NW == 1 ? 256 : NW * 64) v
     u32 take = 0;
     static_assert(E <= 32, "a bit each");
 #pragma unroll
-    for (int e = 0; e < E; ++e) take |= (key[e] > t || (forced == a.keep && key[e] == t) ? 1u : 0u) << e;
-    if (forced < a.keep) place([&](int e) { return key[e] == t; }, [&](int e, int i) { take |= (i < equal ? 1u : 0u) << e; });
+    for (int e = 0; e < E; ++e) take |= (key[e] > t || (key[e] == t && rest[e] >= t2) ? 1u : 0u) << e;
+    if (equal < E * NT) {
+        u32 drop = 0;
+        place([&](int e) { return key[e] == t && rest[e] == t2; }, [&](int e, int i) { drop |= (i < equal ? 0u : 1u) << e; });
+        take &= ~drop;
+    }
     place([&](int e) { return (take >> e & 1) != 0; }, [&](int e, int i) {
         const int j = e * NT + tid;
         out[i] = tab[j];
@@ -224,7 +354,7 @@ template <int NW, int E> __global__ __launch_bounds__(NW == 1 ? 256 : NW * 64) v
 struct SparsePlan {
     int dp, groups, splits;
     bool scored;
-    i64 tokens;  // at a time
+    int nb, nt;  // sequences and tokens of each at a time
     i64 score, table, rows, po, pm, bytes;  // offsets in the workspace
 };
 
@@ -232,16 +362,16 @@ static bool sparse_plan(i64 B, i64 T, i64 H, i64 G, i64 dim, i64 width, i64 page
     const i64 lim = (i64)1 << 30;
     if (B < 0 || T < 1 || H < 1 || G < 1 || dim < 1 || dim > 256 || width < 1 || width > MOST_PAGES || keep < 1 || keep > 1024 ||
         B > lim || T > lim || H > lim || G > 1 << 20 || page < 16 || page > 4096 || (page & (page - 1)) ||
-        width * page > lim || B * T > lim || H * ((G + 15) / 16) > 1 << 20)
+        width * page > lim || B * T > lim || H * ((G + 15) / 16) > 1 << 12)
         return false;
     p.dp = (int)(dim + 63) / 64 * 64, p.groups = (int)(G + 15) / 16, p.scored = width > keep;
-    const i64 tokens = B * T;
-    // a pass takes as many tokens as SLAB holds the scores of, and fewer than 2^24 units
-    p.tokens = tokens;
-    const i64 each = H * width * 8, most_units = ((i64)1 << 24) / (H * p.groups);
-    if (p.scored && p.tokens * each > SLAB) p.tokens = SLAB / each ? SLAB / each : 1;
-    if (p.tokens > most_units) p.tokens = most_units ? most_units : 1;
-    const i64 rows = p.tokens * H, units = rows * p.groups;
+    // a pass takes as many sequences, or (one) sequence's tokens, as SLAB holds the scores of, and fewer than 2^24 units
+    const i64 each = p.scored ? H * width * 8 : 1, most_units = ((i64)1 << 24) / (H * p.groups);
+    i64 most = SLAB / each < most_units ? SLAB / each : most_units;
+    if (most < 16) most = 16;
+    p.nt = (int)(T <= most ? T : most / 16 * 16);
+    p.nb = (int)(T <= most ? (B < most / T ? B : most / T) : 1);
+    const i64 rows = (B ? (i64)p.nb : 0) * p.nt * H, units = rows * p.groups;
     const i64 tiles = ((keep < width ? keep : width) * page + TILE - 1) / TILE;
     i64 splits = units ? (AIM + units - 1) / units : 1;
     p.splits = (int)(splits < tiles ? splits : tiles);
@@ -294,14 +424,27 @@ extern "C" int ng_page_bounds(const void* k, const float* ks, i64 pages, int pag
     }
 }
 
-static int score_rows(const ScoreArgs& a, int dp, hipStream_t st) {
-    const i64 n = a.rows * a.chunks;
+// One token a sequence is scored by vector operations, more on the matrix units, of which a token uses a sixteenth: 4 tokens
+// of 2 sequences over 524288 positions x us there, y by vector operations. A block takes 256 pages, or 64 where that
+// leaves fewer than 1024 blocks.
+static int score_rows(ScoreArgs& a, int nb, int dp, hipStream_t st) {
+    const i64 units = (i64)nb * a.H * (a.T == 1 ? 1 : (a.nt + 15) / 16);
+    i64 per = units * a.width / 1024;
+    per = per < 256 ? (per + 63) / 64 * 64 : 256;
+    a.per = per ? (int)per : 64;
+    a.chunks = (a.width + a.per - 1) / a.per;
+    const i64 n = units * a.chunks;
     if (n >= (i64)1 << 31) return -1;
-    switch (dp) {
-        case 64: score_k<64, 8><<<(unsigned)n, 256, 0, st>>>(a); break;
-        case 128: score_k<128, 16><<<(unsigned)n, 256, 0, st>>>(a); break;
-        case 192: score_k<192, 32><<<(unsigned)n, 256, 0, st>>>(a); break;
-        default: score_k<256, 32><<<(unsigned)n, 256, 0, st>>>(a);
+    if (a.T == 1) switch (dp) {
+        case 64: score_one_k<64, 8><<<(unsigned)n, 256, 0, st>>>(a); break;
+        case 128: score_one_k<128, 16><<<(unsigned)n, 256, 0, st>>>(a); break;
+        case 192: score_one_k<192, 32><<<(unsigned)n, 256, 0, st>>>(a); break;
+        default: score_one_k<256, 32><<<(unsigned)n, 256, 0, st>>>(a);
+    } else switch (dp) {
+        case 64: score_k<64><<<(unsigned)n, 256, 0, st>>>(a); break;
+        case 128: score_k<128><<<(unsigned)n, 256, 0, st>>>(a); break;
+        case 192: score_k<192><<<(unsigned)n, 256, 0, st>>>(a); break;
+        default: score_k<256><<<(unsigned)n, 256, 0, st>>>(a);
     }
     return (int)hipGetLastError();
 }
@@ -325,7 +468,6 @@ extern "C" int ng_sparse_attention(const void* q, i64 qb, i64 qt, i64 qh, int qt
     s.shift = __builtin_ctz((unsigned)page), s.width = width, s.keep = keep, s.first = first, s.last = last;
     s.qtype = qtype, s.vec = ((u64)q & 15) == 0 && (((qb | qt | qh) * 2) & 15) == 0;
     s.score = (u64*)(w + p.score), s.table_out = (int*)(w + p.table), s.row_out = (int2*)(w + p.rows), s.chosen = chosen;
-    s.chunks = (width + 255) / 256;
     SparseArgs r;
     TreeArgs& a = r.a;
     a.q = q, a.qb = qb, a.qt = qt, a.qh = qh, a.k = k, a.v = v, a.ks = ks, a.vs = vs, a.table = s.table_out;
@@ -333,20 +475,24 @@ extern "C" int ng_sparse_attention(const void* q, i64 qb, i64 qt, i64 qh, int qt
     a.po = (float*)(w + p.po), a.pm = (float*)(w + p.pm), a.pages = pages, a.B = B, a.T = 1, a.H = H, a.G = G, a.dim = dim;
     a.shift = s.shift, a.width = keep, a.groups = p.groups, a.qtype = qtype, a.vec = s.vec, a.scale = scale;
     r.rows = s.row_out, r.T = T, r.splits = p.splits;
-    a.pl = a.pm + (p.splits > 1 ? p.tokens * H * p.groups * p.splits * 16 : 0);
+    a.pl = a.pm + (p.splits > 1 ? (i64)p.nb * p.nt * H * p.groups * p.splits * 16 : 0);
     hipStream_t st = (hipStream_t)stream;
-    const i64 tokens = (i64)B * T;
-    for (i64 t0 = 0; t0 < tokens; t0 += p.tokens) {
-        const i64 n = tokens - t0 < p.tokens ? tokens - t0 : p.tokens;
-        s.first_row = t0 * H, s.rows = n * H;
+    for (int b0 = 0; b0 < B; b0 += p.nb)
+    for (int t0 = 0; t0 < T; t0 += p.nt) {
+        const int nb = B - b0 < p.nb ? B - b0 : p.nb;
+        s.b0 = r.b0 = b0, s.t0 = r.t0 = t0, s.nt = r.nt = T - t0 < p.nt ? T - t0 : p.nt;
+        s.rows = (i64)nb * s.nt * H;
         int rc;
-        if (p.scored && (rc = score_rows(s, p.dp, st))) return rc;
-        // by the scores that a row can have: 1024 are a wave's, 4096 four waves'
-        if (width <= 1024) choose_k<1, 16><<<(unsigned)((s.rows + 3) / 4), 256, 0, st>>>(s);
+        if (p.scored && (rc = score_rows(s, nb, p.dp, st))) return rc;
+        // by the scores that a row can have: a wave's, a row a wave; four waves'; a block's
+        if (width <= 256) choose_k<1, 4><<<(unsigned)((s.rows + 3) / 4), 256, 0, st>>>(s);
+        else if (width <= 640) choose_k<1, 10><<<(unsigned)((s.rows + 3) / 4), 256, 0, st>>>(s);
+        else if (width <= 1024) choose_k<1, 16><<<(unsigned)((s.rows + 3) / 4), 256, 0, st>>>(s);
         else if (width <= 4096) choose_k<4, 16><<<(unsigned)s.rows, 256, 0, st>>>(s);
+        else if (width <= 16384) choose_k<16, 16><<<(unsigned)s.rows, 1024, 0, st>>>(s);
         else choose_k<16, 32><<<(unsigned)s.rows, 1024, 0, st>>>(s);
         if ((rc = (int)hipGetLastError())) return rc;
-        r.first_row = s.first_row, r.units = s.rows * p.groups;
+        r.units = s.rows * p.groups;
         switch (codes) {
             case KV_INT8: rc = sparse_codes<KV_INT8>(r, p.dp, st); break;
             case KV_FP8: rc = sparse_codes<KV_FP8>(r, p.dp, st); break;
