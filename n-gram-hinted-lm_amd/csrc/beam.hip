@@ -493,7 +493,7 @@ template <typename U> __global__ __launch_bounds__(256) void gather_rows_k(const
     for (i64 j = (blockIdx.x % parts) * 256 + threadIdx.x; j < units; j += (i64)parts * 256) {
         U x = {};
         if (is) x = s[j];
-        o[j] = x;
+        __builtin_nontemporal_store(x, o + j);
     }
 }
 
@@ -513,7 +513,8 @@ extern "C" int ng_gather_rows(const void* src, i64 stride, i64 rows, i64 bytes, 
     hipStream_t st = (hipStream_t)stream;
     const unsigned grid = (unsigned)(parts * n);
 #define GATHER(U) gather_rows_k<U><<<grid, 256, 0, st>>>((const char*)src, stride, rows, from, units, (int)parts, (char*)out)
-    if (size == 16) GATHER(uint4);
+    typedef u32 words __attribute__((ext_vector_type(4)));
+    if (size == 16) GATHER(words);
     else if (size == 4) GATHER(u32);
     else if (size == 2) GATHER(u16);
     else GATHER(unsigned char);

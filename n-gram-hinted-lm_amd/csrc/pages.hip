@@ -105,7 +105,7 @@ struct Room {
 enum { KEPT = -1, NONE = -2 };
 
 struct Ask {
-    int column, entry;
+    int column, entry, refs;
     bool is, held;
 };
 
@@ -120,7 +120,8 @@ __device__ __forceinline__ Ask ask_of(const Pool& p, const Room& r, int i) {
     q.column = (len >> r.shift) + j;
     q.is = ((i64)q.column << r.shift) < (i64)len + row_count(r, s) && q.column < r.width && row_count(r, s) > 0;
     q.entry = q.is ? r.table[s * r.stride + q.column] : -1;
-    q.held = q.is && is_page(p, q.entry) && p.refs[q.entry] > 0;  // (an entry that was never counted is none)
+    q.refs = q.is && is_page(p, q.entry) ? p.refs[q.entry] : 0;
+    q.held = q.refs > 0;  // (an entry that was never counted is none)
     return q;
 }
 
@@ -145,56 +146,89 @@ __device__ __forceinline__ int scan_block(int x, int* lds, int& total) {
     return before + inc - x;
 }
 
-__global__ __launch_bounds__(1024) void pool_room_k(const Pool p, const Room r) {
-    __shared__ int sums[16];
-    const int n = r.S * r.per, tid = threadIdx.x;
-    // who else asks for a shared page
-    for (int i = tid; i < n; i += 1024) {
-        const Ask q = ask_of(p, r, i);
-        if (q.held && p.refs[q.entry] != 1) {
-            atomicAdd(&p.asks[q.entry], 1);
-            atomicMin(&p.claim[q.entry], i);
+// The requests for a shared page, in LDS where there are no more than 1024: a place for each page, found by probing from its
+// number's.
+#define PLACES 2048
+struct Askers {
+    int page[PLACES], count[PLACES], first[PLACES];
+    __device__ __forceinline__ int place(int p) {
+        for (u32 i = (u32)p * 2654435761u >> 21;; i = (i + 1) % PLACES) {  // (twice as many places as requests: one is empty)
+            const int at = atomicCAS(&page[i], -1, p);
+            if (at == p || at == -1) return (int)i;
         }
     }
-    __syncthreads();
-    int wanted = 0;
+};
+
+// ONE: no more than 1024 requests, each in its thread's registers throughout; else they are read again in each phase.
+template <bool ONE> __global__ __launch_bounds__(1024) void pool_room_k(const Pool p, const Room r) {
+    __shared__ int sums[16];
+    __shared__ int lowest[ONE ? 1024 : 1];
+    __shared__ Askers askers[1];
+    const int n = r.S * r.per, tid = threadIdx.x;
+    int* given = ONE ? lowest : r.given;
+    Ask one;
+    int refs = 0;
+    one.is = one.held = false;
+    const i64 words = (p.pages + 31) / 32;
+    const u32 first = tid < words ? p.free[tid] : 0u;
+    int place = 0;
+    // who else asks for a shared page
+    if constexpr (ONE) {
+        for (int i = tid; i < PLACES; i += 1024) askers->page[i] = -1, askers->count[i] = 0, askers->first[i] = INT_MAX;
+        if (tid < n) one = ask_of(p, r, tid), refs = one.refs;
+        lds_barrier();
+        if (one.held && refs != 1) {
+            place = askers->place(one.entry);
+            atomicAdd(&askers->count[place], 1);
+            atomicMin(&askers->first[place], tid);
+        }
+        lds_barrier();
+    } else {
+        for (int i = tid; i < n; i += 1024) {
+            const Ask q = ask_of(p, r, i);
+            if (q.held && q.refs != 1) {
+                atomicAdd(&p.asks[q.entry], 1);
+                atomicMin(&p.claim[q.entry], i);
+            }
+        }
+        __syncthreads();
+    }
+    int wanted = 0, rank = NONE;
     for (int i0 = 0; i0 < n; i0 += 1024) {
         const int i = i0 + tid;
-        bool want = false, is = false;
-        int entry = -1;
-        if (i < n) {
-            const Ask q = ask_of(p, r, i);
-            is = q.is;
-            want = q.is;
-            if (q.held) {
-                entry = q.entry;
-                const int refs = p.refs[q.entry];
-                want = refs != 1 && !(refs == load_agent(&p.asks[q.entry]) && load_agent(&p.claim[q.entry]) == i);
-            }
+        Ask q = one;
+        if (!ONE && i < n) q = ask_of(p, r, i);
+        bool want = i < n && q.is;
+        if (want && q.held) {
+            const int refs = q.refs;
+            if (ONE) want = refs != 1 && !(refs == askers->count[place] && askers->first[place] == i);
+            else want = refs != 1 && !(refs == load_agent(&p.asks[q.entry]) && load_agent(&p.claim[q.entry]) == i);
         }
         int total;
         const int at = scan_block(want, sums, total);
-        if (i < n) r.rank[i] = want ? wanted + at : is ? KEPT : NONE, r.page[i] = entry;
+        if (i < n) {
+            rank = want ? wanted + at : q.is ? KEPT : NONE;
+            if (!ONE) r.rank[i] = rank, r.page[i] = q.held ? q.entry : -1;
+        }
         wanted += total;
     }
     // the lowest free pages
-    const i64 words = (p.pages + 31) / 32;
     int found = 0;
     for (i64 w0 = 0; w0 < words && found < wanted; w0 += 1024) {
-        u32 bits = w0 + tid < words ? p.free[w0 + tid] : 0u;
+        u32 bits = w0 == 0 ? first : w0 + tid < words ? p.free[w0 + tid] : 0u;
         int total, at = found + scan_block(__popc(bits), sums, total);
-        for (; bits && at < wanted; ++at, bits &= bits - 1) r.given[at] = (int)((w0 + tid) * 32 + __builtin_ctz(bits));
+        for (; bits && at < wanted; ++at, bits &= bits - 1) given[at] = (int)((w0 + tid) * 32 + __builtin_ctz(bits));
         found += total;
     }
     if (found > wanted) found = wanted;
     if (tid == 0 && wanted > found) *p.missing += wanted - found;
     __syncthreads();
     for (int i = tid; i < n; i += 1024) {
-        const int k = r.rank[i], held = r.page[i], s = i / r.per, j = i - s * r.per;
+        const int k = ONE ? rank : r.rank[i], held = !ONE ? r.page[i] : one.held ? one.entry : -1, s = i / r.per, j = i - s * r.per;
         int page = k == KEPT ? held : -1, source = -1;
         if (k >= 0 && k < found) {
-            page = r.given[k];
-            r.table[s * r.stride + ((r.lengths[s] < 0 ? 0 : r.lengths[s]) >> r.shift) + j] = page;
+            page = given[k];
+            r.table[s * r.stride + (ONE ? one.column : ((r.lengths[s] < 0 ? 0 : r.lengths[s]) >> r.shift) + j)] = page;
             p.refs[page] = 1;
             atomicAnd(&p.free[page >> 5], ~(1u << (page & 31)));
             if (held >= 0) {
@@ -202,7 +236,7 @@ __global__ __launch_bounds__(1024) void pool_room_k(const Pool p, const Room r) 
                 source = held;
             }
         }
-        if (held >= 0) p.asks[held] = 0, p.claim[held] = INT_MAX;
+        if (!ONE && held >= 0) p.asks[held] = 0, p.claim[held] = INT_MAX;
         r.page[i] = page;
         if (j == 0) r.source[s] = source;
     }
@@ -222,6 +256,12 @@ struct Parts {
     i64 src_pages, dst_pages;
 };
 
+// A store of lines that nothing reads soon: they leave the L2 while the kernel runs, not at its end.
+__device__ __forceinline__ void stream16(char* p, uint4 x) {
+    typedef u32 words __attribute__((ext_vector_type(4)));
+    __builtin_nontemporal_store(__builtin_bit_cast(words, x), (words*)p);
+}
+
 __device__ __forceinline__ void copy_bytes(const char* s, char* d, i64 bytes) {  // both at multiples of 16 bytes
     const i64 n = bytes / 16;
     i64 i = threadIdx.x;
@@ -230,31 +270,51 @@ __device__ __forceinline__ void copy_bytes(const char* s, char* d, i64 bytes) { 
 #pragma unroll
         for (int k = 0; k < 4; ++k) x[k] = ((const uint4*)s)[i + k * 256];
 #pragma unroll
-        for (int k = 0; k < 4; ++k) ((uint4*)d)[i + k * 256] = x[k];
+        for (int k = 0; k < 4; ++k) stream16(d + (i + k * 256) * 16, x[k]);
     }
     for (; i < n; i += 256) ((uint4*)d)[i] = ((const uint4*)s)[i];
     for (i = n * 4 + threadIdx.x; i < bytes / 4; i += 256) ((u32*)d)[i] = ((const u32*)s)[i];
 }
 
-// A block per (row, head): the slots of the row's positions (head 0), and the rows of a copied page.
-__global__ __launch_bounds__(256) void pool_slots_k(const Pool p, const Room r, const Parts c, i64* __restrict__ slots) {
+// A block per (row, head): the slots of the row's positions (head 0), and the rows of a copied page. (128 threads: the blocks
+// of 512 rows and 8 heads are on the card at once, and what they wait for one after the other they wait for together.)
+__global__ __launch_bounds__(128) void pool_slots_k(const Pool p, const Room r, const Parts c, i64* __restrict__ slots) {
     const int s = blockIdx.x / c.H, h = blockIdx.x - s * c.H;
-    const int len = r.lengths[s] < 0 ? 0 : r.lengths[s], in = (1 << r.shift) - 1;
-    if (h == 0) {
-        const int own = row_count(r, s);
-        for (int i = threadIdx.x; i < r.count; i += 256) {
+    const int l = r.lengths[s], from = r.source[s], to = r.page[s * r.per], own = row_count(r, s);
+    const int len = l < 0 ? 0 : l, in = (1 << r.shift) - 1;
+    if (h == 0)
+        for (int i = threadIdx.x; i < r.count; i += 128) {
             const i64 pos = (i64)len + i;
             const int page = i < own ? r.page[s * r.per + (int)((pos >> r.shift) - (len >> r.shift))] : -1;
             slots[(i64)s * r.count + i] = page < 0 ? -1 : ((i64)page << r.shift) + (pos & in);
         }
-    }
-    const int rows = len & in, from = r.source[s];
+    const int rows = len & in;
     if (!rows || from < 0) return;
-    const int to = r.page[s * r.per];
-    for (int k = 0; k < c.n; ++k) {
-        const Part& t = c.part[k];
-        copy_bytes(t.src + (((i64)from * c.H + h) << c.shift) * t.bytes, t.dst + (((i64)to * c.H + h) << c.shift) * t.bytes,
-                   rows * t.bytes);
+    const i64 a = ((i64)from * c.H + h) << c.shift, b = ((i64)to * c.H + h) << c.shift;
+    // keys and values together, so that a row's loads are all under way before its stores
+    const i64 row = c.part[0].bytes;
+    const int units = (int)(rows * row / 16), t = threadIdx.x;
+    const bool q8 = c.n > 2;
+    u32 ks = 0, vs = 0;
+    if (q8 && t < rows) ks = ((const u32*)c.part[2].src)[a + t], vs = ((const u32*)c.part[3].src)[a + t];
+    for (int i = t; i < units; i += 512) {
+        uint4 x[2][4];
+#pragma unroll
+        for (int k = 0; k < 2; ++k)
+#pragma unroll
+            for (int u = 0; u < 4; ++u)
+                if (i + u * 128 < units) x[k][u] = ((const uint4*)(c.part[k].src + a * row))[i + u * 128];
+#pragma unroll
+        for (int k = 0; k < 2; ++k)
+#pragma unroll
+            for (int u = 0; u < 4; ++u)
+                if (i + u * 128 < units) stream16(c.part[k].dst + b * row + (i + u * 128) * 16ll, x[k][u]);
+    }
+    if (!q8) return;
+    if (t < rows) ((u32*)c.part[2].dst)[b + t] = ks, ((u32*)c.part[3].dst)[b + t] = vs;
+    for (int i = t + 128; i < rows; i += 128) {
+        ((u32*)c.part[2].dst)[b + i] = ((const u32*)c.part[2].src)[a + i];
+        ((u32*)c.part[3].dst)[b + i] = ((const u32*)c.part[3].src)[a + i];
     }
 }
 
@@ -279,31 +339,21 @@ __global__ __launch_bounds__(256) void copy_pages_k(const Parts c, const I* __re
     }
 }
 
-// The live pages in order: list[i] = the i-th, map[p] = its place (-1), and the other pool's state. A block per 1024 words of
-// free bits, which counts the words before its own by itself.
+// The live pages in order: list[i] = the i-th, map[p] = its place (-1), and the other pool's state. A thread a page; a block
+// counts the free bits before its own by itself.
 __global__ __launch_bounds__(1024) void pool_pack_k(const Pool p, const Pool to, int* __restrict__ list, int* __restrict__ map) {
     __shared__ int sums[16];
-    const i64 words = (p.pages + 31) / 32;
-    const int tid = threadIdx.x;
-    auto live = [&](i64 w) {
-        return w < words ? ~p.free[w] & (w * 32 + 32 <= p.pages ? ~0u : (1u << (p.pages & 31)) - 1) : 0u;
-    };
+    const i64 page = (i64)blockIdx.x * 1024 + threadIdx.x;
+    const bool is = page < p.pages && !(p.free[page >> 5] >> (page & 31) & 1);
+    const int refs = is ? p.refs[page] : 0;
     int n = 0, before, total;
-    for (i64 w = tid; w < (i64)blockIdx.x * 1024; w += 1024) n += __popc(live(w));
+    for (i64 w = threadIdx.x; w < (i64)blockIdx.x * 32; w += 1024) n += __popc(~p.free[w]);  // (whole words)
     scan_block(n, sums, before);
-    const i64 w = (i64)blockIdx.x * 1024 + tid;
-    const u32 bits = live(w);
-    int at = before + scan_block(__popc(bits), sums, total);
-    for (int b = 0; b < 32; ++b) {
-        const i64 page = w * 32 + b;
-        if (w >= words || page >= p.pages) break;
-        const bool is = bits >> b & 1;
-        map[page] = is && at < to.pages ? at : -1;
-        if (is && at < to.pages) list[at] = (int)page, to.refs[at] = p.refs[page];
-        at += is;
-    }
+    const int at = before + scan_block(is, sums, total);
+    if (page < p.pages) map[page] = is && at < to.pages ? at : -1;
+    if (is && at < to.pages) list[at] = (int)page, to.refs[at] = refs;
     if (blockIdx.x + 1 < gridDim.x) return;
-    const int all = before + total;  // the last block: what is behind the live pages
+    const int all = before + total, tid = threadIdx.x;  // the last block: what is behind the live pages
     if (tid == 0) *to.missing += all > to.pages ? (int)(all - to.pages) : 0;
     for (i64 i = all + tid; i < to.pages; i += 1024) list[i] = -1, to.refs[i] = 0;
     for (i64 v = tid; v < (to.pages + 31) / 32; v += 1024) {
@@ -418,10 +468,11 @@ extern "C" int ng_pool_room(void* state, i64 pages, int* table, i64 stride, int 
     const i64 n = (i64)S * r.per;
     r.rank = (int*)work, r.page = r.rank + n, r.given = r.page + n, r.source = r.given + n;
     hipStream_t st = (hipStream_t)stream;
-    pool_room_k<<<1, 1024, 0, st>>>(p, r);
+    if (n <= 1024) pool_room_k<true><<<1, 1024, 0, st>>>(p, r);
+    else pool_room_k<false><<<1, 1024, 0, st>>>(p, r);
     const int rc = (int)hipGetLastError();
     if (rc) return rc;
-    pool_slots_k<<<(unsigned)(S * heads), 256, 0, st>>>(p, r, c, slots);
+    pool_slots_k<<<(unsigned)(S * heads), 128, 0, st>>>(p, r, c, slots);
     return (int)hipGetLastError();
 }
 
@@ -471,8 +522,7 @@ extern "C" int ng_pool_move(void* state, i64 pages, const void* k, const void* v
     int* list = (int*)work;
     int* map = list + to_pages;
     hipStream_t st = (hipStream_t)stream;
-    const i64 words = (pages + 31) / 32;
-    pool_pack_k<<<(unsigned)((words + 1023) / 1024), 1024, 0, st>>>(p, to, list, map);
+    pool_pack_k<<<(unsigned)((pages + 1023) / 1024), 1024, 0, st>>>(p, to, list, map);
     int rc = (int)hipGetLastError();
     if (rc) return rc;
     if ((i64)S * width) {

@@ -1,6 +1,7 @@
 // Attention over chosen pages (sparse.hip has the mathematics and the host's side; a file per cache type instantiates it).
 #pragma once
 #include "tree.h"
+#include <type_traits>
 
 struct SparseArgs {
     TreeArgs a;  // q, the cache, out, lse; a.table: the chosen pages [rows, keep], a.width: keep
@@ -154,83 +155,150 @@ template <int CODES> int sparse_codes(const SparseArgs& s, int dp, hipStream_t s
 
 // ------------------------------------------------------------------------------------------------------- the bounds
 
-__device__ __forceinline__ b16 outward(float x, bool up) {  // to the next bfloat16 above (or below) where x is none
-    const u32 u = __float_as_uint(x), near = u & 0xFFFF0000u;
-    if (x != x) return __builtin_bit_cast(b16, (u16)0x7FC0);
-    const bool away = up == !(u >> 31);  // its size grows that way
-    return __builtin_bit_cast(b16, (u16)((away && u != near ? near + 0x10000u : near) >> 16));
+// To the next bfloat16 above (or below) where x is none: towards zero, after 2^16 - 1 more where its size grows that way.
+__device__ __forceinline__ b16 outward(float x, bool up) {
+    const u32 u = __float_as_uint(x), negative = (u32)((int)u >> 31);
+    return __builtin_bit_cast(b16, (u16)((u + ((up ? ~negative : negative) & 0xFFFFu)) >> 16));
 }
 
-// A block per (sequence, page that its tokens touch, head): the elements' smallest and largest over the page's rows, where the
-// tokens complete it.
-template <int CODES, int DP>
+// The smaller of two numbers (no NaN), one operation: fminf brings each operand into form first.
+__device__ __forceinline__ float least(float a, float b) { return __builtin_amdgcn_fmed3f(a, b, -__builtin_inff()); }
+
+// The smaller of a lane's and its partner's, 32 or 16 lanes on, of two values at once: half of the lanes keep each.
+template <int O> __device__ __forceinline__ float halve(float a, float b) {
+    const auto r = O == 32 ? __builtin_amdgcn_permlane32_swap(__float_as_uint(a), __float_as_uint(b), false, false)
+                           : __builtin_amdgcn_permlane16_swap(__float_as_uint(a), __float_as_uint(b), false, false);
+    return least(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+
+// WP waves per (sequence, page that its tokens touch, head): the elements' smallest and largest over the page's rows, where
+// the tokens complete it. A lane holds E elements of a row, four rows' loads at a time. Of the lanes of one place in a row the
+// lower half then keeps the smallest, the upper half the largest (as the smallest of the negatives).
+template <int CODES, int DP, int WP>
 __global__ __launch_bounds__(256) void bounds_k(const void* __restrict__ k, const float* __restrict__ ks, i64 pages, int shift,
                                                 int H, int dim, const int* __restrict__ table, i64 stride, int width,
-                                                const int* __restrict__ start, int count, int per, b16* __restrict__ bounds) {
-    constexpr int L = DP / 8, R = 256 / L;  // lanes a row, rows at a time
-    __shared__ float lows[R][DP], highs[R][DP];
-    const int h = blockIdx.x % H, at = blockIdx.x / H, b = at / per;
-    const i64 from = start[b], column = (from >> shift) + (at - b * per);
-    if (column < 0 || (column + 1) << shift > from + count || column >= width) return;
-    const int e = table[b * stride + column];
-    if ((u32)e >= (u64)pages) return;
-    const int r0 = threadIdx.x / L, d0 = threadIdx.x % L * 8;
-    const i64 first = ((i64)e * H + h) << shift;
-    float lo[8], hi[8];
-    u32 bad = 0;
-#pragma unroll
-    for (int j = 0; j < 8; ++j) lo[j] = __builtin_inff(), hi[j] = -__builtin_inff();
-    if (r0 < R)
-        for (int r = r0; r < 1 << shift; r += R) {
-            float x[8];
-            if constexpr (CODES == KV_INT8 || CODES == KV_FP8) {
-                const float s = ks[first + r];
-                const uint2 w = *(const uint2*)((const char*)k + (first + r) * DP + d0);
-                if constexpr (CODES == KV_INT8) {
-#pragma unroll
-                    for (int j = 0; j < 8; ++j) x[j] = (float)(signed char)((j < 4 ? w.x : w.y) >> (8 * (j & 3))) * s;
-                } else {
-#pragma unroll
-                    for (int i = 0; i < 2; ++i) {
-                        const auto a = __builtin_amdgcn_cvt_pk_f32_fp8((int)(i ? w.y : w.x), false);
-                        const auto c = __builtin_amdgcn_cvt_pk_f32_fp8((int)(i ? w.y : w.x), true);
-                        x[4 * i] = a[0] * s, x[4 * i + 1] = a[1] * s, x[4 * i + 2] = c[0] * s, x[4 * i + 3] = c[1] * s;
-                    }
-                }
-            } else {
-                typedef typename op_t<CODES>::type T;
-                Pack<T, 8> p;
-                p.load((const T*)k + (first + r) * DP + d0);
-#pragma unroll
-                for (int j = 0; j < 8; ++j) x[j] = (float)p.v[j];
-            }
-#pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                lo[j] = fminf(lo[j], x[j]), hi[j] = fmaxf(hi[j], x[j]);
-                bad |= (x[j] != x[j] ? 1u : 0u) << j;
-            }
-        }
-    if (r0 < R)
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            lows[r0][d0 + j] = bad >> j & 1 ? __builtin_nanf("") : lo[j];
-            highs[r0][d0 + j] = hi[j];
-        }
-    __syncthreads();
-    const int d = threadIdx.x;
-    if (d >= DP) return;
-    float l = lows[0][d], g = highs[0][d];
-    bool nan = l != l;
-#pragma unroll
-    for (int r = 1; r < R; ++r) {
-        const float x = lows[r][d];
-        nan |= x != x;
-        l = fminf(l, x), g = fmaxf(g, highs[r][d]);
+                                                const int* __restrict__ start, u32 items, int count, int per,
+                                                b16* __restrict__ bounds) {
+    constexpr bool Q8 = CODES == KV_INT8 || CODES == KV_FP8;
+    constexpr int E = DP == 192 ? 12 : Q8 ? 16 : 8, L = DP / E, R = 64 / L;  // elements a lane, lanes a row, rows a wave
+    constexpr int M = R > 2 ? E / 2 : E;                                     // elements that a lane ends with
+    __shared__ float sides[WP == 1 ? 1 : 4][2][WP == 1 ? 1 : DP];
+    const int wave = threadIdx.x >> 6, part = wave % WP, l = lane_id();
+    const u32 item = blockIdx.x * (4 / WP) + wave / WP, page = item / (u32)H, b = page / (u32)per;
+    const int h = (int)(item - page * H);
+    int e = -1;
+    if (item < items) {
+        const i64 from = start[b], column = (from >> shift) + (page - b * per);
+        if (column >= 0 && (column + 1) << shift <= from + count && column < width) e = table[b * stride + column];
     }
-    if (nan) l = g = __builtin_nanf("");
-    if (d >= dim) l = g = 0.f;
-    b16* o = bounds + (((i64)e * H + h) * 2) * DP + d;
-    o[0] = outward(l, false), o[DP] = outward(g, true);
+    if ((u32)e >= (u64)pages) return;  // (all waves of a page)
+    const int r0 = part * R + l / L, d0 = l % L * E;
+    const i64 first = ((i64)e * H + h) << shift;
+    float x[E], hi[E];
+    u32 bad = 0;     // elements that a NaN was seen in
+    // Minima pass over NaN. That there may be one is noticed by words (a code of NaN, a scale that is not finite; 16 bits: an
+    // element larger than infinity); only then the rows are read again with a look at each element.
+    u32 odd = 0;
+    auto rows = [&](auto careful) {
+        constexpr bool EACH = decltype(careful)::value;
+#pragma unroll
+        for (int j = 0; j < E; ++j) x[j] = __builtin_inff(), hi[j] = -__builtin_inff();
+        for (int r = r0; r < 1 << shift; r += 4 * WP * R) {
+            u32 w[4][E * (Q8 ? 1 : 2) / 4];
+            float s[4];
+#pragma unroll
+            for (int u = 0; u < 4; ++u) {  // (a row past the page is the first of the four again)
+                const int at = r + u * WP * R < 1 << shift ? r + u * WP * R : r;
+                load_words<E * (Q8 ? 1 : 2) / 4>((const char*)k + ((first + at) * DP + d0) * (Q8 ? 1 : 2), w[u]);
+                s[u] = Q8 ? ks[first + at] : 1.f;
+            }
+            float v[4][E];
+#pragma unroll
+            for (int u = 0; u < 4; ++u) {
+                if constexpr (Q8 && !EACH) odd |= finite_f(s[u]) ? 0u : 1u;
+                if constexpr (CODES == KV_FP8) {
+#pragma unroll
+                    for (int i = 0; i < E / 4; ++i) {
+                        const auto p = __builtin_amdgcn_cvt_pk_f32_fp8((int)w[u][i], false);
+                        const auto q = __builtin_amdgcn_cvt_pk_f32_fp8((int)w[u][i], true);
+                        v[u][4 * i] = p[0], v[u][4 * i + 1] = p[1], v[u][4 * i + 2] = q[0], v[u][4 * i + 3] = q[1];
+                        if constexpr (!EACH) odd |= ((w[u][i] & 0x7F7F7F7Fu) + 0x01010101u) & 0x80808080u;
+                    }
+                } else
+#pragma unroll
+                    for (int j = 0; j < E; ++j) {
+                        if constexpr (CODES == KV_INT8) v[u][j] = (float)(signed char)(w[u][j / 4] >> (8 * (j & 3)));
+                        else v[u][j] = (float)__builtin_bit_cast(typename op_t<CODES>::type, (u16)(w[u][j / 2] >> (16 * (j & 1))));
+                        if constexpr (!Q8 && !EACH)
+                            if (j & 1) {
+                                constexpr u32 INF = CODES == KV_BF16 ? 0x7F80u : 0x7C00u;
+                                const u32 size = w[u][j / 2] & 0x7FFF7FFFu;
+                                odd |= (size >> 16 > INF) | ((size & 0xFFFFu) > INF);
+                            }
+                    }
+#pragma unroll
+                for (int j = 0; j < E; ++j) {
+                    if constexpr (Q8) v[u][j] *= s[u];
+                    if constexpr (EACH) bad |= (v[u][j] != v[u][j] ? 1u : 0u) << j;
+                }
+            }
+#pragma unroll
+            for (int j = 0; j < E; ++j) {
+                x[j] = fminf(fminf(x[j], v[0][j]), fminf(v[1][j], fminf(v[2][j], v[3][j])));
+                hi[j] = fmaxf(fmaxf(hi[j], v[0][j]), fmaxf(v[1][j], fmaxf(v[2][j], v[3][j])));
+            }
+        }
+    };
+    rows(std::false_type());
+    if (__any(odd != 0)) {
+        rows(std::true_type());
+#pragma unroll
+        for (int o = L; o < 64; o <<= 1) bad |= (u32)__shfl_xor((int)bad, o, 64);
+    }
+#pragma unroll
+    for (int j = 0; j < E; ++j) x[j] = halve<32>(x[j], -hi[j]);
+    if constexpr (R > 2)
+#pragma unroll
+        for (int j = 0; j < M; ++j) x[j] = halve<16>(x[j], x[M + j]);
+    if constexpr (R > 4)
+#pragma unroll
+        for (int o = 8; o >= L; o >>= 1)
+#pragma unroll
+            for (int j = 0; j < M; ++j) x[j] = least(x[j], __shfl_xor(x[j], o, 64));
+    // lane l: the smallest (l < 32) or the largest of elements d .. d + M - 1
+    const int side = l >> 5, skip = R > 2 ? (l >> 4 & 1) * M : 0, d = d0 + skip;
+    const bool mine = R <= 4 || (l & 15) < L;
+#pragma unroll
+    for (int j = 0; j < M; ++j) x[j] = side ? -x[j] : x[j];
+    if (__any(bad != 0))
+#pragma unroll
+        for (int j = 0; j < M; ++j) x[j] = bad >> (skip + j) & 1 ? __builtin_nanf("") : x[j];
+    if constexpr (WP > 1)
+        if (mine)
+#pragma unroll
+            for (int j = 0; j < M; ++j) sides[wave][side][d + j] = x[j];
+    if constexpr (WP > 1) {
+        __syncthreads();
+        if (part) return;
+#pragma unroll
+        for (int j = 0; j < M; ++j) {
+#pragma unroll
+            for (int w = 1; w < WP; ++w) {
+                const float y = sides[wave + w][side][d + j];
+                x[j] = x[j] != x[j] || y != y ? __builtin_nanf("") : side ? fmaxf(x[j], y) : fminf(x[j], y);
+            }
+        }
+    }
+    if (!mine) return;
+    constexpr int N = M % 4 ? 2 : M == 4 ? 4 : 8;  // elements a store
+    b16* to = bounds + (((i64)e * H + h) * 2 + side) * DP + d;
+#pragma unroll
+    for (int i = 0; i < M; i += N) {
+        Pack<b16, N> o;
+#pragma unroll
+        for (int j = 0; j < N; ++j) o.v[j] = d + i + j < dim ? outward(x[i + j], side != 0) : (b16)0.f;
+        o.store(to + i);
+    }
 }
 
 template <int CODES> int bounds_codes(const void* k, const float* ks, i64 pages, int shift, int H, int dim, const int* table,
@@ -238,9 +306,15 @@ template <int CODES> int bounds_codes(const void* k, const float* ks, i64 pages,
                                       hipStream_t st) {
     const int per = ((count - 1) >> shift) + 2;
     const i64 n = (i64)B * per * H;
+    // pages of more than 64 rows: a block each
+    const int waves = shift > 6 ? 4 : 1;
+    const i64 grid = (n * waves + 3) / 4;
     if (n >= (i64)1 << 31) return -1;
-#define DP_CASE(DP)                                                                                                      \
-    bounds_k<CODES, DP><<<(unsigned)n, 256, 0, st>>>(k, ks, pages, shift, H, dim, table, stride, width, start, count, per, bounds)
+#define BOUNDS_K(DP, WP) \
+    bounds_k<CODES, DP, WP><<<(unsigned)grid, 256, 0, st>>>(k, ks, pages, shift, H, dim, table, stride, width, start, (u32)n, count, per, bounds)
+#define DP_CASE(DP)            \
+    if (waves == 4) BOUNDS_K(DP, 4); \
+    else BOUNDS_K(DP, 1)
     switch ((dim + 63) / 64) {
         case 1: DP_CASE(64); break;
         case 2: DP_CASE(128); break;
@@ -248,5 +322,6 @@ template <int CODES> int bounds_codes(const void* k, const float* ks, i64 pages,
         default: DP_CASE(256);
     }
 #undef DP_CASE
+#undef BOUNDS_K
     return (int)hipGetLastError();
 }
