@@ -15,15 +15,18 @@ template <int CODES> int sparse_codes(const SparseArgs& s, int dp, hipStream_t s
 template <int CODES> int bounds_codes(const void* k, const float* ks, i64 pages, int shift, int H, int dim, const int* table,
                                       i64 stride, int width, const int* start, int B, int count, b16* bounds, hipStream_t st);
 
-// A row's sequence, token and head.
+// A unit's sequence, token, head and group of 16 query heads. The tokens of a head come one after the other (rows lie by
+// sequence, token and head): their pages are the same head's, which an XCD's L2 then holds.
 struct At {
-    i64 b;
-    int t, head;
+    i64 b, row;
+    int t, head, group;
 };
-__device__ __forceinline__ At at_of(const SparseArgs& s, i64 row) {
-    const i64 token = row / s.a.H, b = token / s.nt;
+__device__ __forceinline__ At at_of(const SparseArgs& s, u32 unit) {
+    const u32 x = unit / (u32)s.a.groups, bh = x / (u32)s.nt, b = bh / (u32)s.a.H;
+    const int t = (int)(x - bh * s.nt);
     At p;
-    p.b = s.b0 + b, p.t = s.t0 + (int)(token - b * s.nt), p.head = (int)(row - token * s.a.H);
+    p.group = (int)(unit - x * s.a.groups), p.head = (int)(bh - b * s.a.H), p.b = s.b0 + (i64)b, p.t = s.t0 + t;
+    p.row = ((i64)b * s.nt + t) * s.a.H + p.head;
     return p;
 }
 
@@ -41,11 +44,12 @@ __device__ __forceinline__ Share share_of(int keys, int splits, int split) {
 
 // A block per (row, group of up to 16 query heads, part of its chosen pages): tree attention of one token whose page table is
 // the chosen pages'.
-template <int CODES, int DP> __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void sparse_k(const SparseArgs s) {
-    typedef Tree<CODES, DP, 1> W;
+template <int CODES, int DP> __global__ __launch_bounds__(256, DP <= 64 ? 4 : DP <= 128 ? 3 : 1) void sparse_k(const SparseArgs s) {
+    typedef Tree<CODES, DP, 1, true> W;
     typedef typename W::Lo Lo;
-    __shared__ __align__(16) char lds[sizeof(Lo) * 4 > 16 * W::QLD * 2 ? sizeof(Lo) * 4 : 16 * W::QLD * 2];
-    Lo* lo = (Lo*)lds;  // the waves' sums at the end; before that the queries
+    // the queries, then the waves' keys, at the end their sums
+    __shared__ __align__(16) char lds[sizeof(Lo) > W::STAGE ? sizeof(Lo) * 4 : W::STAGE * 4];
+    Lo* lo = (Lo*)lds;
     __shared__ float lm[4][16], ll[4][16];
     __shared__ typename W::Sizes size;
     __shared__ u64 bits[16];
@@ -54,11 +58,9 @@ template <int CODES, int DP> __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1
     const i64 blocks = s.units * s.splits, a8 = (blocks + 7) / 8, me = (i64)(blockIdx.x % 8) * a8 + blockIdx.x / 8;
     if ((i64)blockIdx.x / 8 >= a8 || me >= blocks) return;
     const i64 unit = me / s.splits;
-    const int split = (int)(me - unit * s.splits), groups = s.a.groups, G = s.a.G;
-    const i64 row = unit / groups;
-    const int group = (int)(unit - row * groups);
-    const At p = at_of(s, row);
-    const int2 r = s.rows[row];
+    const int split = (int)(me - unit * s.splits), G = s.a.G;
+    const At p = at_of(s, (u32)unit);
+    const int2 r = s.rows[p.row];
     const int n = __builtin_amdgcn_readfirstlane(r.x);
     const Share mine = share_of(n, s.splits, split);
     if (split && mine.t1 <= mine.t0) return;
@@ -74,16 +76,18 @@ template <int CODES, int DP> __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1
     const int base = mine.t0 * TILE + wave * 32, stop = mine.t1 * TILE < n ? mine.t1 * TILE : n;
     typename W::State st;
     typename W::Run run;
-    const int* tab = a.table + row * a.width;
+    st.stage = lds + wave * W::STAGE;
+    const int* tab = a.table + p.row * a.width;
     W::begin(a, tab, p.head, base, stop, run);
-    const bool own = W::load_q(a, 0, p.head, q, group * 16, (typename W::T*)lds, size, bits, st);
+    const bool own = W::load_q(a, 0, p.head, q, p.group * 16, (typename W::T*)lds, size, bits, st);
+    lds_barrier();  // (each wave has its queries)
     st.m[0] = -__builtin_inff(), st.l[0] = 0.f;
 #pragma unroll
     for (int j = 0; j < W::NJ; ++j) st.o[0][j] = f4{0.f, 0.f, 0.f, 0.f};
     W::keys(a, tab, p.head, q, base, stop, bits, size, own, run, st, fac[wave]);
     float m, sum, o[W::NJ];
     W::join_waves(st, 0, lo, lm, ll, m, sum, o);
-    const int at = threadIdx.x >> 4, d0 = (threadIdx.x & 15) * W::NJ, h = group * 16 + at;
+    const int at = threadIdx.x >> 4, d0 = (threadIdx.x & 15) * W::NJ, h = p.group * 16 + at;
     if (h >= G) return;
     if (mine.blocks <= 1) {
         const i64 i = (p.b * s.T + p.t) * a.H * G + p.head * G + h;
@@ -106,10 +110,9 @@ template <int CODES, int DP> __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1
 template <int DP> __global__ __launch_bounds__(256) void sparse_join_k(const SparseArgs s, float bias) {
     constexpr int NJ = DP / 16;
     const TreeArgs& a = s.a;
-    const i64 unit = blockIdx.x, row = unit / a.groups;
-    const int h = (int)(unit - row * a.groups) * 16 + (threadIdx.x >> 4);
-    const At p = at_of(s, row);
-    const int parts = share_of(s.rows[row].x, s.splits, 0).blocks;
+    const i64 unit = blockIdx.x;
+    const At p = at_of(s, (u32)unit);
+    const int h = p.group * 16 + (threadIdx.x >> 4), parts = share_of(s.rows[p.row].x, s.splits, 0).blocks;
     if (parts <= 1 || h >= a.G) return;
     const int d0 = (threadIdx.x & 15) * NJ;
     float m = -__builtin_inff(), sum = 0.f, o[NJ];

@@ -260,8 +260,10 @@ template <int N> __device__ __forceinline__ void put(const TreeArgs& a, i64 i, i
     }
 }
 
-// CODES: the cache's; DP: its padded row; R: rows a block / 16, 1 or 2.
-template <int CODES, int DP, int R> struct Tree {
+// CODES: the cache's; DP: its padded row; R: rows a block / 16, 1 or 2. STAGED: a wave's keys come in whole rows, lane by lane,
+// and go to the operands' lanes through LDS. Loaded into those lanes at once, 16 neighbouring lanes read 16 rows: nothing
+// where memory bounds the kernel, but where the keys lie in the L2 it is the lookups of the L1 that do (a lane, a lookup).
+template <int CODES, int DP, int R, bool STAGED = false> struct Tree {
     typedef typename op_t<CODES>::type T;
     typedef T V8 __attribute__((ext_vector_type(8)));
     static constexpr bool Q8 = CODES == KV_INT8 || CODES == KV_FP8;
@@ -294,7 +296,16 @@ template <int CODES, int DP, int R> struct Tree {
     };
     static constexpr bool QLDS = R == 2;  // the queries are read from LDS for every tile: registers go to loads in flight
 
+    static constexpr int ROWB = DP * ES, STAGE = STAGED ? 32 * ROWB : 0;  // bytes of a row, and of a wave's keys in LDS
+
+    // A key's place there: its 16-byte pieces in an order of its own, so that 8 lanes of an operand (keys 0 .. 3 and 8 .. 11 of
+    // 16, one piece) meet no bank twice.
+    static __device__ __forceinline__ int turn(int key) {
+        return ROWB % 128 == 0 ? (key & 3) | (key >> 1 & 4) : (key >> 1 & 1) | (key >> 2 & 2);
+    }
+
     struct State {
+        char* stage;  // this wave's keys in LDS (STAGED)
         V8 q[QLDS ? 1 : R][KS];
         const T* ql;  // the queries in LDS, at this lane's row and quarter
         f4 o[R][NJ];
@@ -432,11 +443,23 @@ template <int CODES, int DP, int R> struct Tree {
     // registers that its keys have just left, the values into the other of two sets.
     static __device__ __forceinline__ void fetch_keys(const TreeArgs& a, int head, int base, const Pages& p, Keys& f) {
         const int c = lane_id() & 15, g = lane_id() >> 4, in = (1 << a.shift) - 1;
-        const i64 pk = (u32)p.k < (u64)a.pages ? p.k : 0, ps = (u32)p.s < (u64)a.pages ? p.s : 0;
-        const i64 rk = ((pk * a.H + head) << a.shift) + ((base + (c >> 2) * 8) & in) + (c & 3);
-        const char* k = (const char*)a.k + rk * (DP * ES) + g * (DP * ES / 4);
-        load_words<KW>(k, f.k[0]);
-        load_words<KW>(k + 4 * DP * ES, f.k[1]);
+        const i64 ps = (u32)p.s < (u64)a.pages ? p.s : 0;
+        if constexpr (STAGED) {
+#pragma unroll
+            for (int i = 0; i < KW / 2; ++i) {  // 1024 bytes each; p.v of lane 16 j is the page of keys 8 j .. 8 j + 7
+                const int o = i * 1024 + lane_id() * 16, key = ROWB % 128 ? o / ROWB : i * 1024 / (8 * ROWB) * 8;
+                const int e = ROWB % 128 ? __shfl(p.v, key / 8 * 16, 64) : __builtin_amdgcn_readlane(p.v, key * 2);
+                const i64 pk = (u32)e < (u64)a.pages ? e : 0;
+                const i64 rk = ((pk * a.H + head) << a.shift) + ((base + key / 8 * 8) & in);
+                load_words<4>((const char*)a.k + rk * ROWB + (o - key / 8 * 8 * ROWB), &f.k[0][0] + 4 * i);
+            }
+        } else {
+            const i64 pk = (u32)p.k < (u64)a.pages ? p.k : 0;
+            const i64 rk = ((pk * a.H + head) << a.shift) + ((base + (c >> 2) * 8) & in) + (c & 3);
+            const char* k = (const char*)a.k + rk * (DP * ES) + g * (DP * ES / 4);
+            load_words<KW>(k, f.k[0]);
+            load_words<KW>(k + 4 * DP * ES, f.k[1]);
+        }
         if constexpr (Q8) {
             const i64 rs = ((ps * a.H + head) << a.shift) + ((base + (lane_id() & 31)) & in);
             f.s = (lane_id() < 32 ? a.ks : a.vs)[rs];
@@ -533,6 +556,28 @@ template <int CODES, int DP, int R> struct Tree {
         const int c = lane_id() & 15, g = lane_id() >> 4;
 #pragma unroll
         for (int r = 0; r < R; ++r) sc[r][0] = sc[r][1] = f4{0.f, 0.f, 0.f, 0.f};
+        if constexpr (STAGED) {
+#pragma unroll
+            for (int i = 0; i < KW / 2; ++i) {
+                const int o = i * 1024 + lane_id() * 16, key = o / ROWB;
+                uint4 w;
+                __builtin_memcpy(&w, &k.k[0][0] + 4 * i, 16);
+                *(uint4*)(s.stage + key * ROWB + ((o % ROWB / 16) ^ turn(key)) * 16) = w;
+            }
+            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront", "local");
+            __builtin_amdgcn_wave_barrier();
+#pragma unroll
+            for (int t = 0; t < 2; ++t) {
+                const int key = (c >> 2) * 8 + t * 4 + (c & 3);
+#pragma unroll
+                for (int i = 0; i < KW / 4; ++i) {
+                    const uint4 w = *(const uint4*)(s.stage + key * ROWB + ((g * (KW / 4) + i) ^ turn(key)) * 16);
+                    __builtin_memcpy(&k.k[t][4 * i], &w, 16);
+                }
+            }
+            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront", "local");
+            __builtin_amdgcn_wave_barrier();
+        }
 #pragma unroll
         for (int st = 0; st < KS; ++st) {
             V8 x[R];
