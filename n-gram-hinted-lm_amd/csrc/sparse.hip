@@ -58,24 +58,22 @@ __device__ __forceinline__ float query_at(const ScoreArgs& a, u16 e) {
     return a.qtype == NG_BF16 ? __uint_as_float((u32)e << 16) : (float)__builtin_bit_cast(f16, e);
 }
 
-// A score as a key: a page of none of the cache's ranks last, one whose score is NaN first.
+// A score as a key, its upper word above 0: a page of none of the cache's ranks last, one whose score is NaN first.
 __device__ __forceinline__ u64 score_key(bool is, double x) {
     const u64 u = (u64)__double_as_longlong(x + 0.);
-    return !is ? 1ull : x != x ? ~1ull : u >> 63 ? ~u : u | 1ull << 63;
+    return !is ? 1ull << 32 : x != x ? ~1ull : u >> 63 ? ~u : u | 1ull << 63;
 }
 
 // The pairs of elements of four words, 16 bits each, in 64 bits.
 __device__ __forceinline__ double low(u32 w) { return (double)__uint_as_float(w << 16); }
 __device__ __forceinline__ double high(u32 w) { return (double)__uint_as_float(w & 0xFFFF0000u); }
 
-// One token a sequence: a block per (row, a.per pages); GS lanes a page, each of 8 elements, 4 pages at a time.
-template <int DP, int GS> __global__ __launch_bounds__(256) void score_one_k(const ScoreArgs a) {
-    constexpr int U = 4, STEP = 256 / GS;
-    const i64 row = blockIdx.x / (u32)a.chunks;
-    const int chunk = (int)(blockIdx.x - row * a.chunks);
+// A token's scores of pages from .. stop - 1, by a block of NT: GS lanes a page, each of 8 elements, 4 pages at a time. put
+// takes those that are wanted.
+template <int DP, int GS, int NT, typename F>
+__device__ __forceinline__ void score_one(const ScoreArgs& a, const Place& p, int from, int stop, F put) {
+    constexpr int U = 4, STEP = NT / GS;
     const int sub = threadIdx.x % GS, group = threadIdx.x / GS, d0 = sub * 8;
-    const Place p = place_of(a, (u32)row);
-    const int from = chunk * a.per, stop = from + a.per < a.width ? from + a.per : a.width;
     const int* tab = a.table + p.b * a.table_stride;
     int e[U], next[U];  // (asked for before the sequence's length is known)
 #pragma unroll
@@ -138,26 +136,47 @@ template <int DP, int GS> __global__ __launch_bounds__(256) void score_one_k(con
         for (int o = GS / 8; o; o >>= 1) x += __shfl_xor(x, o, GS);
         const int u = (a1 ? 2 : 0) + (a2 ? 1 : 0), j = j0 + u * STEP;
         const bool mine = a1 ? (a2 ? is[3] : is[2]) : (a2 ? is[1] : is[0]);
-        if (j >= a.first && j < end && sub % (GS / 4) == 0) a.score[row * a.width + j] = score_key(mine, x);
+        if (j >= a.first && j < end && sub % (GS / 4) == 0) put(j, score_key(mine, x));
 #pragma unroll
         for (int u = 0; u < U; ++u) e[u] = next[u];
     }
 }
 
+// One token a sequence: a block per (row, a.per pages).
+template <int DP, int GS> __global__ __launch_bounds__(256) void score_one_k(const ScoreArgs a) {
+    const i64 row = blockIdx.x / (u32)a.chunks;
+    const int from = (int)(blockIdx.x - row * a.chunks) * a.per, stop = from + a.per < a.width ? from + a.per : a.width;
+    score_one<DP, GS, 256>(a, place_of(a, (u32)row), from, stop, [&](int j, u64 x) { a.score[row * a.width + j] = x; });
+}
+
 typedef double d4 __attribute__((ext_vector_type(4)));
 
-// Several tokens a sequence: a block per (16 tokens of a sequence and head, a.per pages), on the matrix units: tokens x pages,
-// 16 of each a wave at a time. A lane's operand is 8 in 32 elements of a page's bounds (of one page in 16) and the same ones
+// Products of TT tokens and 16 pages over 4 elements: a lane's operands are of token lane % TT, page lane % 16 and element
+// lane / 16, its sums those of tokens 4 r + lane / 16 and page lane % 16.
+template <int TT> struct Sums;
+template <> struct Sums<16> {
+    typedef d4 type;
+    static __device__ __forceinline__ d4 mma(double t, double p, d4 s) { return __builtin_amdgcn_mfma_f64_16x16x4f64(t, p, s, 0, 0, 0); }
+    static __device__ __forceinline__ double at(d4 s, int r) { return s[r]; }
+};
+template <> struct Sums<4> {
+    typedef double type;
+    static __device__ __forceinline__ double mma(double t, double p, double s) { return __builtin_amdgcn_mfma_f64_4x4x4f64(t, p, s, 0, 0, 0); }
+    static __device__ __forceinline__ double at(double s, int) { return s; }
+};
+
+// Several tokens a sequence: a block per (TT tokens, 16 or 4, of a sequence and head, a.per pages), on the matrix units: tokens
+// x pages, 16 pages a wave at a time (TT = 4: as four products of 4 x 4). A lane's operand is 8 in 32 elements of a page's bounds (of one page in 16) and the same ones
 // of a token's sums, which lie in LDS.
-template <int DP> __global__ __launch_bounds__(256, DP <= 128 ? 4 : 2) void score_k(const ScoreArgs a) {
+template <int DP, int TT> __global__ __launch_bounds__(256, DP <= 128 ? 4 : 2) void score_k(const ScoreArgs a) {
     constexpr int LD = 2 * DP + 2;  // (16 rows' reads of 16 bytes meet no bank twice)
-    __shared__ __align__(16) double sums[16 * LD];
+    __shared__ __align__(16) double sums[TT * LD];
     const int c = lane_id() & 15, g = lane_id() >> 4, wave = threadIdx.x >> 6;
-    const u32 tiles = (a.nt + 15) / 16, unit = blockIdx.x / (u32)a.chunks, bh = unit / tiles;  // (sequence, head, 16 tokens)
+    const u32 tiles = (a.nt + TT - 1) / TT, unit = blockIdx.x / (u32)a.chunks, bh = unit / tiles;  // (sequence, head, TT tokens)
     const u32 at = bh / (u32)a.H;
-    const int chunk = (int)(blockIdx.x - unit * a.chunks), tile = (int)(unit - bh * tiles) * 16;
+    const int chunk = (int)(blockIdx.x - unit * a.chunks), tile = (int)(unit - bh * tiles) * TT;
     const int h = (int)(bh - at * a.H), b = a.b0 + (int)at, t0 = a.t0 + tile;
-    const int n = a.nt - tile < 16 ? a.nt - tile : 16;
+    const int n = a.nt - tile < TT ? a.nt - tile : TT;
     const i64 row0 = ((i64)at * a.nt + tile) * a.H + h;
     const Place whole = place_of(a, (u32)(row0 + (i64)(n - 1) * a.H));  // the last token sees the most pages
     const int from = chunk * a.per;
@@ -165,7 +184,7 @@ template <int DP> __global__ __launch_bounds__(256, DP <= 128 ? 4 : 2) void scor
     if (whole.pages <= a.keep || from >= stop) return;
     const int w = a.widths ? a.widths[b] : a.T;
     if (t0 >= w) return;
-    for (int i = threadIdx.x; i < 16 * DP / 8; i += 256) {
+    for (int i = threadIdx.x; i < TT * DP / 8; i += 256) {
         const int t = i / (DP / 8), d0 = i % (DP / 8) * 8;
         double up[8], down[8];
 #pragma unroll
@@ -195,12 +214,12 @@ template <int DP> __global__ __launch_bounds__(256, DP <= 128 ? 4 : 2) void scor
     }
     __syncthreads();
     const int* tab = a.table + b * a.table_stride;
-    const double* mine = sums + c * LD + g * 8;
+    const double* mine = sums + c % TT * LD + g * 8;
     const int steps = (a.dim + 31) / 32;
     u64* out = a.score + (row0 + (i64)g * a.H) * a.width;
-    int ends[4];  // behind the last page that a token's score is wanted of
+    int ends[TT / 4];  // behind the last page that a token's score is wanted of
 #pragma unroll
-    for (int r = 0; r < 4; ++r) {
+    for (int r = 0; r < TT / 4; ++r) {
         const int t = 4 * r + g;
         const i64 keys = whole.len + t0 + t + 1, cap = (i64)a.width << a.shift;
         const int pages = (int)(((keys < cap ? keys : cap) + (1 << a.shift) - 1) >> a.shift);
@@ -215,7 +234,7 @@ template <int DP> __global__ __launch_bounds__(256, DP <= 128 ? 4 : 2) void scor
         const bool is = (u32)e < (u64)a.pages;
         const b16* then = page(next);
         e = next, next = entry(j0 + 128);
-        d4 acc = {0., 0., 0., 0.}, more = {0., 0., 0., 0.};
+        typename Sums<TT>::type acc = {}, more = {};
 #pragma unroll 1
         for (int i = 0; i < steps; ++i) {  // (the next eight elements, or the next page's first, are under way)
             const u32 l[4] = {lo.x, lo.y, lo.z, lo.w}, k[4] = {hi.x, hi.y, hi.z, hi.w};
@@ -224,28 +243,27 @@ template <int DP> __global__ __launch_bounds__(256, DP <= 128 ? 4 : 2) void scor
 #pragma unroll
             for (int j = 0; j < 8; j += 2) {
                 const double2 up = *(const double2*)(mine + i * 32 + j), down = *(const double2*)(mine + DP + i * 32 + j);
-                acc = __builtin_amdgcn_mfma_f64_16x16x4f64(up.x, low(k[j / 2]), acc, 0, 0, 0);
-                more = __builtin_amdgcn_mfma_f64_16x16x4f64(down.x, low(l[j / 2]), more, 0, 0, 0);
-                acc = __builtin_amdgcn_mfma_f64_16x16x4f64(up.y, high(k[j / 2]), acc, 0, 0, 0);
-                more = __builtin_amdgcn_mfma_f64_16x16x4f64(down.y, high(l[j / 2]), more, 0, 0, 0);
+                acc = Sums<TT>::mma(up.x, low(k[j / 2]), acc);
+                more = Sums<TT>::mma(down.x, low(l[j / 2]), more);
+                acc = Sums<TT>::mma(up.y, high(k[j / 2]), acc);
+                more = Sums<TT>::mma(down.y, high(l[j / 2]), more);
             }
         }
         const int j = j0 + c;  // this lane's page; its tokens: 4 r + g
 #pragma unroll
-        for (int r = 0; r < 4; ++r)
-            if (j >= a.first && j < ends[r]) out[(i64)r * 4 * a.H * a.width + j] = score_key(is, acc[r] + more[r]);
+        for (int r = 0; r < TT / 4; ++r)
+            if (j >= a.first && j < ends[r])
+                out[(i64)r * 4 * a.H * a.width + j] = score_key(is, Sums<TT>::at(acc, r) + Sums<TT>::at(more, r));
     }
 }
 
-// The kept pages of a row, by NW waves that hold E of its scores a lane (NW = 1: four rows a block).
-template <int NW, int E> __global__ __launch_bounds__(NW == 1 ? 256 : NW * 64) void choose_k(const ScoreArgs a) {
+// The kept pages of a row, by NW waves that hold E of its scores (score(j)) a lane.
+template <int NW, int E, typename F>
+__device__ __forceinline__ void choose(const ScoreArgs& a, const Place& p, i64 row, F score) {
     constexpr int NT = NW * 64;
     __shared__ int counts[2][NW], before[NW == 1 ? 1 : E * NW];
     __shared__ u32 ends[2][NW];
-    const i64 row = NW == 1 ? (i64)blockIdx.x * 4 + (threadIdx.x >> 6) : (i64)blockIdx.x;
-    if (row >= a.rows) return;
     const int tid = NW == 1 ? lane_id() : (int)threadIdx.x, wave = NW == 1 ? 0 : tid >> 6;
-    const Place p = place_of(a, (u32)row);
     const int* tab = a.table + p.b * a.table_stride;
     int* out = a.table_out + row * a.keep;
     int* chosen = a.chosen ? a.chosen + (((i64)p.b * a.T + p.t) * a.H + p.h) * a.keep : nullptr;
@@ -271,7 +289,7 @@ template <int NW, int E> __global__ __launch_bounds__(NW == 1 ? 256 : NW * 64) v
     for (int e = 0; e < E; ++e) {
         const int j = e * NT + tid;
         u64 k = 0;
-        if (j < n) k = j < a.first || j >= n - a.last ? ~0ull : a.score[row * a.width + j];
+        if (j < n) k = j < a.first || j >= n - a.last ? ~0ull : score(j);
         key[e] = (u32)(k >> 32), rest[e] = (u32)k;
         if (j < n) lo = key[e] < lo ? key[e] : lo;
         if (key[e] != ~0u) hi = key[e] > hi ? key[e] : hi;
@@ -284,6 +302,36 @@ template <int NW, int E> __global__ __launch_bounds__(NW == 1 ? 256 : NW * 64) v
         for (int w = 0; w < NW; ++w) lo = ends[0][w] < lo ? ends[0][w] : lo, hi = ends[1][w] > hi ? ends[1][w] : hi;
     }
     Count<NW> count(counts);
+    auto few = [&](const u32 (&k)[E], u32 least) {  // the keys from `least` on, no more than lanes: one each, 0 behind them
+        __shared__ u32 left[NW == 1 ? 256 : NT];
+        __shared__ int fill[4];
+        u32* mine = left + (NW == 1 ? threadIdx.x / 64 * 64 : 0);
+        int at = 0;
+        if constexpr (NW > 1) {
+            if (tid == 0) fill[0] = 0;
+            mine[tid] = 0;
+            __syncthreads();
+        } else mine[tid] = 0;
+#pragma unroll
+        for (int e = 0; e < E; ++e) {
+            const bool is = k[e] >= least;
+            const u64 m = __ballot(is);
+            int first = at;
+            if constexpr (NW > 1) {
+                if (!m) continue;
+                if (lane_id() == 0) first = atomicAdd(fill, __popcll(m));
+                first = __builtin_amdgcn_readfirstlane(first);
+            }
+            if (is) mine[first + __popcll(m & lanemask_lt())] = k[e];
+            at += __popcll(m);
+        }
+        if constexpr (NW > 1) __syncthreads();
+        else {
+            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront", "local");
+            __builtin_amdgcn_wave_barrier();
+        }
+        return mine[tid];
+    };
     int c;
     // (an upper word of ones: a page always kept, or a NaN, whose lower word is one less; hi is below both)
     u32 t = ~0u, t2 = 0;
@@ -291,7 +339,14 @@ template <int NW, int E> __global__ __launch_bounds__(NW == 1 ? 256 : NW * 64) v
     c = count.at_least(key, t);
     if (c < a.keep) {
         c = n;
-        t = count.threshold(key, lo, hi, a.keep, a.keep, c);
+        // halving with all keys until a key a lane is left, then with those
+        t = count.threshold(key, lo, hi, a.keep, a.keep > NT ? a.keep : NT, c);
+        if (c > a.keep) {
+            if (E > 1 && c <= NT) {
+                u32 one[1] = {few(key, t)};
+                t = count.threshold(one, t, hi, a.keep, a.keep, c);
+            } else t = count.threshold(key, t, hi, a.keep, a.keep, c);
+        }
     }
     if (c > a.keep) {
         const int above = t == ~0u ? 0 : count.at_least(key, t + 1);
@@ -346,9 +401,27 @@ template <int NW, int E> __global__ __launch_bounds__(NW == 1 ? 256 : NW * 64) v
     });
 }
 
+// (NW = 1: four rows a block)
+template <int NW, int E> __global__ __launch_bounds__(NW == 1 ? 256 : NW * 64) void choose_k(const ScoreArgs a) {
+    const i64 row = NW == 1 ? (i64)blockIdx.x * 4 + (threadIdx.x >> 6) : (i64)blockIdx.x;
+    if (row >= a.rows) return;
+    choose<NW, E>(a, place_of(a, (u32)row), row, [&](int j) { return a.score[row * a.width + j]; });
+}
+
+// Both for one token a sequence of few pages, a block a row.
+#define FEW_PAGES 1024
+template <int DP, int GS> __global__ __launch_bounds__(512) void score_choose_k(const ScoreArgs a) {
+    __shared__ u64 scores[FEW_PAGES];
+    const i64 row = blockIdx.x;
+    const Place p = place_of(a, (u32)row);
+    score_one<DP, GS, 512>(a, p, 0, a.width, [&](int j, u64 x) { scores[j] = x; });
+    __syncthreads();
+    choose<8, FEW_PAGES / 512>(a, p, row, [&](int j) { return scores[j]; });
+}
+
 // ------------------------------------------------------------------------------------------------------------ the host
 
-#define SLAB ((i64)256 << 20)  // bytes of scores at a time
+#define SLAB ((i64)256 << 20)  // bytes of scores and kept pages at a time
 #define AIM 512                // blocks that fill the card: 2 a CU
 
 struct SparsePlan {
@@ -365,16 +438,17 @@ static bool sparse_plan(i64 B, i64 T, i64 H, i64 G, i64 dim, i64 width, i64 page
         width * page > lim || B * T > lim || H * ((G + 15) / 16) > 1 << 12)
         return false;
     p.dp = (int)(dim + 63) / 64 * 64, p.groups = (int)(G + 15) / 16, p.scored = width > keep;
-    // a pass takes as many sequences, or (one) sequence's tokens, as SLAB holds the scores of, and fewer than 2^24 units
-    const i64 each = p.scored ? H * width * 8 : 1, most_units = ((i64)1 << 24) / (H * p.groups);
+    // a pass takes as many sequences, or one sequence's tokens, as SLAB holds the scores and kept pages of, fewer than 2^24 units
+    const i64 each = H * ((p.scored ? width * 8 : 0) + keep * 4), most_units = ((i64)1 << 24) / (H * p.groups);
     i64 most = SLAB / each < most_units ? SLAB / each : most_units;
     if (most < 16) most = 16;
     p.nt = (int)(T <= most ? T : most / 16 * 16);
     p.nb = (int)(T <= most ? (B < most / T ? B : most / T) : 1);
     const i64 rows = (B ? (i64)p.nb : 0) * p.nt * H, units = rows * p.groups;
     const i64 tiles = ((keep < width ? keep : width) * page + TILE - 1) / TILE;
-    i64 splits = units ? (AIM + units - 1) / units : 1;
-    p.splits = (int)(splits < tiles ? splits : tiles);
+    // parts of two tiles at least; up to six tiles are left whole: joining their parts costs more than they take
+    i64 splits = units && tiles > 6 ? (AIM + units - 1) / units : 1;
+    p.splits = (int)(splits < (tiles + 1) / 2 ? splits : (tiles + 1) / 2);
     const i64 parts = p.splits > 1 ? units * p.splits * 16 : 0;
     p.score = 0;
     p.rows = p.score + (p.scored ? rows * width * 8 : 0);
@@ -424,27 +498,33 @@ extern "C" int ng_page_bounds(const void* k, const float* ks, i64 pages, int pag
     }
 }
 
-// One token a sequence is scored by vector operations, more on the matrix units, of which a token uses a sixteenth: 4 tokens
-// of 2 sequences over 524288 positions x us there, y by vector operations. A block takes 256 pages, or 64 where that
-// leaves fewer than 1024 blocks.
+template <int TT> static void score_tokens(const ScoreArgs& a, int dp, unsigned grid, hipStream_t st) {
+    switch (dp) {
+        case 64: score_k<64, TT><<<grid, 256, 0, st>>>(a); break;
+        case 128: score_k<128, TT><<<grid, 256, 0, st>>>(a); break;
+        case 192: score_k<192, TT><<<grid, 256, 0, st>>>(a); break;
+        default: score_k<256, TT><<<grid, 256, 0, st>>>(a);
+    }
+}
+
+// One token a sequence is scored by vector operations, more on the matrix units. A block takes 256 pages, or fewer (64 at
+// least) where that leaves fewer than 1024 blocks.
 static int score_rows(ScoreArgs& a, int nb, int dp, hipStream_t st) {
-    const i64 units = (i64)nb * a.H * (a.T == 1 ? 1 : (a.nt + 15) / 16);
+    const int tokens = a.T == 1 ? 1 : a.T <= 4 ? 4 : 16;
+    const i64 units = (i64)nb * a.H * ((a.nt + tokens - 1) / tokens);
     i64 per = units * a.width / 1024;
     per = per < 256 ? (per + 63) / 64 * 64 : 256;
     a.per = per ? (int)per : 64;
     a.chunks = (a.width + a.per - 1) / a.per;
     const i64 n = units * a.chunks;
     if (n >= (i64)1 << 31) return -1;
-    if (a.T == 1) switch (dp) {
+    if (tokens == 4) score_tokens<4>(a, dp, (unsigned)n, st);
+    else if (tokens == 16) score_tokens<16>(a, dp, (unsigned)n, st);
+    else switch (dp) {
         case 64: score_one_k<64, 8><<<(unsigned)n, 256, 0, st>>>(a); break;
         case 128: score_one_k<128, 16><<<(unsigned)n, 256, 0, st>>>(a); break;
         case 192: score_one_k<192, 32><<<(unsigned)n, 256, 0, st>>>(a); break;
         default: score_one_k<256, 32><<<(unsigned)n, 256, 0, st>>>(a);
-    } else switch (dp) {
-        case 64: score_k<64><<<(unsigned)n, 256, 0, st>>>(a); break;
-        case 128: score_k<128><<<(unsigned)n, 256, 0, st>>>(a); break;
-        case 192: score_k<192><<<(unsigned)n, 256, 0, st>>>(a); break;
-        default: score_k<256><<<(unsigned)n, 256, 0, st>>>(a);
     }
     return (int)hipGetLastError();
 }
@@ -483,14 +563,25 @@ extern "C" int ng_sparse_attention(const void* q, i64 qb, i64 qt, i64 qh, int qt
         s.b0 = r.b0 = b0, s.t0 = r.t0 = t0, s.nt = r.nt = T - t0 < p.nt ? T - t0 : p.nt;
         s.rows = (i64)nb * s.nt * H;
         int rc;
-        if (p.scored && (rc = score_rows(s, nb, p.dp, st))) return rc;
-        // by the scores that a row can have: a wave's, a row a wave; four waves'; a block's
-        if (width <= 256) choose_k<1, 4><<<(unsigned)((s.rows + 3) / 4), 256, 0, st>>>(s);
-        else if (width <= 640) choose_k<1, 10><<<(unsigned)((s.rows + 3) / 4), 256, 0, st>>>(s);
-        else if (width <= 1024) choose_k<1, 16><<<(unsigned)((s.rows + 3) / 4), 256, 0, st>>>(s);
-        else if (width <= 4096) choose_k<4, 16><<<(unsigned)s.rows, 256, 0, st>>>(s);
-        else if (width <= 16384) choose_k<16, 16><<<(unsigned)s.rows, 1024, 0, st>>>(s);
-        else choose_k<16, 32><<<(unsigned)s.rows, 1024, 0, st>>>(s);
+        // one token a sequence: both at once where the rows fill half the CUs, a block each (32 sequences over 32768: 17.9 us
+        // against 15.2 and 7.4; one over 5000, 8 rows: 12.8 against 5.3 and 5.8)
+        if (p.scored && T == 1 && width <= FEW_PAGES && s.rows >= 128) {
+            switch (p.dp) {
+                case 64: score_choose_k<64, 8><<<(unsigned)s.rows, 512, 0, st>>>(s); break;
+                case 128: score_choose_k<128, 16><<<(unsigned)s.rows, 512, 0, st>>>(s); break;
+                case 192: score_choose_k<192, 32><<<(unsigned)s.rows, 512, 0, st>>>(s); break;
+                default: score_choose_k<256, 32><<<(unsigned)s.rows, 512, 0, st>>>(s);
+            }
+        } else {
+            if (p.scored && (rc = score_rows(s, nb, p.dp, st))) return rc;
+            // by the scores that a row can have: a wave's, a row a wave; four waves'; a block's
+            if (width <= 256) choose_k<1, 4><<<(unsigned)((s.rows + 3) / 4), 256, 0, st>>>(s);
+            else if (width <= 640) choose_k<1, 10><<<(unsigned)((s.rows + 3) / 4), 256, 0, st>>>(s);
+            else if (width <= 1024) choose_k<1, 16><<<(unsigned)((s.rows + 3) / 4), 256, 0, st>>>(s);
+            else if (width <= 4096) choose_k<4, 16><<<(unsigned)s.rows, 256, 0, st>>>(s);
+            else if (width <= 16384) choose_k<16, 16><<<(unsigned)s.rows, 1024, 0, st>>>(s);
+            else choose_k<16, 32><<<(unsigned)s.rows, 1024, 0, st>>>(s);
+        }
         if ((rc = (int)hipGetLastError())) return rc;
         r.units = s.rows * p.groups;
         switch (codes) {

@@ -20,6 +20,7 @@ import functools
 from typing import NamedTuple, Sequence
 
 import torch
+from torch.autograd import forward_ad
 
 from .kvcache import DTYPES, refuse_gradients
 from .lib import Entry, Lib, float32
@@ -53,9 +54,9 @@ def _work(B: int, W: int, V: int, K: int) -> int:
     return n
 
 
-def _check(name: str, t: torch.Tensor, shape: tuple, dtype: torch.dtype, like: torch.Tensor) -> torch.Tensor:
-    if t.dtype != dtype or t.shape != shape or t.device != like.device:
-        raise ValueError(f"{name} must be {dtype} {tuple(shape)} on {like.device}: got {tuple(t.shape)} {t.dtype} on {t.device}")
+def _check(name: str, t: torch.Tensor, shape: tuple, dtype: torch.dtype, device: int) -> torch.Tensor:
+    if t.dtype != dtype or t.shape != shape or t.get_device() != device:
+        raise ValueError(f"{name} must be {dtype} {tuple(shape)} on GPU {device}: got {tuple(t.shape)} {t.dtype} on {t.device}")
     return t.contiguous()
 
 
@@ -88,22 +89,25 @@ def beam_step(logits: torch.Tensor, scores: torch.Tensor, lengths: torch.Tensor 
     alpha = float32("alpha", alpha)
     if alpha < 0 or (alpha and lengths is None):
         raise ValueError(f"alpha must be 0 or more, and needs lengths: {alpha}")
-    refuse_gradients("beam_step", logits, scores)
-    scores = _check("scores", scores, (B, W), torch.float32, logits)
+    if logits.requires_grad or scores.requires_grad or forward_ad._current_level >= 0:
+        refuse_gradients("beam_step", logits, scores)
+    gpu = logits.get_device()
+    scores = _check("scores", scores, (B, W), torch.float32, gpu)
     if lengths is not None:
-        lengths = _check("lengths", lengths, (B, W), torch.int32 if lengths.dtype == torch.int32 else torch.int64, logits)
+        lengths = _check("lengths", lengths, (B, W), torch.int32 if lengths.dtype == torch.int32 else torch.int64, gpu)
     if finished is not None:
-        finished = _check("finished", finished, (B, W), torch.bool, logits)
+        finished = _check("finished", finished, (B, W), torch.bool, gpu)
     if logits.stride(2) != 1 and V > 1:
         logits = logits.contiguous()
     device, shape = logits.device, (B, keep)
     out = torch.empty(shape, dtype=torch.float32, device=device)
-    parents, tokens = torch.empty(shape, dtype=torch.int64, device=device), torch.empty(shape, dtype=torch.int64, device=device)
+    # (one tensor's parts: an allocation costs a call of this size more than a view)
+    parents, tokens, *more = torch.empty((2 if lengths is None else 3, B, keep), dtype=torch.int64, device=device).unbind(0)
+    grown = more[0] if more else None
     done = torch.empty(shape, dtype=torch.bool, device=device) if finished is not None or end is not None else None
-    grown = torch.empty(shape, dtype=torch.int64, device=device) if lengths is not None else None
     scratch = torch.empty(work, dtype=torch.uint8, device=device)
     at = _at
-    _entries()[0](logits.get_device(), logits.data_ptr(), logits.stride(0), logits.stride(1), DTYPES[dtype], scores.data_ptr(),
+    _entries()[0](gpu, logits.data_ptr(), logits.stride(0), logits.stride(1), DTYPES[dtype], scores.data_ptr(),
                   at(lengths), 0 if lengths is None else lengths.element_size(), at(finished), B, W, V, keep, -1 if end is None else end, -1 if pad is None else pad, alpha,
                   out.data_ptr(), parents.data_ptr(), tokens.data_ptr(), at(done), at(grown), scratch.data_ptr())
     return BeamStep(out, parents, tokens, done, grown)
@@ -124,15 +128,16 @@ def reorder(states: torch.Tensor | Sequence[torch.Tensor], parents: torch.Tensor
 def _reordered(state: torch.Tensor, parents: torch.Tensor) -> torch.Tensor:
     if state.dim() < 1 or not state.is_cuda:
         raise ValueError(f"states must be [rows, ...] on the GPU: got {tuple(state.shape)} on {state.device}")
-    if parents.dtype != torch.int64 or parents.device != state.device:
+    if parents.dtype != torch.int64 or parents.get_device() != state.get_device():
         raise ValueError(f"parents must be int64 on {state.device}: got {parents.dtype} on {parents.device}")
-    refuse_gradients("reorder", state)
+    if state.requires_grad or forward_ad._current_level >= 0:
+        refuse_gradients("reorder", state)
     rows, rest, size = state.shape[0], state.shape[1:], state.element_size()
     row = rest.numel() * size
-    if rows and not state[0].is_contiguous():
+    if not state.is_contiguous() and rows and not state[0].is_contiguous():
         state = state.contiguous()
-    parents = parents.reshape(-1).contiguous()
-    n = parents.shape[0]
+    parents = parents.contiguous()
+    n = parents.numel()
     out = torch.empty((n, *rest), dtype=state.dtype, device=state.device)
     _entries()[1](state.get_device(), state.data_ptr(), state.stride(0) * size, rows, row, parents.data_ptr(), n, out.data_ptr())
     return out

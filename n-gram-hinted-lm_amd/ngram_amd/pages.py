@@ -14,8 +14,8 @@ what it has written). Every table's entries must be counted: by hold, by a fork 
 
 Pages and counts are whole numbers and choices go by order (the lowest free pages, in the order of rows), so the same calls
 give the same pages on every run. Everything runs on the current stream and nothing synchronizes: where the pages do not
-suffice, `missing` on the device counts the ones that were not to be had, and their positions' slots are -1. csrc/pages.hip
-has the kernels."""
+suffice, `missing` on the device counts the ones that were not to be had, and their positions' slots are -1. A pool is one
+state: calls on it from several streams must be ordered by the caller. csrc/pages.hip has the kernels."""
 
 from __future__ import annotations
 
@@ -83,7 +83,7 @@ class PagePool:
         if parents.dtype != torch.int64 or parents.numel() != S or parents.get_device() != self.cache.device:
             raise ValueError(f"parents must be int64 of {S} rows on {self.cache.k.device}: got {tuple(parents.shape)} "
                              f"{parents.dtype} on {parents.device}")
-        parents = parents.reshape(-1).contiguous()
+        parents = parents.contiguous()
         work = torch.empty(_size("ng_pool_fork_work", S, width), dtype=torch.uint8, device=table.device)
         _entries()[2](self.cache.device, self._state.data_ptr(), self.cache.pages, table.data_ptr(), table.stride(0), S, width,
                       lengths.data_ptr(), parents.data_ptr(), work.data_ptr())

@@ -140,6 +140,13 @@ def test_pages_always_kept(gpu, keep, first, last):
     _check(*_make(keep, 3, 2, 2, 2, 64, "int8", torch.bfloat16, [16 * 40 - 1, 333, 16 * 41]), keep, first=first, last=last)
 
 
+@pytest.mark.parametrize("dim", [64, 100, 192, 250])
+@pytest.mark.parametrize("B,T,n", [(2, 1, 300), (66, 1, 40), (2, 2, 300), (1, 4, 70), (1, 5, 300), (1, 17, 33)])
+def test_scores_of_every_row_size(gpu, dim, B, T, n):
+    """One token by vector operations, apart from the choice and with it; up to four and more on the matrix units."""
+    _check(*_make(dim + T, B, T, 2, 3, dim, "fp8", torch.bfloat16, [16 * n - 7 * b % 50 for b in range(B)]), 7)
+
+
 @pytest.mark.parametrize("n,keep", [(1024, 1000), (1025, 17), (1023, 64), (4096, 100), (4097, 33), (9000, 500), (32768, 7)])
 def test_many_pages(gpu, n, keep):
     """Sequences of as many pages as a wave, four waves or a block hold scores of, and one more."""
