@@ -446,8 +446,9 @@ static bool sparse_plan(i64 B, i64 T, i64 H, i64 G, i64 dim, i64 width, i64 page
     p.nb = (int)(T <= most ? (B < most / T ? B : most / T) : 1);
     const i64 rows = (B ? (i64)p.nb : 0) * p.nt * H, units = rows * p.groups;
     const i64 tiles = ((keep < width ? keep : width) * page + TILE - 1) / TILE;
-    // parts of two tiles at least; up to six tiles are left whole: joining their parts costs more than they take
-    i64 splits = units && tiles > 6 ? (AIM + units - 1) / units : 1;
+    // A block a unit where the units fill the CUs (256: 30.0 us and no joining; in two parts each 28.3 and 4.3), else parts that
+    // make AIM blocks, of two tiles at least. Up to six tiles are left whole: joining their parts costs more than they take.
+    i64 splits = units && units < 256 && tiles > 6 ? (AIM + units - 1) / units : 1;
     p.splits = (int)(splits < (tiles + 1) / 2 ? splits : (tiles + 1) / 2);
     const i64 parts = p.splits > 1 ? units * p.splits * 16 : 0;
     p.score = 0;
