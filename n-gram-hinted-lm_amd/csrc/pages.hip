@@ -5,8 +5,8 @@
 //
 // Fork: row s of a table becomes what row parents[s] was. refs[p] += children(row) - 1 for each entry of each row, one atomic
 // an entry and none where a row has one child; every holder's change is -1 at least and refs counts them all, so a count
-// reaches 0 only by its last change, which sets the free bit. The entries go through a scratch table (rows read each
-// other), only the rows that move.
+// reaches 0 only by its last change, which sets the free bit. Rows read each other: up to 1024 rows' entries go through LDS, a
+// strip of columns a block, more through a scratch table (only the rows that move).
 //
 // Room: positions length .. length + count - 1 of each row, a request per page that holds any of them. A request is met by
 // the entry it finds where no other row holds that page, or where all that hold it request it here and this is the first of
@@ -78,6 +78,34 @@ __global__ __launch_bounds__(256) void pool_fork_k(const Pool p, const int* __re
         if (from != s) moved[(i64)s * width + c] = is ? table[from * stride + c] : -1;
     }
     if (blockIdx.y == 0 && tid == 0) moved_len[s] = is ? lengths[from] : 0;
+}
+
+// Up to MANY rows: a block takes a strip of columns of all rows, which go through its LDS.
+#define MANY 1024
+#define HELD 2048  // entries of a strip
+__global__ __launch_bounds__(1024) void pool_fork_few_k(const Pool p, int* __restrict__ table, i64 stride, int S, int width,
+                                                        int* __restrict__ lengths, const i64* __restrict__ parents, int shift) {
+    __shared__ int held[HELD], from[MANY], children[MANY], len[MANY];
+    const int tid = threadIdx.x, columns = 1 << shift, c0 = blockIdx.x << shift, n = width - c0;
+    if (tid < S) {
+        const i64 f = parents[tid];
+        from[tid] = (u64)f < (u64)S ? (int)f : -1;
+        children[tid] = 0;
+        if (blockIdx.x == 0) len[tid] = lengths[tid];
+    }
+    for (int i = tid; i < S << shift; i += 1024) {
+        const int s = i >> shift, c = i & (columns - 1);
+        held[i] = c < n ? table[s * stride + c0 + c] : -1;
+    }
+    __syncthreads();
+    if (tid < S && from[tid] >= 0) atomicAdd(&children[from[tid]], 1);
+    __syncthreads();
+    for (int i = tid; i < S << shift; i += 1024) {
+        const int s = i >> shift, c = i & (columns - 1), change = children[s] - 1, e = held[i], f = from[s];
+        if (change && is_page(p, e) && atomicAdd(&p.refs[e], change) + change == 0) atomicOr(&p.free[e >> 5], 1u << (e & 31));
+        if (f != s && c < n) table[s * stride + c0 + c] = f < 0 ? -1 : held[(f << shift) + c];
+    }
+    if (blockIdx.x == 0 && tid < S && from[tid] != tid) lengths[tid] = from[tid] < 0 ? 0 : len[from[tid]];
 }
 
 __global__ __launch_bounds__(256) void pool_moved_k(int* __restrict__ table, i64 stride, int width, int* __restrict__ lengths,
@@ -407,7 +435,8 @@ extern "C" int ng_pool_hold(void* state, i64 pages, const int* table, i64 stride
 }
 
 extern "C" i64 ng_pool_fork_work(i64 S, i64 width) {
-    return S < 0 || width < 1 || S > 1 << 24 || width > 1 << 26 || S * width >= (i64)1 << 40 ? -1 : (S * width + S) * 4;
+    if (S < 0 || width < 1 || S > 1 << 24 || width > 1 << 26 || S * width >= (i64)1 << 40) return -1;
+    return S <= MANY ? 0 : (S * width + S) * 4;
 }
 
 extern "C" int ng_pool_fork(void* state, i64 pages, int* table, i64 stride, int S, int width, int* lengths,
@@ -415,6 +444,13 @@ extern "C" int ng_pool_fork(void* state, i64 pages, int* table, i64 stride, int 
     Pool p;
     if (!pool_of(state, pages, p) || ng_pool_fork_work(S, width) < 0) return -1;
     if (S == 0) return 0;
+    if (S <= MANY) {
+        int shift = 5;  // 32 columns, 2 for 1024 rows
+        while (S << shift > HELD) --shift;
+        pool_fork_few_k<<<(unsigned)(((i64)width + (1 << shift) - 1) >> shift), 1024, 0, (hipStream_t)stream>>>(
+            p, table, stride, S, width, lengths, parents, shift);
+        return (int)hipGetLastError();
+    }
     int* moved = (int*)work;
     int* moved_len = moved + (i64)S * width;
     const dim3 grid(S, (width + STRIP - 1) / STRIP);

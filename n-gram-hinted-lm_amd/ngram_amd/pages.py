@@ -84,9 +84,10 @@ class PagePool:
             raise ValueError(f"parents must be int64 of {S} rows on {self.cache.k.device}: got {tuple(parents.shape)} "
                              f"{parents.dtype} on {parents.device}")
         parents = parents.contiguous()
-        work = torch.empty(_size("ng_pool_fork_work", S, width), dtype=torch.uint8, device=table.device)
+        size = _size("ng_pool_fork_work", S, width)
+        work = torch.empty(size, dtype=torch.uint8, device=table.device) if size else None
         _entries()[2](self.cache.device, self._state.data_ptr(), self.cache.pages, table.data_ptr(), table.stride(0), S, width,
-                      lengths.data_ptr(), parents.data_ptr(), work.data_ptr())
+                      lengths.data_ptr(), parents.data_ptr(), None if work is None else work.data_ptr())
 
     def reserve(self, table: torch.Tensor, lengths: torch.Tensor, count: int, counts: torch.Tensor | None = None) -> torch.Tensor:
         """Room behind each row's tokens for `count` more (or counts[s], int32 [rows], held to 0 .. count): int64 [rows,

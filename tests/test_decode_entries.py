@@ -43,7 +43,7 @@ def test_sizes(library):
         assert size("ng_beam_work", *bad) == -1, bad
     assert size("ng_pool_state", 33) == (3 * 33 + 2 + 1) * 4
     assert size("ng_pool_state", 0) == size("ng_pool_state", 1 << 31) == -1
-    assert size("ng_pool_fork_work", 3, 5) == 72 and size("ng_pool_fork_work", 1, 1 << 27) == -1
+    assert size("ng_pool_fork_work", 1024, 5) == 0 and size("ng_pool_fork_work", 1025, 5) == 1025 * 6 * 4 and size("ng_pool_fork_work", 1, 1 << 27) == -1
     assert size("ng_pool_room_work", 2, 1, 16) == (3 * 4 + 2) * 4 and size("ng_pool_room_work", 2, 18, 16) == (3 * 6 + 2) * 4
     for bad in ((1, 0, 16), (1, 1, 8), (1, 1, 48), (1, 1 << 30, 16), (1 << 27, 100, 16)):
         assert size("ng_pool_room_work", *bad) == -1, bad

@@ -237,6 +237,32 @@ def test_part_of_a_table(gpu):
     assert b.pool.refs.tolist() == b.plain.refs()
 
 
+@pytest.mark.parametrize("S,width", [(1, 1), (1, 70), (255, 33), (257, 100), (1000, 17), (1024, 9), (1025, 9), (1300, 2100)])
+def test_forks_of_every_size(gpu, S, width):
+    """Few rows through LDS, many through a scratch table; against indexing."""
+    g = torch.Generator().manual_seed(S + width)
+    cache = KVCache.empty(500, 16, 1, 1, "bf16")
+    pool = PagePool(cache)
+    wide = torch.randint(-1, 500, (S, width + 3), generator=g).int().cuda()
+    start, behind = wide[:, :width].clone(), wide[:, width:].clone()
+    table, lengths = wide[:, :width], torch.randint(0, 999, (S,), generator=g).int().cuda()
+    was = lengths.clone()
+    pool.hold(table)
+    parents = torch.randint(-1, S, (S,), generator=g).cuda()
+    parents[::3] = torch.arange(S).cuda()[::3]
+    parents[S // 2] = S
+    pool.fork(table, lengths, parents)
+    there = (parents >= 0) & (parents < S)
+    want = torch.where(there[:, None], start[parents.clamp(0, S - 1)], -1)
+    assert torch.equal(table, want) and torch.equal(wide[:, width:], behind)
+    assert torch.equal(lengths, torch.where(there, was[parents.clamp(0, S - 1)], 0))
+    assert torch.equal(pool.refs, torch.bincount(want[want >= 0].long(), minlength=500).int())
+    free = torch.full((1, 500), -1, dtype=torch.int32).cuda()
+    slots = pool.reserve(free, torch.zeros(1, dtype=torch.int32).cuda(), 500 * 16)[0, ::16] // 16
+    n = int((torch.bincount(want[want >= 0].long(), minlength=500) == 0).sum())
+    assert (slots >= 0).sum() == n and (pool.refs[slots[:n]] == 1).all()
+
+
 def test_wide_tables(gpu):
     """Rows of more columns than a block takes."""
     width, S = 5000, 7
