@@ -52,11 +52,15 @@ __device__ __forceinline__ int few(int K) { return K + K / 2 + 12; }
 __device__ __forceinline__ void write_ranked(u64* list, int n, int K_, u64* out, int threads) {
     if (threadIdx.x < 3) list[n + threadIdx.x] = 0;
     __syncthreads();
-    for (int i = threadIdx.x; i < n; i += threads) {
-        const u64 mine = list[i];
+    for (int i0 = 0; i0 < n; i0 += threads / 4) {  // four lanes a key
+        const int i = i0 + threadIdx.x / 4;
+        const u64 mine = i < n ? list[i] : 0;
         int r = 0;
-        for (int j = 0; j < n; j += 4) r += (list[j] > mine) + (list[j + 1] > mine) + (list[j + 2] > mine) + (list[j + 3] > mine);
-        if (r < K_) out[r] = mine;
+        for (int j = (threadIdx.x & 3) * 4; j < n; j += 16)
+            r += (list[j] > mine) + (list[j + 1] > mine) + (list[j + 2] > mine) + (list[j + 3] > mine);
+        r += __shfl_xor(r, 1, WAVE);
+        r += __shfl_xor(r, 2, WAVE);
+        if (i < n && r < K_ && (threadIdx.x & 3) == 0) out[r] = mine;
     }
     for (int i = n + threadIdx.x; i < K_; i += threads) out[i] = 0;
 }
@@ -132,11 +136,10 @@ template <typename T, int E> __global__ __launch_bounds__(256, 8) void beam_part
     __shared__ u32 most[4], least[4];
     __shared__ double sums[4];
     __shared__ int fill;
-    const i64 row = blockIdx.x / a.chunks;
+    const u32 row = blockIdx.x / (u32)a.chunks, b = row / (u32)a.W;
     const int chunk = (int)(blockIdx.x - row * a.chunks), tid = threadIdx.x, wave = tid >> 6;
     if (ended(a, row)) return;
-    const i64 b = row / a.W;
-    const T* __restrict__ x = (const T*)a.logits + b * a.sb + (row - b * a.W) * a.sw;
+    const T* __restrict__ x = (const T*)a.logits + b * a.sb + (i64)(row - b * a.W) * a.sw;
     const int from = chunk * 256 * E + tid * N;
     Logits<T, E> v;
     v.load(x, from, a.V, (i64)(chunk + 1) * 256 * E <= a.V);
@@ -190,7 +193,7 @@ template <typename T, int E> __global__ __launch_bounds__(256, 8) void beam_part
                 }
     __syncthreads();
     if (fill > ROOM) crowded<T, E>(x, from, a, t, hi, count, list, &fill);
-    const i64 at = row * a.chunks + chunk;
+    const i64 at = blockIdx.x;
     write_ranked(list, fill, a.K, a.part + at * a.K, 256);
     if (tid == 0) {
         const double off = near ? 0.69314718055994531 * ((double)L * m + (double)c) : 0.;  // below 2^-11: exp by its series
@@ -250,7 +253,7 @@ template <int NW, int E> __global__ __launch_bounds__(NW * 64) void beam_row_k(c
         const int i = e * NT + threadIdx.x;
         key[e] = i < have ? a.part[row * have + i] : 0;
         mine = key[e] > mine ? key[e] : mine;
-        if (i % a.K == a.K - 1) full = key[e] > full ? key[e] : full;
+        if ((u32)i % (u32)a.K == (u32)a.K - 1) full = key[e] > full ? key[e] : full;
     }
     u64 lo, hi;
     ends(mine, full, most, hi, lo);
@@ -316,11 +319,11 @@ template <int NW, int E> __global__ __launch_bounds__(NW * 64) void beam_join_k(
         const int i = e * NT + tid;
         key[e] = 0;
         if (i < have) {
-            const int w = i / per;
+            const int w = (int)((u32)i / (u32)per);
             const u64 c = done[w] ? 0ull : HOLD ? held[HOLD ? e : 0] : a.part[b * have + i];
             if (c) key[e] = key_of((scores[w] + ((double)of_key((u32)(c >> 32)) - lses[w])) * norms[w]);
             if (done[w] && i == w * per) key[e] = key_of(scores[w] * norms[w]);
-            if (i % a.K == a.K - 1) full = key[e] > full ? key[e] : full;
+            if ((u32)i % (u32)a.K == (u32)a.K - 1) full = key[e] > full ? key[e] : full;
         }
         mine = key[e] > mine ? key[e] : mine;
     }
@@ -330,7 +333,7 @@ template <int NW, int E> __global__ __launch_bounds__(NW * 64) void beam_join_k(
     int n = count.at_least(key, lo);
     const u64 t = count.threshold(key, lo, hi, a.K, few(a.K), n);
     auto second = [&](int e) {
-        const int i = e * NT + tid, w = i / per;
+        const int i = e * NT + tid, w = (int)((u32)i / (u32)per);
         const u64 c = done[w] ? 0xFFFFFFFFull << 32 | (u32)~a.pad : HOLD ? held[HOLD ? e : 0] : a.part[b * have + i];
         return (u64)(MOST - 1 - w) << 57 | c >> 32 << TOKEN_BITS | ((u32)c & ((1u << TOKEN_BITS) - 1));
     };
@@ -367,16 +370,19 @@ template <int NW, int E> __global__ __launch_bounds__(NW * 64) void beam_join_k(
         if (a.out_finished) a.out_finished[o] = done[w] || token == a.end;
         if (a.out_lengths) a.out_lengths[o] = length_of(a, b * a.W + w) + (done[w] ? 0 : 1);
     };
-    for (int i = tid; i < n; i += NT) {
-        const u64 k = list[i].x, s = list[i].y;
+    for (int i0 = 0; i0 < n; i0 += NT / 4) {  // four lanes a candidate
+        const int i = i0 + tid / 4;
+        const u64 k = i < n ? list[i].x : 0, s = i < n ? list[i].y : 0;
         int r = 0;
-        for (int j = 0; j < n; j += 4)
+        for (int j = (tid & 3) * 4; j < n; j += 16)
 #pragma unroll
             for (int u = 0; u < 4; ++u) {
                 const ulonglong2 x = list[j + u];
                 r += x.x > k || (x.x == k && x.y > s);
             }
-        if (r >= a.K) continue;
+        r += __shfl_xor(r, 1, WAVE);
+        r += __shfl_xor(r, 2, WAVE);
+        if (i >= n || r >= a.K || (tid & 3)) continue;
         const int w = MOST - 1 - (int)(s >> 57), token = (1 << TOKEN_BITS) - 1 - (int)(s & ((1u << TOKEN_BITS) - 1));
         put(r, w, token, (float)(done[w] ? scores[w] : scores[w] + ((double)of_key((u32)(s >> TOKEN_BITS)) - lses[w])));
     }
