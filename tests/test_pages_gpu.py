@@ -143,6 +143,18 @@ def test_histories(gpu, codes, page, rows, count):
     assert not b.pool.refs.any() and not b.table.ge(0).any()
 
 
+@pytest.mark.parametrize("codes", ["int8", "bf16"])
+def test_many_requests(gpu, codes):
+    """More requests in a call than a block's threads, for pages in common among them."""
+    rows, g = 700, torch.Generator().manual_seed(8)
+    b = Both(rows * 7, 16, rows, 6, codes, heads=1)
+    b.append(20, [20 if s % 3 else 0 for s in range(rows)])
+    for _ in range(2):
+        b.fork(torch.randint(0, rows // 4, (rows,), generator=g).tolist())
+        b.append(3)
+    b.append(30, torch.randint(-5, 31, (rows,), generator=g).tolist())
+
+
 def test_pages_run_out(gpu):
     """What was to be had goes to the first rows; the others' slots are -1 and nobody's rows are touched."""
     b = Both(7, 16, 4, 4)
