@@ -37,9 +37,9 @@ def _entries() -> tuple[Entry, ...]:
 
 @functools.lru_cache(maxsize=1024)
 def _size(name: str, *args: int) -> int:
-    n = Lib().size(name, *args)
+    n = Lib().size("ng_" + name, *args)
     if n < 0:
-        raise ValueError(f"{name[3:]} of {args}: out of range")
+        raise ValueError(f"{name} of {args}: out of range")
     return n
 
 
@@ -50,7 +50,7 @@ class PagePool:
         if bounds is not None and bounds.cache is not cache:
             raise ValueError("the bounds are another cache's")
         self.cache, self.bounds = cache, bounds
-        self._state = torch.empty(_size("ng_pool_state", cache.pages) // 4, dtype=torch.int32, device=cache.k.device)
+        self._state = torch.empty(_size("pool_state", cache.pages) // 4, dtype=torch.int32, device=cache.k.device)
         self.clear()
 
     # refs: the entries that hold each page. missing: pages that reservations and moves did not get, since the pool was cleared.
@@ -84,7 +84,7 @@ class PagePool:
             raise ValueError(f"parents must be int64 of {S} rows on {self.cache.k.device}: got {tuple(parents.shape)} "
                              f"{parents.dtype} on {parents.device}")
         parents = parents.contiguous()
-        size = _size("ng_pool_fork_work", S, width)
+        size = _size("pool_fork_work", S, width)
         work = torch.empty(size, dtype=torch.uint8, device=table.device) if size else None
         _entries()[2](self.cache.device, self._state.data_ptr(), self.cache.pages, table.data_ptr(), table.stride(0), S, width,
                       lengths.data_ptr(), parents.data_ptr(), None if work is None else work.data_ptr())
@@ -104,7 +104,7 @@ class PagePool:
             counts = counts.contiguous()
         slots = torch.empty((S, count), dtype=torch.int64, device=table.device)
         if S and count:
-            work = torch.empty(_size("ng_pool_room_work", S, count, c.page), dtype=torch.uint8, device=table.device)
+            work = torch.empty(_size("pool_room_work", S, count, c.page), dtype=torch.uint8, device=table.device)
             _entries()[3](c.device, self._state.data_ptr(), c.pages, table.data_ptr(), table.stride(0), S, width,
                           lengths.data_ptr(), None if counts is None else counts.data_ptr(), count, *c.addresses(), c.page,
                           c.heads, c.dim, c.code, slots.data_ptr(), work.data_ptr())
@@ -123,7 +123,7 @@ class PagePool:
         if (self.bounds is None) != (into.bounds is None):
             raise ValueError("both pools need bounds, or neither")
         out = torch.empty((S, width), dtype=torch.int32, device=table.device)
-        work = torch.empty(_size("ng_pool_move_work", a.pages, b.pages), dtype=torch.uint8, device=table.device)
+        work = torch.empty(_size("pool_move_work", a.pages, b.pages), dtype=torch.uint8, device=table.device)
         _entries()[4](a.device, self._state.data_ptr(), a.pages, *a.addresses(), _bounds(self.bounds), into._state.data_ptr(),
                       b.pages, *b.addresses(), _bounds(into.bounds), a.page, a.heads, a.dim, a.code, table.data_ptr(),
                       table.stride(0), S, width, out.data_ptr(), work.data_ptr())

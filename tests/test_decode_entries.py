@@ -36,23 +36,25 @@ def test_declared_types_match_the_header(library):
 
 
 def test_sizes(library):
-    size = library.size
-    assert size("ng_beam_work", 1, 4, 50257, 4) > 0 and size("ng_beam_work", 0, 1, 1, 1) >= 0
+    assert library.size("ng_beam_work", 1, 4, 50257, 4) > 0
+    assert library.size("ng_beam_work", 0, 1, 1, 1) >= 0
     for bad in ((-1, 1, 9, 1), (1, 0, 9, 1), (1, 129, 9, 1), (1, 1, 0, 1), (1, 1, 9, 0), (1, 1, 9, 10), (1, 2, 900, 129),
                 (1, 1, (1 << 25) + 1, 1), (1, 1, 1 << 21, 128)):
-        assert size("ng_beam_work", *bad) == -1, bad
-    assert size("ng_pool_state", 33) == (3 * 33 + 2 + 1) * 4
-    assert size("ng_pool_state", 0) == size("ng_pool_state", 1 << 31) == -1
-    assert size("ng_pool_fork_work", 1024, 5) == 0 and size("ng_pool_fork_work", 1025, 5) == 1025 * 6 * 4 and size("ng_pool_fork_work", 1, 1 << 27) == -1
-    assert size("ng_pool_room_work", 2, 1, 16) == (3 * 4 + 2) * 4 and size("ng_pool_room_work", 2, 18, 16) == (3 * 6 + 2) * 4
+        assert library.size("ng_beam_work", *bad) == -1, bad
+    assert library.size("ng_pool_state", 33) == (3 * 33 + 2 + 1) * 4
+    assert library.size("ng_pool_state", 0) == library.size("ng_pool_state", 1 << 31) == -1
+    assert library.size("ng_pool_fork_work", 1024, 5) == 0 and library.size("ng_pool_fork_work", 1025, 5) == 1025 * 6 * 4
+    assert library.size("ng_pool_fork_work", 1, 1 << 27) == -1
+    assert library.size("ng_pool_room_work", 2, 1, 16) == (3 * 4 + 2) * 4
+    assert library.size("ng_pool_room_work", 2, 18, 16) == (3 * 6 + 2) * 4
     for bad in ((1, 0, 16), (1, 1, 8), (1, 1, 48), (1, 1 << 30, 16), (1 << 27, 100, 16)):
-        assert size("ng_pool_room_work", *bad) == -1, bad
-    assert size("ng_pool_move_work", 4, 9) == 52 and size("ng_pool_move_work", 0, 9) == -1
-    assert size("ng_sparse_work", 1, 1, 8, 4, 128, 320, 16, 32) > 0
+        assert library.size("ng_pool_room_work", *bad) == -1, bad
+    assert library.size("ng_pool_move_work", 4, 9) == 52 and library.size("ng_pool_move_work", 0, 9) == -1
+    assert library.size("ng_sparse_work", 1, 1, 8, 4, 128, 320, 16, 32) > 0
     for bad in ((1, 0, 8, 4, 128, 320, 16, 32), (1, 1, 0, 4, 128, 320, 16, 32), (1, 1, 8, 0, 128, 320, 16, 32),
                 (1, 1, 8, 4, 257, 320, 16, 32), (1, 1, 8, 4, 128, 32769, 16, 32), (1, 1, 8, 4, 128, 320, 24, 32),
                 (1, 1, 8, 4, 128, 320, 16, 1025), (1, 1, 8, 4, 128, 320, 16, 0)):
-        assert size("ng_sparse_work", *bad) == -1, bad
+        assert library.size("ng_sparse_work", *bad) == -1, bad
 
 
 def test_refused_before_a_launch(library, host):
