@@ -106,10 +106,10 @@ def beam_step(logits: torch.Tensor, scores: torch.Tensor, lengths: torch.Tensor 
     grown = more[0] if more else None
     done = torch.empty(shape, dtype=torch.bool, device=device) if finished is not None or end is not None else None
     scratch = torch.empty(work, dtype=torch.uint8, device=device)
-    at = _at
-    _entries()[0](gpu, logits.data_ptr(), logits.stride(0), logits.stride(1), DTYPES[dtype], scores.data_ptr(),
-                  at(lengths), 0 if lengths is None else lengths.element_size(), at(finished), B, W, V, keep, -1 if end is None else end, -1 if pad is None else pad, alpha,
-                  out.data_ptr(), parents.data_ptr(), tokens.data_ptr(), at(done), at(grown), scratch.data_ptr())
+    _entries()[0](gpu, logits.data_ptr(), logits.stride(0), logits.stride(1), DTYPES[dtype], scores.data_ptr(), _at(lengths),
+                  0 if lengths is None else lengths.element_size(), _at(finished), B, W, V, keep, -1 if end is None else end,
+                  -1 if pad is None else pad, alpha, out.data_ptr(), parents.data_ptr(), tokens.data_ptr(), _at(done),
+                  _at(grown), scratch.data_ptr())
     return BeamStep(out, parents, tokens, done, grown)
 
 

@@ -9,9 +9,9 @@ zero (or too small for its inverse) has scale 0; one that holds a NaN or an infi
 reads back as NaN and nothing of it enters where it is masked. A scale of 0 stands for zeros whatever the codes are.
 
 A token's slot is page * page size + its row there; a sequence's page table lists its pages in order, and -1 stands for no
-slot. Which page belongs to whom is the caller's. Quantising has no backward pass: keys and values that require gradients
-(with gradients on) or carry tangents raise. Everything runs on the current stream, and nothing here synchronizes.
-csrc/kvcache.hip has the kernels."""
+slot. Which page belongs to whom is the caller's, or a pool's (pages.py). Quantising has no backward pass: keys and values
+that require gradients (with gradients on) or carry tangents raise. Everything runs on the current stream, and nothing here
+synchronizes. csrc/kvcache.hip has the kernels."""
 
 from __future__ import annotations
 
