@@ -455,7 +455,8 @@ static bool sparse_plan(i64 B, i64 T, i64 H, i64 G, i64 dim, i64 width, i64 page
     const i64 rows = (B ? (i64)p.nb : 0) * p.nt * H, units = rows * p.groups;
     const i64 tiles = ((keep < width ? keep : width) * page + TILE - 1) / TILE;
     // A block a unit where the units fill the CUs (256: 30.0 us and no joining; in two parts each 28.3 and 4.3), else parts that
-    // make AIM blocks, of two tiles at least. Up to six tiles are left whole: joining their parts costs more than they take.
+    // make AIM blocks, of two tiles at least. Up to six tiles are left whole: joining their parts costs more than they take (8
+    // units of four tiles: 10.8 us, in halves 8.7 and 2.6 in two launches).
     i64 splits = units && units < 256 && tiles > 6 ? (AIM + units - 1) / units : 1;
     p.splits = (int)(splits < (tiles + 1) / 2 ? splits : (tiles + 1) / 2);
     const i64 parts = p.splits > 1 ? units * p.splits * 16 : 0;
@@ -516,8 +517,9 @@ template <int TT> static void score_tokens(const ScoreArgs& a, int dp, unsigned 
     }
 }
 
-// One token a sequence is scored by vector operations, more on the matrix units. A block takes 256 pages, or fewer (64 at
-// least) where that leaves fewer than 1024 blocks.
+// One token a sequence is scored by vector operations (32 over up to 512 pages: 14.7 us, on the matrix units 17.2), more on the
+// matrix units, up to four by products of 4 x 4 (2 x 4 over 8192 pages: 21.5 us, by 16 x 16 26.6). A block takes 256 pages, or
+// fewer (64 at least) where that leaves fewer than 1024 blocks.
 static int score_rows(ScoreArgs& a, int nb, int dp, hipStream_t st) {
     const int tokens = a.T == 1 ? 1 : a.T <= 4 ? 4 : 16;
     const i64 units = (i64)nb * a.H * ((a.nt + tokens - 1) / tokens);
@@ -583,7 +585,8 @@ extern "C" int ng_sparse_attention(const void* q, i64 qb, i64 qt, i64 qh, int qt
             }
         } else {
             if (p.scored && (rc = score_rows(s, nb, p.dp, st))) return rc;
-            // by the scores that a row can have: a wave's, a row a wave; four waves'; a block's
+            // by the scores that a row can have: a wave's, a row a wave (5120 rows of 533: 11.0 us, by four waves each 32; 8
+            // rows of 313: 5.4 and 7.8); four waves'; a block's
             if (width <= 256) choose_k<1, 4><<<(unsigned)((s.rows + 3) / 4), 256, 0, st>>>(s);
             else if (width <= 640) choose_k<1, 10><<<(unsigned)((s.rows + 3) / 4), 256, 0, st>>>(s);
             else if (width <= 1024) choose_k<1, 16><<<(unsigned)((s.rows + 3) / 4), 256, 0, st>>>(s);
