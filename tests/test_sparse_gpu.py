@@ -242,7 +242,7 @@ def test_scores_that_are_not_finite(gpu):
 
 
 @pytest.mark.parametrize("codes,dtype", CODES)
-@pytest.mark.parametrize("dim,page", [(64, 16), (100, 32), (192, 128), (256, 64), (1, 16)])
+@pytest.mark.parametrize("dim,page", [(64, 16), (100, 32), (192, 128), (256, 64), (1, 16), (130, 256), (33, 512)])
 def test_bounds(gpu, codes, dtype, dim, page):
     """The smallest and largest of a page's values, outward; of the pages that the positions complete and no other."""
     g = torch.Generator().manual_seed(dim)
