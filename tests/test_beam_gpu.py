@@ -5,8 +5,9 @@ refusals; the states' reordering.
 Tolerances. A row's log-sum: a term 2^t beside the largest (1) has its exponent rounded once, off by |t| 2^-24, so itself by
 0.7 |t| 2^-24, and the instruction adds 2^-23; of V <= 2^17 terms those with |t| > 20 weigh less than 2^-3 of the largest
 together and less the further they lie, so a sum is off by 20 * 0.7 * 2^-24 < 2^-20 and 2^-23 of itself at most; a thread's
-sum of up to 32 terms adds 31 * 2^-24, the rest is 64 bits: LSE = 2^-20 + 2^-23 + 31 * 2^-24. A score is rounded to float32 once: 2^-24 of itself more. Two candidates may come in the other order where their exact ranks
-differ by less than twice LSE (over their lengths' norms, which are 1 at least); within a beam the order is the logits'."""
+sum of up to 32 terms adds 31 * 2^-24, the rest is 64 bits: LSE = 2^-20 + 2^-23 + 31 * 2^-24. A score is rounded to float32
+once: 2^-24 of itself more. Two candidates may come in the other order where their exact ranks differ by less than twice LSE
+(over their lengths' norms, which are 1 at least); within a beam the order is the logits'."""
 
 import math
 
