@@ -9,8 +9,10 @@
 // strip of columns a block, more through a scratch table (only the rows that move).
 //
 // Room: positions length .. length + count - 1 of each row, a request per page that holds any of them. A request is met by
-// the entry it finds where no other row holds that page, or where all that hold it request it here and this is the first of
-// them (atomic minimum and count: the order of atomics changes nothing); else by the lowest free pages in the order of rows.
+// the entry it finds where no other row holds that page, or where all that hold it request it here and this is the longest of
+// them, of equal ones the first (an atomic maximum and count: the order of atomics changes nothing); else by the lowest free
+// pages in the order of rows. (The longest: where the pages run out, a row that gets none is left with the page it shares, and
+// what the keeper writes there must lie behind that row's tokens.)
 // One block does this, since each page given depends on all before it: the requests are scanned 1024 at a time and the free
 // bits 32768 pages at a time, up to the last one needed. The rows of a shared page that lie before the length are copied by
 // a second kernel, a block per row and head, which also writes the slots.
@@ -139,7 +141,7 @@ struct Room {
 enum { KEPT = -1, NONE = -2 };
 
 struct Ask {
-    int column, entry, refs;
+    int column, entry, refs, len;
     bool is, held;
 };
 
@@ -148,10 +150,12 @@ __device__ __forceinline__ int row_count(const Room& r, int s) {
     return n < 0 ? 0 : n < r.count ? n : r.count;
 }
 
+__device__ __forceinline__ int row_len(const Room& r, int s) { return r.lengths[s] < 0 ? 0 : r.lengths[s]; }
+
 __device__ __forceinline__ Ask ask_of(const Pool& p, const Room& r, int i) {
-    const int s = i / r.per, j = i - s * r.per, len = r.lengths[s] < 0 ? 0 : r.lengths[s];
+    const int s = i / r.per, j = i - s * r.per, len = row_len(r, s);
     Ask q;
-    q.column = (len >> r.shift) + j;
+    q.len = len, q.column = (len >> r.shift) + j;
     q.is = ((i64)q.column << r.shift) < (i64)len + row_count(r, s) && q.column < r.width && row_count(r, s) > 0;
     q.entry = q.is ? r.table[s * r.stride + q.column] : -1;
     q.refs = q.is && is_page(p, q.entry) ? p.refs[q.entry] : 0;
@@ -184,7 +188,8 @@ __device__ __forceinline__ int scan_block(int x, int* lds, int& total) {
 // number's.
 #define PLACES 2048
 struct Askers {
-    int page[PLACES], count[PLACES], first[PLACES];
+    int page[PLACES], count[PLACES];
+    u64 best[PLACES];  // the largest of longest()
     __device__ __forceinline__ int place(int p) {
         for (u32 i = (u32)p * 2654435761u >> 21;; i = (i + 1) % PLACES) {  // (twice as many places as requests: one is empty)
             const int at = atomicCAS(&page[i], -1, p);
@@ -192,6 +197,19 @@ struct Askers {
         }
     }
 };
+
+// A request as a number that is larger for longer rows, of equal ones for the first.
+__device__ __forceinline__ u64 longest(int len, int i) { return (u64)len << 32 | (u32)~i; }
+
+// The request that page e goes to so far, in its claim, against request i. Each exchange puts a larger one there: it ends.
+__device__ __forceinline__ void claim_page(const Pool& p, const Room& r, int e, int len, int i) {
+    int cur = load_agent(&p.claim[e]);
+    while (cur == INT_MAX || longest(len, i) > longest(row_len(r, cur / r.per), cur)) {
+        const int was = atomicCAS(&p.claim[e], cur, i);
+        if (was == cur) break;
+        cur = was;
+    }
+}
 
 // ONE: no more than 1024 requests, each in its thread's registers throughout; else they are read again in each phase (1024
 // requests so: 11.0 us against 8.2).
@@ -209,13 +227,13 @@ template <bool ONE> __global__ __launch_bounds__(1024) void pool_room_k(const Po
     int place = 0;
     // who else asks for a shared page
     if constexpr (ONE) {
-        for (int i = tid; i < PLACES; i += 1024) askers->page[i] = -1, askers->count[i] = 0, askers->first[i] = INT_MAX;
+        for (int i = tid; i < PLACES; i += 1024) askers->page[i] = -1, askers->count[i] = 0, askers->best[i] = 0;
         if (tid < n) one = ask_of(p, r, tid), refs = one.refs;
         lds_barrier();
         if (one.held && refs != 1) {
             place = askers->place(one.entry);
             atomicAdd(&askers->count[place], 1);
-            atomicMin(&askers->first[place], tid);
+            atomicMax(&askers->best[place], longest(one.len, tid));
         }
         lds_barrier();
     } else {
@@ -223,7 +241,7 @@ template <bool ONE> __global__ __launch_bounds__(1024) void pool_room_k(const Po
             const Ask q = ask_of(p, r, i);
             if (q.held && q.refs != 1) {
                 atomicAdd(&p.asks[q.entry], 1);
-                atomicMin(&p.claim[q.entry], i);
+                claim_page(p, r, q.entry, q.len, i);
             }
         }
         __syncthreads();
@@ -236,7 +254,7 @@ template <bool ONE> __global__ __launch_bounds__(1024) void pool_room_k(const Po
         bool want = i < n && q.is;
         if (want && q.held) {
             const int refs = q.refs;
-            if (ONE) want = refs != 1 && !(refs == askers->count[place] && askers->first[place] == i);
+            if (ONE) want = refs != 1 && !(refs == askers->count[place] && askers->best[place] == longest(q.len, i));
             else want = refs != 1 && !(refs == load_agent(&p.asks[q.entry]) && load_agent(&p.claim[q.entry]) == i);
         }
         int total;
@@ -263,7 +281,7 @@ template <bool ONE> __global__ __launch_bounds__(1024) void pool_room_k(const Po
         int page = k == KEPT ? held : -1, source = -1;
         if (k >= 0 && k < found) {
             page = given[k];
-            r.table[s * r.stride + (ONE ? one.column : ((r.lengths[s] < 0 ? 0 : r.lengths[s]) >> r.shift) + j)] = page;
+            r.table[s * r.stride + (ONE ? one.column : (row_len(r, s) >> r.shift) + j)] = page;
             p.refs[page] = 1;
             atomicAnd(&p.free[page >> 5], ~(1u << (page & 31)));
             if (held >= 0) {
@@ -315,8 +333,8 @@ __device__ __forceinline__ void copy_bytes(const char* s, char* d, i64 bytes) { 
 // of 512 rows and 8 heads are on the card at once, and what they wait for one after the other they wait for together.)
 __global__ __launch_bounds__(128) void pool_slots_k(const Pool p, const Room r, const Parts c, i64* __restrict__ slots) {
     const int s = blockIdx.x / c.H, h = blockIdx.x - s * c.H;
-    const int l = r.lengths[s], from = r.source[s], to = r.page[s * r.per], own = row_count(r, s);
-    const int len = l < 0 ? 0 : l, in = (1 << r.shift) - 1;
+    const int len = row_len(r, s), from = r.source[s], to = r.page[s * r.per], own = row_count(r, s);
+    const int in = (1 << r.shift) - 1;
     if (h == 0)
         for (int i = threadIdx.x; i < r.count; i += 128) {
             const i64 pos = (i64)len + i;

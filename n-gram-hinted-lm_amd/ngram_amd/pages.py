@@ -93,7 +93,8 @@ class PagePool:
         """Room behind each row's tokens for `count` more (or counts[s], int32 [rows], held to 0 .. count): int64 [rows,
         count], their slots, -1 past a row's own count, past the table and where no page was to be had (`missing`). A page
         that others hold is left to them: the row gets another, with a copy of the rows before its length; where all that
-        hold it ask in this call, the first of them keeps it."""
+        hold it ask in this call, the longest of them keeps it, of equal ones the first, so that what it writes lies behind
+        the tokens of a row that gets none and is left with the shared page."""
         S, width = self._rows(table, lengths)
         if not 0 <= count < 1 << 30:
             raise ValueError(f"count must be 0 to 2^30 - 1: {count}")
