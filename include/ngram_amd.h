@@ -580,11 +580,17 @@ int ng_tree_mask(const int* parents, int B, int T, ng_u64* bits, void* stream);
  * max(length + 1, 1)^alpha; a finished beam has one, `pad` at its own score and length. out_scores, parents (b * W + w), tokens
  * [B, K]; out_finished bytes [B, K] (token == end, or a finished parent) or NULL; out_lengths [B, K] or NULL; work:
  * ng_beam_work(B, W, V, K) bytes (-1: out of range; W, K <= 128, V <= 2^25, K * V <= 2^27).
+ * ng_beam_step_alpha64: with the exponent in 64 bits (as a float 0.6 is 0.60000002: beams of different lengths whose ranks lie
+ * within 2^-22 of each other then come in another order).
  * ng_gather_rows: out row i = src row from[i], of `bytes` bytes at a multiple of `stride` bytes; zeros outside [0, rows). */
 ng_i64 ng_beam_work(ng_i64 B, ng_i64 W, ng_i64 V, ng_i64 K);
 int ng_beam_step(const void* logits, ng_i64 sb, ng_i64 sw, int dtype, const float* scores, const void* lengths,
                  int lsize, const void* finished, int B, int W, int V, int K, int end, int pad, float alpha, float* out_scores,
                  ng_i64* parents, ng_i64* tokens, void* out_finished, ng_i64* out_lengths, void* work, void* stream);
+int ng_beam_step_alpha64(const void* logits, ng_i64 sb, ng_i64 sw, int dtype, const float* scores, const void* lengths,
+                         int lsize, const void* finished, int B, int W, int V, int K, int end, int pad, double alpha,
+                         float* out_scores, ng_i64* parents, ng_i64* tokens, void* out_finished, ng_i64* out_lengths, void* work,
+                         void* stream);
 int ng_gather_rows(const void* src, ng_i64 stride, ng_i64 rows, ng_i64 bytes, const ng_i64* from, ng_i64 n, void* out,
                    void* stream);
 

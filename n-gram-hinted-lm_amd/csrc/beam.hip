@@ -455,13 +455,14 @@ template <typename T> static void beam_part(const BeamArgs& a, int E, hipStream_
     else beam_part_k<T, 8><<<grid, 256, 0, st>>>(a);
 }
 
-extern "C" int ng_beam_step(const void* logits, i64 sb, i64 sw, int dtype, const float* scores, const void* lengths,
-                            int lsize, const void* finished, int B, int W, int V, int K, int end, int pad, float alpha,
-                            float* out_scores, i64* parents, i64* tokens, void* out_finished, i64* out_lengths, void* work,
-                            void* stream) {
+extern "C" int ng_beam_step_alpha64(const void* logits, i64 sb, i64 sw, int dtype, const float* scores, const void* lengths,
+                                    int lsize, const void* finished, int B, int W, int V, int K, int end, int pad,
+                                    double alpha, float* out_scores, i64* parents, i64* tokens, void* out_finished,
+                                    i64* out_lengths, void* work, void* stream) {
     BeamPlan p;
-    if (!beam_plan(B, W, V, K, p) || dtype < NG_F32 || dtype > NG_F16 || !(alpha >= 0.f) || (out_lengths && !lengths) ||
-        (alpha != 0.f && !lengths) || (lengths && lsize != 4 && lsize != 8) || (finished && (pad < 0 || pad >= V)))
+    if (!beam_plan(B, W, V, K, p) || dtype < NG_F32 || dtype > NG_F16 || !(alpha >= 0. && alpha < __builtin_inf()) ||
+        (out_lengths && !lengths) ||
+        (alpha != 0. && !lengths) || (lengths && lsize != 4 && lsize != 8) || (finished && (pad < 0 || pad >= V)))
         return -1;
     if (B == 0) return 0;
     BeamArgs a;
@@ -493,6 +494,14 @@ extern "C" int ng_beam_step(const void* logits, i64 sb, i64 sw, int dtype, const
     else if (have <= 4096) beam_join_k<16, 4><<<B, 1024, 0, st>>>(a);
     else beam_join_k<16, 16><<<B, 1024, 0, st>>>(a);
     return (int)hipGetLastError();
+}
+
+extern "C" int ng_beam_step(const void* logits, i64 sb, i64 sw, int dtype, const float* scores, const void* lengths,
+                            int lsize, const void* finished, int B, int W, int V, int K, int end, int pad, float alpha,
+                            float* out_scores, i64* parents, i64* tokens, void* out_finished, i64* out_lengths, void* work,
+                            void* stream) {
+    return ng_beam_step_alpha64(logits, sb, sw, dtype, scores, lengths, lsize, finished, B, W, V, K, end, pad, alpha, out_scores,
+                                parents, tokens, out_finished, out_lengths, work, stream);
 }
 
 // Rows copied in a given order: out[i] = src[from[i]], zeros where that is no row. U: the unit of a copy; a block takes 256

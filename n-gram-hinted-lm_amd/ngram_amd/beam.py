@@ -17,13 +17,14 @@ synchronizes; everything runs on the current stream. csrc/beam.hip has the kerne
 from __future__ import annotations
 
 import functools
+import math
 from typing import NamedTuple, Sequence
 
 import torch
 from torch.autograd import forward_ad
 
 from .kvcache import DTYPES, refuse_gradients
-from .lib import Entry, Lib, float32
+from .lib import Entry, Lib
 
 MOST = 128  # beams of a sequence, and candidates kept
 
@@ -43,6 +44,11 @@ class BeamStep(NamedTuple):
 @functools.lru_cache(maxsize=None)
 def _entries() -> tuple[Entry, Entry]:
     return (Entry(name="ng_beam_step", types="pqqippipiiiiiifpppppp"), Entry(name="ng_gather_rows", types="pqqqpqp"))
+
+
+@functools.lru_cache(maxsize=None)
+def _step() -> Entry:
+    return Entry(name="ng_beam_step_alpha64", types="pqqippipiiiiiidpppppp")
 
 
 @functools.lru_cache(maxsize=1024)
@@ -86,9 +92,9 @@ def beam_step(logits: torch.Tensor, scores: torch.Tensor, lengths: torch.Tensor 
     pad = end if pad is None else pad
     if finished is not None and pad is None:
         raise ValueError("finished beams go on with a padding token: give end or pad")
-    alpha = float32("alpha", alpha)
-    if alpha < 0 or (alpha and lengths is None):
-        raise ValueError(f"alpha must be 0 or more, and needs lengths: {alpha}")
+    alpha = float(alpha)
+    if not 0 <= alpha < math.inf or (alpha and lengths is None):
+        raise ValueError(f"alpha must be finite, 0 or more, and needs lengths: {alpha}")
     if logits.requires_grad or scores.requires_grad or forward_ad._current_level >= 0:
         refuse_gradients("beam_step", logits, scores)
     gpu = logits.get_device()
@@ -106,10 +112,10 @@ def beam_step(logits: torch.Tensor, scores: torch.Tensor, lengths: torch.Tensor 
     grown = more[0] if more else None
     done = torch.empty(shape, dtype=torch.bool, device=device) if finished is not None or end is not None else None
     scratch = torch.empty(work, dtype=torch.uint8, device=device)
-    _entries()[0](gpu, logits.data_ptr(), logits.stride(0), logits.stride(1), DTYPES[dtype], scores.data_ptr(), _at(lengths),
-                  0 if lengths is None else lengths.element_size(), _at(finished), B, W, V, keep, -1 if end is None else end,
-                  -1 if pad is None else pad, alpha, out.data_ptr(), parents.data_ptr(), tokens.data_ptr(), _at(done),
-                  _at(grown), scratch.data_ptr())
+    _step()(gpu, logits.data_ptr(), logits.stride(0), logits.stride(1), DTYPES[dtype], scores.data_ptr(), _at(lengths),
+            0 if lengths is None else lengths.element_size(), _at(finished), B, W, V, keep, -1 if end is None else end,
+            -1 if pad is None else pad, alpha, out.data_ptr(), parents.data_ptr(), tokens.data_ptr(), _at(done), _at(grown),
+            scratch.data_ptr())
     return BeamStep(out, parents, tokens, done, grown)
 
 

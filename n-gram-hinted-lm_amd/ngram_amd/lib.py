@@ -131,13 +131,13 @@ def float32(name: str, x: float) -> float:
     return x
 
 
-_TYPES = {"p": _ptr, "q": _i64, "i": _i32, "f": ctypes.c_float}
+_TYPES = {"p": _ptr, "q": _i64, "i": _i32, "f": ctypes.c_float, "d": ctypes.c_double}
 
 
 class Entry:
     """One entry point with its argument types declared, for calls whose host time counts (ctypes then converts plain ints
     and floats itself): `Entry(name="ng_x", types="ppqi")` has a letter an argument before the stream, p a pointer (an address or
-    None), q int64, i int, f float. Called with the device's index first; the stream is that device's current one."""
+    None), q int64, i int, f float, d double. Called with the device's index first; the stream is that device's current one."""
 
     def __init__(self, name: str, types: str, path: str | Path | None = None):
         self.name, self.types = name, types
