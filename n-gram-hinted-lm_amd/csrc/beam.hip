@@ -12,9 +12,12 @@
 // candidates; where there are many, a block a row first leaves K of them.
 //
 // Precision. Candidates of different beams lie close to each other, so what decides between them is held in 64 bits: sums
-// over more than a thread's 32 elements, the logarithm, totals and ranks. An exponential is a 32-bit one: its argument's
-// rounding and the instruction's are off by 2^-20 of a term, and average out over a row's terms. (Putting each argument's
-// rounding back took 5 more operations an element: 20.5 us a chunk's pass against 17.3 for 64 x 8 rows of 50257.)
+// over more than a thread's 32 elements, the logarithm, totals and ranks (quotients, as they are defined: by the mean of its
+// tokens a beam of -n over n of them ranks -1 for every n, where a product with exp(-log n) is an ulp off for some, and beams of
+// equal ranks come in their order).
+// An exponential is a 32-bit one: its argument's rounding and the instruction's are off by 2^-20 of a term, and average out over
+// a row's terms. (Putting each argument's rounding back took 5 more operations an element: 20.5 us a chunk's pass against 17.3
+// for 64 x 8 rows of 50257.)
 //
 // Measured (in a trace, us): 64 x 8 rows of 50257 bfloat16 logits, a fifth of the beams finished (41 MB): chunks 17.7 (2.3
 // TB/s), joining 7.4; 8 x 32 rows of 100003 float32 ones, a tenth finished, 64 kept (92 MB): chunks 28 (3.3 TB/s), rows 7.1,
@@ -312,7 +315,8 @@ template <int NW, int E> __global__ __launch_bounds__(NW * 64) void beam_join_k(
         }
         if ((lane_id() & 15) == 0) {
             lses[w] = lse, scores[w] = score, done[w] = end;
-            norms[w] = a.alpha == 0. || len <= 1 ? 1. : exp(-a.alpha * log((double)len));
+            const double n = len > 1 ? (double)len : 1.;
+            norms[w] = a.alpha == 0. ? 1. : a.alpha == 1. ? n : pow(n, a.alpha);  // (pow(n, 1) is an ulp off n for some n)
         }
     }
     if (tid == 0) fill = 0;
@@ -327,8 +331,8 @@ template <int NW, int E> __global__ __launch_bounds__(NW * 64) void beam_join_k(
         if (i < have) {
             const int w = (int)((u32)i / (u32)per);
             const u64 c = done[w] ? 0ull : HOLD ? held[HOLD ? e : 0] : a.part[b * have + i];
-            if (c) key[e] = key_of((scores[w] + ((double)of_key((u32)(c >> 32)) - lses[w])) * norms[w]);
-            if (done[w] && i == w * per) key[e] = key_of(scores[w] * norms[w]);
+            if (c) key[e] = key_of((scores[w] + ((double)of_key((u32)(c >> 32)) - lses[w])) / norms[w]);
+            if (done[w] && i == w * per) key[e] = key_of(scores[w] / norms[w]);
             if ((u32)i % (u32)a.K == (u32)a.K - 1) full = key[e] > full ? key[e] : full;
         }
         mine = key[e] > mine ? key[e] : mine;

@@ -38,3 +38,11 @@ def test_ranks_of_an_example(gpu):
     scores = torch.tensor([[-16778.74609375, -384.02536]]).cuda()
     step = beam_step(torch.zeros((1, 2, 3)).cuda(), scores, _dev([[542, 1]]), torch.ones((1, 2), dtype=torch.bool).cuda(), end=0, alpha=0.6)
     assert step.parents.tolist() == [[1, 0]]
+
+
+def test_equal_ranks_of_different_lengths(gpu):
+    """Scores of -n over n tokens: all rank -1, and the lower beam comes first."""
+    n = torch.randperm(128, generator=torch.Generator().manual_seed(4))[None] + 1
+    step = beam_step(torch.zeros((1, 128, 3)).cuda(), -n.float().cuda(), n.cuda(), torch.ones((1, 128), dtype=torch.bool).cuda(), end=0,
+                     alpha=1.0)
+    assert step.parents[0].tolist() == list(range(128))
