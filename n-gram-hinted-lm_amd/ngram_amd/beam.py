@@ -103,8 +103,8 @@ def beam_step(logits: torch.Tensor, scores: torch.Tensor, lengths: torch.Tensor 
         lengths = _check("lengths", lengths, (B, W), torch.int32 if lengths.dtype == torch.int32 else torch.int64, gpu)
     if finished is not None:
         finished = _check("finished", finished, (B, W), torch.bool, gpu)
-    if logits.stride(2) != 1 and V > 1:
-        logits = logits.contiguous()
+    if logits.stride(2) != 1:
+        logits = logits.resolve_neg().contiguous()
     device, shape = logits.device, (B, keep)
     out = torch.empty(shape, dtype=torch.float32, device=device)
     # (one tensor's parts: an allocation costs a call of this size more than a view)
@@ -138,6 +138,8 @@ def _reordered(state: torch.Tensor, parents: torch.Tensor) -> torch.Tensor:
         raise ValueError(f"parents must be int64 on {state.device}: got {parents.dtype} on {parents.device}")
     if state.requires_grad or forward_ad._current_level >= 0:
         refuse_gradients("reorder", state)
+    if state.is_conj() or state.is_neg():  # (a bit of the tensor: its memory holds other values)
+        state = state.resolve_conj().resolve_neg()
     rows, rest, size = state.shape[0], state.shape[1:], state.element_size()
     row = rest.numel() * size
     if not state.is_contiguous() and rows and not state[0].is_contiguous():

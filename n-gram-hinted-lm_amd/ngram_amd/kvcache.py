@@ -123,7 +123,7 @@ class KVCache:
             raise ValueError(f"k and v must be on {self.k.device}")
         (kt, kh, kd), (vt, vh, vd) = k.stride(), v.stride()
         if kd != 1 or vd != 1:
-            k, v = k.contiguous(), v.contiguous()
+            k, v = k.resolve_neg().contiguous(), v.resolve_neg().contiguous()
             (kt, kh, _), (vt, vh, _) = k.stride(), v.stride()
         if k.requires_grad or v.requires_grad or forward_ad._current_level >= 0:
             refuse_gradients("KVCache.write", k, v)

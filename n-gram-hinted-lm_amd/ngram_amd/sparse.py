@@ -121,8 +121,8 @@ def sparse_attention(q: torch.Tensor, cache: KVCache, bounds: PageBounds, table:
         widths = _check("widths", widths, (B,), torch.int32, cache)
     scale = 1 / math.sqrt(dim) if scale is None else float32("scale", scale)
     qb, qt, qh, qd = q.stride()
-    if qd != 1 and dim > 1:
-        q = q.contiguous()
+    if qd != 1:  # (of one element a row, too, which torch calls contiguous and may have negated by a bit alone)
+        q = q.resolve_neg().contiguous()
         qb, qt, qh, _ = q.stride()
     device, group = cache.k.device, heads // cache.heads
     work = torch.empty(_work(B, T, cache.heads, group, dim, width, cache.page, keep), dtype=torch.uint8, device=device)

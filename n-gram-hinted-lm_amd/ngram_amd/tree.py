@@ -97,8 +97,8 @@ def tree_attention(q: torch.Tensor, cache: KVCache, table: torch.Tensor, lengths
         widths = _check("widths", widths, (B,), torch.int32, cache)
     scale = 1 / math.sqrt(dim) if scale is None else float32("scale", scale)
     qb, qt, qh, qd = q.stride()
-    if qd != 1 and dim > 1:
-        q = q.contiguous()
+    if qd != 1:  # (of one element a row, too, which torch calls contiguous and may have negated by a bit alone)
+        q = q.resolve_neg().contiguous()
         qb, qt, qh, _ = q.stride()
     device, group = cache.k.device, heads // cache.heads
     out = torch.empty(size, dtype=dtype, device=device)
