@@ -2,7 +2,7 @@
 //
 //   bounds[page, head]   (min, max) over the page's keys of each element, outward to bfloat16
 //   score(token, head, page) = sum over the group's query heads g and elements d of max(q[g, d] lo[d], q[g, d] hi[d])
-//                            = sum_d (sum_g max(q[g, d], 0)) hi[d] + (sum_g min(q[g, d], 0)) lo[d]
+//                            = sum_d (sum_g max(q[g, d], 0)) hi[d] + (sum_g min(q[g, d], 0)) lo[d],  a zero counting nothing
 //   kept: of the pages that hold positions 0 .. the token's own, the first and the last ones and the best others
 //   o = softmax attention over the kept pages' keys at positions up to the token's own
 //
@@ -76,6 +76,10 @@ __device__ __forceinline__ u64 score_key(bool is, double x) {
 __device__ __forceinline__ double low(u32 w) { return (double)__uint_as_float(w << 16); }
 __device__ __forceinline__ double high(u32 w) { return (double)__uint_as_float(w & 0xFFFF0000u); }
 
+// A sum of queries of one sign times a bound. Without such queries nothing of the bound counts: 0 where it is infinite, too
+// (its product with 0 is NaN; sums that come out as NaN are taken again so).
+__device__ __forceinline__ double times(double q, double x) { return q == 0. && __builtin_isinf(x) ? 0. : q * x; }
+
 // A token's scores of pages from .. stop - 1, by a block of NT: GS lanes a page, each of 8 elements, 4 pages at a time. put
 // takes those that are wanted.
 template <int DP, int GS, int NT, typename F>
@@ -135,6 +139,16 @@ __device__ __forceinline__ void score_one(const ScoreArgs& a, const Place& p, in
                 acc[u] = fma(down[j], x, fma(up[j], y, acc[u]));
             }
         }
+        // (the bounds are read again: held for this they would cost every call 20 registers)
+        if (__any(acc[0] != acc[0] || acc[1] != acc[1] || acc[2] != acc[2] || acc[3] != acc[3]))
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                if (!is[u] || acc[u] == acc[u]) continue;
+                const b16* x = a.bounds + ((i64)e[u] * a.H + p.h) * 2 * DP + d0;
+                acc[u] = 0.;
+#pragma unroll
+                for (int j = 0; j < 8; ++j) acc[u] += times(down[j], (double)(float)x[j]) + times(up[j], (double)(float)x[DP + j]);
+            }
         // the four pages' sums over the lanes, each step for half as many pages: a quarter of the lanes ends with each
         const bool a1 = sub & (GS / 2), a2 = sub & (GS / 4);
         double x = (a1 ? acc[2] : acc[0]) + __shfl_xor(a1 ? acc[0] : acc[2], GS / 2, GS);
@@ -240,7 +254,7 @@ template <int DP, int TT> __global__ __launch_bounds__(256, DP <= 128 ? 4 : 2) v
     uint4 lo = *(const uint4*)x, hi = *(const uint4*)(x + DP);
     for (int j0 = from + wave * 16; j0 < stop; j0 += 64) {
         const bool is = (u32)e < (u64)a.pages;
-        const b16* then = page(next);
+        const b16 *now = page(e) - g * 8, *then = page(next);
         e = next, next = entry(j0 + 128);
         typename Sums<TT>::type acc = {}, more = {};
 #pragma unroll 1
@@ -260,8 +274,16 @@ template <int DP, int TT> __global__ __launch_bounds__(256, DP <= 128 ? 4 : 2) v
         const int j = j0 + c;  // this lane's page; its tokens: 4 r + g
 #pragma unroll
         for (int r = 0; r < TT / 4; ++r)
-            if (j >= a.first && j < ends[r])
-                out[(i64)r * 4 * a.H * a.width + j] = score_key(is, Sums<TT>::at(acc, r) + Sums<TT>::at(more, r));
+            if (j >= a.first && j < ends[r]) {
+                double x = Sums<TT>::at(acc, r) + Sums<TT>::at(more, r);
+                if (is && x != x) {
+                    const double *up = sums + (4 * r + g) * LD, *down = up + DP;
+                    x = 0.;
+#pragma unroll 1
+                    for (int d = 0; d < a.dim; ++d) x += times(down[d], (double)(float)now[d]) + times(up[d], (double)(float)now[DP + d]);
+                }
+                out[(i64)r * 4 * a.H * a.width + j] = score_key(is, x);
+            }
     }
 }
 

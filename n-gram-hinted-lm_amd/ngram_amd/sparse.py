@@ -6,8 +6,8 @@ of the cache no longer grows with the context.
   sparse_attention(q, cache, bounds, table, lengths, keep, ...)
 
 A page's bounds are the smallest and largest of each element of its keys, per head. Its score for a token is the sum over
-the query heads that share a cached head of sum_d max(q_d smallest_d, q_d largest_d): no key of the page has a larger sum of
-products with them. Of the pages that hold positions up to its own, a token keeps the `first` and the `last` ones (the last
+the query heads that share a cached head of sum_d max(q_d smallest_d, q_d largest_d), a q_d of 0 counting nothing: no key of
+the page has a larger sum of products with them. Of the pages that hold positions up to its own, a token keeps the `first` and the `last` ones (the last
 is its own page, which may be incomplete) and the best-scoring others, `keep` in all, for each cached head; equal scores go
 to the lower page. A page whose score is NaN is kept first, one that is no page of the cache last (its keys are masked).
 
