@@ -62,29 +62,43 @@ __global__ __launch_bounds__(256) void pool_hold_k(const Pool p, const int* __re
 
 #define STRIP 2048  // a block's columns
 
+// Each row's children, in the places of the lengths to come.
+__global__ __launch_bounds__(256) void pool_zero_k(int* __restrict__ x, int n) {
+    const int i = blockIdx.x * 256 + threadIdx.x;
+    if (i < n) x[i] = 0;
+}
+__global__ __launch_bounds__(256) void pool_children_k(const i64* __restrict__ parents, int S, int* __restrict__ children) {
+    const int i = blockIdx.x * 256 + threadIdx.x;
+    if (i < S && (u64)parents[i] < (u64)S) atomicAdd(&children[parents[i]], 1);
+}
+
+// A block a row. COUNTED: its children are counted already (the count is read before the length goes in its place); else it
+// finds them among all the parents.
+template <bool COUNTED>
 __global__ __launch_bounds__(256) void pool_fork_k(const Pool p, const int* __restrict__ table, i64 stride, int S, int width,
                                                    const int* __restrict__ lengths, const i64* __restrict__ parents,
-                                                   int* __restrict__ moved, int* __restrict__ moved_len) {
+                                                   int* __restrict__ moved, int* moved_len) {
     __shared__ int children;
     const int s = blockIdx.x, tid = threadIdx.x;
-    if (tid == 0) children = 0;
+    if (tid == 0) children = COUNTED ? moved_len[s] : 0;
     __syncthreads();
-    int n = 0;
-    for (int i = tid; i < S; i += 256) n += parents[i] == s;
-    if (n) atomicAdd(&children, n);
-    __syncthreads();
+    if constexpr (!COUNTED) {
+        int n = 0;
+        for (int i = tid; i < S; i += 256) n += parents[i] == s;
+        if (n) atomicAdd(&children, n);
+        __syncthreads();
+    }
     const int change = children - 1;
     const i64 from = parents[s];
     const bool is = (u64)from < (u64)S;
-    const int c1 = (blockIdx.y + 1) * STRIP < width ? (blockIdx.y + 1) * STRIP : width;
-    for (int c = blockIdx.y * STRIP + tid; c < c1; c += 256) {
+    for (int c = tid; c < width; c += 256) {
         if (change) {
             const int e = table[s * stride + c];
             if (is_page(p, e) && atomicAdd(&p.refs[e], change) + change == 0) atomicOr(&p.free[e >> 5], 1u << (e & 31));
         }
         if (from != s) moved[(i64)s * width + c] = is ? table[from * stride + c] : -1;
     }
-    if (blockIdx.y == 0 && tid == 0) moved_len[s] = is ? lengths[from] : 0;
+    if (tid == 0) moved_len[s] = is ? lengths[from] : 0;
 }
 
 // Up to MANY rows: a block takes a strip of columns of all rows, which go through its LDS (512 rows of 65 entries: 6.7 us; by
@@ -480,7 +494,15 @@ extern "C" int ng_pool_fork(void* state, i64 pages, int* table, i64 stride, int 
     int* moved_len = moved + (i64)S * width;
     const dim3 grid(S, (width + STRIP - 1) / STRIP);
     hipStream_t st = (hipStream_t)stream;
-    pool_fork_k<<<grid, 256, 0, st>>>(p, table, stride, S, width, lengths, parents, moved, moved_len);
+    // Looking for the children costs rows squared, counting them two launches: 2048 rows of 65 entries 18.7 and 21.9 us, 4096
+    // 28.5 and 27.4, 16384 160 and 59, 65536 of 17 1880 and 78, 262144 of 2 28600 and 245.
+    if (S <= 4096) pool_fork_k<false><<<S, 256, 0, st>>>(p, table, stride, S, width, lengths, parents, moved, moved_len);
+    else {
+        const unsigned blocks = (S + 255) / 256;
+        pool_zero_k<<<blocks, 256, 0, st>>>(moved_len, S);
+        pool_children_k<<<blocks, 256, 0, st>>>(parents, S, moved_len);
+        pool_fork_k<true><<<S, 256, 0, st>>>(p, table, stride, S, width, lengths, parents, moved, moved_len);
+    }
     const int rc = (int)hipGetLastError();
     if (rc) return rc;
     pool_moved_k<<<grid, 256, 0, st>>>(table, stride, width, lengths, parents, moved, moved_len);
