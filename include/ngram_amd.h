@@ -576,10 +576,11 @@ int ng_tree_attention(const void* q, ng_i64 qb, ng_i64 qt, ng_i64 qh, int qtype,
 int ng_tree_mask(const int* parents, int B, int T, ng_u64* bits, void* stream);
 
 /* A beam search's step: of the candidates of W beams (logits [B, W, V] of dtype, strides sb, sw in elements; scores float32
- * [B, W]; lengths [B, W] of lsize bytes (4, 8) or NULL; finished bytes [B, W] or NULL) the K best, ranked by (score + logit - log sum exp) /
- * max(length + 1, 1)^alpha; a finished beam has one, `pad` at its own score and length. out_scores, parents (b * W + w), tokens
- * [B, K]; out_finished bytes [B, K] (token == end, or a finished parent) or NULL; out_lengths [B, K] or NULL; work:
- * ng_beam_work(B, W, V, K) bytes (-1: out of range; W, K <= 128, V <= 2^25, K * V <= 2^27).
+ * [B, W]; lengths [B, W] of lsize bytes (4, 8) or NULL; finished bytes [B, W] or NULL) the K best, ranked by (score + logit -
+ * log sum exp) / max(length + 1, 1)^alpha; a finished beam has one, `pad` at its own score and length. out_scores, parents
+ * (b * W + w), tokens [B, K]; out_finished bytes [B, K] (token == end, or a finished parent) or NULL; out_lengths [B, K] or
+ * NULL; work: ng_beam_work(B, W, V, K) bytes (-1: out of range; B <= 2^24, W, K <= 128, V <= 2^25, K <= W * V, K * ceil(V /
+ * 8192) <= 16384, B * W * ceil(V / 8192) < 2^31).
  * ng_beam_step_alpha64: with the exponent in 64 bits (as a float 0.6 is 0.60000002: beams of different lengths whose ranks lie
  * within 2^-22 of each other then come in another order).
  * ng_gather_rows: out row i = src row from[i], of `bytes` bytes at a multiple of `stride` bytes; zeros outside [0, rows). */

@@ -55,8 +55,8 @@ def _step() -> Entry:
 def _work(B: int, W: int, V: int, K: int) -> int:
     n = Lib().size("ng_beam_work", B, W, V, K)
     if n < 0:
-        raise ValueError(f"{B} sequences of {W} beams, {V} tokens, {K} kept: at most {MOST} beams and {MOST} kept, kept * tokens "
-                         "at most 2^27")
+        raise ValueError(f"{B} sequences of {W} beams, {V} tokens, {K} kept: at most 2^24 sequences, {MOST} beams and {MOST} "
+                         "kept, 2^25 tokens, kept * ceil(tokens / 8192) at most 16384, and B * W * ceil(tokens / 8192) below 2^31")
     return n
 
 
@@ -69,7 +69,8 @@ def _check(name: str, t: torch.Tensor, shape: tuple, dtype: torch.dtype, device:
 def beam_step(logits: torch.Tensor, scores: torch.Tensor, lengths: torch.Tensor | None = None,
               finished: torch.Tensor | None = None, keep: int | None = None, end: int | None = None, pad: int | None = None,
               alpha: float = 0.0) -> BeamStep:
-    """The `keep` best candidates (W by default) of each of B sequences' W beams.
+    """The `keep` best candidates (W by default) of each of B sequences' W beams: at most 2^25 tokens, and keep * ceil(V / 8192)
+    at most 16384 (every keep up to 128 over 2^20 tokens).
 
     logits    [B, W, V] in float32, bfloat16 or float16, any strides over sequences and beams
     scores    float32 [B, W]: the beams' scores so far

@@ -40,3 +40,18 @@ def test_exponents_refused_before_a_launch(step):
         for B in (0, 1):
             with pytest.raises(RuntimeError, match="returned -1"):
                 call(B, alpha, lengths)
+
+
+@pytest.mark.parametrize("V", [1, 8192, 8193, 50257, (1 << 20) - 1, 1 << 20, (1 << 20) + 1, 1056831, 3_000_000, 1 << 25, (1 << 25) + 1])
+def test_stated_limits(step, V):
+    """Sizes are taken up to the limits that the header and the refusal state, and no further."""
+    chunks = -(-V // 8192)
+    for B, W in ((0, 1), (1, 1), (1, 128), (1, 129), (1 << 24, 1), ((1 << 24) + 1, 1), (1 << 24, 128), (1 << 20, 64), (4, 8)):
+        for K in (1, 2, 4, 5, 63, 64, 100, 126, 127, 128, 129):
+            within = (B <= 1 << 24 and W <= 128 and K <= 128 and V <= 1 << 25 and K <= W * V and K * chunks <= 16384
+                      and B * W * chunks < 1 << 31)
+            size = lib.Lib().size("ng_beam_work", B, W, V, K)
+            assert (size >= 0) == within, (B, W, V, K)
+            if not within:
+                with pytest.raises(ValueError, match="16384"):
+                    beam._work(B, W, V, K)
