@@ -45,6 +45,7 @@ struct BeamArgs {
     double* sum;    // [B * W, chunks]
     int B, W, V, K, chunks, lsize;
     int end, pad;   // -1: none
+    i64 row0;       // the rows before this launch's first
     double alpha;
 };
 
@@ -376,7 +377,7 @@ template <int NW, int E> __global__ __launch_bounds__(NW * 64) void beam_join_k(
     __syncthreads();
     auto put = [&](int r, int w, int token, float score) {
         const i64 o = b * a.K + r;
-        a.out_scores[o] = score, a.parents[o] = b * a.W + w, a.tokens[o] = token;
+        a.out_scores[o] = score, a.parents[o] = a.row0 + b * a.W + w, a.tokens[o] = token;
         if (a.out_finished) a.out_finished[o] = done[w] || token == a.end;
         if (a.out_lengths) a.out_lengths[o] = length_of(a, b * a.W + w) + (done[w] ? 0 : 1);
     };
@@ -420,8 +421,12 @@ template <int NW, int E> __global__ __launch_bounds__(NW * 64) void beam_join_k(
 struct BeamPlan {
     int E, chunks;
     bool merge;
+    i64 nb;                                    // sequences a launch
     i64 part, top, sum, rows, row_sum, bytes;  // offsets in the workspace
 };
+
+// A launch has fewer than 2^32 threads: as many sequences at a time as leave blocks of 1024 fewer than that.
+#define MOST_BLOCKS (((i64)1 << 22) - 1)
 
 // A chunk is 8192 logits, or fewer where that leaves less than 1024 blocks (4 a CU): 4 rows of 50257 take 5.9 us and 6.5 of
 // joining in chunks of 2048, 7.5 and 5.4 in chunks of 8192; 256 rows of 100003 34 us in chunks of 4096, 29 in chunks of 8192.
@@ -437,12 +442,13 @@ static bool beam_plan(i64 B, i64 W, i64 V, i64 K, BeamPlan& p) {
     if (chunks * K > 16384 || B * W * chunks >= (i64)1 << 31) return false;
     p.chunks = (int)chunks;
     p.merge = W * chunks * K > 4096;
-    const i64 n = B * W * chunks;
+    p.nb = B < MOST_BLOCKS / (W * chunks) ? B : MOST_BLOCKS / (W * chunks);
+    const i64 n = p.nb * W * chunks;
     p.part = 0;
     p.sum = p.part + n * K * 8;
     p.rows = p.sum + n * 8;
-    p.row_sum = p.rows + (p.merge ? B * W * K * 8 : 0);
-    p.top = p.row_sum + (p.merge ? B * W * 8 : 0);
+    p.row_sum = p.rows + (p.merge ? p.nb * W * K * 8 : 0);
+    p.top = p.row_sum + (p.merge ? p.nb * W * 8 : 0);
     p.bytes = p.top + n * 4;
     return true;
 }
@@ -453,30 +459,13 @@ extern "C" i64 ng_beam_work(i64 B, i64 W, i64 V, i64 K) {
 }
 
 template <typename T> static void beam_part(const BeamArgs& a, int E, hipStream_t st) {
-    const unsigned grid = (unsigned)((i64)a.B * a.W * a.chunks);
+    const unsigned grid = (unsigned)(a.B * a.W * a.chunks);
     if (E == 32) beam_part_k<T, 32><<<grid, 256, 0, st>>>(a);
     else if (E == 16) beam_part_k<T, 16><<<grid, 256, 0, st>>>(a);
     else beam_part_k<T, 8><<<grid, 256, 0, st>>>(a);
 }
 
-extern "C" int ng_beam_step_alpha64(const void* logits, i64 sb, i64 sw, int dtype, const float* scores, const void* lengths,
-                                    int lsize, const void* finished, int B, int W, int V, int K, int end, int pad,
-                                    double alpha, float* out_scores, i64* parents, i64* tokens, void* out_finished,
-                                    i64* out_lengths, void* work, void* stream) {
-    BeamPlan p;
-    if (!beam_plan(B, W, V, K, p) || dtype < NG_F32 || dtype > NG_F16 || !(alpha >= 0. && alpha < __builtin_inf()) ||
-        (out_lengths && !lengths) ||
-        (alpha != 0. && !lengths) || (lengths && lsize != 4 && lsize != 8) || (finished && (pad < 0 || pad >= V)))
-        return -1;
-    if (B == 0) return 0;
-    BeamArgs a;
-    char* w = (char*)work;
-    a.logits = logits, a.sb = sb, a.sw = sw, a.scores = scores, a.lengths = lengths, a.lsize = lsize;
-    a.finished = (const unsigned char*)finished, a.out_scores = out_scores, a.parents = parents, a.tokens = tokens;
-    a.out_finished = (unsigned char*)out_finished, a.out_lengths = out_lengths;
-    a.part = (u64*)(w + p.part), a.top = (float*)(w + p.top), a.sum = (double*)(w + p.sum);
-    a.B = B, a.W = W, a.V = V, a.K = K, a.chunks = p.chunks, a.end = end, a.pad = pad, a.alpha = alpha;
-    hipStream_t st = (hipStream_t)stream;
+static int beam_launch(BeamArgs a, const BeamPlan& p, int dtype, char* w, hipStream_t st) {
     switch (dtype) {
         case NG_F32: beam_part<float>(a, p.E, st); break;
         case NG_BF16: beam_part<b16>(a, p.E, st); break;
@@ -487,17 +476,47 @@ extern "C" int ng_beam_step_alpha64(const void* logits, i64 sb, i64 sw, int dtyp
     if (p.merge) {
         u64* rows = (u64*)(w + p.rows);
         double* lses = (double*)(w + p.row_sum);
-        if (a.chunks * K <= 1024) beam_row_k<4, 4><<<(unsigned)(B * W), 256, 0, st>>>(a, rows, lses);
-        else beam_row_k<16, 16><<<(unsigned)(B * W), 1024, 0, st>>>(a, rows, lses);
+        const unsigned grid = (unsigned)(a.B * a.W);
+        if (a.chunks * a.K <= 1024) beam_row_k<4, 4><<<grid, 256, 0, st>>>(a, rows, lses);
+        else beam_row_k<16, 16><<<grid, 1024, 0, st>>>(a, rows, lses);
         if ((rc = (int)hipGetLastError())) return rc;
         a.part = rows, a.top = nullptr, a.sum = lses, a.chunks = 1;
     }
-    const int have = W * a.chunks * K;
-    if (have <= 1024) beam_join_k<4, 4><<<B, 256, 0, st>>>(a);
-    else if (have <= 2048) beam_join_k<8, 4><<<B, 512, 0, st>>>(a);
-    else if (have <= 4096) beam_join_k<16, 4><<<B, 1024, 0, st>>>(a);
-    else beam_join_k<16, 16><<<B, 1024, 0, st>>>(a);
+    const int have = a.W * a.chunks * a.K;
+    if (have <= 1024) beam_join_k<4, 4><<<a.B, 256, 0, st>>>(a);
+    else if (have <= 2048) beam_join_k<8, 4><<<a.B, 512, 0, st>>>(a);
+    else if (have <= 4096) beam_join_k<16, 4><<<a.B, 1024, 0, st>>>(a);
+    else beam_join_k<16, 16><<<a.B, 1024, 0, st>>>(a);
     return (int)hipGetLastError();
+}
+
+extern "C" int ng_beam_step_alpha64(const void* logits, i64 sb, i64 sw, int dtype, const float* scores, const void* lengths,
+                                    int lsize, const void* finished, int B, int W, int V, int K, int end, int pad,
+                                    double alpha, float* out_scores, i64* parents, i64* tokens, void* out_finished,
+                                    i64* out_lengths, void* work, void* stream) {
+    BeamPlan p;
+    if (!beam_plan(B, W, V, K, p) || dtype < NG_F32 || dtype > NG_F16 || !(alpha >= 0. && alpha < __builtin_inf()) ||
+        (out_lengths && !lengths) || (alpha != 0. && !lengths) || (lengths && lsize != 4 && lsize != 8) ||
+        (finished && (pad < 0 || pad >= V)))
+        return -1;
+    hipStream_t st = (hipStream_t)stream;
+    for (i64 b0 = 0; b0 < B; b0 += p.nb) {
+        BeamArgs a;
+        const i64 r0 = b0 * W, o = b0 * K;
+        char* w = (char*)work;
+        a.logits = (const char*)logits + b0 * sb * (dtype == NG_F32 ? 4 : 2), a.sb = sb, a.sw = sw, a.scores = scores + r0;
+        a.lengths = lengths ? (const char*)lengths + r0 * lsize : nullptr, a.lsize = lsize;
+        a.finished = finished ? (const unsigned char*)finished + r0 : nullptr;
+        a.out_scores = out_scores + o, a.parents = parents + o, a.tokens = tokens + o;
+        a.out_finished = out_finished ? (unsigned char*)out_finished + o : nullptr;
+        a.out_lengths = out_lengths ? out_lengths + o : nullptr;
+        a.part = (u64*)(w + p.part), a.top = (float*)(w + p.top), a.sum = (double*)(w + p.sum);
+        a.B = (int)(B - b0 < p.nb ? B - b0 : p.nb), a.W = W, a.V = V, a.K = K, a.chunks = p.chunks, a.end = end, a.pad = pad;
+        a.alpha = alpha, a.row0 = r0;
+        const int rc = beam_launch(a, p, dtype, w, st);
+        if (rc) return rc;
+    }
+    return 0;
 }
 
 extern "C" int ng_beam_step(const void* logits, i64 sb, i64 sw, int dtype, const float* scores, const void* lengths,
@@ -535,15 +554,19 @@ extern "C" int ng_gather_rows(const void* src, i64 stride, i64 rows, i64 bytes, 
     i64 parts = (units + 1023) / 1024;
     const i64 most = (16384 + n - 1) / n;
     parts = parts < most ? parts : most;
-    if (parts * n >= (i64)1 << 31) parts = 1;
     hipStream_t st = (hipStream_t)stream;
-    const unsigned grid = (unsigned)(parts * n);
+    const i64 step = MOST_BLOCKS / parts;  // (parts is 16384 at most)
+    for (i64 i0 = 0; i0 < n; i0 += step, from += step, out = (char*)out + step * bytes) {
+        const unsigned grid = (unsigned)(parts * (n - i0 < step ? n - i0 : step));
 #define GATHER(U) gather_rows_k<U><<<grid, 256, 0, st>>>((const char*)src, stride, rows, from, units, (int)parts, (char*)out)
-    typedef u32 words __attribute__((ext_vector_type(4)));
-    if (size == 16) GATHER(words);
-    else if (size == 4) GATHER(u32);
-    else if (size == 2) GATHER(u16);
-    else GATHER(unsigned char);
+        typedef u32 words __attribute__((ext_vector_type(4)));
+        if (size == 16) GATHER(words);
+        else if (size == 4) GATHER(u32);
+        else if (size == 2) GATHER(u16);
+        else GATHER(unsigned char);
 #undef GATHER
-    return (int)hipGetLastError();
+        const int rc = (int)hipGetLastError();
+        if (rc) return rc;
+    }
+    return 0;
 }
