@@ -345,8 +345,9 @@ __device__ __forceinline__ void copy_bytes(const char* s, char* d, i64 bytes) { 
 
 // A block per (row, head): the slots of the row's positions (head 0), and the rows of a copied page. (128 threads: the blocks
 // of 512 rows and 8 heads are on the card at once, and what they wait for one after the other they wait for together.)
-__global__ __launch_bounds__(128) void pool_slots_k(const Pool p, const Room r, const Parts c, i64* __restrict__ slots) {
-    const int s = blockIdx.x / c.H, h = blockIdx.x - s * c.H;
+__global__ __launch_bounds__(128) void pool_slots_k(const Pool p, const Room r, const Parts c, i64* __restrict__ slots,
+                                                    int s0) {
+    const int at = blockIdx.x / c.H, h = blockIdx.x - at * c.H, s = s0 + at;
     const int len = row_len(r, s), from = r.source[s], to = r.page[s * r.per], own = row_count(r, s);
     const int in = (1 << r.shift) - 1;
     if (h == 0)
@@ -385,23 +386,24 @@ __global__ __launch_bounds__(128) void pool_slots_k(const Pool p, const Room r, 
     }
 }
 
-// Page dst[i] of one cache := page src[i] of another, in pieces of PIECE bytes; entries that are no pages are passed over.
-// (src NULL: the list of `from`'s live pages, packed.)
+// Page dst[i] of one cache := page src[i] of another, in pieces of PIECE bytes, from i0 on; entries that are no pages are passed
+// over. (dst NULL: page i, for a move's list of live pages.)
 #define PIECE 65536
 template <typename I>
-__global__ __launch_bounds__(256) void copy_pages_k(const Parts c, const I* __restrict__ src, const I* __restrict__ dst, i64 n,
-                                                    int pieces) {
-    const i64 i = blockIdx.x / pieces;
-    const int piece = (int)(blockIdx.x - i * pieces);
+__global__ __launch_bounds__(256) void copy_pages_k(const Parts c, const I* __restrict__ src, const I* __restrict__ dst,
+                                                    i64 i0, int pieces) {
+    const u32 at = blockIdx.x / (u32)pieces;
+    const i64 i = i0 + at;
+    const int piece = (int)(blockIdx.x - at * pieces);
     const i64 a = src[i], b = dst ? (i64)dst[i] : i;
     if ((u64)a >= (u64)c.src_pages || (u64)b >= (u64)c.dst_pages) return;
-    i64 at = (i64)piece * PIECE, end = at + PIECE;
+    i64 from = (i64)piece * PIECE, end = from + PIECE;
     for (int k = 0; k < c.n; ++k) {  // the parts laid end to end
         const Part& t = c.part[k];
         const i64 size = t.bytes * c.H << (k < 4 ? c.shift : 0);
-        const i64 x = at < 0 ? 0 : at, y = end < size ? end : size;
+        const i64 x = from < 0 ? 0 : from, y = end < size ? end : size;
         if (x < y) copy_bytes(t.src + a * size + x, t.dst + b * size + x, y - x);
-        at -= size, end -= size;
+        from -= size, end -= size;
         if (end <= 0) break;
     }
 }
@@ -451,6 +453,8 @@ static bool pool_of(void* state, i64 pages, Pool& p) {
     return true;
 }
 
+#define MOST_BLOCKS (((i64)1 << 24) - 1)  // of a launch, of up to 256 threads: fewer than 2^32 in all
+
 static int some_blocks(i64 n) {
     const int g = grid_for(n, 256);
     return g < 2048 ? g : 2048;
@@ -474,7 +478,7 @@ extern "C" int ng_pool_hold(void* state, i64 pages, const int* table, i64 stride
 }
 
 extern "C" i64 ng_pool_fork_work(i64 S, i64 width) {
-    if (S < 0 || width < 1 || S > 1 << 24 || width > 1 << 26 || S * width >= (i64)1 << 40) return -1;
+    if (S < 0 || width < 1 || S > MOST_BLOCKS || width > 1 << 26 || S * width >= (i64)1 << 40) return -1;
     return S <= MANY ? 0 : (S * width + S) * 4;
 }
 
@@ -542,7 +546,7 @@ extern "C" int ng_pool_room(void* state, i64 pages, int* table, i64 stride, int 
     const void* const src[5] = {k, v, ks, vs, nullptr};
     void* const dst[5] = {k, v, ks, vs, nullptr};
     if (!pool_of(state, pages, p) || S < 0 || width < 1 || ng_pool_room_work(S, count, page) < 0 ||
-        !parts_of(src, dst, pages, pages, page, heads, dim, codes, c) || (i64)S * heads >= (i64)1 << 31)
+        !parts_of(src, dst, pages, pages, page, heads, dim, codes, c) || heads > MOST_BLOCKS)
         return -1;
     if (S == 0) return 0;
     Room r;
@@ -555,8 +559,14 @@ extern "C" int ng_pool_room(void* state, i64 pages, int* table, i64 stride, int 
     else pool_room_k<false><<<1, 1024, 0, st>>>(p, r);
     const int rc = (int)hipGetLastError();
     if (rc) return rc;
-    pool_slots_k<<<(unsigned)(S * heads), 128, 0, st>>>(p, r, c, slots);
-    return (int)hipGetLastError();
+    const i64 most = MOST_BLOCKS / heads;  // rows a launch
+    for (i64 s0 = 0; s0 < S; s0 += most) {
+        const i64 rows = S - s0 < most ? S - s0 : most;
+        pool_slots_k<<<(unsigned)(rows * heads), 128, 0, st>>>(p, r, c, slots, (int)s0);
+        const int rc = (int)hipGetLastError();
+        if (rc) return rc;
+    }
+    return 0;
 }
 
 static i64 page_pieces(const Parts& c, bool bounds) {
@@ -569,9 +579,15 @@ static i64 page_pieces(const Parts& c, bool bounds) {
 template <typename I> static int copy_list(Parts c, bool bounds, const I* src, const I* dst, i64 n, hipStream_t st) {
     const i64 pieces = page_pieces(c, bounds);
     if (bounds) c.n = 5;  // (a 16-bit cache's scales have rows of no bytes)
-    if (n * pieces >= (i64)1 << 31) return -1;
-    copy_pages_k<I><<<(unsigned)(n * pieces), 256, 0, st>>>(c, src, dst, n, (int)pieces);
-    return (int)hipGetLastError();
+    if (pieces > MOST_BLOCKS) return -1;
+    const i64 most = MOST_BLOCKS / pieces;  // pages a launch
+    for (i64 i0 = 0; i0 < n; i0 += most) {
+        const i64 pages = n - i0 < most ? n - i0 : most;
+        copy_pages_k<I><<<(unsigned)(pages * pieces), 256, 0, st>>>(c, src, dst, i0, (int)pieces);
+        const int rc = (int)hipGetLastError();
+        if (rc) return rc;
+    }
+    return 0;
 }
 
 extern "C" int ng_copy_pages(const void* k, const void* v, const void* ks, const void* vs, const void* bounds, i64 pages,
