@@ -191,8 +191,8 @@ __global__ __launch_bounds__(256) void bounds_k(const void* __restrict__ k, cons
     const int h = (int)(item - page * H);
     int e = -1;
     if (item < items) {
-        const i64 from = start[b], column = (from >> shift) + (page - b * per);
-        if (column >= 0 && (column + 1) << shift <= from + count && column < width) e = table[b * stride + column];
+        const i64 from = start[b], column = (from < 0 ? 0 : from >> shift) + (page - b * per);
+        if ((column + 1) << shift <= from + count && column < width) e = table[b * stride + column];
     }
     if ((u32)e >= (u64)pages) return;  // (all waves of a page)
     const int r0 = part * R + l / L, d0 = l % L * E;
@@ -307,25 +307,30 @@ __global__ __launch_bounds__(256) void bounds_k(const void* __restrict__ k, cons
 template <int CODES> int bounds_codes(const void* k, const float* ks, i64 pages, int shift, int H, int dim, const int* table,
                                       i64 stride, int width, const int* start, int B, int count, b16* bounds,
                                       hipStream_t st) {
-    const int per = ((count - 1) >> shift) + 2;
-    const i64 n = (i64)B * per * H;
+    const int touched = ((count - 1) >> shift) + 2, per = touched < width ? touched : width;  // pages a sequence
     // A wave a page and head, or a block where the page is larger: 64 sequences' pages of 8 heads of 128 in 8 bits take 10.5 us
     // by waves and 13.2 by blocks at 256 rows, 28.2 and 24.8 at 1024; in 16 bits 8.6 and 7.7 at 128.
     const int waves = shift > (CODES == KV_INT8 || CODES == KV_FP8 ? 8 : 6) ? 4 : 1;
-    const i64 grid = (n * waves + 3) / 4;
-    if (n >= (i64)1 << 31) return -1;
+    // a launch has fewer than 2^32 threads: so many sequences at a time
+    const i64 each = (i64)per * H, most = ((((i64)1 << 26) - 4) / waves) / each;
+    if (most < 1) return -1;
+    for (i64 b0 = 0; b0 < B; b0 += most, table += most * stride, start += most) {
+        const i64 n = (B - b0 < most ? B - b0 : most) * each, grid = (n * waves + 3) / 4;
 #define BOUNDS_K(DP, WP) \
     bounds_k<CODES, DP, WP><<<(unsigned)grid, 256, 0, st>>>(k, ks, pages, shift, H, dim, table, stride, width, start, (u32)n, count, per, bounds)
 #define DP_CASE(DP)            \
     if (waves == 4) BOUNDS_K(DP, 4); \
     else BOUNDS_K(DP, 1)
-    switch ((dim + 63) / 64) {
-        case 1: DP_CASE(64); break;
-        case 2: DP_CASE(128); break;
-        case 3: DP_CASE(192); break;
-        default: DP_CASE(256);
+        switch ((dim + 63) / 64) {
+            case 1: DP_CASE(64); break;
+            case 2: DP_CASE(128); break;
+            case 3: DP_CASE(192); break;
+            default: DP_CASE(256);
+        }
+        const int rc = (int)hipGetLastError();
+        if (rc) return rc;
     }
 #undef DP_CASE
 #undef BOUNDS_K
-    return (int)hipGetLastError();
+    return 0;
 }

@@ -468,8 +468,9 @@ static bool sparse_plan(i64 B, i64 T, i64 H, i64 G, i64 dim, i64 width, i64 page
         width * page > lim || B * T > lim || H * ((G + 15) / 16) > 1 << 12)
         return false;
     p.dp = (int)(dim + 63) / 64 * 64, p.groups = (int)(G + 15) / 16, p.scored = width > keep;
-    // a pass takes as many sequences, or one sequence's tokens, as SLAB holds the scores and kept pages of, fewer than 2^24 units
-    const i64 each = H * ((p.scored ? width * 8 : 0) + keep * 4), most_units = ((i64)1 << 24) / (H * p.groups);
+    // a pass takes as many sequences, or one sequence's tokens, as SLAB holds the scores and kept pages of, fewer than 2^23 units
+    // (blocks of up to 512 threads, fewer than 2^32 in a launch)
+    const i64 each = H * ((p.scored ? width * 8 : 0) + keep * 4), most_units = (((i64)1 << 23) - 1) / (H * p.groups);
     i64 most = SLAB / each < most_units ? SLAB / each : most_units;
     if (most < 16) most = 16;
     p.nt = (int)(T <= most ? T : most / 16 * 16);
@@ -550,7 +551,7 @@ static int score_rows(ScoreArgs& a, int nb, int dp, hipStream_t st) {
     a.per = per ? (int)per : 64;
     a.chunks = (a.width + a.per - 1) / a.per;
     const i64 n = units * a.chunks;
-    if (n >= (i64)1 << 31) return -1;
+    if (n >= (i64)1 << 24) return -1;  // (a pass has fewer)
     if (tokens == 4) score_tokens<4>(a, dp, (unsigned)n, st);
     else if (tokens == 16) score_tokens<16>(a, dp, (unsigned)n, st);
     else switch (dp) {
