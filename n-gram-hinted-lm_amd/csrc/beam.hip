@@ -17,12 +17,15 @@
 // equal ranks come in their order).
 // An exponential is a 32-bit one: its argument's rounding and the instruction's are off by 2^-20 of a term, and average out over
 // a row's terms. (Putting each argument's rounding back took 5 more operations an element: 20.5 us a chunk's pass against 17.3
-// for 64 x 8 rows of 50257.)
+// for 64 x 8 rows of 50257.) One part does not average out: log2(e) as a float is 1.34e-8 of itself low, so a term is (m - v)
+// 1.34e-8 of itself large, m the row's largest logit, and a log-sum by 1.34e-8 times the mean of m - v under the softmax's
+// weights. That is no more than their entropy, ln V at most: 2^-22 for any V.
 //
 // Measured (in a trace, us): 64 x 8 rows of 50257 bfloat16 logits, a fifth of the beams finished (41 MB): chunks 17.7 (2.3
-// TB/s), joining 7.4; 8 x 32 rows of 100003 float32 ones, a tenth finished, 64 kept (92 MB): chunks 28 (3.3 TB/s), rows 7.1,
-// joining 9.4; one sequence of 4 beams: 6.0 and 6.4. The chunks' pass is bound by its vector instructions (a maximum, an
-// exponential and a comparison an element) and the halvings' barriers, the joining by one block's chain of them.
+// TB/s), joining 8.2; 8 x 32 rows of 100003 float32 ones, a tenth finished, 64 kept (92 MB): chunks 29 (3.2 TB/s), rows 7.2,
+// joining 9.3; one sequence of 4 beams: 6.0 and 6.5. The chunks' pass issues vector instructions in 55 and 61 % of its time (some
+// 500 and 900 a wave of 32 elements a lane, by counters), and its waves spend 54 and 46 % of theirs waiting, for the loads and at
+// the halvings' barriers; the joining is one block's chain of these. Finding a threshold without halvings has not been tried.
 #include "choose.h"
 #include "vals.h"
 

@@ -19,10 +19,12 @@
 //
 // Counts and pages are whole numbers and every choice is by order, so a call gives the same pages on every run.
 //
-// Measured (in a trace, us): 64 prompts of 8 rows forked (512 x 65 entries) 6.8, room for a token each 8.1, 448 copies of a
-// part of a page of 64 x 8 heads x 128 codes with the slots 8.5; a prompt of 4 rows 2.7, 4.9 and 2.9. The room is one block's
-// chain of loads, scans and barriers; what it must read is less than a microsecond's. A third of 8192 pages of 256 KiB packed
-// into another cache: 4.7, 4.6 and 267 (1.4 GB moved, 5.3 TB/s: memory bounds it).
+// Measured (in a trace, us): 64 prompts of 8 rows forked (512 x 65 entries) 6.7, room for a token each 8.5, 448 copies of a
+// part of a page of 64 x 8 heads x 128 codes with the slots 8.6; a prompt of 4 rows 2.7, 4.9 and 2.9. Where the table lies in the
+// caches, a fork of 512 rows takes 3.1 to read strips of four entries of each row, 0.7 more where the rows change places and 1.1
+// more where pages' counts change (4 rows: 1.9, 0.4 and 0.5). The room is one block's chain of loads, scans and barriers; what it
+// must read is less than a microsecond's. A third of 8192 pages of 256 KiB packed into
+// another cache: 4.7, 4.6 and 269 (1.4 GB moved, 5.3 TB/s: memory bounds it).
 #include "vals.h"
 #include <climits>
 

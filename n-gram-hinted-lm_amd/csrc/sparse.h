@@ -177,6 +177,9 @@ template <int O> __device__ __forceinline__ float halve(float a, float b) {
 // WP waves per (sequence, page that its tokens touch, head): the elements' smallest and largest over the page's rows, where
 // the tokens complete it. A lane holds E elements of a row, four rows' loads at a time. Of the lanes of one place in a row the
 // lower half then keeps the smallest, the upper half the largest (as the smallest of the negatives).
+// Pages of 32 rows of 8 heads of 128, 1125 of them: 12.7 us in 8 bits (3.4 TB/s), bound by vector instructions, 640 a wave of 64
+// elements a lane (75 % of the time by counters; the sums over lanes at a page's end, 16 elements each, among them); 15.3 in 16
+// bits (5.1 TB/s: memory).
 template <int CODES, int DP, int WP>
 __global__ __launch_bounds__(256) void bounds_k(const void* __restrict__ k, const float* __restrict__ ks, i64 pages, int shift,
                                                 int H, int dim, const int* __restrict__ table, i64 stride, int width,

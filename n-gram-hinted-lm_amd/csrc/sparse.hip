@@ -280,7 +280,8 @@ template <int DP, int TT> __global__ __launch_bounds__(256, DP <= 128 ? 4 : 2) v
                     const double *up = sums + (4 * r + g) * LD, *down = up + DP;
                     x = 0.;
 #pragma unroll 1
-                    for (int d = 0; d < a.dim; ++d) x += times(down[d], (double)(float)now[d]) + times(up[d], (double)(float)now[DP + d]);
+                    for (int d = 0; d < a.dim; ++d)
+                        x += times(down[d], (double)(float)now[d]) + times(up[d], (double)(float)now[DP + d]);
                 }
                 out[(i64)r * 4 * a.H * a.width + j] = score_key(is, x);
             }
@@ -597,8 +598,10 @@ extern "C" int ng_sparse_attention(const void* q, i64 qb, i64 qt, i64 qh, int qt
         s.b0 = r.b0 = b0, s.t0 = r.t0 = t0, s.nt = r.nt = T - t0 < p.nt ? T - t0 : p.nt;
         s.rows = (i64)nb * s.nt * H;
         int rc;
-        // one token a sequence: both at once where the rows fill half the CUs, a block each (32 sequences over 32768: 17.9 us
-        // against 15.2 and 7.4; one over 5000, 8 rows: 12.8 against 5.3 and 5.8)
+        // one token a sequence: both at once where the rows fill half the CUs, a block each. At once, and as scores and choice, in
+        // us: 128 rows of 313 pages 16.1, 9.1 and 8.2, of 512 18.2, 10.6 and 8.6, of 1024 23.5, 13.9 and 12.1; 96 rows 16.1, 7.0
+        // and 7.8, 17.4, 9.5 and 8.4, 23.6, 11.9 and 11.7. (Of few pages the two launches are shorter at 512 rows, too: of 128
+        // 17.0, 11.0 and 4.8.)
         if (p.scored && T == 1 && width <= FEW_PAGES && s.rows >= 128) {
             switch (p.dp) {
                 case 64: score_choose_k<64, 8><<<(unsigned)s.rows, 512, 0, st>>>(s); break;
@@ -608,8 +611,10 @@ extern "C" int ng_sparse_attention(const void* q, i64 qb, i64 qt, i64 qh, int qt
             }
         } else {
             if (p.scored && (rc = score_rows(s, nb, p.dp, st))) return rc;
-            // by the scores that a row can have: a wave's, a row a wave (5120 rows of 533: 11.0 us, by four waves each 32; 8
-            // rows of 313: 5.4 and 7.8); four waves'; a block's
+            // by the scores that a row can have, the fewest that a lane can hold, in us for 8 and for 5120 rows: 256 scores by
+            // 4 a lane 5.3 and 8.1, by 10 6.2 and 10.6; 640 by 10 a lane 7.8 and 13.4, by 16 8.9 and 16.0; 1024 by a wave 10.0
+            // and 18.0, by four 11.4 and 47.7. For 8 and 512 rows: 4096 by four waves 12.9 and 15.7, by sixteen 16.5 and 33.3;
+            // 16384 by 16 a lane 20.9 and 41.8, by 32 28.4 and 55.8
             if (width <= 256) choose_k<1, 4><<<(unsigned)((s.rows + 3) / 4), 256, 0, st>>>(s);
             else if (width <= 640) choose_k<1, 10><<<(unsigned)((s.rows + 3) / 4), 256, 0, st>>>(s);
             else if (width <= 1024) choose_k<1, 16><<<(unsigned)((s.rows + 3) / 4), 256, 0, st>>>(s);
