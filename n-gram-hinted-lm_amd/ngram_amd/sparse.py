@@ -6,10 +6,10 @@ of the cache no longer grows with the context.
   sparse_attention(q, cache, bounds, table, lengths, keep, ...)
 
 A page's bounds are the smallest and largest of each element of its keys, per head. Its score for a token is the sum over
-the query heads that share a cached head of sum_d max(q_d smallest_d, q_d largest_d), a q_d of 0 counting nothing: no key of
-the page has a larger sum of products with them. Of the pages that hold positions up to its own, a token keeps the `first` and the `last` ones (the last
-is its own page, which may be incomplete) and the best-scoring others, `keep` in all, for each cached head; equal scores go
-to the lower page. A page whose score is NaN is kept first, one that is no page of the cache last (its keys are masked).
+the query heads that share a cached head of sum_d max(q_d smallest_d, q_d largest_d), where a q_d of 0 counts nothing but
+beside a NaN: no key of the page has a larger sum of products with them. Of the pages that hold positions up to its own, a
+token keeps the `first` and the `last` ones (the last is its own page, which may be incomplete) and the best-scoring others,
+`keep` in all, for each cached head; equal scores go to the lower page. A page whose score is NaN is kept first, one that is no page of the cache last (its keys are masked).
 
 Scores are computed in 64 bits, so the choice does not depend on the order of sums. The attention over the kept pages is tree
 attention's (tree.py), with the same rounding. There is no backward pass; everything runs on the current stream, lengths
